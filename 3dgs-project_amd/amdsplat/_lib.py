@@ -68,6 +68,62 @@ class GsAdamGroup(C.Structure):
     ]
 
 
+GS_ROTARY_ADJACENT, GS_ROTARY_SHARED, GS_ROTARY_INVERSE = 1, 2, 4  # gs_rotary.flags
+
+
+class GsRotary(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_out", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("tokens", C.c_int64),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("base", C.c_double),
+        ("q_heads", C.c_int32),
+        ("k_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("axes", C.c_int32),
+        ("sections", C.c_int32 * 4),
+        ("dtype", C.c_int32),
+        ("flags", C.c_int32),
+    ]
+
+
+class GsAttention(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("q_offsets", C.c_void_p),
+        ("k_offsets", C.c_void_p),
+        ("k_lengths", C.c_void_p),
+        ("prefix", C.c_void_p),
+        ("q_tokens", C.c_int64),
+        ("k_tokens", C.c_int64),
+        ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64),
+        ("k_token_stride", C.c_int64),
+        ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("v_head_stride", C.c_int64),
+        ("docs", C.c_int32),
+        ("heads", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("dim", C.c_int32),
+        ("dtype", C.c_int32),
+        ("causal", C.c_int32),
+        ("softcap", C.c_float),
+        ("scale", C.c_float),
+    ]
+
+
 class AmdSplatError(RuntimeError):
     pass
 
@@ -115,6 +171,15 @@ _SIGS = {
     "gs_preprocess_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, C.POINTER(GsCamera), _vp, _vp,
                                  _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "gs_adam_step": (_i32, [C.POINTER(GsAdamGroup), _i32, _i64, _vp, _vp]),
+    "gs_adam_step_scaled": (_i32, [C.POINTER(GsAdamGroup), _i32, _i64, _vp, _vp, _vp]),
+    "gs_grad_norm_workspace_size": (_sz, [_vp, _i32]),
+    "gs_grad_norm": (_i32, [_vp, _vp, _vp, _i32, C.c_double, _vp, _vp, _vp, _sz, _vp]),
+    "gs_grad_scale": (_i32, [_vp, _vp, _vp, _vp, _i32, _vp, _vp]),
+    "gs_rotary_axes": (_i32, [_vp, _vp]),
+    "gs_attention_fwd_workspace_size": (_sz, [_vp]),
+    "gs_attention_fwd": (_i32, [_vp, _vp, _sz, _vp]),
+    "gs_attention_bwd_workspace_size": (_sz, [_vp]),
+    "gs_attention_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "gs_densification_stats": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp]),
     "gs_l1_ssim_workspace_size": (_sz, [_i32, _i32, _i32]),
     "gs_l1_ssim_fwd": (_i32, [_vp, _vp, _i32, _i32, _i32, C.c_float, _vp, _vp, _vp, _sz, _vp]),

@@ -21,6 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr
+from .clip import check_max_norm, clip_coefficient
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -48,11 +49,15 @@ def _group(grad, param, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps) -> _li
                             _dtype_code(exp_avg), int(step), float(lr), float(beta1), float(beta2), float(eps))
 
 
-def _launch(groups, n_primitives: int, visibility, device) -> None:
+def _launch(groups, n_primitives: int, visibility, device, grad_scale=None) -> None:
     for i in range(0, len(groups), _lib.GS_ADAM_MAX_GROUPS):
         chunk = groups[i:i + _lib.GS_ADAM_MAX_GROUPS]
         arr = (_lib.GsAdamGroup * len(chunk))(*chunk)
-        call("gs_adam_step", arr, len(chunk), int(n_primitives), ptr(visibility), _lib.stream_handle(device))
+        if grad_scale is None:
+            call("gs_adam_step", arr, len(chunk), int(n_primitives), ptr(visibility), _lib.stream_handle(device))
+        else:
+            call("gs_adam_step_scaled", arr, len(chunk), int(n_primitives), ptr(visibility), ptr(grad_scale),
+                 _lib.stream_handle(device))
 
 
 def _visibility(visibility, n_primitives: int):
@@ -100,16 +105,21 @@ class FusedAdam(torch.optim.Adam):
         _Rasterize.track_visibility = sparse
 
     @torch.no_grad()
-    def step(self, visibility: torch.Tensor | None = None) -> None:
+    def step(self, visibility: torch.Tensor | None = None, max_norm: float | None = None) -> torch.Tensor | None:
         """visibility: int32 [n_primitives] (> 0 = update), e.g. aux["visibility"] of the view's
-        forward; None takes the last differentiable forward's (sparse only)."""
+        forward; None takes the last differentiable forward's (sparse only). max_norm: the update
+        uses the gradients clipped to this global norm (of all groups' rows, visible or not), which
+        the call returns as a 0-dim device tensor; the gradients themselves are left unscaled."""
         from .raster3d import _Rasterize3D
 
+        if max_norm is not None:
+            max_norm = check_max_norm(max_norm)
         if not self.sparse:
             visibility = None
         elif visibility is None:
             visibility = _Rasterize3D.last_visibility
         batches: dict = {}
+        grads = []
         for group in self.param_groups:
             assert len(group["params"]) == 1, "more than one tensor in group"
             param = group["params"][0]
@@ -128,6 +138,7 @@ class FusedAdam(torch.optim.Adam):
             state["step"] += 1
             grad = param.grad.contiguous()
             _check(param, grad, state["exp_avg"], state["exp_avg_sq"])
+            grads.append(grad)
             n_prim = param.shape[0]
             vis = visibility
             if vis is not None and vis.numel() != n_prim:
@@ -138,5 +149,11 @@ class FusedAdam(torch.optim.Adam):
             batches.setdefault(key, (vis, []))[1].append(
                 _group(grad, param, state["exp_avg"], state["exp_avg_sq"], state["step"], group["lr"], b1, b2,
                        group["eps"]))
+        norm = scale = None
+        if max_norm is not None:
+            if not grads:
+                return torch.zeros(())
+            norm, scale = clip_coefficient(grads, max_norm)
         for (n_prim, _, device), (vis, groups) in batches.items():
-            _launch(groups, n_prim, _visibility(vis, n_prim), device)
+            _launch(groups, n_prim, _visibility(vis, n_prim), device, scale)
+        return norm

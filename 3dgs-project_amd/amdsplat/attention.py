@@ -1,0 +1,160 @@
+"""Softmax attention over packed documents on the GPU (gs_attention_fwd / gs_attention_bwd).
+
+`attention(q, k, v, ...)` is what a splat predictor (a transformer over the tokens of posed views
+whose output is a set of Gaussians) runs between its projections. The tokens of several scenes are
+packed one after the other; a scene is a document and sees itself only. Query heads may share key
+heads; scores may be capped by a tanh; the causal mask may leave a prefix that all tokens see; keys
+and values may be a cache that is longer than what it holds. bfloat16 or float32 CUDA tensors;
+statistics and sums are float32. Nothing is read back to the host.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from ._lib import call, ptr
+
+MAX_DIM = 128  # GS_ATTENTION_MAX_DIM
+_DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8)}
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """t itself if the kernels can read it through its strides, otherwise a contiguous copy."""
+    per = _DTYPES[t.dtype][1]
+    st, sh, sd = t.stride()
+    if t.numel() == 0:
+        return t
+    ok = ((sd == 1 or t.shape[2] == 1) and 0 <= st < 1 << 24 and 0 <= sh < 1 << 24 and st % per == 0 and sh % per == 0
+          and t.data_ptr() % 16 == 0)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _args(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale) -> _lib.GsAttention:
+    docs = 1 if offsets is None else offsets.numel() - 1
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if not q.numel():
+        qs = (0, 0, 1)
+    if not k.numel():
+        ks = vs = (0, 0, 1)
+    return _lib.GsAttention(ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(offsets), ptr(k_offsets), ptr(k_lengths),
+                            ptr(prefix), q.shape[0], k.shape[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], docs,
+                            q.shape[1], k.shape[1], q.shape[2], _DTYPES[q.dtype][0], int(causal), softcap, scale)
+
+
+def _workspace(name: str, args, device):
+    n = _lib.size_call(name, C.byref(args))
+    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+
+
+def _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale):
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    args = _args(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale)
+    ws, n = _workspace("gs_attention_fwd_workspace_size", args, q.device)
+    call("gs_attention_fwd", C.byref(args), ptr(ws), n, _lib.stream_handle(q.device))
+    return out, lse
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale):
+        q, k, v = _readable(q), _readable(k), _readable(v)
+        out, lse = _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale)
+        ctx.save_for_backward(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix)
+        ctx.rule = (causal, softcap, scale)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, _d_lse):
+        q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix = ctx.saved_tensors
+        d_out = d_out.contiguous()
+        if d_out.numel() and d_out.data_ptr() % 16:
+            d_out = d_out.clone()
+        d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        args = _args(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix, *ctx.rule)
+        ws, n = _workspace("gs_attention_bwd_workspace_size", args, q.device)
+        call("gs_attention_bwd", C.byref(args), ptr(d_out), ptr(d_q), ptr(d_k), ptr(d_v), ptr(ws), n,
+             _lib.stream_handle(q.device))
+        return (d_q, d_k, d_v) + (None,) * 7
+
+
+def _table(t, name: str, n: int, device) -> None:
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
+            and t.device == device):
+        raise ValueError(f"{name} must be a contiguous int32 tensor on the tensors' device")
+    if t.numel() != n:
+        raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: torch.Tensor | None = None,
+              k_offsets: torch.Tensor | None = None, k_lengths: torch.Tensor | None = None, causal: bool = False,
+              prefix: torch.Tensor | None = None, softcap: float = 0.0, scale: float | None = None,
+              return_lse: bool = False):
+    """out [Tq, heads, D] (and with return_lse the float32 log-sum-exp [Tq, heads], which takes no
+    gradient) of q [Tq, heads, D] over k, v [Tk, kv_heads, D]; differentiable in q, k and v.
+
+    offsets [docs + 1] int32, non-decreasing: document d's tokens are offsets[d] .. offsets[d + 1]
+    (None: one document of all tokens). k_offsets: the same for the keys (None: as the queries).
+    k_lengths [docs] int32: of a document's key tokens only the first so many are there (a cache);
+    the rest may hold anything. causal: query i of a document of Lq queries and Lk keys sees key j
+    if j <= i + Lk - Lq; prefix [docs] int32 (with causal): or if j < prefix[d]. softcap c > 0: scores
+    s become c tanh(s / c). scale: of the scores before the cap (default 1 / sqrt(D)).
+
+    A query that sees no key gets 0 and -infinity. D up to 128 (padded to a multiple of 8 by a copy).
+    Tensors are read through their strides where these and the addresses are multiples of 16 bytes
+    and the last dimension is contiguous; otherwise they are copied first."""
+    if not (q.dim() == k.dim() == v.dim() == 3):
+        raise ValueError("q, k and v must be [tokens, heads, D]")
+    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v must share a dtype, float32 or bfloat16: got {q.dtype}, {k.dtype}, {v.dtype}")
+    device = q.device
+    if not q.is_cuda or k.device != device or v.device != device:
+        raise ValueError("q, k and v must be on one GPU")
+    (tq, heads, d), (tk, kv_heads, _) = q.shape, k.shape
+    if k.shape != v.shape or k.shape[2] != d:
+        raise ValueError(f"shape mismatch: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if not 1 <= d <= MAX_DIM:
+        raise ValueError(f"head size {d}: 1 to {MAX_DIM} are provided")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} heads are not a multiple of {kv_heads} key heads")
+    if offsets is None and k_offsets is not None:
+        raise ValueError("k_offsets without offsets")
+    docs = 1
+    if offsets is not None:
+        docs = offsets.numel() - 1
+        if docs < 1:
+            raise ValueError("offsets must have at least 2 entries")
+        _table(offsets, "offsets", docs + 1, device)
+        if k_offsets is None:
+            if tk != tq:
+                raise ValueError(f"{tk} keys for {tq} queries: pass k_offsets")
+            k_offsets = offsets
+        else:
+            _table(k_offsets, "k_offsets", docs + 1, device)
+    if k_lengths is not None:
+        _table(k_lengths, "k_lengths", docs, device)
+    if prefix is not None:
+        if not causal:
+            raise ValueError("a prefix needs causal=True")
+        _table(prefix, "prefix", docs, device)
+    softcap = float(softcap)
+    if not (softcap >= 0.0 and math.isfinite(softcap)):
+        raise ValueError("softcap must be finite and >= 0")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if d % 8:
+        q, k, v = (torch.nn.functional.pad(t, (0, -d % 8)) for t in (q, k, v))
+    rest = (offsets, k_offsets, k_lengths, prefix, bool(causal), softcap, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _Attention.apply(q, k, v, *rest)
+    else:
+        out, lse = _forward(_readable(q), _readable(k), _readable(v), *rest)
+    if d % 8:
+        out = out[..., :d]
+    return (out, lse) if return_lse else out

@@ -20,7 +20,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT = HERE / "amdsplat" / "libamdsplat.so"
 SOURCES = ["capi.hip", "preprocess.hip", "binning.hip", "blend.hip", "view.hip", "raster2d.hip", "adam.hip", "loss.hip",
-           "probe.hip"]
+           "attention.hip", "rotary.hip", "clip.hip", "probe.hip"]
 
 HIPCC_FLAGS = [
     "-O3",

@@ -23,12 +23,14 @@ struct AdamGroupK {
   uint32_t seed;
   int lowp;
   float step_size, beta1, beta2, eps, bc2;
+  float new1, new2;  // 1 - beta, rounded from double (the scaled update's weights)
 };
 
 struct AdamArgs {
   AdamGroupK g[GS_ADAM_MAX_GROUPS];
   int n_groups;
   const int32_t* vis;
+  const float* scale;  // factor of every gradient (a clipping coefficient), one device float
 };
 
 // Integer hash of the stochastic rounding (the 32-bit "lowbias32" finaliser: xor-shift,
@@ -46,15 +48,28 @@ __device__ __forceinline__ uint16_t to_bf16_sr(float f, uint32_t rnd) {
   return static_cast<uint16_t>((__float_as_uint(f) + (rnd & 0xffffu)) >> 16);
 }
 
+// The scaled update weights the new value by 1 - beta as rounded from double. The plain one keeps the
+// reference's form, where the rounding of beta2 itself (0.999 to float32) leaves 1 - beta2, and with
+// it a fresh v, off by 1.3e-5.
+template <bool SCALED>
 __device__ __forceinline__ void adam_elem(const AdamGroupK& G, float g, float& p, float& m, float& v) {
   const float gsq = g * g;
-  m = fmaf(G.beta1, m - g, g);
-  v = fmaf(G.beta2, v - gsq, gsq);
+  if constexpr (SCALED) {
+    m = fmaf(G.new1, g - m, m);
+    v = fmaf(G.new2, gsq - v, v);
+  } else {
+    m = fmaf(G.beta1, m - g, g);
+    v = fmaf(G.beta2, v - gsq, gsq);
+  }
   const float denom = sqrtf(v) * G.bc2 + G.eps;
   p = p - (G.step_size * m) / denom;
 }
 
+// SCALED: the gradient is multiplied by *a.scale as it is read, so a clipped step takes no pass of its
+// own over the gradients (8 bytes per element beside the update's 28).
+template <bool SCALED>
 __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
+  const float scale = SCALED ? *a.scale : 1.0f;
   int gi = 0;
 #pragma unroll
   for (int k = 1; k < GS_ADAM_MAX_GROUPS; ++k)
@@ -94,6 +109,10 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
     const float4 g4 = *reinterpret_cast<const float4*>(G.grad + e0);
     const float4 p4 = *reinterpret_cast<const float4*>(G.param + e0);
     g[0] = g4.x; g[1] = g4.y; g[2] = g4.z; g[3] = g4.w;
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int k = 0; k < kAdamPerThread; ++k) g[k] *= scale;
+    }
     p[0] = p4.x; p[1] = p4.y; p[2] = p4.z; p[3] = p4.w;
     if (!G.lowp && ((reinterpret_cast<uintptr_t>(static_cast<float*>(G.m) + e0) |
                      reinterpret_cast<uintptr_t>(static_cast<float*>(G.v) + e0)) & 15u) == 0) {
@@ -103,7 +122,7 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
       v[0] = v4.x; v[1] = v4.y; v[2] = v4.z; v[3] = v4.w;
 #pragma unroll
       for (int k = 0; k < kAdamPerThread; ++k)
-        if (live[k]) adam_elem(G, g[k], p[k], m[k], v[k]);
+        if (live[k]) adam_elem<SCALED>(G, g[k], p[k], m[k], v[k]);
       *reinterpret_cast<float4*>(G.param + e0) = make_float4(p[0], p[1], p[2], p[3]);
       *reinterpret_cast<float4*>(static_cast<float*>(G.m) + e0) = make_float4(m[0], m[1], m[2], m[3]);
       *reinterpret_cast<float4*>(static_cast<float*>(G.v) + e0) = make_float4(v[0], v[1], v[2], v[3]);
@@ -120,7 +139,7 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
         m[k] = __uint_as_float(((mw[k >> 1] >> sh) & 0xffffu) << 16);
         v[k] = __uint_as_float(((vw[k >> 1] >> sh) & 0xffffu) << 16);
         if (!live[k]) continue;
-        adam_elem(G, g[k], p[k], m[k], v[k]);
+        adam_elem<SCALED>(G, g[k], p[k], m[k], v[k]);
         const int64_t idx = e0 + k;
         const uint32_t r1 = sr_hash(static_cast<uint32_t>(idx) ^ G.seed);
         const uint32_t r2 = sr_hash(r1);
@@ -146,7 +165,7 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
       mk = static_cast<const float*>(G.m)[idx];
       vk = static_cast<const float*>(G.v)[idx];
     }
-    adam_elem(G, G.grad[idx], pk, mk, vk);
+    adam_elem<SCALED>(G, SCALED ? G.grad[idx] * scale : G.grad[idx], pk, mk, vk);
     G.param[idx] = pk;
     if (G.lowp) {
       const uint32_t r1 = sr_hash(static_cast<uint32_t>(idx) ^ G.seed);
@@ -164,15 +183,15 @@ __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
 
 using namespace gs;
 
-extern "C" int gs_adam_step(const gs_adam_group* groups, int n_groups, int64_t n_primitives,
-                            const int32_t* visibility, void* stream) {
-  clear_error();
+static int adam_launch(const gs_adam_group* groups, int n_groups, int64_t n_primitives, const int32_t* visibility,
+                       const float* grad_scale, void* stream) {
   GS_REQUIRE(groups && n_groups >= 1 && n_groups <= GS_ADAM_MAX_GROUPS, GS_ERR_ARG,
              "need 1 to %d parameter groups", GS_ADAM_MAX_GROUPS);
   GS_REQUIRE(n_primitives >= 0, GS_ERR_ARG, "n_primitives must be >= 0");
   AdamArgs a = {};
   a.n_groups = n_groups;
   a.vis = visibility;
+  a.scale = grad_scale;
   int64_t blocks = 0;
   for (int i = 0; i < n_groups; ++i) {
     const gs_adam_group& q = groups[i];
@@ -203,12 +222,31 @@ extern "C" int gs_adam_step(const gs_adam_group* groups, int n_groups, int64_t n
     g.beta1 = static_cast<float>(q.beta1);
     g.beta2 = static_cast<float>(q.beta2);
     g.eps = static_cast<float>(q.eps);
+    g.new1 = static_cast<float>(1.0 - q.beta1);
+    g.new2 = static_cast<float>(1.0 - q.beta2);
     g.bc2 = static_cast<float>(bc2);
     blocks += (q.n_elements + kAdamBlockElems - 1) / kAdamBlockElems;
   }
   for (int i = n_groups; i < GS_ADAM_MAX_GROUPS; ++i) a.g[i].block0 = INT64_MAX;
   if (blocks == 0) return GS_OK;
   GS_REQUIRE(blocks < (int64_t(1) << 31), GS_ERR_ARG, "too many elements");
-  hipLaunchKernelGGL(adam_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kAdamThreads), 0, as_stream(stream), a);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(kAdamThreads);
+  if (grad_scale)
+    hipLaunchKernelGGL(adam_kernel<true>, grid, block, 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(adam_kernel<false>, grid, block, 0, as_stream(stream), a);
   return check_launch("adam_step");
+}
+
+extern "C" int gs_adam_step(const gs_adam_group* groups, int n_groups, int64_t n_primitives,
+                            const int32_t* visibility, void* stream) {
+  clear_error();
+  return adam_launch(groups, n_groups, n_primitives, visibility, nullptr, stream);
+}
+
+extern "C" int gs_adam_step_scaled(const gs_adam_group* groups, int n_groups, int64_t n_primitives,
+                                   const int32_t* visibility, const float* grad_scale, void* stream) {
+  clear_error();
+  GS_REQUIRE(grad_scale && aligned(grad_scale, 4), GS_ERR_ARG, "adam_step_scaled: needs the gradients' factor");
+  return adam_launch(groups, n_groups, n_primitives, visibility, grad_scale, stream);
 }

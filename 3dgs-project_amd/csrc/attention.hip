@@ -1,0 +1,513 @@
+// Softmax attention over packed documents, forward and backward (see gs_attention.h for the layout
+// of the products). A query row is a (token, head of the group) pair: the heads that share a key
+// head are rows of one tile, so a key tile is read once for all of them and the gradients of shared
+// heads are summed inside one workgroup, in a fixed order, without atomics.
+#include "gs_attention.h"
+
+namespace gs {
+
+constexpr int kAttnWaves = 4;
+constexpr int kAttnThreads = kAttnWaves * kWave;
+constexpr int kAttnRows = kAttnWaves * 32;  // query rows (or keys, in the key gradients) of a workgroup
+constexpr int kAttnKeys = 64;               // keys (or query rows) of a tile in LDS
+
+// Copies rows [0, valid) of a strided matrix to a tile, zero beyond them and beyond `dim`.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void stage(char* lds, const T* src, int64_t stride, int valid, int dim) {
+  using L = Tile<T, DP>;
+#pragma unroll
+  for (int i = 0; i < ROWS * L::kChunks / kAttnThreads; ++i) {
+    const int e = i * kAttnThreads + static_cast<int>(threadIdx.x);
+    const int row = e / L::kChunks, chunk = e % L::kChunks;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row < valid && chunk * L::kElemsPerChunk < dim)
+      v = *reinterpret_cast<const f32x4*>(src + row * stride + chunk * L::kElemsPerChunk);
+    *reinterpret_cast<f32x4*>(lds + L::at(row, chunk)) = v;
+  }
+}
+
+// The rows of a tile of (token, head of the group) pairs.
+struct RowMap {
+  int64_t token0;
+  int group, head0;
+};
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void stage_rows(char* lds, const T* src, int64_t token_stride, int64_t head_stride,
+                                           const RowMap& m, int row0, int valid, int dim) {
+  using L = Tile<T, DP>;
+#pragma unroll
+  for (int i = 0; i < ROWS * L::kChunks / kAttnThreads; ++i) {
+    const int e = i * kAttnThreads + static_cast<int>(threadIdx.x);
+    const int row = e / L::kChunks, chunk = e % L::kChunks;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (row < valid && chunk * L::kElemsPerChunk < dim) {
+      const int r = row0 + row, t = r / m.group;
+      v = *reinterpret_cast<const f32x4*>(src + (m.token0 + t) * token_stride +
+                                          (m.head0 + r - t * m.group) * head_stride + chunk * L::kElemsPerChunk);
+    }
+    *reinterpret_cast<f32x4*>(lds + L::at(row, chunk)) = v;
+  }
+}
+
+// Score in units of ln 2 (the softmax is taken in base 2), and the capped score's slope.
+template <typename T, bool CAP>
+__device__ __forceinline__ float score(float s, float scale2, float in_scale, float cap2) {
+  if constexpr (CAP) return cap2 * tanh_of<T>(s * in_scale);
+  return s * scale2;
+}
+
+template <typename T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int C = DP / 16;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kAttnKeys * L::kRowBytes];
+  char* lk = lds;
+  char* lv = lds + kAttnKeys * L::kRowBytes;
+  const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
+  const int64_t tile = a.n_tiles - 1 - static_cast<int64_t>(blockIdx.x / a.kv_heads);
+  int64_t first;
+  const int di = find_stretch(a.q_offsets, a.q_tokens, a.docs, a.group, kAttnRows, tile, &first);
+  const Doc doc = doc_of(a, di);
+  const int rows = static_cast<int>(doc.q_len) * a.group;
+  const int64_t base = (tile - first) * kAttnRows;
+  if (base >= rows) return;
+  const int row0 = static_cast<int>(base);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int wrow = row0 + wave * 32;
+  const int row = wrow + (lane & 31);
+  const bool live = row < rows;
+  const int rc = live ? row : rows - 1;
+  const int tok = rc / a.group, head = hk * a.group + rc - tok * a.group;
+  const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
+  Frag<T> q[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) q[c] = load_frag<T>(qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
+  const int vis = visible(a, doc, tok);
+  const int wave_min = visible(a, doc, min(wrow, rows - 1) / a.group);
+  const int end = visible(a, doc, min(row0 + kAttnRows, rows) == 0 ? 0 : (min(row0 + kAttnRows, rows) - 1) / a.group);
+  const float scale2 = a.scale * kLog2e;
+  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  f32x16 o[DP / 32] = {};
+  float m = -INFINITY, l = 0.0f;
+  const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
+  for (int k0 = 0; k0 < end; k0 += kAttnKeys) {
+    const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
+    __syncthreads();
+    stage<T, DP, kAttnKeys>(lk, kp + k0 * a.k_token, a.k_token, valid, a.dim);
+    stage<T, DP, kAttnKeys>(lv, vp + k0 * a.v_token, a.v_token, valid, a.dim);
+    __syncthreads();
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) mma(s[st], L::rows(lk, 32 * st, c, lane), q[c]);
+    const bool mask = k0 + kAttnKeys > wave_min;
+    float top = m;
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = score<T, CAP>(s[st][r], scale2, in_scale, cap2);
+        if (mask && k0 + 32 * st + 8 * (r / 4) + 4 * h + r % 4 >= vis) x = -INFINITY;
+        s[st][r] = x;
+        top = fmaxf(top, x);
+      }
+    top = half_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float alpha = exp2_hw(m - ref);
+    m = top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[st][r] = exp2_hw(s[st][r] - ref);
+        sum += s[st][r];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= alpha;
+#pragma unroll
+    for (int kc = 0; kc < 4; ++kc) {
+      const Frag<T> p = acc_frag<T>(s[kc / 2], kc % 2);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], L::cols(lv, 32 * dt, 16 * kc, lane), p);
+    }
+  }
+  if (!live) return;
+  l = half_sum(l);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  T* op = static_cast<T*>(a.out) + ((doc.q0 + tok) * a.heads + head) * a.dim;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * h;
+      if (d < a.dim) store4(op + d, o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv);
+    }
+  if (h == 0) a.lse[(doc.q0 + tok) * a.heads + head] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// Query gradients, and delta_i = dO_i . O_i for the key gradients.
+template <typename T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int C = DP / 16;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kAttnKeys * L::kRowBytes];
+  char* lk = lds;
+  char* lv = lds + kAttnKeys * L::kRowBytes;
+  const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
+  const int64_t tile = a.n_tiles - 1 - static_cast<int64_t>(blockIdx.x / a.kv_heads);
+  int64_t first;
+  const int di = find_stretch(a.q_offsets, a.q_tokens, a.docs, a.group, kAttnRows, tile, &first);
+  const Doc doc = doc_of(a, di);
+  const int rows = static_cast<int>(doc.q_len) * a.group;
+  const int64_t base = (tile - first) * kAttnRows;
+  if (base >= rows) return;
+  const int row0 = static_cast<int>(base);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int wrow = row0 + wave * 32;
+  const int row = wrow + (lane & 31);
+  const bool live = row < rows;
+  const int rc = live ? row : rows - 1;
+  const int tok = rc / a.group, head = hk * a.group + rc - tok * a.group;
+  const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
+  const int64_t at = ((doc.q0 + tok) * a.heads + head) * a.dim;
+  const T* gp = static_cast<const T*>(a.d_out) + at;
+  const T* op = static_cast<const T*>(a.out) + at;
+  Frag<T> q[C], g[C];
+  float delta = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const bool in = 16 * c + 8 * h < a.dim;
+    q[c] = load_frag<T>(qp + 16 * c + 8 * h, in);
+    g[c] = load_frag<T>(gp + 16 * c + 8 * h, in);
+    const Frag<T> o = load_frag<T>(op + 16 * c + 8 * h, in);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta = fmaf(static_cast<float>(g[c][j]), static_cast<float>(o[j]), delta);
+  }
+  delta = half_sum(delta);
+  const int64_t stat = (doc.q0 + tok) * a.heads + head;
+  if (live && h == 0) a.delta[stat] = delta;
+  const float lse = a.lse[stat];
+  const float lse2 = lse == -INFINITY ? 0.0f : lse * kLog2e;
+  const int vis = live ? visible(a, doc, tok) : 0;
+  const int wave_min = wrow + 31 < rows ? visible(a, doc, wrow / a.group) : 0;
+  const int end = visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group);
+  const float scale2 = a.scale * kLog2e;
+  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  f32x16 dq[DP / 32] = {};
+  const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
+  for (int k0 = 0; k0 < end; k0 += kAttnKeys) {
+    const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
+    __syncthreads();
+    stage<T, DP, kAttnKeys>(lk, kp + k0 * a.k_token, a.k_token, valid, a.dim);
+    stage<T, DP, kAttnKeys>(lv, vp + k0 * a.v_token, a.v_token, valid, a.dim);
+    __syncthreads();
+    const bool mask = k0 + kAttnKeys > wave_min;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        mma(s, L::rows(lk, 32 * st, c, lane), q[c]);
+        mma(dp, L::rows(lv, 32 * st, c, lane), g[c]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float ds;
+        if constexpr (CAP) {
+          const float t = tanh_of<T>(s[r] * in_scale);
+          ds = exp2_hw(fmaf(cap2, t, -lse2)) * (dp[r] - delta) * fmaf(-t, t, 1.0f);
+        } else {
+          ds = exp2_hw(fmaf(s[r], scale2, -lse2)) * (dp[r] - delta);
+        }
+        if (mask && k0 + 32 * st + 8 * (r / 4) + 4 * h + r % 4 >= vis) ds = 0.0f;
+        s[r] = ds;
+      }
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        const Frag<T> p = acc_frag<T>(s, kc);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) mma(dq[dt], L::cols(lk, 32 * dt, 32 * st + 16 * kc, lane), p);
+      }
+    }
+  }
+  if (!live) return;
+  T* dp = static_cast<T*>(a.d_q) + at;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * h;
+      if (d < a.dim)
+        store4(dp + d, dq[dt][r] * a.scale, dq[dt][r + 1] * a.scale, dq[dt][r + 2] * a.scale,
+               dq[dt][r + 3] * a.scale);
+    }
+}
+
+// Key and value gradients: a lane owns one key, the workgroup walks over the query rows that see it.
+template <typename T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int C = DP / 16;
+  constexpr int R = 32;  // query rows of a tile
+  __shared__ __attribute__((aligned(16))) char lds[2 * R * L::kRowBytes];
+  __shared__ __attribute__((aligned(16))) float l_lse[R], l_delta[R];
+  __shared__ __attribute__((aligned(16))) int l_vis[R];
+  char* lq = lds;
+  char* lg = lds + R * L::kRowBytes;
+  const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
+  const int64_t tile = blockIdx.x / a.kv_heads;
+  int64_t first;
+  const int di = find_stretch(a.k_offsets, a.k_tokens, a.docs, 1, kAttnRows, tile, &first);
+  const Doc doc = doc_of(a, di);
+  const int64_t base = (tile - first) * kAttnRows;
+  if (base >= doc.k_cap) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int key0 = static_cast<int>(base), wkey = key0 + wave * 32;
+  const int key = wkey + (lane & 31);
+  const bool live = key < doc.k_len;
+  Frag<T> k[C], v[C];
+  const T* kp = static_cast<const T*>(a.k) + (doc.k0 + key) * a.k_token + hk * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + (doc.k0 + key) * a.v_token + hk * a.v_head;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const bool in = live && 16 * c + 8 * h < a.dim;
+    k[c] = load_frag<T>(kp + 16 * c + 8 * h, in);
+    v[c] = load_frag<T>(vp + 16 * c + 8 * h, in);
+  }
+  const int rows = static_cast<int>(doc.q_len) * a.group;
+  // the first token that sees key0 (none of this tile's keys is seen by one before it)
+  int row_begin = 0;
+  if (a.causal && key0 >= doc.prefix) {
+    const int64_t t = key0 - doc.k_len + doc.q_len;
+    if (t > 0) row_begin = static_cast<int>(t < doc.q_len ? t : doc.q_len) * a.group;
+  }
+  if (key0 >= doc.k_len) row_begin = rows;
+  const float scale2 = a.scale * kLog2e;
+  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+  const RowMap map = {doc.q0, a.group, hk * a.group};
+  for (int r0 = row_begin; r0 < rows; r0 += R) {
+    const int valid = min(R, rows - r0);
+    __syncthreads();
+    stage_rows<T, DP, R>(lq, static_cast<const T*>(a.q), a.q_token, a.q_head, map, r0, valid, a.dim);
+    stage_rows<T, DP, R>(lg, static_cast<const T*>(a.d_out), static_cast<int64_t>(a.heads) * a.dim, a.dim, map, r0,
+                         valid, a.dim);
+    if (threadIdx.x < R) {
+      const int r = r0 + threadIdx.x;
+      float lse = 0.0f, delta = 0.0f;
+      int vis = 0;
+      if (r < rows) {
+        const int t = r / a.group;
+        const int64_t stat = (doc.q0 + t) * a.heads + hk * a.group + r - t * a.group;
+        lse = a.lse[stat];
+        lse = lse == -INFINITY ? 0.0f : lse * kLog2e;
+        delta = a.delta[stat];
+        vis = visible(a, doc, t);
+      }
+      l_lse[threadIdx.x] = lse;
+      l_delta[threadIdx.x] = delta;
+      l_vis[threadIdx.x] = vis;
+    }
+    __syncthreads();
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      mma(s, L::rows(lq, 0, c, lane), k[c]);
+      mma(dp, L::rows(lg, 0, c, lane), v[c]);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = 8 * (r / 4) + 4 * h + r % 4;
+      float p, ds;
+      if constexpr (CAP) {
+        const float t = tanh_of<T>(s[r] * in_scale);
+        p = exp2_hw(fmaf(cap2, t, -l_lse[i]));
+        ds = p * (dp[r] - l_delta[i]) * fmaf(-t, t, 1.0f);
+      } else {
+        p = exp2_hw(fmaf(s[r], scale2, -l_lse[i]));
+        ds = p * (dp[r] - l_delta[i]);
+      }
+      if (key >= l_vis[i]) p = ds = 0.0f;
+      s[r] = p;
+      dp[r] = ds;
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      const Frag<T> p = acc_frag<T>(s, kc), ds = acc_frag<T>(dp, kc);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) {
+        mma(dv[dt], L::cols(lg, 32 * dt, 16 * kc, lane), p);
+        mma(dk[dt], L::cols(lq, 32 * dt, 16 * kc, lane), ds);
+      }
+    }
+  }
+  if (key >= doc.k_cap) return;
+  const int64_t at = ((doc.k0 + key) * a.kv_heads + hk) * a.dim;
+  T* dkp = static_cast<T*>(a.d_k) + at;
+  T* dvp = static_cast<T*>(a.d_v) + at;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int d = 32 * dt + 2 * r + 4 * h;
+      if (d < a.dim) {
+        store4(dkp + d, dk[dt][r] * a.scale, dk[dt][r + 1] * a.scale, dk[dt][r + 2] * a.scale,
+               dk[dt][r + 3] * a.scale);
+        store4(dvp + d, dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]);
+      }
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+static int attn_setup(const gs_attention* p, bool backward, AttnArgs& a) {
+  GS_REQUIRE(p != nullptr, GS_ERR_ARG, "attention: arguments are NULL");
+  GS_REQUIRE(p->dtype == GS_FLOAT32 || p->dtype == GS_BFLOAT16, GS_ERR_ARG,
+             "attention: dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(p->heads >= 1 && p->kv_heads >= 1 && p->heads % p->kv_heads == 0, GS_ERR_ARG,
+             "attention: %d heads are not a multiple of %d key heads", p->heads, p->kv_heads);
+  GS_REQUIRE(p->dim >= 8 && p->dim <= GS_ATTENTION_MAX_DIM && p->dim % 8 == 0, GS_ERR_ARG,
+             "attention: head size must be a multiple of 8 up to %d (got %d)", GS_ATTENTION_MAX_DIM, p->dim);
+  GS_REQUIRE(p->docs >= 1, GS_ERR_ARG, "attention: need at least one document");
+  GS_REQUIRE(p->docs == 1 || (p->q_offsets && p->k_offsets), GS_ERR_ARG,
+             "attention: several documents need their offsets");
+  GS_REQUIRE(p->q_tokens >= 0 && p->k_tokens >= 0, GS_ERR_ARG, "attention: token counts must be >= 0");
+  const int64_t group = p->heads / p->kv_heads;
+  GS_REQUIRE(p->q_tokens * group < (int64_t(1) << 30) && p->k_tokens < (int64_t(1) << 30) &&
+                 p->docs < (1 << 26), GS_ERR_ARG, "attention: too many tokens or documents");
+  GS_REQUIRE(p->prefix == nullptr || p->causal, GS_ERR_ARG, "attention: a prefix needs the causal mask");
+  GS_REQUIRE(p->scale == p->scale && p->softcap >= 0.0f && p->softcap <= FLT_MAX &&
+                 p->scale <= FLT_MAX && p->scale >= -FLT_MAX, GS_ERR_ARG,
+             "attention: scale must be finite, softcap finite and >= 0");
+  const bool has_q = p->q_tokens > 0, has_k = p->k_tokens > 0;
+  GS_REQUIRE((!has_q || (p->q && p->out && p->lse)) && (!has_k || (p->k && p->v)), GS_ERR_ARG,
+             "attention: null pointer");
+  const int64_t elems = p->dtype == GS_BFLOAT16 ? 8 : 4;
+  const int64_t strides[6] = {p->q_token_stride, p->q_head_stride, p->k_token_stride,
+                              p->k_head_stride, p->v_token_stride, p->v_head_stride};
+  for (int i = 0; i < 6; ++i)
+    GS_REQUIRE(strides[i] >= 0 && strides[i] < (int64_t(1) << 24) && strides[i] % elems == 0, GS_ERR_ALIGN,
+               "attention: strides must be multiples of 16 bytes, below 2^24 elements (got %lld)",
+               static_cast<long long>(strides[i]));
+  GS_REQUIRE(aligned(p->q, 16) && aligned(p->k, 16) && aligned(p->v, 16) && aligned(p->out, 16) &&
+                 aligned(p->lse, 4), GS_ERR_ALIGN, "attention: tensors must be 16-byte aligned");
+  a = {};
+  a.q = p->q;
+  a.k = p->k;
+  a.v = p->v;
+  a.out = p->out;
+  a.lse = p->lse;
+  a.q_offsets = p->q_offsets;
+  a.k_offsets = p->k_offsets;
+  a.k_lengths = p->k_lengths;
+  a.prefix = p->prefix;
+  a.q_tokens = p->q_tokens;
+  a.k_tokens = p->k_tokens;
+  a.q_token = p->q_token_stride;
+  a.q_head = p->q_head_stride;
+  a.k_token = p->k_token_stride;
+  a.k_head = p->k_head_stride;
+  a.v_token = p->v_token_stride;
+  a.v_head = p->v_head_stride;
+  a.docs = p->docs;
+  a.heads = p->heads;
+  a.kv_heads = p->kv_heads;
+  a.group = static_cast<int>(group);
+  a.dim = p->dim;
+  a.causal = p->causal != 0;
+  a.softcap = p->softcap;
+  a.scale = p->scale;
+  return GS_OK;
+}
+
+// Tiles of `rows` rows that `tokens` tokens of `per` rows in docs + 2 stretches can take.
+static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { return tokens * per / rows + docs + 2; }
+
+#define GS_ATTN_LAUNCH(KERNEL, GRID)                                                                       \
+  do {                                                                                                     \
+    const dim3 grid_(static_cast<unsigned>(GRID)), block_(kAttnThreads);                                   \
+    const bool cap_ = a.softcap > 0.0f, wide_ = a.dim > 64;                                                \
+    if (p->dtype == GS_BFLOAT16) {                                                                         \
+      if (wide_ && cap_) hipLaunchKernelGGL((KERNEL<__bf16, 128, true>), grid_, block_, 0, st, a);         \
+      else if (wide_) hipLaunchKernelGGL((KERNEL<__bf16, 128, false>), grid_, block_, 0, st, a);           \
+      else if (cap_) hipLaunchKernelGGL((KERNEL<__bf16, 64, true>), grid_, block_, 0, st, a);              \
+      else hipLaunchKernelGGL((KERNEL<__bf16, 64, false>), grid_, block_, 0, st, a);                       \
+    } else {                                                                                               \
+      if (wide_ && cap_) hipLaunchKernelGGL((KERNEL<float, 128, true>), grid_, block_, 0, st, a);          \
+      else if (wide_) hipLaunchKernelGGL((KERNEL<float, 128, false>), grid_, block_, 0, st, a);            \
+      else if (cap_) hipLaunchKernelGGL((KERNEL<float, 64, true>), grid_, block_, 0, st, a);               \
+      else hipLaunchKernelGGL((KERNEL<float, 64, false>), grid_, block_, 0, st, a);                        \
+    }                                                                                                      \
+  } while (0)
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" size_t gs_attention_fwd_workspace_size(const gs_attention* p) {
+  clear_error();
+  (void)p;
+  return 0;
+}
+
+extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  (void)workspace;
+  (void)workspace_bytes;
+  AttnArgs a;
+  if (const int rc = attn_setup(p, false, a)) return rc;
+  if (p->q_tokens == 0) return GS_OK;
+  const hipStream_t st = as_stream(stream);
+  const int64_t tiles = tiles_of(a.q_tokens, a.group, kAttnRows, a.docs);
+  GS_REQUIRE(tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG, "attention: too many tokens, documents or heads");
+  a.n_tiles = static_cast<int>(tiles);
+  GS_ATTN_LAUNCH(attn_fwd_kernel, tiles * a.kv_heads);
+  return check_launch("attention");
+}
+
+extern "C" size_t gs_attention_bwd_workspace_size(const gs_attention* p) {
+  clear_error();
+  if (p == nullptr || p->q_tokens <= 0 || p->heads <= 0) return 0;
+  return static_cast<size_t>(p->q_tokens) * p->heads * sizeof(float);
+}
+
+extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* d_q, void* d_k, void* d_v,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  AttnArgs a;
+  if (const int rc = attn_setup(p, true, a)) return rc;
+  GS_REQUIRE((p->q_tokens == 0 || (d_out && d_q)) && (p->k_tokens == 0 || (d_k && d_v)), GS_ERR_ARG,
+             "attention backward: null pointer");
+  GS_REQUIRE(aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16), GS_ERR_ALIGN,
+             "attention backward: tensors must be 16-byte aligned");
+  GS_REQUIRE(workspace_bytes >= gs_attention_bwd_workspace_size(p) && (workspace || p->q_tokens == 0),
+             GS_ERR_WORKSPACE, "attention backward: workspace too small");
+  GS_REQUIRE(aligned(workspace, 4), GS_ERR_ALIGN, "attention backward: workspace must be 4-byte aligned");
+  a.d_out = d_out;
+  a.d_q = d_q;
+  a.d_k = d_k;
+  a.d_v = d_v;
+  a.delta = static_cast<float*>(workspace);
+  const hipStream_t st = as_stream(stream);
+  const int64_t q_tiles = tiles_of(a.q_tokens, a.group, kAttnRows, a.docs);
+  const int64_t k_tiles = tiles_of(a.k_tokens, 1, kAttnRows, a.docs);
+  GS_REQUIRE(q_tiles * a.kv_heads < (int64_t(1) << 31) && k_tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG,
+             "attention: too many tokens, documents or heads");
+  if (p->q_tokens > 0) {
+    a.n_tiles = static_cast<int>(q_tiles);
+    GS_ATTN_LAUNCH(attn_bwd_q_kernel, q_tiles * a.kv_heads);
+    if (const int rc = check_launch("attention backward (queries)")) return rc;
+  }
+  if (p->k_tokens > 0) {
+    a.n_tiles = static_cast<int>(k_tiles);
+    GS_ATTN_LAUNCH(attn_bwd_kv_kernel, k_tiles * a.kv_heads);
+    return check_launch("attention backward (keys)");
+  }
+  return GS_OK;
+}

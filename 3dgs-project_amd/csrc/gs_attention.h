@@ -1,0 +1,250 @@
+// Tiles, fragments and document lookup of the attention kernels.
+//
+// Every product is an outer product of 32x32 tiles (v_mfma_f32_32x32x16_bf16, or eight
+// v_mfma_f32_32x32x2_f32 in float32) arranged so that a wavefront's lane owns one query (or, in the
+// key and value gradients, one key): lane l holds column l % 32 of the accumulator and, with
+// h = l / 32, its rows 8 (r / 4) + 4 h + r % 4 for r = 0 .. 15. Scores are therefore formed
+// transposed (keys down, queries across): a query's maximum, sum, log-sum-exp and rescaling factor
+// are scalars of its lane, and the probabilities are already the B operand of the next product if
+// that product's A operand lists the contraction indexes in the order the accumulator has them
+// (slots 0 .. 7 of half h = rows 4 h + 0 .. 3 and 8 + 4 h + 0 .. 3 of a group of 16): no value moves
+// between lanes.
+#pragma once
+
+#include <float.h>
+
+#include "gs_host.h"
+
+namespace gs {
+
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using bf16x4 = __bf16 __attribute__((ext_vector_type(4)));
+using f32x8 = float __attribute__((ext_vector_type(8)));
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using f32x16 = float __attribute__((ext_vector_type(16)));
+using i16x4 = short __attribute__((ext_vector_type(4)));
+
+
+// Eight contraction slots of one row (A) or column (B) per lane.
+template <typename T>
+struct FragOf;
+template <>
+struct FragOf<__bf16> {
+  using type = bf16x8;
+};
+template <>
+struct FragOf<float> {
+  using type = f32x8;
+};
+template <typename T>
+using Frag = typename FragOf<T>::type;
+
+__device__ __forceinline__ void mma(f32x16& c, bf16x8 a, bf16x8 b) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(f32x16& c, f32x8 a, f32x8 b) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+}
+
+// Accumulator registers 8 k .. 8 k + 7 as a B operand. In bfloat16 the probabilities (and their
+// gradients) are rounded here, to nearest; every sum of them is taken in float32.
+template <typename T>
+__device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int k) {
+  Frag<T> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = static_cast<T>(c[8 * k + j]);
+  return f;
+}
+
+// A tile in LDS: rows of DP elements, the 16-byte chunks of a row permuted by XOR with bits of the
+// row number so that both kinds of read below fall on distinct banks: eight consecutive rows at one
+// chunk, and four consecutive rows at a pair of chunks.
+template <typename T, int DP>
+struct Tile {
+  static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kElemsPerChunk = 16 / static_cast<int>(sizeof(T));
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (kChunks == 8) return ((row & 6) | ((row >> 3) & 1));
+    return ((row << 1) & 14) | ((row >> 3) & 1);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return row * kRowBytes + ((chunk ^ swizzle(row)) << 4);
+  }
+  // A operand: row row0 + l % 32, elements 16 c + 8 h .. + 7
+  static __device__ __forceinline__ Frag<T> rows(const char* lds, int row0, int c, int lane) {
+    const int row = row0 + (lane & 31), h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      return *reinterpret_cast<const bf16x8*>(lds + at(row, 2 * c + h));
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + at(row, 4 * c + 2 * h));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + at(row, 4 * c + 2 * h + 1));
+      return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  }
+  // A operand of the transposed tile: element col0 + l % 32, rows row0 + 4 h + 0 .. 3 and
+  // row0 + 8 + 4 h + 0 .. 3. In bfloat16 the LDS unit transposes: of 16 lanes, lane i gives the
+  // address of four elements of row i / 4 and receives column i of the four rows.
+  static __device__ __forceinline__ Frag<T> cols(const char* lds, int col0, int row0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+      const int i = lane & 15;
+      const int col = col0 + (lane & 16) + 4 * (i & 3);
+      const int r = row0 + 4 * h + (i >> 2);
+      const int in = (col & 7) * 2;
+      const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + at(r, col >> 3) + in));
+      const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + at(r + 8, col >> 3) + in));
+      using i16x8 = short __attribute__((ext_vector_type(8)));
+      return __builtin_bit_cast(bf16x8, i16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    } else {
+      const int col = col0 + (lane & 31);
+      f32x8 f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = row0 + (j & 4) * 2 + 4 * h + (j & 3);
+        f[j] = *reinterpret_cast<const float*>(lds + at(r, col >> 2) + (col & 3) * 4);
+      }
+      return f;
+    }
+  }
+};
+
+// Eight elements of a row from global memory (16-byte aligned), zero outside.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* p, bool valid) {
+  Frag<T> f;
+  if (valid) {
+    if constexpr (sizeof(T) == 2) {
+      f = *reinterpret_cast<const bf16x8*>(p);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+      f = f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = static_cast<T>(0.0f);
+  }
+  return f;
+}
+
+// Four consecutive accumulator rows of one column, rounded to nearest and stored.
+__device__ __forceinline__ void store4(__bf16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<bf16x4*>(p) = bf16x4{static_cast<__bf16>(a), static_cast<__bf16>(b), static_cast<__bf16>(c),
+                                         static_cast<__bf16>(d)};
+}
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d};
+}
+
+// v of lane l and of lane l ^ 32, added (or the larger one): the two halves of a query's keys.
+__device__ __forceinline__ float half_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// 2^x by the hardware instruction (1 ulp; results below the smallest normal number are zero).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh. bfloat16: 1 - 2 / (1 + e^2x) from the hardware exponential and reciprocal (absolute error
+// 2e-7; both ends saturate). float32: the library's, which keeps the relative error near zero.
+template <typename T>
+__device__ __forceinline__ float tanh_of(float x) {
+  if constexpr (sizeof(T) == 2)
+    return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + exp2_hw(2.0f * kLog2e * x)), 1.0f);
+  else
+    return tanhf(x);
+}
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int32_t *q_offsets, *k_offsets, *k_lengths, *prefix;
+  int64_t q_tokens, k_tokens;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides in elements
+  int docs, heads, kv_heads, group, dim, causal;
+  float softcap, scale;
+  // backward
+  const void* d_out;
+  void *d_q, *d_k, *d_v;
+  float* delta;
+  int n_tiles;
+};
+
+// The tokens in order belong to docs + 2 stretches: those before the first document's offset, the
+// documents, those after the last one's. The two outer ones have no keys. Offsets are clamped to
+// the tensors, so whatever the arrays hold every access stays inside.
+__device__ __forceinline__ int64_t edge(const int32_t* off, int64_t tokens, int docs, int i) {
+  if (i <= 0) return 0;
+  if (i >= docs + 2) return tokens;
+  if (off == nullptr) return i == 1 ? 0 : tokens;
+  const int64_t v = off[i - 1];
+  return v < 0 ? 0 : (v > tokens ? tokens : v);
+}
+
+struct Doc {
+  int64_t q0, k0;   // first token
+  int64_t q_len;
+  int64_t k_cap;    // tokens of the key stretch
+  int64_t k_len;    // of them valid
+  int64_t prefix;
+  int64_t tile;     // tile within the document
+};
+
+// The stretch and the tile in it of tile t, where stretch i (of `per` rows a token) starts at tile
+// floor(edge(i) per / rows) + i: at least as many tiles as it needs, with no sums over the documents.
+// 64 stretches are looked at in one step (a load each), then 64 within the interval found.
+__device__ __forceinline__ int find_stretch(const int32_t* off, int64_t tokens, int docs, int64_t per, int rows,
+                                            int64_t t, int64_t* first) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int lo = 0, n = docs + 2;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + kWave - 1) / kWave;
+    const int i = lo + lane * step;
+    const bool before = lane * step < n && edge(off, tokens, docs, i) * per / rows + i <= t;
+    const uint64_t b = __ballot(before);
+    const int last = b ? 63 - __builtin_clzll(b) : 0;
+    n = min(step, n - last * step);
+    lo += last * step;
+  }
+  *first = edge(off, tokens, docs, lo) * per / rows + lo;
+  return lo;
+}
+
+__device__ __forceinline__ Doc doc_of(const AttnArgs& a, int i) {
+  Doc d;
+  d.q0 = edge(a.q_offsets, a.q_tokens, a.docs, i);
+  d.q_len = edge(a.q_offsets, a.q_tokens, a.docs, i + 1) - d.q0;
+  d.k0 = edge(a.k_offsets, a.k_tokens, a.docs, i);
+  d.k_cap = edge(a.k_offsets, a.k_tokens, a.docs, i + 1) - d.k0;
+  if (d.q_len < 0) d.q_len = 0;
+  if (d.k_cap < 0) d.k_cap = 0;
+  d.k_len = d.k_cap;
+  d.prefix = 0;
+  if (i < 1 || i > a.docs) {
+    d.k_len = 0;
+  } else {
+    if (a.k_lengths) {
+      const int64_t n = a.k_lengths[i - 1];
+      d.k_len = n < 0 ? 0 : (n < d.k_cap ? n : d.k_cap);
+    }
+    if (a.prefix) d.prefix = a.prefix[i - 1];
+  }
+  return d;
+}
+
+// Keys that token t of the document sees: always the first so many.
+__device__ __forceinline__ int visible(const AttnArgs& a, const Doc& d, int64_t t) {
+  if (!a.causal) return static_cast<int>(d.k_len);
+  int64_t n = t + 1 + d.k_len - d.q_len;
+  if (n < d.prefix) n = d.prefix;
+  return static_cast<int>(n < 0 ? 0 : (n < d.k_len ? n : d.k_len));
+}
+
+}  // namespace gs

@@ -563,6 +563,98 @@ int gs_stage_marks_read(float* ms, const char** names, int max);
 int gs_l1_ssim_fwd_noalloc(const float* image, const float* target, int channels, int height, int width,
                            float lambda_dssim, float* dmap, float* loss, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * gs_adam_step with every gradient multiplied by *grad_scale (a device float, e.g. the clipping
+ * coefficient of gs_grad_norm) as it is read; the gradients themselves stay as they are. The moments are
+ *   m' = fma(1 - beta1, g - m, m);  v' = fma(1 - beta2, g*g - v, v)
+ * with 1 - beta computed in double and rounded to float; the rest is gs_adam_step's.
+ * ------------------------------------------------------------------------------------- */
+int gs_adam_step_scaled(const gs_adam_group* groups, int n_groups, int64_t n_primitives,
+                        const int32_t* visibility, const float* grad_scale, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Operators of a splat predictor (a transformer over image tokens whose output is a set of
+ * Gaussians) and of its training step. No counterpart in the reference. float32 or bfloat16;
+ * sums, softmax statistics and norms in float32 or float64.
+ *
+ * The global norm of n gradient tensors, norm = sqrt(sum of all squares), and the clipping
+ * coefficient coef = min(1, max_norm / (norm + 1e-6)) (coef may be NULL): device floats. grads,
+ * sizes (elements) and dtypes (GS_FLOAT32 or GS_BFLOAT16) are host arrays of n; the tensors are
+ * contiguous. Summed in float64 in a fixed order: the same inputs give the same bits. A norm that
+ * is not finite gives coef 0 (infinity) or NaN, and gs_grad_scale then writes what the products
+ * are. gs_grad_scale writes out[i] = grads[i] * *coef (out[i] may be grads[i]; otherwise they do
+ * not overlap).
+ * ------------------------------------------------------------------------------------- */
+size_t gs_grad_norm_workspace_size(const int64_t* sizes, int n);
+int gs_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int n, double max_norm,
+                 float* norm, float* coef, void* workspace, size_t workspace_bytes, void* stream);
+int gs_grad_scale(const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes, int n,
+                  const float* coef, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Rotary positions with several axes (e.g. view, row, column). Pair p of a head, of P = sum of
+ * sections pairs, belongs to the axis whose section holds p and is turned by positions[token,
+ * axis] * base^-x, x = (p - the section's first pair) / section, or with GS_ROTARY_SHARED x = p / P:
+ *   (u, w) -> (u cos - w sin, u sin + w cos),
+ * on the elements (p, p + P), or with GS_ROTARY_ADJACENT (2 p, 2 p + 1); the elements from 2 P on
+ * are copied. GS_ROTARY_INVERSE negates the angle (the gradient). q [tokens, q_heads, dim] and k
+ * [tokens, k_heads, dim] (k_heads 0: none) are read through their strides (elements; the last
+ * dimension is contiguous) and written contiguously. positions: [tokens, axes] float32.
+ * ------------------------------------------------------------------------------------- */
+#define GS_ROTARY_MAX_AXES 4
+#define GS_ROTARY_MAX_PAIRS 256
+#define GS_ROTARY_ADJACENT 1
+#define GS_ROTARY_SHARED 2
+#define GS_ROTARY_INVERSE 4
+typedef struct gs_rotary {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const float* positions;
+  int64_t tokens;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  double base;
+  int32_t q_heads, k_heads, dim, axes;
+  int32_t sections[GS_ROTARY_MAX_AXES];
+  int32_t dtype, flags;
+} gs_rotary;
+int gs_rotary_axes(const gs_rotary* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Softmax attention over packed documents. q [q_tokens, heads, dim], k and v [k_tokens, kv_heads,
+ * dim] through strides (elements; the last dimension contiguous; strides multiples of 16 bytes,
+ * pointers 16-byte aligned); heads a multiple of kv_heads: query head h reads key head
+ * h / (heads / kv_heads). Document d owns the query tokens q_offsets[d] .. q_offsets[d + 1] and of
+ * the key tokens k_offsets[d] .. k_offsets[d + 1] the first k_lengths[d] (NULL: all): device int32,
+ * offsets non-decreasing, docs + 1 of them (NULL for one document: all tokens). With Lq, Lk the
+ * document's counts, query i sees key j < Lk if not causal, or j <= i + Lk - Lq, or j < prefix[d]
+ * (device int32, may be NULL; only with causal). Scores s = scale q.k, or with softcap > 0
+ * softcap tanh(scale q.k / softcap).
+ *   out [q_tokens, heads, dim] = sum_j softmax(s)_j v_j, lse [q_tokens, heads] float32 = ln sum_j e^s_j.
+ * A query that sees nothing, and one outside every document, gets 0 and -infinity. Key tokens
+ * outside the documents and their lengths are never used, whatever they hold. Offsets and lengths
+ * outside the tensors are cut to them.
+ * gs_attention_bwd takes out and lse of the forward and d_out [q_tokens, heads, dim], and writes
+ * d_q, d_k, d_v (contiguous, every element; keys that nothing sees get 0). No atomics: the same
+ * inputs give the same bits.
+ * ------------------------------------------------------------------------------------- */
+#define GS_ATTENTION_MAX_DIM 128
+typedef struct gs_attention {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int32_t *q_offsets, *k_offsets, *k_lengths, *prefix;
+  int64_t q_tokens, k_tokens;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int32_t docs, heads, kv_heads, dim;
+  int32_t dtype, causal;
+  float softcap, scale;
+} gs_attention;
+size_t gs_attention_fwd_workspace_size(const gs_attention* args);
+int gs_attention_fwd(const gs_attention* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t gs_attention_bwd_workspace_size(const gs_attention* args);
+int gs_attention_bwd(const gs_attention* args, const void* d_out, void* d_q, void* d_k, void* d_v,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
