@@ -27,7 +27,7 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     st, sh, sd = t.stride()
     if t.numel() == 0:
         return t
-    ok = ((sd == 1 or t.shape[2] == 1) and 0 <= st < 1 << 24 and 0 <= sh < 1 << 24 and st % per == 0 and sh % per == 0
+    ok = ((sd == 1 or t.shape[2] == 1) and 0 <= st < 1 << 22 and 0 <= sh < 1 << 40 and st % per == 0 and sh % per == 0
           and t.data_ptr() % 16 == 0)
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 

@@ -2,6 +2,8 @@
 // of the products). A query row is a (token, head of the group) pair: the heads that share a key
 // head are rows of one tile, so a key tile is read once for all of them and the gradients of shared
 // heads are summed inside one workgroup, in a fixed order, without atomics.
+#include <algorithm>
+
 #include "gs_attention.h"
 
 namespace gs {
@@ -72,6 +74,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
   const int64_t base = (tile - first) * kAttnRows;
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
+  const Piece piece = piece_of(a, visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group), blockIdx.y);
+  if (static_cast<int>(blockIdx.y) >= piece.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wrow = row0 + wave * 32;
   const int row = wrow + (lane & 31);
@@ -84,14 +88,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
   for (int c = 0; c < C; ++c) q[c] = load_frag<T>(qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
   const int vis = visible(a, doc, tok);
   const int wave_min = visible(a, doc, min(wrow, rows - 1) / a.group);
-  const int end = visible(a, doc, min(row0 + kAttnRows, rows) == 0 ? 0 : (min(row0 + kAttnRows, rows) - 1) / a.group);
   const float scale2 = a.scale * kLog2e;
   const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
   f32x16 o[DP / 32] = {};
   float m = -INFINITY, l = 0.0f;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
-  for (int k0 = 0; k0 < end; k0 += kAttnKeys) {
+  for (int k0 = piece.begin; k0 < piece.stop; k0 += kAttnKeys) {
     const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
     __syncthreads();
     stage<T, DP, kAttnKeys>(lk, kp + k0 * a.k_token, a.k_token, valid, a.dim);
@@ -137,6 +140,24 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
   }
   if (!live) return;
   l = half_sum(l);
+  if (a.splits > 1) {
+    const int64_t at = (doc.q0 + tok) * a.heads + head;
+    const int64_t part = blockIdx.y * a.q_tokens * a.heads + at;
+    float* pp = a.part + part * a.dim;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * dt + 2 * r + 4 * h;
+        if (d < a.dim) store4(pp + d, o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+      }
+    if (h == 0) {
+      a.part_stat[2 * part] = m;
+      a.part_stat[2 * part + 1] = l;
+      if (blockIdx.y == 0) a.part_n[at] = piece.n;
+    }
+    return;
+  }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   T* op = static_cast<T*>(a.out) + ((doc.q0 + tok) * a.heads + head) * a.dim;
 #pragma unroll
@@ -147,6 +168,194 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
       if (d < a.dim) store4(op + d, o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv);
     }
   if (h == 0) a.lse[(doc.q0 + tok) * a.heads + head] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+// Few query rows (single tokens) against long keys: HBM-bound, so a workgroup's wavefronts each walk
+// over keys of their own, 32 at a time, for the same 32 rows, and join at the end. The next keys' and
+// values' loads (16 KB a wavefront at 128 elements of bfloat16) are in flight while the present ones are
+// multiplied; they pass through the wavefront's own LDS (rows to be read across and along), with no
+// barrier in the loop.
+template <typename T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int C = DP / 16;
+  constexpr int kLoads = 32 * L::kChunks / kWave;  // 16-byte loads a lane for 32 rows
+  constexpr int kTileBytes = 32 * L::kRowBytes;
+  static_assert(2 * kTileBytes >= 32 * DP * 4, "the join reuses the wavefront's tiles");
+  __shared__ __attribute__((aligned(16))) char lds[kAttnWaves * 2 * kTileBytes];
+  __shared__ float l_m[kAttnWaves][32], l_l[kAttnWaves][32];
+  const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
+  const int64_t tile = static_cast<int64_t>(blockIdx.x / a.kv_heads);
+  int64_t first;
+  const int di = find_stretch(a.q_offsets, a.q_tokens, a.docs, a.group, 32, tile, &first);
+  const Doc doc = doc_of(a, di);
+  const int rows = static_cast<int>(doc.q_len) * a.group;
+  const int64_t base = (tile - first) * 32;
+  if (base >= rows) return;
+  const int row0 = static_cast<int>(base);
+  const int n_rows = min(32, rows - row0);
+  const Piece piece = piece_of(a, visible(a, doc, (row0 + n_rows - 1) / a.group), blockIdx.y);
+  if (static_cast<int>(blockIdx.y) >= piece.n) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int row = row0 + (lane & 31);
+  const bool live = row < rows;
+  const int rc = live ? row : rows - 1;
+  const int tok = rc / a.group, head = hk * a.group + rc - tok * a.group;
+  const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
+  const int vis = min(visible(a, doc, tok), piece.stop);
+  const int all_min = min(visible(a, doc, row0 / a.group), piece.stop);
+  const float scale2 = a.scale * kLog2e;
+  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  f32x16 o[DP / 32] = {};
+  float m = -INFINITY, l = 0.0f;
+  const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
+  char* lk = lds + wave * 2 * kTileBytes;
+  char* lv = lk + kTileBytes;
+  f32x4 pk[kLoads], pv[kLoads];
+  uint32_t at_k[kLoads], at_v[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int e = i * kWave + lane, r = e / L::kChunks, c = (e % L::kChunks) * L::kElemsPerChunk;
+    at_k[i] = c < a.dim ? static_cast<uint32_t>((r * a.k_token + c) * sizeof(T)) : kNowhere;
+    at_v[i] = c < a.dim ? static_cast<uint32_t>((r * a.v_token + c) * sizeof(T)) : kNowhere;
+  }
+  const auto fetch = [&](int k0) {
+    const auto bk = row_buffer(kp + k0 * a.k_token, a.k_token, min(32, piece.stop - k0), a.dim);
+    const auto bv = row_buffer(vp + k0 * a.v_token, a.v_token, min(32, piece.stop - k0), a.dim);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) pk[i] = load16(bk, at_k[i]);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) pv[i] = load16(bv, at_v[i]);
+  };
+  int k0 = piece.begin + __builtin_amdgcn_readfirstlane(wave) * 32;
+  if (k0 < piece.stop) fetch(k0);
+  Frag<T> q[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) q[c] = load_frag<T>(qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
+  for (; k0 < piece.stop; k0 += kAttnWaves * 32) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int e = i * kWave + lane;
+      *reinterpret_cast<f32x4*>(lk + L::at(e / L::kChunks, e % L::kChunks)) = pk[i];
+      *reinterpret_cast<f32x4*>(lv + L::at(e / L::kChunks, e % L::kChunks)) = pv[i];
+    }
+    wave_sync();
+    if (k0 + kAttnWaves * 32 < piece.stop) fetch(k0 + kAttnWaves * 32);
+    f32x16 s = {};
+#pragma unroll
+    for (int c = 0; c < C; ++c) mma(s, L::rows(lk, 0, c, lane), q[c]);
+    const bool mask = k0 + 32 > all_min;
+    float top = m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float x = score<T, CAP>(s[r], scale2, in_scale, cap2);
+      if (mask && k0 + 8 * (r / 4) + 4 * h + r % 4 >= vis) x = -INFINITY;
+      s[r] = x;
+      top = fmaxf(top, x);
+    }
+    top = half_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float alpha = exp2_hw(m - ref);
+    m = top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = exp2_hw(s[r] - ref);
+      sum += s[r];
+    }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= alpha;
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      const Frag<T> p = acc_frag<T>(s, kc);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], L::cols(lv, 32 * dt, 16 * kc, lane), p);
+    }
+    wave_sync();
+  }
+  // join: every wavefront leaves its rows, statistics and (in its own tiles) sums; then all threads
+  // take the same rows' elements and add the wavefronts' in order
+  l = half_sum(l);
+  float* own = reinterpret_cast<float*>(lk);
+  if (live) {
+    if (h == 0) {
+      l_m[wave][lane & 31] = m;
+      l_l[wave][lane & 31] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store4(own + (lane & 31) * DP + 32 * dt + 2 * r + 4 * h, o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_rows * (DP / 4); e += kAttnThreads) {
+    const int i = e / (DP / 4), d = e % (DP / 4) * 4;
+    float top = l_m[0][i];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, l_m[w][i]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) {
+      const float f = exp2_hw(l_m[w][i] - ref);
+      sum += f * l_l[w][i];
+      x += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 2 * kTileBytes) + i * DP + d);
+    }
+    const int t = (row0 + i) / a.group;
+    const int64_t at = (doc.q0 + t) * a.heads + hk * a.group + row0 + i - t * a.group;
+    if (a.splits > 1) {
+      const int64_t part = blockIdx.y * a.q_tokens * a.heads + at;
+      if (d < a.dim) *reinterpret_cast<f32x4*>(a.part + part * a.dim + d) = x;
+      if (d == 0) {
+        a.part_stat[2 * part] = top;
+        a.part_stat[2 * part + 1] = sum;
+        if (blockIdx.y == 0) a.part_n[at] = piece.n;
+      }
+    } else {
+      const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+      if (d < a.dim) store4(static_cast<T*>(a.out) + at * a.dim + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      if (d == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    }
+  }
+}
+
+// Joins the pieces of a (token, head), a wavefront each, in order. Rows outside every document have
+// no keys, hence one piece.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kAttnWaves + threadIdx.x / kWave;
+  const int64_t all = a.q_tokens * a.heads;
+  if (at >= all) return;
+  const int lane = threadIdx.x & 63;
+  const int n = a.part_n[at];
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += kWave) top = fmaxf(top, a.part_stat[2 * (i * all + at)]);
+#pragma unroll
+  for (int b = 1; b < kWave; b *= 2) top = fmaxf(top, __shfl_xor(top, b));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
+  const int d = 2 * lane;
+  for (int i = 0; i < n; ++i) {
+    const int64_t part = i * all + at;
+    const float f = exp2_hw(a.part_stat[2 * part] - ref);
+    sum += f * a.part_stat[2 * part + 1];
+    if (d < a.dim) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part + part * a.dim + d);
+      x0 = fmaf(f, v.x, x0);
+      x1 = fmaf(f, v.y, x1);
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  if (d < a.dim) {
+    T* out = static_cast<T*>(a.out) + at * a.dim + d;
+    out[0] = static_cast<T>(x0 * inv);
+    out[1] = static_cast<T>(x1 * inv);
+  }
+  if (lane == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 // Query gradients, and delta_i = dO_i . O_i for the key gradients.
@@ -366,7 +575,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
-static int attn_setup(const gs_attention* p, bool backward, AttnArgs& a) {
+static int attn_setup(const gs_attention* p, AttnArgs& a) {
   GS_REQUIRE(p != nullptr, GS_ERR_ARG, "attention: arguments are NULL");
   GS_REQUIRE(p->dtype == GS_FLOAT32 || p->dtype == GS_BFLOAT16, GS_ERR_ARG,
              "attention: dtype must be GS_FLOAT32 or GS_BFLOAT16");
@@ -392,9 +601,9 @@ static int attn_setup(const gs_attention* p, bool backward, AttnArgs& a) {
   const int64_t strides[6] = {p->q_token_stride, p->q_head_stride, p->k_token_stride,
                               p->k_head_stride, p->v_token_stride, p->v_head_stride};
   for (int i = 0; i < 6; ++i)
-    GS_REQUIRE(strides[i] >= 0 && strides[i] < (int64_t(1) << 24) && strides[i] % elems == 0, GS_ERR_ALIGN,
-               "attention: strides must be multiples of 16 bytes, below 2^24 elements (got %lld)",
-               static_cast<long long>(strides[i]));
+    GS_REQUIRE(strides[i] >= 0 && strides[i] < (int64_t(1) << (i % 2 ? 40 : 22)) && strides[i] % elems == 0,
+               GS_ERR_ALIGN, "attention: strides must be multiples of 16 bytes, token strides below 2^22 elements "
+               "(got %lld)", static_cast<long long>(strides[i]));
   GS_REQUIRE(aligned(p->q, 16) && aligned(p->k, 16) && aligned(p->v, 16) && aligned(p->out, 16) &&
                  aligned(p->lse, 4), GS_ERR_ALIGN, "attention: tensors must be 16-byte aligned");
   a = {};
@@ -423,6 +632,7 @@ static int attn_setup(const gs_attention* p, bool backward, AttnArgs& a) {
   a.causal = p->causal != 0;
   a.softcap = p->softcap;
   a.scale = p->scale;
+  a.splits = 1;
   return GS_OK;
 }
 
@@ -431,7 +641,7 @@ static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { retur
 
 #define GS_ATTN_LAUNCH(KERNEL, GRID)                                                                       \
   do {                                                                                                     \
-    const dim3 grid_(static_cast<unsigned>(GRID)), block_(kAttnThreads);                                   \
+    const dim3 grid_(static_cast<unsigned>(GRID), static_cast<unsigned>(a.splits)), block_(kAttnThreads);                                   \
     const bool cap_ = a.softcap > 0.0f, wide_ = a.dim > 64;                                                \
     if (p->dtype == GS_BFLOAT16) {                                                                         \
       if (wide_ && cap_) hipLaunchKernelGGL((KERNEL<__bf16, 128, true>), grid_, block_, 0, st, a);         \
@@ -446,29 +656,79 @@ static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { retur
     }                                                                                                      \
   } while (0)
 
+// How a forward call is laid out, by sizes alone (so that the workspace can be asked for first).
+struct FwdPlan {
+  bool few;       // the kernel for few rows
+  int64_t tiles;  // row tiles
+  int splits;     // pieces of the keys
+};
+constexpr int kFewSplitKeys = 512, kTileSplitKeys = 256;
+constexpr int kFewBlocks = 2048, kTileBlocks = 512, kMaxSplits = 256;
+
+static FwdPlan plan_fwd(const AttnArgs& a) {
+  FwdPlan f;
+  // few: at most 32 rows to a document and key head on average. There the tile kernel's 128 rows are
+  // mostly padding and each workgroup's keys one long chain.
+  f.few = a.q_tokens * a.group <= 32 * static_cast<int64_t>(a.docs);
+  f.tiles = tiles_of(a.q_tokens, a.group, f.few ? 32 : kAttnRows, a.docs);
+  // Pieces until the chip has its workgroups, each of split_keys at least. Ragged documents: up to twice
+  // the average length is provided for; a longer one gets longer pieces.
+  const int64_t work = (f.few ? std::max<int64_t>(a.docs, a.q_tokens * a.group / 32)
+                              : a.q_tokens * a.group / kAttnRows + 1) * a.kv_heads;
+  const int64_t keys = a.docs == 1 ? a.k_tokens : 2 * (a.k_tokens / a.docs);
+  const int64_t want = (f.few ? kFewBlocks : kTileBlocks) / work;
+  const int64_t most = keys / (f.few ? kFewSplitKeys : kTileSplitKeys);
+  f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
+  return f;
+}
+
+static size_t fwd_workspace(const AttnArgs& a, const FwdPlan& f) {
+  if (f.splits == 1) return 0;
+  const size_t rows = static_cast<size_t>(a.q_tokens) * a.heads;
+  return rows * (static_cast<size_t>(f.splits) * (a.dim + 2) + 1) * sizeof(float);
+}
+
 }  // namespace gs
 
 using namespace gs;
 
 extern "C" size_t gs_attention_fwd_workspace_size(const gs_attention* p) {
   clear_error();
-  (void)p;
-  return 0;
+  AttnArgs a;
+  if (attn_setup(p, a) || p->q_tokens == 0) return 0;
+  return fwd_workspace(a, plan_fwd(a));
 }
 
 extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  (void)workspace;
-  (void)workspace_bytes;
   AttnArgs a;
-  if (const int rc = attn_setup(p, false, a)) return rc;
+  if (const int rc = attn_setup(p, a)) return rc;
   if (p->q_tokens == 0) return GS_OK;
+  const FwdPlan f = plan_fwd(a);
+  GS_REQUIRE(f.tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG, "attention: too many tokens, documents or heads");
+  GS_REQUIRE(workspace_bytes >= fwd_workspace(a, f) && (workspace || f.splits == 1), GS_ERR_WORKSPACE,
+             "attention: workspace too small");
+  GS_REQUIRE(aligned(workspace, 16), GS_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
   const hipStream_t st = as_stream(stream);
-  const int64_t tiles = tiles_of(a.q_tokens, a.group, kAttnRows, a.docs);
-  GS_REQUIRE(tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG, "attention: too many tokens, documents or heads");
-  a.n_tiles = static_cast<int>(tiles);
-  GS_ATTN_LAUNCH(attn_fwd_kernel, tiles * a.kv_heads);
-  return check_launch("attention");
+  a.n_tiles = static_cast<int>(f.tiles);
+  a.splits = f.splits;
+  a.split_keys = f.few ? kFewSplitKeys : kTileSplitKeys;
+  const int64_t rows = a.q_tokens * a.heads;
+  a.part = static_cast<float*>(workspace);
+  a.part_stat = a.part + rows * a.splits * a.dim;
+  a.part_n = reinterpret_cast<int32_t*>(a.part_stat + rows * a.splits * 2);
+  if (f.few)
+    GS_ATTN_LAUNCH(attn_few_kernel, f.tiles * a.kv_heads);
+  else
+    GS_ATTN_LAUNCH(attn_fwd_kernel, f.tiles * a.kv_heads);
+  if (const int rc = check_launch("attention")) return rc;
+  if (a.splits == 1) return GS_OK;
+  const dim3 grid(static_cast<unsigned>((rows + kAttnWaves - 1) / kAttnWaves)), block(kAttnThreads);
+  if (p->dtype == GS_BFLOAT16)
+    hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL(attn_join_kernel<float>, grid, block, 0, st, a);
+  return check_launch("attention (join)");
 }
 
 extern "C" size_t gs_attention_bwd_workspace_size(const gs_attention* p) {
@@ -481,7 +741,7 @@ extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* 
                                 void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   AttnArgs a;
-  if (const int rc = attn_setup(p, true, a)) return rc;
+  if (const int rc = attn_setup(p, a)) return rc;
   GS_REQUIRE((p->q_tokens == 0 || (d_out && d_q)) && (p->k_tokens == 0 || (d_k && d_v)), GS_ERR_ARG,
              "attention backward: null pointer");
   GS_REQUIRE(aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16), GS_ERR_ALIGN,

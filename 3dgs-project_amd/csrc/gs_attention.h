@@ -129,6 +129,20 @@ __device__ __forceinline__ Frag<T> load_frag(const T* p, bool valid) {
   return f;
 }
 
+// Rows [0, rows) of a strided matrix as a buffer: loads beyond the last row, and at kNowhere, give
+// zero. Its base is set per tile, so that offsets stay within 32 bits however long the matrix is
+// (token strides are below 2^22 elements, tiles have at most 128 rows).
+constexpr uint32_t kNowhere = 0xffffff00u;
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* base, int64_t stride, int rows, int dim) {
+  const int bytes = rows > 0 ? static_cast<int>(((rows - 1) * stride + dim) * static_cast<int64_t>(sizeof(T))) : 0;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ f32x4 load16(__amdgpu_buffer_rsrc_t b, uint32_t offset) {
+  using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(f32x4, static_cast<u32x4>(__builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0)));
+}
+
 // Four consecutive accumulator rows of one column, rounded to nearest and stored.
 __device__ __forceinline__ void store4(__bf16* p, float a, float b, float c, float d) {
   *reinterpret_cast<bf16x4*>(p) = bf16x4{static_cast<__bf16>(a), static_cast<__bf16>(b), static_cast<__bf16>(c),
@@ -175,7 +189,24 @@ struct AttnArgs {
   void *d_q, *d_k, *d_v;
   float* delta;
   int n_tiles;
+  // keys of a row tile cut into up to `splits` pieces of at least split_keys, joined by a second launch
+  int splits, split_keys;
+  float* part;        // [splits][q_tokens][heads][dim], unnormalised
+  float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
+  int32_t* part_n;    // [q_tokens][heads] pieces
 };
+
+// The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one).
+struct Piece {
+  int begin, stop, n;
+};
+__device__ __forceinline__ Piece piece_of(const AttnArgs& a, int end, int split) {
+  if (a.splits == 1) return {0, end, 1};
+  int per = (end + a.splits - 1) / a.splits;
+  per = max((per + 127) & ~127, a.split_keys);
+  const int n = max(1, (end + per - 1) / per);
+  return {min(split * per, end), min((split + 1) * per, end), n};
+}
 
 // The tokens in order belong to docs + 2 stretches: those before the first document's offset, the
 // documents, those after the last one's. The two outer ones have no keys. Offsets are clamped to

@@ -622,7 +622,7 @@ int gs_rotary_axes(const gs_rotary* args, void* stream);
 /* ---------------------------------------------------------------------------------------
  * Softmax attention over packed documents. q [q_tokens, heads, dim], k and v [k_tokens, kv_heads,
  * dim] through strides (elements; the last dimension contiguous; strides multiples of 16 bytes,
- * pointers 16-byte aligned); heads a multiple of kv_heads: query head h reads key head
+ * token strides below 2^22 elements, pointers 16-byte aligned); heads a multiple of kv_heads: query head h reads key head
  * h / (heads / kv_heads). Document d owns the query tokens q_offsets[d] .. q_offsets[d + 1] and of
  * the key tokens k_offsets[d] .. k_offsets[d + 1] the first k_lengths[d] (NULL: all): device int32,
  * offsets non-decreasing, docs + 1 of them (NULL for one document: all tokens). With Lq, Lk the

@@ -49,7 +49,7 @@ def attention_args(**kw):
     (dict(v=None), ARG, "null"),
     (dict(k_token_stride=129), ALIGN, "strides"),
     (dict(v_head_stride=-64), ALIGN, "strides"),
-    (dict(q_token_stride=1 << 24), ALIGN, "strides"),
+    (dict(q_token_stride=1 << 22), ALIGN, "strides"),
     (dict(k=264), ALIGN, "aligned"),
     (dict(out=258), ALIGN, "aligned"),
 ])
