@@ -51,20 +51,105 @@ __device__ __forceinline__ void stage_rows(char* lds, const T* src, int64_t toke
   }
 }
 
-// Score in units of ln 2 (the softmax is taken in base 2), and the capped score's slope.
-template <typename T, bool CAP>
-__device__ __forceinline__ float score(float s, float scale2, float in_scale, float cap2) {
-  if constexpr (CAP) return cap2 * tanh_of<T>(s * in_scale);
-  return s * scale2;
+// Base-2 exponent of a score, up to the reference that p = 2^(x - ref) takes off. Plain scores stay as
+// they come (monotone in x: the scale is positive) and are scaled in the same fma that subtracts.
+struct Rule {
+  float scale2;    // plain: scale log2 e
+  float in_scale;  // capped: scale / cap
+  float cap2;      // capped: cap log2 e
+};
+template <int MODE>
+__device__ __forceinline__ Rule rule_of(const AttnArgs& a) {
+  const float scale = fabsf(a.scale);
+  return {fmaxf(scale * kLog2e, 1e-30f), MODE == kPlain ? 0.0f : scale / a.softcap, a.softcap * kLog2e};
+}
+template <typename T, int MODE>
+__device__ __forceinline__ float exponent(const Rule& u, float s) {
+  if constexpr (MODE == kPlain) return s;
+  return u.cap2 * tanh_of<T>(s * u.in_scale);
+}
+template <int MODE>
+__device__ __forceinline__ float prob(const Rule& u, float x, float ref) {
+  if constexpr (MODE == kPlain) return exp2_hw(fmaf(x, u.scale2, -ref));
+  return exp2_hw(x - ref);
 }
 
-template <typename T, int DP, bool CAP>
-__global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
+// Softmax state of a lane's query: running maximum of the exponents (kept within 2^8 of the true one:
+// the accumulators are rescaled only when some lane's maximum grows by more), sum.
+struct Softmax {
+  float m = -INFINITY, l = 0.0f;
+};
+
+// Turns N tiles of 32 scores into probabilities; `o` is rescaled where the reference moves. Key i of the
+// lane's registers is seen if it is below `vis`.
+template <typename T, int MODE, int N, int M>
+__device__ __forceinline__ void softmax_step(const Rule& u, f32x16 (&s)[N], f32x16 (&o)[M], Softmax& st, bool mask,
+                                             int vis, int h) {
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[t][r] = exponent<T, MODE>(u, s[t][r]);
+  if (mask) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (32 * t + 8 * (r / 4) + 4 * h + r % 4 >= vis) s[t][r] = -INFINITY;
+  }
+  float ref;
+  if constexpr (MODE == kCapFixed) {
+    ref = u.cap2 - kFixedTop;
+    st.m = ref;
+  } else {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top[r % 4] = fmaxf(top[r % 4], s[t][r]);
+    float x = half_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+    if constexpr (MODE == kPlain) x *= u.scale2;
+    if (__any(x > st.m + 8.0f)) {
+      const float m = fmaxf(st.m, x);
+      const float f = exp2_hw(st.m - (m == -INFINITY ? 0.0f : m));
+      st.m = m;
+      st.l *= f;
+#pragma unroll
+      for (int i = 0; i < M; ++i) o[i] *= f;
+    }
+    ref = st.m == -INFINITY ? 0.0f : st.m;
+  }
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[t][r] = prob<MODE>(u, s[t][r], ref);
+      sum[r % 4] += s[t][r];
+    }
+  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// The query's sign takes the scale's, so that scores are scaled by |scale|.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_query(const AttnArgs& a, const T* p, bool valid) {
+  Frag<T> f = load_frag<T>(p, valid);
+  if (a.scale < 0.0f) f = -f;
+  return f;
+}
+
+// Keeps the instructions on either side apart: groups of LDS reads are issued together, ahead of the
+// products that use them, where the compiler would read, wait and multiply one by one.
+template <typename T>
+__device__ __forceinline__ void keep_order() {
+  if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+}
+
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kAttnKeys * L::kRowBytes];
-  char* lk = lds;
-  char* lv = lds + kAttnKeys * L::kRowBytes;
+  constexpr int kTileBytes = kAttnKeys * L::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = a.n_tiles - 1 - static_cast<int64_t>(blockIdx.x / a.kv_heads);
   int64_t first;
@@ -85,61 +170,60 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
   const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
   Frag<T> q[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) q[c] = load_frag<T>(qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
+  for (int c = 0; c < C; ++c) q[c] = load_query<T>(a, qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
   const int vis = visible(a, doc, tok);
   const int wave_min = visible(a, doc, min(wrow, rows - 1) / a.group);
-  const float scale2 = a.scale * kLog2e;
-  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  const Rule rule = rule_of<MODE>(a);
   f32x16 o[DP / 32] = {};
-  float m = -INFINITY, l = 0.0f;
+  Softmax st;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
-  for (int k0 = piece.begin; k0 < piece.stop; k0 += kAttnKeys) {
+  const TileCopy<T, DP, kAttnKeys, kAttnThreads> copy_k(a.k_token, a.dim), copy_v(a.v_token, a.dim);
+  const auto fetch = [&](int k0, char* to) {
     const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
+    copy_k(to, row_buffer(kp + k0 * a.k_token, a.k_token, valid, a.dim));
+    copy_v(to + kTileBytes, row_buffer(vp + k0 * a.v_token, a.v_token, valid, a.dim));
+  };
+  if (piece.begin < piece.stop) fetch(piece.begin, lds);
+  int buf = 0;
+  for (int k0 = piece.begin; k0 < piece.stop; k0 += kAttnKeys, buf ^= 1) {
+    const char* lk = lds + buf * 2 * kTileBytes;
+    const char* lv = lk + kTileBytes;
+    copies_done();
     __syncthreads();
-    stage<T, DP, kAttnKeys>(lk, kp + k0 * a.k_token, a.k_token, valid, a.dim);
-    stage<T, DP, kAttnKeys>(lv, vp + k0 * a.v_token, a.v_token, valid, a.dim);
-    __syncthreads();
+    if (k0 + kAttnKeys < piece.stop) fetch(k0 + kAttnKeys, lds + (buf ^ 1) * 2 * kTileBytes);
     f32x16 s[2] = {};
+    {
+      Frag<T> ka[C], kb[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) ka[c] = L::rows(lk, 0, c, lane);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) mma(s[st], L::rows(lk, 32 * st, c, lane), q[c]);
-    const bool mask = k0 + kAttnKeys > wave_min;
-    float top = m;
+      for (int c = 0; c < C; ++c) kb[c] = L::rows(lk, 32, c, lane);
+      keep_order<T>();
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+      for (int c = 0; c < C; ++c) mma(s[0], ka[c], q[c]);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float x = score<T, CAP>(s[st][r], scale2, in_scale, cap2);
-        if (mask && k0 + 32 * st + 8 * (r / 4) + 4 * h + r % 4 >= vis) x = -INFINITY;
-        s[st][r] = x;
-        top = fmaxf(top, x);
-      }
-    top = half_max(top);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float alpha = exp2_hw(m - ref);
-    m = top;
-    float sum = 0.0f;
+      for (int c = 0; c < C; ++c) mma(s[1], kb[c], q[c]);
+    }
+    Frag<T> v[2][DP / 32];
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[st][r] = exp2_hw(s[st][r] - ref);
-        sum += s[st][r];
-      }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= alpha;
+    for (int dt = 0; dt < DP / 32; ++dt) v[0][dt] = L::cols(lv, 32 * dt, 0, lane);
+    keep_order<T>();
+    softmax_step<T, MODE>(rule, s, o, st, k0 + kAttnKeys > wave_min, vis - k0, h);
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc) {
+      if (kc < 3) {
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) v[(kc + 1) & 1][dt] = L::cols(lv, 32 * dt, 16 * (kc + 1), lane);
+        keep_order<T>();
+      }
       const Frag<T> p = acc_frag<T>(s[kc / 2], kc % 2);
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], L::cols(lv, 32 * dt, 16 * kc, lane), p);
+      for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], v[kc & 1][dt], p);
     }
   }
   if (!live) return;
-  l = half_sum(l);
+  const float m = st.m, l = half_sum(st.l);
   if (a.splits > 1) {
     const int64_t at = (doc.q0 + tok) * a.heads + head;
     const int64_t part = blockIdx.y * a.q_tokens * a.heads + at;
@@ -175,7 +259,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_fwd_kernel(AttnArgs a) {
 // values' loads (16 KB a wavefront at 128 elements of bfloat16) are in flight while the present ones are
 // multiplied; they pass through the wavefront's own LDS (rows to be read across and along), with no
 // barrier in the loop.
-template <typename T, int DP, bool CAP>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
@@ -204,10 +288,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
   const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
   const int vis = min(visible(a, doc, tok), piece.stop);
   const int all_min = min(visible(a, doc, row0 / a.group), piece.stop);
-  const float scale2 = a.scale * kLog2e;
-  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  const Rule rule = rule_of<MODE>(a);
   f32x16 o[DP / 32] = {};
-  float m = -INFINITY, l = 0.0f;
+  Softmax st;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
   char* lk = lds + wave * 2 * kTileBytes;
@@ -232,7 +315,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
   if (k0 < piece.stop) fetch(k0);
   Frag<T> q[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) q[c] = load_frag<T>(qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
+  for (int c = 0; c < C; ++c) q[c] = load_query<T>(a, qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
   for (; k0 < piece.stop; k0 += kAttnWaves * 32) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -242,34 +325,13 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
     }
     wave_sync();
     if (k0 + kAttnWaves * 32 < piece.stop) fetch(k0 + kAttnWaves * 32);
-    f32x16 s = {};
+    f32x16 s[1] = {};
 #pragma unroll
-    for (int c = 0; c < C; ++c) mma(s, L::rows(lk, 0, c, lane), q[c]);
-    const bool mask = k0 + 32 > all_min;
-    float top = m;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float x = score<T, CAP>(s[r], scale2, in_scale, cap2);
-      if (mask && k0 + 8 * (r / 4) + 4 * h + r % 4 >= vis) x = -INFINITY;
-      s[r] = x;
-      top = fmaxf(top, x);
-    }
-    top = half_max(top);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float alpha = exp2_hw(m - ref);
-    m = top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = exp2_hw(s[r] - ref);
-      sum += s[r];
-    }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= alpha;
+    for (int c = 0; c < C; ++c) mma(s[0], L::rows(lk, 0, c, lane), q[c]);
+    softmax_step<T, MODE>(rule, s, o, st, k0 + 32 > all_min, vis - k0, h);
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
-      const Frag<T> p = acc_frag<T>(s, kc);
+      const Frag<T> p = acc_frag<T>(s[0], kc);
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], L::cols(lv, 32 * dt, 16 * kc, lane), p);
     }
@@ -277,7 +339,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
   }
   // join: every wavefront leaves its rows, statistics and (in its own tiles) sums; then all threads
   // take the same rows' elements and add the wavefronts' in order
-  l = half_sum(l);
+  const float m = st.m, l = half_sum(st.l);
   float* own = reinterpret_cast<float*>(lk);
   if (live) {
     if (h == 0) {
@@ -359,7 +421,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
 }
 
 // Query gradients, and delta_i = dO_i . O_i for the key gradients.
-template <typename T, int DP, bool CAP>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
@@ -404,6 +466,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
   const int vis = live ? visible(a, doc, tok) : 0;
   const int wave_min = wrow + 31 < rows ? visible(a, doc, wrow / a.group) : 0;
   const int end = visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group);
+  constexpr bool CAP = MODE != kPlain;
   const float scale2 = a.scale * kLog2e;
   const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
   f32x16 dq[DP / 32] = {};
@@ -458,7 +521,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
 }
 
 // Key and value gradients: a lane owns one key, the workgroup walks over the query rows that see it.
-template <typename T, int DP, bool CAP>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
@@ -496,6 +559,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
     if (t > 0) row_begin = static_cast<int>(t < doc.q_len ? t : doc.q_len) * a.group;
   }
   if (key0 >= doc.k_len) row_begin = rows;
+  constexpr bool CAP = MODE != kPlain;
   const float scale2 = a.scale * kLog2e;
   const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
@@ -639,22 +703,37 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
 // Tiles of `rows` rows that `tokens` tokens of `per` rows in docs + 2 stretches can take.
 static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { return tokens * per / rows + docs + 2; }
 
-#define GS_ATTN_LAUNCH(KERNEL, GRID)                                                                       \
-  do {                                                                                                     \
-    const dim3 grid_(static_cast<unsigned>(GRID), static_cast<unsigned>(a.splits)), block_(kAttnThreads);                                   \
-    const bool cap_ = a.softcap > 0.0f, wide_ = a.dim > 64;                                                \
-    if (p->dtype == GS_BFLOAT16) {                                                                         \
-      if (wide_ && cap_) hipLaunchKernelGGL((KERNEL<__bf16, 128, true>), grid_, block_, 0, st, a);         \
-      else if (wide_) hipLaunchKernelGGL((KERNEL<__bf16, 128, false>), grid_, block_, 0, st, a);           \
-      else if (cap_) hipLaunchKernelGGL((KERNEL<__bf16, 64, true>), grid_, block_, 0, st, a);              \
-      else hipLaunchKernelGGL((KERNEL<__bf16, 64, false>), grid_, block_, 0, st, a);                       \
-    } else {                                                                                               \
-      if (wide_ && cap_) hipLaunchKernelGGL((KERNEL<float, 128, true>), grid_, block_, 0, st, a);          \
-      else if (wide_) hipLaunchKernelGGL((KERNEL<float, 128, false>), grid_, block_, 0, st, a);            \
-      else if (cap_) hipLaunchKernelGGL((KERNEL<float, 64, true>), grid_, block_, 0, st, a);               \
-      else hipLaunchKernelGGL((KERNEL<float, 64, false>), grid_, block_, 0, st, a);                        \
-    }                                                                                                      \
-  } while (0)
+template <template <typename, int, int> class K, typename T, int DP>
+static void launch_mode(const AttnArgs& a, dim3 grid, hipStream_t st) {
+  if (a.softcap == 0.0f) K<T, DP, kPlain>::launch(a, grid, st);
+  else if (K<T, DP, kCap>::kFixed && a.softcap * kLog2e <= kFixedCap) K<T, DP, kCapFixed>::launch(a, grid, st);
+  else K<T, DP, kCap>::launch(a, grid, st);
+}
+template <template <typename, int, int> class K>
+static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.splits));
+  if (dtype == GS_BFLOAT16) {
+    if (a.dim > 64) launch_mode<K, __bf16, 128>(a, grid, st);
+    else launch_mode<K, __bf16, 64>(a, grid, st);
+  } else {
+    if (a.dim > 64) launch_mode<K, float, 128>(a, grid, st);
+    else launch_mode<K, float, 64>(a, grid, st);
+  }
+}
+#define GS_ATTN_KERNEL(NAME, KERNEL, FIXED)                                            \
+  template <typename T, int DP, int MODE>                                              \
+  struct NAME {                                                                        \
+    static constexpr bool kFixed = FIXED;                                              \
+    static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                 \
+      constexpr int mode = !FIXED && MODE == kCapFixed ? static_cast<int>(kCap) : MODE; \
+      hipLaunchKernelGGL((KERNEL<T, DP, mode>), grid, dim3(kAttnThreads), 0, st, a);   \
+    }                                                                                  \
+  }
+GS_ATTN_KERNEL(FwdKernel, attn_fwd_kernel, true);
+GS_ATTN_KERNEL(FewKernel, attn_few_kernel, true);
+GS_ATTN_KERNEL(BwdQKernel, attn_bwd_q_kernel, false);
+GS_ATTN_KERNEL(BwdKvKernel, attn_bwd_kv_kernel, false);
+#undef GS_ATTN_KERNEL
 
 // How a forward call is laid out, by sizes alone (so that the workspace can be asked for first).
 struct FwdPlan {
@@ -718,9 +797,9 @@ extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t w
   a.part_stat = a.part + rows * a.splits * a.dim;
   a.part_n = reinterpret_cast<int32_t*>(a.part_stat + rows * a.splits * 2);
   if (f.few)
-    GS_ATTN_LAUNCH(attn_few_kernel, f.tiles * a.kv_heads);
+    launch_attn<FewKernel>(a, p->dtype, f.tiles * a.kv_heads, st);
   else
-    GS_ATTN_LAUNCH(attn_fwd_kernel, f.tiles * a.kv_heads);
+    launch_attn<FwdKernel>(a, p->dtype, f.tiles * a.kv_heads, st);
   if (const int rc = check_launch("attention")) return rc;
   if (a.splits == 1) return GS_OK;
   const dim3 grid(static_cast<unsigned>((rows + kAttnWaves - 1) / kAttnWaves)), block(kAttnThreads);
@@ -761,12 +840,12 @@ extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* 
              "attention: too many tokens, documents or heads");
   if (p->q_tokens > 0) {
     a.n_tiles = static_cast<int>(q_tiles);
-    GS_ATTN_LAUNCH(attn_bwd_q_kernel, q_tiles * a.kv_heads);
+    launch_attn<BwdQKernel>(a, p->dtype, q_tiles * a.kv_heads, st);
     if (const int rc = check_launch("attention backward (queries)")) return rc;
   }
   if (p->k_tokens > 0) {
     a.n_tiles = static_cast<int>(k_tiles);
-    GS_ATTN_LAUNCH(attn_bwd_kv_kernel, k_tiles * a.kv_heads);
+    launch_attn<BwdKvKernel>(a, p->dtype, k_tiles * a.kv_heads, st);
     return check_launch("attention backward (keys)");
   }
   return GS_OK;

@@ -131,8 +131,9 @@ __device__ __forceinline__ Frag<T> load_frag(const T* p, bool valid) {
 
 // Rows [0, rows) of a strided matrix as a buffer: loads beyond the last row, and at kNowhere, give
 // zero. Its base is set per tile, so that offsets stay within 32 bits however long the matrix is
-// (token strides are below 2^22 elements, tiles have at most 128 rows).
-constexpr uint32_t kNowhere = 0xffffff00u;
+// (token strides are below 2^22 elements, tiles have at most 64 rows: 2^30 bytes, so kNowhere is
+// outside with any row's offset added).
+constexpr uint32_t kNowhere = 0x80000000u;
 template <typename T>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* base, int64_t stride, int rows, int dim) {
   const int bytes = rows > 0 ? static_cast<int>(((rows - 1) * stride + dim) * static_cast<int64_t>(sizeof(T))) : 0;
@@ -142,6 +143,43 @@ __device__ __forceinline__ f32x4 load16(__amdgpu_buffer_rsrc_t b, uint32_t offse
   using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(f32x4, static_cast<u32x4>(__builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0)));
 }
+
+// Copies a tile from a row_buffer straight to LDS (no registers), rows beyond the buffer's and columns
+// beyond `dim` as zeros. The copy is under way when the call returns: copies_done() waits for the
+// wavefront's own, a barrier after it for the others'. The LDS side is linear in the lanes, so it is
+// the global side that a lane permutes: it fetches the chunk that belongs to its place in the tile.
+// The instruction is written out because the compiler, given its builtin, waits for every copy under
+// way before each transposed LDS read. It has no output registers; M0 (the LDS base), a register that
+// the compiler keeps nothing in from one instruction to the next, needs one wait state before its use.
+template <typename T, int DP, int ROWS, int THREADS>
+struct TileCopy {
+  using L = Tile<T, DP>;
+  static constexpr int kRowsPerStep = THREADS / L::kChunks;
+  static constexpr bool kOneOffset = kRowsPerStep % 16 == 0;  // rows 16 apart are permuted alike
+  uint32_t offset, step;
+  int64_t stride;
+  int dim;
+  __device__ __forceinline__ uint32_t at(int row) const {
+    const int c = ((threadIdx.x % L::kChunks) ^ L::swizzle(row)) * L::kElemsPerChunk;
+    return c < dim ? static_cast<uint32_t>((row * stride + c) * sizeof(T)) : kNowhere;
+  }
+  __device__ __forceinline__ TileCopy(int64_t stride_, int dim_) : stride(stride_), dim(dim_) {
+    offset = at(threadIdx.x / L::kChunks);
+    step = static_cast<uint32_t>(kRowsPerStep * stride * sizeof(T));
+  }
+  __device__ __forceinline__ void operator()(char* lds, __amdgpu_buffer_rsrc_t src) const {
+    typedef __attribute__((address_space(3))) char* lds_ptr;
+    const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)lds)) +
+                        __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
+#pragma unroll
+    for (int i = 0; i < ROWS / kRowsPerStep; ++i) {
+      const uint32_t from = kOneOffset ? offset + i * step : at(threadIdx.x / L::kChunks + i * kRowsPerStep);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to + i * (THREADS * 16)), "v"(from), "s"(src) : "memory");
+    }
+  }
+};
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Four consecutive accumulator rows of one column, rounded to nearest and stored.
 __device__ __forceinline__ void store4(__bf16* p, float a, float b, float c, float d) {
@@ -164,6 +202,13 @@ __device__ __forceinline__ float half_max(float v) {
 
 // 2^x by the hardware instruction (1 ulp; results below the smallest normal number are zero).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// How scores become base-2 exponents.
+enum { kPlain = 0, kCap = 1, kCapFixed = 2 };
+// kCapFixed: scores capped at cap2 (base 2) <= kFixedCap need no running maximum: relative to cap2 -
+// 60 every exponent lies in [-120, 60], so no probability under- or overflows and a sum over 2^30 keys
+// stays below 2^90.
+constexpr float kFixedCap = 90.0f, kFixedTop = 60.0f;
 
 // tanh. bfloat16: 1 - 2 / (1 + e^2x) from the hardware exponential and reciprocal (absolute error
 // 2e-7; both ends saturate). float32: the library's, which keeps the relative error near zero.
