@@ -21,14 +21,15 @@ MAX_DIM = 128  # GS_ATTENTION_MAX_DIM
 _DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8)}
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """t itself if the kernels can read it through its strides, otherwise a contiguous copy."""
+def _readable(t: torch.Tensor, group: int = 0) -> torch.Tensor:
+    """t itself if the kernels can read it through its strides, otherwise a contiguous copy. group: query
+    heads to a key head (q: 64 consecutive rows have to span less than 2^28 elements)."""
     per = _DTYPES[t.dtype][1]
     st, sh, sd = t.stride()
     if t.numel() == 0:
         return t
     ok = ((sd == 1 or t.shape[2] == 1) and 0 <= st < 1 << 22 and 0 <= sh < 1 << 40 and st % per == 0 and sh % per == 0
-          and t.data_ptr() % 16 == 0)
+          and t.data_ptr() % 16 == 0 and (not group or (64 // group + 2) * st + group * sh < 1 << 28))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -61,7 +62,7 @@ def _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, sc
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale):
-        q, k, v = _readable(q), _readable(k), _readable(v)
+        q, k, v = _readable(q, q.shape[1] // k.shape[1]), _readable(k), _readable(v)
         out, lse = _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale)
         ctx.save_for_backward(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix)
         ctx.rule = (causal, softcap, scale)
@@ -122,6 +123,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
         raise ValueError(f"head size {d}: 1 to {MAX_DIM} are provided")
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} heads are not a multiple of {kv_heads} key heads")
+    if heads // kv_heads > 512:
+        raise ValueError("at most 512 heads may share a key head")
     if offsets is None and k_offsets is not None:
         raise ValueError("k_offsets without offsets")
     docs = 1
@@ -154,7 +157,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _Attention.apply(q, k, v, *rest)
     else:
-        out, lse = _forward(_readable(q), _readable(k), _readable(v), *rest)
+        out, lse = _forward(_readable(q, heads // kv_heads), _readable(k), _readable(v), *rest)
     if d % 8:
         out = out[..., :d]
     return (out, lse) if return_lse else out

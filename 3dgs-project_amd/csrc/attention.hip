@@ -3,6 +3,7 @@
 // head are rows of one tile, so a key tile is read once for all of them and the gradients of shared
 // heads are summed inside one workgroup, in a fixed order, without atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_attention.h"
 
@@ -12,44 +13,6 @@ constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = kAttnWaves * kWave;
 constexpr int kAttnRows = kAttnWaves * 32;  // query rows (or keys, in the key gradients) of a workgroup
 constexpr int kAttnKeys = 64;               // keys (or query rows) of a tile in LDS
-
-// Copies rows [0, valid) of a strided matrix to a tile, zero beyond them and beyond `dim`.
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void stage(char* lds, const T* src, int64_t stride, int valid, int dim) {
-  using L = Tile<T, DP>;
-#pragma unroll
-  for (int i = 0; i < ROWS * L::kChunks / kAttnThreads; ++i) {
-    const int e = i * kAttnThreads + static_cast<int>(threadIdx.x);
-    const int row = e / L::kChunks, chunk = e % L::kChunks;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row < valid && chunk * L::kElemsPerChunk < dim)
-      v = *reinterpret_cast<const f32x4*>(src + row * stride + chunk * L::kElemsPerChunk);
-    *reinterpret_cast<f32x4*>(lds + L::at(row, chunk)) = v;
-  }
-}
-
-// The rows of a tile of (token, head of the group) pairs.
-struct RowMap {
-  int64_t token0;
-  int group, head0;
-};
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void stage_rows(char* lds, const T* src, int64_t token_stride, int64_t head_stride,
-                                           const RowMap& m, int row0, int valid, int dim) {
-  using L = Tile<T, DP>;
-#pragma unroll
-  for (int i = 0; i < ROWS * L::kChunks / kAttnThreads; ++i) {
-    const int e = i * kAttnThreads + static_cast<int>(threadIdx.x);
-    const int row = e / L::kChunks, chunk = e % L::kChunks;
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row < valid && chunk * L::kElemsPerChunk < dim) {
-      const int r = row0 + row, t = r / m.group;
-      v = *reinterpret_cast<const f32x4*>(src + (m.token0 + t) * token_stride +
-                                          (m.head0 + r - t * m.group) * head_stride + chunk * L::kElemsPerChunk);
-    }
-    *reinterpret_cast<f32x4*>(lds + L::at(row, chunk)) = v;
-  }
-}
 
 // Base-2 exponent of a score, up to the reference that p = 2^(x - ref) takes off. Plain scores stay as
 // they come (monotone in x: the scale is positive) and are scaled in the same fma that subtracts.
@@ -420,14 +383,65 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
   if (lane == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-// Query gradients, and delta_i = dO_i . O_i for the key gradients.
+// Score gradient of one (query, key): p = e^(s - lse), ds = p (dp - delta) ds/ds_raw.
+template <typename T, int MODE>
+__device__ __forceinline__ void score_grad(const Rule& u, float s, float dp, float lse2, float delta, float* p,
+                                           float* ds) {
+  if constexpr (MODE == kPlain) {
+    *p = exp2_hw(fmaf(s, u.scale2, -lse2));
+    *ds = *p * (dp - delta);
+  } else {
+    const float t = tanh_of<T>(s * u.in_scale);
+    *p = exp2_hw(fmaf(u.cap2, t, -lse2));
+    *ds = *p * fmaf(-t, t, 1.0f) * (dp - delta);
+  }
+}
+
+// S and dP of 32 rows of a pair of tiles against a lane's column, the rows' fragments read first.
+template <typename T, int DP>
+__device__ __forceinline__ void two_products(const char* la, const char* lb, int row0, int lane,
+                                             const Frag<T> (&a)[DP / 16], const Frag<T> (&b)[DP / 16], f32x16& s,
+                                             f32x16& dp) {
+  using L = Tile<T, DP>;
+  constexpr int C = DP / 16;
+  Frag<T> x[C], y[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) x[c] = L::rows(la, row0, c, lane);
+#pragma unroll
+  for (int c = 0; c < C; ++c) y[c] = L::rows(lb, row0, c, lane);
+  s = dp = f32x16{};
+#pragma unroll
+  for (int c = 0; c < C; ++c) mma(s, x[c], a[c]);
+#pragma unroll
+  for (int c = 0; c < C; ++c) mma(dp, y[c], b[c]);
+}
+
+// acc += (tile rows row0 .. row0 + 31, transposed) x p
+template <typename T, int DP>
+__device__ __forceinline__ void add_product(const char* lds, int row0, int lane, const f32x16& p,
+                                            f32x16 (&acc)[DP / 32]) {
+  using L = Tile<T, DP>;
+  Frag<T> x[2][DP / 32];
+#pragma unroll
+  for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) x[kc][dt] = L::cols(lds, 32 * dt, row0 + 16 * kc, lane);
+#pragma unroll
+  for (int kc = 0; kc < 2; ++kc) {
+    const Frag<T> f = acc_frag<T>(p, kc);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) mma(acc[dt], x[kc][dt], f);
+  }
+}
+
+// Query gradients, and delta_i = dO_i . O_i for the key gradients. Like the forward, a lane owns a
+// query; its score gradients are the B operand of dQ = dS K.
 template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kAttnKeys * L::kRowBytes];
-  char* lk = lds;
-  char* lv = lds + kAttnKeys * L::kRowBytes;
+  constexpr int kTileBytes = kAttnKeys * L::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = a.n_tiles - 1 - static_cast<int64_t>(blockIdx.x / a.kv_heads);
   int64_t first;
@@ -437,12 +451,22 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
   const int64_t base = (tile - first) * kAttnRows;
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
+  const int end = visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wrow = row0 + wave * 32;
   const int row = wrow + (lane & 31);
   const bool live = row < rows;
   const int rc = live ? row : rows - 1;
   const int tok = rc / a.group, head = hk * a.group + rc - tok * a.group;
+  const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
+  const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
+  const TileCopy<T, DP, kAttnKeys, kAttnThreads> copy_k(a.k_token, a.dim), copy_v(a.v_token, a.dim);
+  const auto fetch = [&](int k0, char* to) {
+    const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
+    copy_k(to, row_buffer(kp + k0 * a.k_token, a.k_token, valid, a.dim));
+    copy_v(to + kTileBytes, row_buffer(vp + k0 * a.v_token, a.v_token, valid, a.dim));
+  };
+  if (end > 0) fetch(0, lds);
   const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
   const int64_t at = ((doc.q0 + tok) * a.heads + head) * a.dim;
   const T* gp = static_cast<const T*>(a.d_out) + at;
@@ -452,7 +476,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const bool in = 16 * c + 8 * h < a.dim;
-    q[c] = load_frag<T>(qp + 16 * c + 8 * h, in);
+    q[c] = load_query<T>(a, qp + 16 * c + 8 * h, in);
     g[c] = load_frag<T>(gp + 16 * c + 8 * h, in);
     const Frag<T> o = load_frag<T>(op + 16 * c + 8 * h, in);
 #pragma unroll
@@ -465,72 +489,71 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
   const float lse2 = lse == -INFINITY ? 0.0f : lse * kLog2e;
   const int vis = live ? visible(a, doc, tok) : 0;
   const int wave_min = wrow + 31 < rows ? visible(a, doc, wrow / a.group) : 0;
-  const int end = visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group);
-  constexpr bool CAP = MODE != kPlain;
-  const float scale2 = a.scale * kLog2e;
-  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  const Rule rule = rule_of<MODE>(a);
   f32x16 dq[DP / 32] = {};
-  const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
-  const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
-  for (int k0 = 0; k0 < end; k0 += kAttnKeys) {
-    const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
+  int buf = 0;
+  for (int k0 = 0; k0 < end; k0 += kAttnKeys, buf ^= 1) {
+    const char* lk = lds + buf * 2 * kTileBytes;
+    const char* lv = lk + kTileBytes;
+    copies_done();
     __syncthreads();
-    stage<T, DP, kAttnKeys>(lk, kp + k0 * a.k_token, a.k_token, valid, a.dim);
-    stage<T, DP, kAttnKeys>(lv, vp + k0 * a.v_token, a.v_token, valid, a.dim);
-    __syncthreads();
-    const bool mask = k0 + kAttnKeys > wave_min;
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        mma(s, L::rows(lk, 32 * st, c, lane), q[c]);
-        mma(dp, L::rows(lv, 32 * st, c, lane), g[c]);
-      }
+    if (k0 + kAttnKeys < end) fetch(k0 + kAttnKeys, lds + (buf ^ 1) * 2 * kTileBytes);
+    const auto grads = [&](f32x16& s, f32x16& dp, int sub, auto masked) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float ds;
-        if constexpr (CAP) {
-          const float t = tanh_of<T>(s[r] * in_scale);
-          ds = exp2_hw(fmaf(cap2, t, -lse2)) * (dp[r] - delta) * fmaf(-t, t, 1.0f);
-        } else {
-          ds = exp2_hw(fmaf(s[r], scale2, -lse2)) * (dp[r] - delta);
-        }
-        if (mask && k0 + 32 * st + 8 * (r / 4) + 4 * h + r % 4 >= vis) ds = 0.0f;
+        float p, ds;
+        score_grad<T, MODE>(rule, s[r], dp[r], lse2, delta, &p, &ds);
+        if (masked.value && k0 + 32 * sub + 8 * (r / 4) + 4 * h + r % 4 >= vis) ds = 0.0f;
         s[r] = ds;
       }
+    };
+    const auto body = [&](auto masked) {
+      f32x16 s[2], dp[2];
+      if constexpr (sizeof(T) == 2) {
+        // the second half's products beside the first half's exponentials
+        two_products<T, DP>(lk, lv, 0, lane, q, g, s[0], dp[0]);
+        two_products<T, DP>(lk, lv, 32, lane, q, g, s[1], dp[1]);
+        grads(s[0], dp[0], 0, masked);
+        add_product<T, DP>(lk, 0, lane, s[0], dq);
+        grads(s[1], dp[1], 1, masked);
+        add_product<T, DP>(lk, 32, lane, s[1], dq);
+      } else {
 #pragma unroll
-      for (int kc = 0; kc < 2; ++kc) {
-        const Frag<T> p = acc_frag<T>(s, kc);
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) mma(dq[dt], L::cols(lk, 32 * dt, 32 * st + 16 * kc, lane), p);
+        for (int t = 0; t < 2; ++t) {
+          two_products<T, DP>(lk, lv, 32 * t, lane, q, g, s[t], dp[t]);
+          grads(s[t], dp[t], t, masked);
+          add_product<T, DP>(lk, 32 * t, lane, s[t], dq);
+        }
       }
-    }
+    };
+    if (k0 + kAttnKeys > wave_min) body(std::true_type{});
+    else body(std::false_type{});
   }
   if (!live) return;
-  T* dp = static_cast<T*>(a.d_q) + at;
+  T* to = static_cast<T*>(a.d_q) + at;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * h;
       if (d < a.dim)
-        store4(dp + d, dq[dt][r] * a.scale, dq[dt][r + 1] * a.scale, dq[dt][r + 2] * a.scale,
+        store4(to + d, dq[dt][r] * a.scale, dq[dt][r + 1] * a.scale, dq[dt][r + 2] * a.scale,
                dq[dt][r + 3] * a.scale);
     }
 }
 
-// Key and value gradients: a lane owns one key, the workgroup walks over the query rows that see it.
+// Key and value gradients: a lane owns one key, the workgroup walks over the query rows that see it,
+// 64 at a time. Rows past the document's end need no mask: their q, dO, lse and delta are zero, and so
+// is what they add. The lanes of keys past the valid length gather nothing that is kept.
 template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
-  constexpr int R = 32;  // query rows of a tile
-  __shared__ __attribute__((aligned(16))) char lds[2 * R * L::kRowBytes];
-  __shared__ __attribute__((aligned(16))) float l_lse[R], l_delta[R];
-  __shared__ __attribute__((aligned(16))) int l_vis[R];
-  char* lq = lds;
-  char* lg = lds + R * L::kRowBytes;
+  constexpr int R = 64;
+  constexpr int kTileBytes = R * L::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) float l_lse[2][R], l_delta[2][R];
+  __shared__ __attribute__((aligned(16))) int l_vis[2][R];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = blockIdx.x / a.kv_heads;
   int64_t first;
@@ -542,6 +565,44 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
   const int key0 = static_cast<int>(base), wkey = key0 + wave * 32;
   const int key = wkey + (lane & 31);
   const bool live = key < doc.k_len;
+  const int rows = static_cast<int>(doc.q_len) * a.group;
+  // the first token that sees key0 (none of this tile's keys is seen by one before it)
+  RowStart start = {0, 0};
+  if (a.causal && key0 >= doc.prefix) {
+    const int64_t t = key0 - doc.k_len + doc.q_len;
+    if (t > 0) start.token = static_cast<int>(t < doc.q_len ? t : doc.q_len);
+  }
+  const int row_begin = key0 >= doc.k_len ? rows : start.token * a.group;
+  const RowTileCopy<T, DP, R, kAttnThreads> copy_q = {a.q_token, a.q_head};
+  const RowTileCopy<T, DP, R, kAttnThreads> copy_g = {static_cast<int64_t>(a.heads) * a.dim, a.dim};
+  float n_lse = 0.0f, n_delta = 0.0f;
+  int n_vis = 0;
+  const auto fetch = [&](int r0, char* to) {
+    const int64_t token = doc.q0 + start.token;
+    copy_q(a, to, static_cast<const T*>(a.q) + token * a.q_token + hk * a.group * a.q_head, start.g, rows - r0);
+    copy_g(a, to + kTileBytes, static_cast<const T*>(a.d_out) + (token * a.heads + hk * a.group) * a.dim, start.g,
+           rows - r0);
+    if (threadIdx.x < R) {
+      n_lse = n_delta = 0.0f;
+      n_vis = 0;
+      if (r0 + static_cast<int>(threadIdx.x) < rows) {
+        const int n = start.g + threadIdx.x, t = static_cast<int>((n * a.group_magic) >> 20);
+        const int64_t stat = (token + t) * a.heads + hk * a.group + n - t * a.group;
+        n_lse = a.lse[stat];
+        n_delta = a.delta[stat];
+        n_vis = visible(a, doc, start.token + t);
+      }
+    }
+    start.advance(a, R);
+  };
+  const auto keep = [&](int b) {
+    if (threadIdx.x < R) {
+      l_lse[b][threadIdx.x] = n_lse == -INFINITY ? 0.0f : n_lse * kLog2e;
+      l_delta[b][threadIdx.x] = n_delta;
+      l_vis[b][threadIdx.x] = n_vis;
+    }
+  };
+  if (row_begin < rows) fetch(row_begin, lds);
   Frag<T> k[C], v[C];
   const T* kp = static_cast<const T*>(a.k) + (doc.k0 + key) * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + (doc.k0 + key) * a.v_token + hk * a.v_head;
@@ -549,75 +610,61 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
   for (int c = 0; c < C; ++c) {
     const bool in = live && 16 * c + 8 * h < a.dim;
     k[c] = load_frag<T>(kp + 16 * c + 8 * h, in);
+    if (a.scale < 0.0f) k[c] = -k[c];
     v[c] = load_frag<T>(vp + 16 * c + 8 * h, in);
   }
-  const int rows = static_cast<int>(doc.q_len) * a.group;
-  // the first token that sees key0 (none of this tile's keys is seen by one before it)
-  int row_begin = 0;
-  if (a.causal && key0 >= doc.prefix) {
-    const int64_t t = key0 - doc.k_len + doc.q_len;
-    if (t > 0) row_begin = static_cast<int>(t < doc.q_len ? t : doc.q_len) * a.group;
-  }
-  if (key0 >= doc.k_len) row_begin = rows;
-  constexpr bool CAP = MODE != kPlain;
-  const float scale2 = a.scale * kLog2e;
-  const float in_scale = CAP ? a.scale / a.softcap : 0.0f, cap2 = a.softcap * kLog2e;
+  const Rule rule = rule_of<MODE>(a);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  const RowMap map = {doc.q0, a.group, hk * a.group};
-  for (int r0 = row_begin; r0 < rows; r0 += R) {
-    const int valid = min(R, rows - r0);
+  int buf = 0;
+  for (int r0 = row_begin; r0 < rows; r0 += R, buf ^= 1) {
+    const char* lq = lds + buf * 2 * kTileBytes;
+    const char* lg = lq + kTileBytes;
+    keep(buf);
+    copies_done();
     __syncthreads();
-    stage_rows<T, DP, R>(lq, static_cast<const T*>(a.q), a.q_token, a.q_head, map, r0, valid, a.dim);
-    stage_rows<T, DP, R>(lg, static_cast<const T*>(a.d_out), static_cast<int64_t>(a.heads) * a.dim, a.dim, map, r0,
-                         valid, a.dim);
-    if (threadIdx.x < R) {
-      const int r = r0 + threadIdx.x;
-      float lse = 0.0f, delta = 0.0f;
-      int vis = 0;
-      if (r < rows) {
-        const int t = r / a.group;
-        const int64_t stat = (doc.q0 + t) * a.heads + hk * a.group + r - t * a.group;
-        lse = a.lse[stat];
-        lse = lse == -INFINITY ? 0.0f : lse * kLog2e;
-        delta = a.delta[stat];
-        vis = visible(a, doc, t);
+    // every row of the tile sees all of this wavefront's keys?
+    const bool mask = a.causal && __builtin_amdgcn_readfirstlane(l_vis[buf][0]) < wkey + 32;
+    if (r0 + R < rows) fetch(r0 + R, lds + (buf ^ 1) * 2 * kTileBytes);
+    const auto grads = [&](f32x16& s, f32x16& dp, int sub, auto masked) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = 32 * sub + 8 * i + 4 * h;
+        const f32x4 lse2 = *reinterpret_cast<const f32x4*>(&l_lse[buf][at]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&l_delta[buf][at]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * i + j;
+          float p, ds;
+          score_grad<T, MODE>(rule, s[r], dp[r], lse2[j], delta[j], &p, &ds);
+          if (masked.value && key >= l_vis[buf][at + j]) p = ds = 0.0f;
+          s[r] = p;
+          dp[r] = ds;
+        }
       }
-      l_lse[threadIdx.x] = lse;
-      l_delta[threadIdx.x] = delta;
-      l_vis[threadIdx.x] = vis;
-    }
-    __syncthreads();
-    f32x16 s = {}, dp = {};
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      mma(s, L::rows(lq, 0, c, lane), k[c]);
-      mma(dp, L::rows(lg, 0, c, lane), v[c]);
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int i = 8 * (r / 4) + 4 * h + r % 4;
-      float p, ds;
-      if constexpr (CAP) {
-        const float t = tanh_of<T>(s[r] * in_scale);
-        p = exp2_hw(fmaf(cap2, t, -l_lse[i]));
-        ds = p * (dp[r] - l_delta[i]) * fmaf(-t, t, 1.0f);
+    };
+    const auto body = [&](auto masked) {
+      f32x16 s[2], dp[2];
+      if constexpr (sizeof(T) == 2) {
+        two_products<T, DP>(lq, lg, 0, lane, k, v, s[0], dp[0]);
+        two_products<T, DP>(lq, lg, 32, lane, k, v, s[1], dp[1]);
+        grads(s[0], dp[0], 0, masked);
+        add_product<T, DP>(lg, 0, lane, s[0], dv);
+        add_product<T, DP>(lq, 0, lane, dp[0], dk);
+        grads(s[1], dp[1], 1, masked);
+        add_product<T, DP>(lg, 32, lane, s[1], dv);
+        add_product<T, DP>(lq, 32, lane, dp[1], dk);
       } else {
-        p = exp2_hw(fmaf(s[r], scale2, -l_lse[i]));
-        ds = p * (dp[r] - l_delta[i]);
-      }
-      if (key >= l_vis[i]) p = ds = 0.0f;
-      s[r] = p;
-      dp[r] = ds;
-    }
 #pragma unroll
-    for (int kc = 0; kc < 2; ++kc) {
-      const Frag<T> p = acc_frag<T>(s, kc), ds = acc_frag<T>(dp, kc);
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
-        mma(dv[dt], L::cols(lg, 32 * dt, 16 * kc, lane), p);
-        mma(dk[dt], L::cols(lq, 32 * dt, 16 * kc, lane), ds);
+        for (int t = 0; t < 2; ++t) {
+          two_products<T, DP>(lq, lg, 32 * t, lane, k, v, s[t], dp[t]);
+          grads(s[t], dp[t], t, masked);
+          add_product<T, DP>(lg, 32 * t, lane, s[t], dv);
+          add_product<T, DP>(lq, 32 * t, lane, dp[t], dk);
+        }
       }
-    }
+    };
+    if (mask) body(std::true_type{});
+    else body(std::false_type{});
   }
   if (key >= doc.k_cap) return;
   const int64_t at = ((doc.k0 + key) * a.kv_heads + hk) * a.dim;
@@ -628,11 +675,14 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * h;
-      if (d < a.dim) {
-        store4(dkp + d, dk[dt][r] * a.scale, dk[dt][r + 1] * a.scale, dk[dt][r + 2] * a.scale,
-               dk[dt][r + 3] * a.scale);
-        store4(dvp + d, dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]);
+      if (d >= a.dim) continue;
+      f32x4 x = {}, y = {};
+      if (live) {
+        x = f32x4{dk[dt][r], dk[dt][r + 1], dk[dt][r + 2], dk[dt][r + 3]} * a.scale;
+        y = f32x4{dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]};
       }
+      store4(dkp + d, x[0], x[1], x[2], x[3]);
+      store4(dvp + d, y[0], y[1], y[2], y[3]);
     }
 }
 
@@ -654,6 +704,7 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
   const int64_t group = p->heads / p->kv_heads;
   GS_REQUIRE(p->q_tokens * group < (int64_t(1) << 30) && p->k_tokens < (int64_t(1) << 30) &&
                  p->docs < (1 << 26), GS_ERR_ARG, "attention: too many tokens or documents");
+  GS_REQUIRE(group <= 512, GS_ERR_ARG, "attention: at most 512 heads share a key head");
   GS_REQUIRE(p->prefix == nullptr || p->causal, GS_ERR_ARG, "attention: a prefix needs the causal mask");
   GS_REQUIRE(p->scale == p->scale && p->softcap >= 0.0f && p->softcap <= FLT_MAX &&
                  p->scale <= FLT_MAX && p->scale >= -FLT_MAX, GS_ERR_ARG,
@@ -668,6 +719,9 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
     GS_REQUIRE(strides[i] >= 0 && strides[i] < (int64_t(1) << (i % 2 ? 40 : 22)) && strides[i] % elems == 0,
                GS_ERR_ALIGN, "attention: strides must be multiples of 16 bytes, token strides below 2^22 elements "
                "(got %lld)", static_cast<long long>(strides[i]));
+  // what 64 consecutive rows (token, head of a group) of q span, 2^31 bytes at most
+  GS_REQUIRE((64 / group + 2) * p->q_token_stride + group * p->q_head_stride < (int64_t(1) << 28), GS_ERR_ALIGN,
+             "attention: q's strides are too large");
   GS_REQUIRE(aligned(p->q, 16) && aligned(p->k, 16) && aligned(p->v, 16) && aligned(p->out, 16) &&
                  aligned(p->lse, 4), GS_ERR_ALIGN, "attention: tensors must be 16-byte aligned");
   a = {};
@@ -693,6 +747,7 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
   a.kv_heads = p->kv_heads;
   a.group = static_cast<int>(group);
   a.dim = p->dim;
+  a.group_magic = static_cast<uint32_t>(((1 << 20) + group - 1) / group);
   a.causal = p->causal != 0;
   a.softcap = p->softcap;
   a.scale = p->scale;

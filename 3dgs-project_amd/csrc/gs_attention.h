@@ -129,6 +129,28 @@ __device__ __forceinline__ Frag<T> load_frag(const T* p, bool valid) {
   return f;
 }
 
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int32_t *q_offsets, *k_offsets, *k_lengths, *prefix;
+  int64_t q_tokens, k_tokens;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides in elements
+  int docs, heads, kv_heads, group, dim, causal;
+  uint32_t group_magic;  // ceil(2^20 / group)
+  float softcap, scale;
+  // backward
+  const void* d_out;
+  void *d_q, *d_k, *d_v;
+  float* delta;
+  int n_tiles;
+  // keys of a row tile cut into up to `splits` pieces of at least split_keys, joined by a second launch
+  int splits, split_keys;
+  float* part;        // [splits][q_tokens][heads][dim], unnormalised
+  float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
+  int32_t* part_n;    // [q_tokens][heads] pieces
+};
+
 // Rows [0, rows) of a strided matrix as a buffer: loads beyond the last row, and at kNowhere, give
 // zero. Its base is set per tile, so that offsets stay within 32 bits however long the matrix is
 // (token strides are below 2^22 elements, tiles have at most 64 rows: 2^30 bytes, so kNowhere is
@@ -179,6 +201,42 @@ struct TileCopy {
     }
   }
 };
+// The same for rows that are (token, head of the group) pairs. The first row's token and head are kept
+// as a pair and advanced, a row's own are found by a multiplication: (n magic) >> 20 is n / group for
+// n < group + 64 (group <= 512).
+struct RowStart {
+  int token, g;
+  __device__ __forceinline__ void advance(const AttnArgs& a, int rows) {
+    g += rows;
+    const int t = static_cast<int>((static_cast<uint32_t>(g) * a.group_magic) >> 20);
+    token += t;
+    g -= t * a.group;
+  }
+};
+template <typename T, int DP, int ROWS, int THREADS>
+struct RowTileCopy {
+  using L = Tile<T, DP>;
+  static constexpr int kRowsPerStep = THREADS / L::kChunks;
+  int64_t token_stride, head_stride;
+  // base: the first token's first head of the group. Rows from `valid` on, and columns from dim on, are zero.
+  __device__ __forceinline__ void operator()(const AttnArgs& a, char* lds, const T* base, int g0, int valid) const {
+    typedef __attribute__((address_space(3))) char* lds_ptr;
+    const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, 0x00027000);
+    const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)lds)) +
+                        __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
+#pragma unroll
+    for (int i = 0; i < ROWS / kRowsPerStep; ++i) {
+      const int row = threadIdx.x / L::kChunks + i * kRowsPerStep;
+      const int c = ((threadIdx.x % L::kChunks) ^ L::swizzle(row)) * L::kElemsPerChunk;
+      const uint32_t n = g0 + row, t = (n * a.group_magic) >> 20;
+      const uint32_t at = t * static_cast<uint32_t>(token_stride) +
+                          (n - t * a.group) * static_cast<uint32_t>(head_stride) + c;
+      const uint32_t from = row < valid && c < a.dim ? at * static_cast<uint32_t>(sizeof(T)) : kNowhere;
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "s"(to + i * (THREADS * 16)), "v"(from), "s"(src) : "memory");
+    }
+  }
+};
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // Four consecutive accumulator rows of one column, rounded to nearest and stored.
@@ -219,27 +277,6 @@ __device__ __forceinline__ float tanh_of(float x) {
   else
     return tanhf(x);
 }
-
-struct AttnArgs {
-  const void *q, *k, *v;
-  void* out;
-  float* lse;
-  const int32_t *q_offsets, *k_offsets, *k_lengths, *prefix;
-  int64_t q_tokens, k_tokens;
-  int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // strides in elements
-  int docs, heads, kv_heads, group, dim, causal;
-  float softcap, scale;
-  // backward
-  const void* d_out;
-  void *d_q, *d_k, *d_v;
-  float* delta;
-  int n_tiles;
-  // keys of a row tile cut into up to `splits` pieces of at least split_keys, joined by a second launch
-  int splits, split_keys;
-  float* part;        // [splits][q_tokens][heads][dim], unnormalised
-  float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
-  int32_t* part_n;    // [q_tokens][heads] pieces
-};
 
 // The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one).
 struct Piece {
