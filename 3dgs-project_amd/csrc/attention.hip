@@ -383,61 +383,92 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
   if (lane == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-// Score gradient of one (query, key): p = e^(s - lse), ds = p (dp - delta) ds/ds_raw.
-template <typename T, int MODE>
-__device__ __forceinline__ void score_grad(const Rule& u, float s, float dp, float lse2, float delta, float* p,
-                                           float* ds) {
-  if constexpr (MODE == kPlain) {
-    *p = exp2_hw(fmaf(s, u.scale2, -lse2));
-    *ds = *p * (dp - delta);
-  } else {
-    const float t = tanh_of<T>(s * u.in_scale);
-    *p = exp2_hw(fmaf(u.cap2, t, -lse2));
-    *ds = *p * fmaf(-t, t, 1.0f) * (dp - delta);
+// Lays out the instructions since the last keep_order as M times one matrix instruction and V vector
+// ones, after N LDS reads: the vector work then runs in the products' shadow within one wavefront.
+template <int N, int M, int V>
+__device__ __forceinline__ void interleave() {
+  if constexpr (N > 0) __builtin_amdgcn_sched_group_barrier(0x100, N, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // matrix
+    __builtin_amdgcn_sched_group_barrier(0x2, V, 0);  // vector
   }
 }
 
-// S and dP of 32 rows of a pair of tiles against a lane's column, the rows' fragments read first.
+// The fragments of 32 rows of a tile, along (rows) and across (cols).
 template <typename T, int DP>
-__device__ __forceinline__ void two_products(const char* la, const char* lb, int row0, int lane,
-                                             const Frag<T> (&a)[DP / 16], const Frag<T> (&b)[DP / 16], f32x16& s,
-                                             f32x16& dp) {
-  using L = Tile<T, DP>;
-  constexpr int C = DP / 16;
-  Frag<T> x[C], y[C];
+struct Rows {
+  Frag<T> f[DP / 16];
+  __device__ __forceinline__ void read(const char* lds, int row0, int lane) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) x[c] = L::rows(la, row0, c, lane);
+    for (int c = 0; c < DP / 16; ++c) f[c] = Tile<T, DP>::rows(lds, row0, c, lane);
+  }
+  __device__ __forceinline__ void times(const Frag<T> (&b)[DP / 16], f32x16& acc) const {
+    acc = f32x16{};
 #pragma unroll
-  for (int c = 0; c < C; ++c) y[c] = L::rows(lb, row0, c, lane);
-  s = dp = f32x16{};
+    for (int c = 0; c < DP / 16; ++c) mma(acc, f[c], b[c]);
+  }
+};
+template <typename T, int DP>
+struct Cols {
+  Frag<T> f[2][DP / 32];
+  __device__ __forceinline__ void read(const char* lds, int row0, int lane) {
 #pragma unroll
-  for (int c = 0; c < C; ++c) mma(s, x[c], a[c]);
+    for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
-  for (int c = 0; c < C; ++c) mma(dp, y[c], b[c]);
+      for (int dt = 0; dt < DP / 32; ++dt) f[kc][dt] = Tile<T, DP>::cols(lds, 32 * dt, row0 + 16 * kc, lane);
+  }
+  __device__ __forceinline__ void add_times(const Frag<T> (&p)[2], f32x16 (&acc)[DP / 32]) const {
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) mma(acc[dt], f[kc][dt], p[kc]);
+  }
+};
+template <typename T>
+__device__ __forceinline__ void acc_frags(const f32x16& c, Frag<T> (&f)[2]) {
+  f[0] = acc_frag<T>(c, 0);
+  f[1] = acc_frag<T>(c, 1);
 }
 
-// acc += (tile rows row0 .. row0 + 31, transposed) x p
-template <typename T, int DP>
-__device__ __forceinline__ void add_product(const char* lds, int row0, int lane, const f32x16& p,
-                                            f32x16 (&acc)[DP / 32]) {
-  using L = Tile<T, DP>;
-  Frag<T> x[2][DP / 32];
+// The same products in float32, whose fragments are twice as large: read as they are used.
+template <int DP>
+__device__ __forceinline__ void rows_times(const char* lds, int row0, int lane, const f32x8 (&b)[DP / 16], f32x16& acc) {
+  acc = f32x16{};
 #pragma unroll
-  for (int kc = 0; kc < 2; ++kc)
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) x[kc][dt] = L::cols(lds, 32 * dt, row0 + 16 * kc, lane);
+  for (int c = 0; c < DP / 16; ++c) {
+    mma(acc, Tile<float, DP>::rows(lds, row0, c, lane), b[c]);
+    if (c % 2) __builtin_amdgcn_sched_barrier(0);
+  }
+}
+template <int DP>
+__device__ __forceinline__ void add_cols_times(const char* lds, int row0, int lane, const f32x16& p,
+                                               f32x16 (&acc)[DP / 32]) {
 #pragma unroll
   for (int kc = 0; kc < 2; ++kc) {
-    const Frag<T> f = acc_frag<T>(p, kc);
+    const f32x8 f = acc_frag<float>(p, kc);
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) mma(acc[dt], x[kc][dt], f);
+    for (int dt = 0; dt < DP / 32; ++dt) {
+      mma(acc[dt], Tile<float, DP>::cols(lds, 32 * dt, row0 + 16 * kc, lane), f);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
+}
+
+// Probability of a score, p = e^(s - lse), and (capped) the score's slope 1 - tanh^2. The raw score's
+// gradient is p slope (dp - delta).
+template <typename T, int MODE>
+__device__ __forceinline__ float prob_of(const Rule& u, float s, float lse2, float* slope) {
+  if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.scale2, -lse2));
+  const float t = tanh_of<T>(s * u.in_scale);
+  *slope = fmaf(-t, t, 1.0f);
+  return exp2_hw(fmaf(u.cap2, t, -lse2));
 }
 
 // Query gradients, and delta_i = dO_i . O_i for the key gradients. Like the forward, a lane owns a
 // query; its score gradients are the B operand of dQ = dS K.
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
   constexpr int kTileBytes = kAttnKeys * L::kRowBytes;
@@ -498,31 +529,46 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
     copies_done();
     __syncthreads();
     if (k0 + kAttnKeys < end) fetch(k0 + kAttnKeys, lds + (buf ^ 1) * 2 * kTileBytes);
-    const auto grads = [&](f32x16& s, f32x16& dp, int sub, auto masked) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float p, ds;
-        score_grad<T, MODE>(rule, s[r], dp[r], lse2, delta, &p, &ds);
-        if (masked.value && k0 + 32 * sub + 8 * (r / 4) + 4 * h + r % 4 >= vis) ds = 0.0f;
-        s[r] = ds;
-      }
-    };
     const auto body = [&](auto masked) {
-      f32x16 s[2], dp[2];
-      if constexpr (sizeof(T) == 2) {
-        // the second half's products beside the first half's exponentials
-        two_products<T, DP>(lk, lv, 0, lane, q, g, s[0], dp[0]);
-        two_products<T, DP>(lk, lv, 32, lane, q, g, s[1], dp[1]);
-        grads(s[0], dp[0], 0, masked);
-        add_product<T, DP>(lk, 0, lane, s[0], dq);
-        grads(s[1], dp[1], 1, masked);
-        add_product<T, DP>(lk, 32, lane, s[1], dq);
-      } else {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          two_products<T, DP>(lk, lv, 32 * t, lane, q, g, s[t], dp[t]);
-          grads(s[t], dp[t], t, masked);
-          add_product<T, DP>(lk, 32 * t, lane, s[t], dq);
+      for (int t = 0; t < 2; ++t) {
+        f32x16 s, dp;
+        const auto probs = [&] {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float slope = 1.0f;
+            s[r] = prob_of<T, MODE>(rule, s[r], lse2, &slope);
+            if constexpr (MODE != kPlain) s[r] *= slope;
+            if (masked.value && k0 + 32 * t + 8 * (r / 4) + 4 * h + r % 4 >= vis) s[r] = 0.0f;
+          }
+        };
+        const auto grads = [&] {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+        };
+        if constexpr (sizeof(T) == 2) {
+          Rows<T, DP> x, y;
+          Cols<T, DP> z;
+          Frag<T> f[2];
+          x.read(lk, 32 * t, lane);
+          y.read(lv, 32 * t, lane);
+          x.times(q, s);
+          keep_order<T>();
+          y.times(g, dp);
+          probs();
+          interleave<0, C, MODE == kPlain ? 6 : 12>();
+          keep_order<T>();
+          z.read(lk, 32 * t, lane);
+          grads();
+          acc_frags<T>(s, f);
+          z.add_times(f, dq);
+          keep_order<T>();
+        } else {
+          rows_times<DP>(lk, 32 * t, lane, q, s);
+          rows_times<DP>(lv, 32 * t, lane, g, dp);
+          probs();
+          grads();
+          add_cols_times<DP>(lk, 32 * t, lane, s, dq);
         }
       }
     };
@@ -545,15 +591,32 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_q_kernel(AttnArgs a) {
 // Key and value gradients: a lane owns one key, the workgroup walks over the query rows that see it,
 // 64 at a time. Rows past the document's end need no mask: their q, dO, lse and delta are zero, and so
 // is what they add. The lanes of keys past the valid length gather nothing that is kept.
-template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
+//
+// At 128 elements of bfloat16 both gradients' accumulators (128 registers beside K and V's 64) leave no
+// room for a second wavefront on the SIMD, and the compiler then moves operands between the register
+// files. There, workgroups with blockIdx.y = 0 gather dK (three products) and the others dV (S again, two
+// products): five products for four, but two wavefronts a SIMD that fill each other's gaps. Measured at
+// 8192 tokens, 16 heads of 128: 1663 us together, KVSPLIT us apart. Smaller heads keep both in one.
+template <typename T, int DP>
+constexpr bool kSplitKv = sizeof(T) == 2 && DP == 128;
+
+constexpr int kKvRows = 64;  // query rows of a tile
+template <typename T, int DP>
+struct KvShared {
+  char tiles[4 * kKvRows * Tile<T, DP>::kRowBytes];
+  float lse[2][kKvRows], delta[2][kKvRows];
+  int vis[2][kKvRows];
+};
+
+template <typename T, int DP, int MODE, bool DK, bool DV>
+__device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& sh) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
-  constexpr int R = 64;
+  constexpr int R = kKvRows;
   constexpr int kTileBytes = R * L::kRowBytes;
-  __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
-  __shared__ __attribute__((aligned(16))) float l_lse[2][R], l_delta[2][R];
-  __shared__ __attribute__((aligned(16))) int l_vis[2][R];
+  char* lds = sh.tiles;
+  const auto &l_lse = sh.lse, &l_delta = sh.delta;
+  const auto& l_vis = sh.vis;
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = blockIdx.x / a.kv_heads;
   int64_t first;
@@ -597,9 +660,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
   };
   const auto keep = [&](int b) {
     if (threadIdx.x < R) {
-      l_lse[b][threadIdx.x] = n_lse == -INFINITY ? 0.0f : n_lse * kLog2e;
-      l_delta[b][threadIdx.x] = n_delta;
-      l_vis[b][threadIdx.x] = n_vis;
+      sh.lse[b][threadIdx.x] = n_lse == -INFINITY ? 0.0f : n_lse * kLog2e;
+      sh.delta[b][threadIdx.x] = n_delta;
+      sh.vis[b][threadIdx.x] = n_vis;
     }
   };
   if (row_begin < rows) fetch(row_begin, lds);
@@ -611,7 +674,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
     const bool in = live && 16 * c + 8 * h < a.dim;
     k[c] = load_frag<T>(kp + 16 * c + 8 * h, in);
     if (a.scale < 0.0f) k[c] = -k[c];
-    v[c] = load_frag<T>(vp + 16 * c + 8 * h, in);
+    if constexpr (DK) v[c] = load_frag<T>(vp + 16 * c + 8 * h, in);
   }
   const Rule rule = rule_of<MODE>(a);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
@@ -625,41 +688,75 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
     // every row of the tile sees all of this wavefront's keys?
     const bool mask = a.causal && __builtin_amdgcn_readfirstlane(l_vis[buf][0]) < wkey + 32;
     if (r0 + R < rows) fetch(r0 + R, lds + (buf ^ 1) * 2 * kTileBytes);
-    const auto grads = [&](f32x16& s, f32x16& dp, int sub, auto masked) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = 32 * sub + 8 * i + 4 * h;
-        const f32x4 lse2 = *reinterpret_cast<const f32x4*>(&l_lse[buf][at]);
-        const f32x4 delta = *reinterpret_cast<const f32x4*>(&l_delta[buf][at]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 4 * i + j;
-          float p, ds;
-          score_grad<T, MODE>(rule, s[r], dp[r], lse2[j], delta[j], &p, &ds);
-          if (masked.value && key >= l_vis[buf][at + j]) p = ds = 0.0f;
-          s[r] = p;
-          dp[r] = ds;
-        }
-      }
-    };
     const auto body = [&](auto masked) {
-      f32x16 s[2], dp[2];
-      if constexpr (sizeof(T) == 2) {
-        two_products<T, DP>(lq, lg, 0, lane, k, v, s[0], dp[0]);
-        two_products<T, DP>(lq, lg, 32, lane, k, v, s[1], dp[1]);
-        grads(s[0], dp[0], 0, masked);
-        add_product<T, DP>(lg, 0, lane, s[0], dv);
-        add_product<T, DP>(lq, 0, lane, dp[0], dk);
-        grads(s[1], dp[1], 1, masked);
-        add_product<T, DP>(lg, 32, lane, s[1], dv);
-        add_product<T, DP>(lq, 32, lane, dp[1], dk);
-      } else {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          two_products<T, DP>(lq, lg, 32 * t, lane, k, v, s[t], dp[t]);
-          grads(s[t], dp[t], t, masked);
-          add_product<T, DP>(lg, 32 * t, lane, s[t], dv);
-          add_product<T, DP>(lq, 32 * t, lane, dp[t], dk);
+      for (int t = 0; t < 2; ++t) {
+        f32x16 s, dp, sl;
+        const auto probs = [&] {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = 32 * t + 8 * i + 4 * h;
+            const f32x4 lse2 = *reinterpret_cast<const f32x4*>(&l_lse[buf][at]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int r = 4 * i + j;
+              float slope = 1.0f;
+              s[r] = prob_of<T, MODE>(rule, s[r], lse2[j], &slope);
+              if constexpr (MODE != kPlain && DV) sl[r] = slope;
+              if constexpr (MODE != kPlain && !DV) s[r] *= slope;
+              if (masked.value && key >= l_vis[buf][at + j]) s[r] = 0.0f;
+            }
+          }
+        };
+        const auto grads = [&] {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 delta = *reinterpret_cast<const f32x4*>(&l_delta[buf][32 * t + 8 * i + 4 * h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int r = 4 * i + j;
+              dp[r] = s[r] * (dp[r] - delta[j]);
+              if constexpr (MODE != kPlain && DV) dp[r] *= sl[r];
+            }
+          }
+        };
+        if constexpr (sizeof(T) == 2) {
+          // products of C matrix instructions; the probabilities are formed in the second's shadow, the
+          // score gradients in the third's, and an operand is read during the product before its own
+          Rows<T, DP> x, y;
+          Cols<T, DP> zg, zq;
+          Frag<T> f[2], e[2];
+          x.read(lq, 32 * t, lane);
+          if constexpr (DK && DV) y.read(lg, 32 * t, lane);
+          x.times(k, s);
+          if constexpr (DV) zg.read(lg, 32 * t, lane);
+          keep_order<T>();
+          if constexpr (DK && !DV) y.read(lg, 32 * t, lane);
+          if constexpr (DK) y.times(v, dp);
+          probs();
+          if constexpr (DV) acc_frags<T>(s, f);
+          if constexpr (DK && DV) zq.read(lq, 32 * t, lane);
+          if constexpr (DK) interleave<0, C, MODE == kPlain ? 7 : 13>();
+          keep_order<T>();
+          if constexpr (DK && !DV) zq.read(lq, 32 * t, lane);
+          if constexpr (DV) zg.add_times(f, dv);
+          if constexpr (DK) {
+            grads();
+            acc_frags<T>(dp, e);
+            if constexpr (DV) {
+              interleave<0, C, MODE == kPlain ? 5 : 7>();
+              keep_order<T>();
+            }
+            zq.add_times(e, dk);
+          }
+          keep_order<T>();
+        } else {
+          rows_times<DP>(lq, 32 * t, lane, k, s);
+          rows_times<DP>(lg, 32 * t, lane, v, dp);
+          probs();
+          grads();
+          add_cols_times<DP>(lg, 32 * t, lane, s, dv);
+          add_cols_times<DP>(lq, 32 * t, lane, dp, dk);
         }
       }
     };
@@ -681,9 +778,17 @@ __global__ __launch_bounds__(kAttnThreads) void attn_bwd_kv_kernel(AttnArgs a) {
         x = f32x4{dk[dt][r], dk[dt][r + 1], dk[dt][r + 2], dk[dt][r + 3]} * a.scale;
         y = f32x4{dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]};
       }
-      store4(dkp + d, x[0], x[1], x[2], x[3]);
-      store4(dvp + d, y[0], y[1], y[2], y[3]);
+      if constexpr (DK) store4(dkp + d, x[0], x[1], x[2], x[3]);
+      if constexpr (DV) store4(dvp + d, y[0], y[1], y[2], y[3]);
     }
+}
+
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
+  __shared__ __attribute__((aligned(16))) KvShared<T, DP> sh;
+  if constexpr (!kSplitKv<T, DP>) attn_bwd_kv<T, DP, MODE, true, true>(a, sh);
+  else if (blockIdx.y == 0) attn_bwd_kv<T, DP, MODE, true, false>(a, sh);
+  else attn_bwd_kv<T, DP, MODE, false, true>(a, sh);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -765,8 +870,8 @@ static void launch_mode(const AttnArgs& a, dim3 grid, hipStream_t st) {
   else K<T, DP, kCap>::launch(a, grid, st);
 }
 template <template <typename, int, int> class K>
-static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.splits));
+static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts, hipStream_t st) {
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
   if (dtype == GS_BFLOAT16) {
     if (a.dim > 64) launch_mode<K, __bf16, 128>(a, grid, st);
     else launch_mode<K, __bf16, 64>(a, grid, st);
@@ -852,9 +957,9 @@ extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t w
   a.part_stat = a.part + rows * a.splits * a.dim;
   a.part_n = reinterpret_cast<int32_t*>(a.part_stat + rows * a.splits * 2);
   if (f.few)
-    launch_attn<FewKernel>(a, p->dtype, f.tiles * a.kv_heads, st);
+    launch_attn<FewKernel>(a, p->dtype, f.tiles * a.kv_heads, a.splits, st);
   else
-    launch_attn<FwdKernel>(a, p->dtype, f.tiles * a.kv_heads, st);
+    launch_attn<FwdKernel>(a, p->dtype, f.tiles * a.kv_heads, a.splits, st);
   if (const int rc = check_launch("attention")) return rc;
   if (a.splits == 1) return GS_OK;
   const dim3 grid(static_cast<unsigned>((rows + kAttnWaves - 1) / kAttnWaves)), block(kAttnThreads);
@@ -895,12 +1000,13 @@ extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* 
              "attention: too many tokens, documents or heads");
   if (p->q_tokens > 0) {
     a.n_tiles = static_cast<int>(q_tiles);
-    launch_attn<BwdQKernel>(a, p->dtype, q_tiles * a.kv_heads, st);
+    launch_attn<BwdQKernel>(a, p->dtype, q_tiles * a.kv_heads, 1, st);
     if (const int rc = check_launch("attention backward (queries)")) return rc;
   }
   if (p->k_tokens > 0) {
     a.n_tiles = static_cast<int>(k_tiles);
-    launch_attn<BwdKvKernel>(a, p->dtype, k_tiles * a.kv_heads, st);
+    launch_attn<BwdKvKernel>(a, p->dtype, k_tiles * a.kv_heads,
+                             p->dtype == GS_BFLOAT16 && kSplitKv<__bf16, 128> && a.dim > 64 ? 2 : 1, st);
     return check_launch("attention backward (keys)");
   }
   return GS_OK;

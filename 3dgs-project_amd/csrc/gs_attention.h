@@ -151,6 +151,16 @@ struct AttnArgs {
   int32_t* part_n;    // [q_tokens][heads] pieces
 };
 
+// A value that is the same in every lane, as a scalar (the compiler cannot always tell).
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename T>
+__device__ __forceinline__ T* uniform(T* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<T*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // Rows [0, rows) of a strided matrix as a buffer: loads beyond the last row, and at kNowhere, give
 // zero. Its base is set per tile, so that offsets stay within 32 bits however long the matrix is
 // (token strides are below 2^22 elements, tiles have at most 64 rows: 2^30 bytes, so kNowhere is
@@ -159,7 +169,7 @@ constexpr uint32_t kNowhere = 0x80000000u;
 template <typename T>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* base, int64_t stride, int rows, int dim) {
   const int bytes = rows > 0 ? static_cast<int>(((rows - 1) * stride + dim) * static_cast<int64_t>(sizeof(T))) : 0;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, bytes, 0x00027000);
+  return __builtin_amdgcn_make_buffer_rsrc(uniform(const_cast<T*>(base)), 0, uniform(bytes), 0x00027000);
 }
 __device__ __forceinline__ f32x4 load16(__amdgpu_buffer_rsrc_t b, uint32_t offset) {
   using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
@@ -221,7 +231,7 @@ struct RowTileCopy {
   // base: the first token's first head of the group. Rows from `valid` on, and columns from dim on, are zero.
   __device__ __forceinline__ void operator()(const AttnArgs& a, char* lds, const T* base, int g0, int valid) const {
     typedef __attribute__((address_space(3))) char* lds_ptr;
-    const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, 0x00027000);
+    const auto src = __builtin_amdgcn_make_buffer_rsrc(uniform(const_cast<T*>(base)), 0, 0x7fffffff, 0x00027000);
     const uint32_t to = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)lds)) +
                         __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * (kWave * 16);
 #pragma unroll
