@@ -635,20 +635,29 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
     const int64_t t = key0 - doc.k_len + doc.q_len;
     if (t > 0) start.token = static_cast<int>(t < doc.q_len ? t : doc.q_len);
   }
-  const int row_begin = key0 >= doc.k_len ? rows : start.token * a.group;
+  int row_begin = key0 >= doc.k_len ? rows : start.token * a.group;
+  int row_end = rows;
+  if (a.row_parts > 1) {
+    const int part = blockIdx.z, per = ((rows - row_begin) / a.row_parts + R) / R * R;
+    const int from = min(part * per, rows - row_begin);
+    start.token += from / a.group;
+    start.g = from % a.group;
+    row_begin += from;
+    row_end = min(row_begin + per, rows);
+  }
   const RowTileCopy<T, DP, R, kAttnThreads> copy_q = {a.q_token, a.q_head};
   const RowTileCopy<T, DP, R, kAttnThreads> copy_g = {static_cast<int64_t>(a.heads) * a.dim, a.dim};
   float n_lse = 0.0f, n_delta = 0.0f;
   int n_vis = 0;
   const auto fetch = [&](int r0, char* to) {
     const int64_t token = doc.q0 + start.token;
-    copy_q(a, to, static_cast<const T*>(a.q) + token * a.q_token + hk * a.group * a.q_head, start.g, rows - r0);
+    copy_q(a, to, static_cast<const T*>(a.q) + token * a.q_token + hk * a.group * a.q_head, start.g, row_end - r0);
     copy_g(a, to + kTileBytes, static_cast<const T*>(a.d_out) + (token * a.heads + hk * a.group) * a.dim, start.g,
-           rows - r0);
+           row_end - r0);
     if (threadIdx.x < R) {
       n_lse = n_delta = 0.0f;
       n_vis = 0;
-      if (r0 + static_cast<int>(threadIdx.x) < rows) {
+      if (r0 + static_cast<int>(threadIdx.x) < row_end) {
         const int n = start.g + threadIdx.x, t = static_cast<int>((n * a.group_magic) >> 20);
         const int64_t stat = (token + t) * a.heads + hk * a.group + n - t * a.group;
         n_lse = a.lse[stat];
@@ -665,7 +674,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
       sh.vis[b][threadIdx.x] = n_vis;
     }
   };
-  if (row_begin < rows) fetch(row_begin, lds);
+  if (row_begin < row_end) fetch(row_begin, lds);
   Frag<T> k[C], v[C];
   const T* kp = static_cast<const T*>(a.k) + (doc.k0 + key) * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + (doc.k0 + key) * a.v_token + hk * a.v_head;
@@ -679,7 +688,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
   const Rule rule = rule_of<MODE>(a);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   int buf = 0;
-  for (int r0 = row_begin; r0 < rows; r0 += R, buf ^= 1) {
+  for (int r0 = row_begin; r0 < row_end; r0 += R, buf ^= 1) {
     const char* lq = lds + buf * 2 * kTileBytes;
     const char* lg = lq + kTileBytes;
     keep(buf);
@@ -687,7 +696,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
     __syncthreads();
     // every row of the tile sees all of this wavefront's keys?
     const bool mask = a.causal && __builtin_amdgcn_readfirstlane(l_vis[buf][0]) < wkey + 32;
-    if (r0 + R < rows) fetch(r0 + R, lds + (buf ^ 1) * 2 * kTileBytes);
+    if (r0 + R < row_end) fetch(r0 + R, lds + (buf ^ 1) * 2 * kTileBytes);
     const auto body = [&](auto masked) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -778,6 +787,13 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
         x = f32x4{dk[dt][r], dk[dt][r + 1], dk[dt][r + 2], dk[dt][r + 3]} * a.scale;
         y = f32x4{dv[dt][r], dv[dt][r + 1], dv[dt][r + 2], dv[dt][r + 3]};
       }
+      if (a.row_parts > 1) {
+        const int64_t all = a.k_tokens * a.kv_heads * a.dim;
+        float* to = a.part_kv + blockIdx.z * all + at + d;
+        if constexpr (DK) *reinterpret_cast<f32x4*>(to) = x;
+        if constexpr (DV) *reinterpret_cast<f32x4*>(to + a.row_parts * all) = y;
+        continue;
+      }
       if constexpr (DK) store4(dkp + d, x[0], x[1], x[2], x[3]);
       if constexpr (DV) store4(dvp + d, y[0], y[1], y[2], y[3]);
     }
@@ -789,6 +805,18 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   if constexpr (!kSplitKv<T, DP>) attn_bwd_kv<T, DP, MODE, true, true>(a, sh);
   else if (blockIdx.y == 0) attn_bwd_kv<T, DP, MODE, true, false>(a, sh);
   else attn_bwd_kv<T, DP, MODE, false, true>(a, sh);
+}
+
+// Adds the row parts' gradients, in order, four elements a thread: blockIdx.y 0 dK, 1 dV.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_kv_join_kernel(AttnArgs a) {
+  const int64_t all = a.k_tokens * a.kv_heads * a.dim;
+  const int64_t e = (static_cast<int64_t>(blockIdx.x) * kAttnThreads + threadIdx.x) * 4;
+  if (e >= all) return;
+  const float* from = a.part_kv + blockIdx.y * a.row_parts * all + e;
+  f32x4 x = *reinterpret_cast<const f32x4*>(from);
+  for (int i = 1; i < a.row_parts; ++i) x += *reinterpret_cast<const f32x4*>(from + i * all);
+  store4(static_cast<T*>(blockIdx.y ? a.d_v : a.d_k) + e, x[0], x[1], x[2], x[3]);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -857,6 +885,7 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
   a.softcap = p->softcap;
   a.scale = p->scale;
   a.splits = 1;
+  a.row_parts = 1;
   return GS_OK;
 }
 
@@ -871,7 +900,7 @@ static void launch_mode(const AttnArgs& a, dim3 grid, hipStream_t st) {
 }
 template <template <typename, int, int> class K>
 static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts, hipStream_t st) {
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts));
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts), static_cast<unsigned>(a.row_parts));
   if (dtype == GS_BFLOAT16) {
     if (a.dim > 64) launch_mode<K, __bf16, 128>(a, grid, st);
     else launch_mode<K, __bf16, 64>(a, grid, st);
@@ -970,10 +999,40 @@ extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t w
   return check_launch("attention (join)");
 }
 
+namespace gs {
+
+// How a backward call is laid out. A key tile's workgroup walks over every row that sees it, times the
+// heads of its group: with few key heads that is one long chain on a part of the chip. The rows are then
+// cut into parts, until the longest chain is about half of what each of the chip's 512 workgroups has to
+// do on average (a causal tile has half the rows on average); the parts' sums are joined in float32.
+// Measured at 9001 causal tokens, 16 heads on 4 of 128: ROWPARTS.
+struct BwdPlan {
+  int64_t q_tiles, k_tiles;
+  int kv_roles, row_parts;
+  size_t delta, part;  // workspace floats
+};
+static BwdPlan plan_bwd(const AttnArgs& a, int dtype) {
+  BwdPlan b;
+  b.q_tiles = tiles_of(a.q_tokens, a.group, kAttnRows, a.docs);
+  b.k_tiles = tiles_of(a.k_tokens, 1, kAttnRows, a.docs);
+  b.kv_roles = dtype == GS_BFLOAT16 && kSplitKv<__bf16, 128> && a.dim > 64 ? 2 : 1;
+  const int64_t blocks = (a.k_tokens + kAttnRows - 1) / kAttnRows * a.kv_heads * b.kv_roles;
+  const int64_t rows = a.q_tokens * a.group / a.docs;
+  const int64_t want = blocks > 0 ? (a.causal ? 4 : 2) * 512 / blocks : 1;
+  b.row_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, rows / 512, 8})));
+  b.delta = (static_cast<size_t>(a.q_tokens) * a.heads + 3) / 4 * 4;
+  b.part = b.row_parts > 1 ? 2 * static_cast<size_t>(b.row_parts) * a.k_tokens * a.kv_heads * a.dim : 0;
+  return b;
+}
+
+}  // namespace gs
+
 extern "C" size_t gs_attention_bwd_workspace_size(const gs_attention* p) {
   clear_error();
-  if (p == nullptr || p->q_tokens <= 0 || p->heads <= 0) return 0;
-  return static_cast<size_t>(p->q_tokens) * p->heads * sizeof(float);
+  AttnArgs a;
+  if (attn_setup(p, a)) return 0;
+  const BwdPlan b = plan_bwd(a, p->dtype);
+  return (b.delta + b.part) * sizeof(float);
 }
 
 extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* d_q, void* d_k, void* d_v,
@@ -985,29 +1044,39 @@ extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* 
              "attention backward: null pointer");
   GS_REQUIRE(aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16), GS_ERR_ALIGN,
              "attention backward: tensors must be 16-byte aligned");
-  GS_REQUIRE(workspace_bytes >= gs_attention_bwd_workspace_size(p) && (workspace || p->q_tokens == 0),
-             GS_ERR_WORKSPACE, "attention backward: workspace too small");
-  GS_REQUIRE(aligned(workspace, 4), GS_ERR_ALIGN, "attention backward: workspace must be 4-byte aligned");
+  const BwdPlan b = plan_bwd(a, p->dtype);
+  const size_t need = (b.delta + b.part) * sizeof(float);
+  GS_REQUIRE(workspace_bytes >= need && (workspace || need == 0), GS_ERR_WORKSPACE,
+             "attention backward: workspace too small");
+  GS_REQUIRE(aligned(workspace, 16), GS_ERR_ALIGN, "attention backward: workspace must be 16-byte aligned");
+  GS_REQUIRE(b.q_tiles * a.kv_heads < (int64_t(1) << 31) && b.k_tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG,
+             "attention: too many tokens, documents or heads");
   a.d_out = d_out;
   a.d_q = d_q;
   a.d_k = d_k;
   a.d_v = d_v;
   a.delta = static_cast<float*>(workspace);
+  a.part_kv = a.delta + b.delta;
   const hipStream_t st = as_stream(stream);
-  const int64_t q_tiles = tiles_of(a.q_tokens, a.group, kAttnRows, a.docs);
-  const int64_t k_tiles = tiles_of(a.k_tokens, 1, kAttnRows, a.docs);
-  GS_REQUIRE(q_tiles * a.kv_heads < (int64_t(1) << 31) && k_tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG,
-             "attention: too many tokens, documents or heads");
   if (p->q_tokens > 0) {
-    a.n_tiles = static_cast<int>(q_tiles);
-    launch_attn<BwdQKernel>(a, p->dtype, q_tiles * a.kv_heads, 1, st);
+    a.n_tiles = static_cast<int>(b.q_tiles);
+    launch_attn<BwdQKernel>(a, p->dtype, b.q_tiles * a.kv_heads, 1, st);
     if (const int rc = check_launch("attention backward (queries)")) return rc;
   }
   if (p->k_tokens > 0) {
-    a.n_tiles = static_cast<int>(k_tiles);
-    launch_attn<BwdKvKernel>(a, p->dtype, k_tiles * a.kv_heads,
-                             p->dtype == GS_BFLOAT16 && kSplitKv<__bf16, 128> && a.dim > 64 ? 2 : 1, st);
-    return check_launch("attention backward (keys)");
+    a.n_tiles = static_cast<int>(b.k_tiles);
+    a.row_parts = b.row_parts;
+    launch_attn<BwdKvKernel>(a, p->dtype, b.k_tiles * a.kv_heads, b.kv_roles, st);
+    if (const int rc = check_launch("attention backward (keys)")) return rc;
+    if (b.row_parts > 1) {
+      const int64_t quads = a.k_tokens * a.kv_heads * a.dim / 4;
+      const dim3 grid(static_cast<unsigned>((quads + kAttnThreads - 1) / kAttnThreads), 2), block(kAttnThreads);
+      if (p->dtype == GS_BFLOAT16)
+        hipLaunchKernelGGL(attn_kv_join_kernel<__bf16>, grid, block, 0, st, a);
+      else
+        hipLaunchKernelGGL(attn_kv_join_kernel<float>, grid, block, 0, st, a);
+      return check_launch("attention backward (join)");
+    }
   }
   return GS_OK;
 }

@@ -149,6 +149,9 @@ struct AttnArgs {
   float* part;        // [splits][q_tokens][heads][dim], unnormalised
   float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
   int32_t* part_n;    // [q_tokens][heads] pieces
+  // backward: query rows of a key tile cut into `row_parts`, each part's dK and dV in float32
+  int row_parts;
+  float* part_kv;     // [dK, dV][row_parts][k_tokens][kv_heads][dim]
 };
 
 // A value that is the same in every lane, as a scalar (the compiler cannot always tell).

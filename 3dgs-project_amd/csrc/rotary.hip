@@ -3,6 +3,8 @@
 // The gradient is the same with the angle negated.
 #include <float.h>
 
+#include <algorithm>
+
 #include "gs_host.h"
 
 namespace gs {
@@ -19,6 +21,7 @@ struct RotaryArgs {
   const float* positions;
   int64_t tokens;
   int axes, pairs, dim, adjacent;
+  int tokens_per_block;
   int section_end[GS_ROTARY_MAX_AXES];
   float sign;
   // frequency in turns, as the sum of two floats
@@ -26,44 +29,89 @@ struct RotaryArgs {
 };
 
 constexpr int kRotaryThreads = 256;
+constexpr int kRotaryTable = 1024;  // (token, pair) angles of a workgroup
 
 // cos and sin of 2 pi pos f. The product is formed to about 48 bits and reduced to a turn before
 // anything is rounded, so the angle's error does not grow with the position.
-__device__ __forceinline__ void turn(float pos, float hi, float lo, float* c, float* s) {
+__device__ __forceinline__ float2 turn(float pos, float hi, float lo) {
   const float ph = pos * hi;
   const float pl = fmaf(pos, lo, fmaf(pos, hi, -ph));
   const float f = (ph - rintf(ph)) + pl;
-  sincospif(2.0f * f, s, c);
+  float2 r;
+  sincospif(2.0f * f, &r.y, &r.x);
+  return r;
 }
 
-template <typename T>
+// HBM-bound: every element is read and written once, in vectors of V. A workgroup takes a few tokens:
+// it forms their angles' cos and sin once, in LDS, for all heads of both tensors (a sincos costs as much
+// as moving some 30 elements), then its threads run over (token, head, V pairs), neighbours in memory
+// next to each other. V is 16 bytes' worth where the pairs, the copied rest, the strides and the
+// addresses are multiples of it, else one element: REALROTARY.
+template <typename T, int V>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
-  const int per_head = a.dim - a.pairs;  // pairs, then copied elements
-  const int heads = a.x[0].heads + a.x[1].heads;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * kRotaryThreads + threadIdx.x;
-  if (e >= a.tokens * heads * per_head) return;
-  const int p = static_cast<int>(e % per_head);
-  const int64_t th = e / per_head;
-  int head = static_cast<int>(th % heads);
-  const int64_t token = th / heads;
-  const int which = head >= a.x[0].heads;
-  head -= which ? a.x[0].heads : 0;
-  const RotaryTensor& x = a.x[which];
-  const T* in = static_cast<const T*>(x.in) + token * x.token_stride + head * x.head_stride;
-  T* out = static_cast<T*>(x.out) + (token * x.heads + head) * a.dim;
-  if (p >= a.pairs) {
-    out[p + a.pairs] = in[p + a.pairs];
-    return;
+  using Vec = T __attribute__((ext_vector_type(V)));
+  __shared__ float2 table[kRotaryTable];
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block;
+  const int n_tokens = static_cast<int>(min<int64_t>(a.tokens_per_block, a.tokens - token0));
+  for (int e = threadIdx.x; e < n_tokens * a.pairs; e += kRotaryThreads) {
+    const int t = e / a.pairs, p = e - t * a.pairs;
+    int axis = 0;
+    while (axis + 1 < a.axes && p >= a.section_end[axis]) ++axis;
+    float2 cs = turn(a.positions[(token0 + t) * a.axes + axis], a.freq_hi[p], a.freq_lo[p]);
+    cs.y *= a.sign;
+    table[e] = cs;
   }
-  int axis = 0;
-  while (axis + 1 < a.axes && p >= a.section_end[axis]) ++axis;
-  float c, s;
-  turn(a.positions[token * a.axes + axis], a.freq_hi[p], a.freq_lo[p], &c, &s);
-  s *= a.sign;
-  const int i = a.adjacent ? 2 * p : p, j = a.adjacent ? 2 * p + 1 : p + a.pairs;
-  const float u = static_cast<float>(in[i]), w = static_cast<float>(in[j]);
-  out[i] = static_cast<T>(fmaf(u, c, -(w * s)));
-  out[j] = static_cast<T>(fmaf(u, s, w * c));
+  __syncthreads();
+  const int turns = a.pairs / V, per_head = turns + (a.dim - 2 * a.pairs) / V;
+  const int heads = a.x[0].heads + a.x[1].heads;
+  const int per_token = heads * per_head;
+  for (int e = threadIdx.x; e < n_tokens * per_token; e += kRotaryThreads) {
+    const int t = e / per_token, th = e - t * per_token;
+    int head = th / per_head;
+    const int c = th - head * per_head;
+    const int which = head >= a.x[0].heads;
+    head -= which ? a.x[0].heads : 0;
+    const RotaryTensor& x = a.x[which];
+    const int64_t token = token0 + t;
+    const T* in = static_cast<const T*>(x.in) + token * x.token_stride + head * x.head_stride;
+    T* out = static_cast<T*>(x.out) + (token * x.heads + head) * a.dim;
+    if (c >= turns) {
+      const int i = 2 * a.pairs + (c - turns) * V;
+      *reinterpret_cast<Vec*>(out + i) = *reinterpret_cast<const Vec*>(in + i);
+      continue;
+    }
+    const int p = c * V;
+    const int i = a.adjacent ? 2 * p : p, j = a.adjacent ? 2 * p + V : p + a.pairs;
+    const Vec b0 = *reinterpret_cast<const Vec*>(in + i), b1 = *reinterpret_cast<const Vec*>(in + j);
+    T u[2 * V], y[2 * V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      u[k] = b0[k];
+      u[V + k] = b1[k];
+    }
+    const float2* cs = table + t * a.pairs + p;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float f = static_cast<float>(a.adjacent ? u[2 * k] : u[k]);
+      const float w = static_cast<float>(a.adjacent ? u[2 * k + 1] : u[V + k]);
+      const T f1 = static_cast<T>(fmaf(f, cs[k].x, -(w * cs[k].y))), w1 = static_cast<T>(fmaf(f, cs[k].y, w * cs[k].x));
+      if (a.adjacent) {
+        y[2 * k] = f1;
+        y[2 * k + 1] = w1;
+      } else {
+        y[k] = f1;
+        y[V + k] = w1;
+      }
+    }
+    Vec y0, y1;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      y0[k] = y[k];
+      y1[k] = y[V + k];
+    }
+    *reinterpret_cast<Vec*>(out + i) = y0;
+    *reinterpret_cast<Vec*>(out + j) = y1;
+  }
 }
 
 }  // namespace gs
@@ -114,13 +162,29 @@ extern "C" int gs_rotary_axes(const gs_rotary* p, void* stream) {
       a.freq_hi[i] = static_cast<float>(f);
       a.freq_lo[i] = static_cast<float>(f - a.freq_hi[i]);
     }
-  const int64_t n = p->tokens * (p->q_heads + p->k_heads) * (p->dim - a.pairs);
-  const int64_t blocks = (n + kRotaryThreads - 1) / kRotaryThreads;
-  GS_REQUIRE(blocks < (int64_t(1) << 31), GS_ERR_ARG, "rotary: too many elements");
-  const dim3 grid(static_cast<unsigned>(blocks)), block(kRotaryThreads);
-  if (p->dtype == GS_BFLOAT16)
-    hipLaunchKernelGGL(rotary_kernel<__bf16>, grid, block, 0, as_stream(stream), a);
-  else
-    hipLaunchKernelGGL(rotary_kernel<float>, grid, block, 0, as_stream(stream), a);
+  const auto fits = [&](int v) {
+    bool ok = a.pairs % v == 0 && p->dim % v == 0;
+    for (const RotaryTensor& x : a.x)
+      ok = ok && (x.heads == 0 || (x.token_stride % v == 0 && x.head_stride % v == 0 && aligned(x.in, v * es) &&
+                                   aligned(x.out, v * es)));
+    return ok;
+  };
+  const int v = fits(static_cast<int>(16 / es)) ? static_cast<int>(16 / es) : 1;
+  // Tokens of a workgroup: eight items a thread, if that leaves workgroups for the whole chip.
+  const int64_t items = static_cast<int64_t>(p->q_heads + p->k_heads) * ((p->dim - a.pairs) / v);
+  GS_REQUIRE(items < (1 << 26), GS_ERR_ARG, "rotary: too many heads");
+  int64_t per = (8 * kRotaryThreads + items - 1) / items;
+  per = std::min<int64_t>({per, kRotaryTable / a.pairs, (p->tokens + 1023) / 1024});
+  a.tokens_per_block = static_cast<int>(std::max<int64_t>(1, per));
+  const dim3 grid(static_cast<unsigned>((p->tokens + a.tokens_per_block - 1) / a.tokens_per_block));
+  const dim3 block(kRotaryThreads);
+  const hipStream_t st = as_stream(stream);
+  if (p->dtype == GS_BFLOAT16) {
+    if (v == 8) hipLaunchKernelGGL((rotary_kernel<__bf16, 8>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rotary_kernel<__bf16, 1>), grid, block, 0, st, a);
+  } else {
+    if (v == 4) hipLaunchKernelGGL((rotary_kernel<float, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((rotary_kernel<float, 1>), grid, block, 0, st, a);
+  }
   return check_launch("rotary");
 }
