@@ -42,6 +42,13 @@ __device__ __forceinline__ float2 turn(float pos, float hi, float lo) {
   return r;
 }
 
+template <typename T>
+__device__ __forceinline__ void rotate(T u, T w, float2 cs, T* u1, T* w1) {
+  const float f = static_cast<float>(u), g = static_cast<float>(w);
+  *u1 = static_cast<T>(fmaf(f, cs.x, -(g * cs.y)));
+  *w1 = static_cast<T>(fmaf(f, cs.y, g * cs.x));
+}
+
 // HBM-bound: every element is read and written once, in vectors of V. A workgroup takes a few tokens:
 // it forms their angles' cos and sin once, in LDS, for all heads of both tensors (a sincos costs as much
 // as moving some 30 elements), then its threads run over (token, head, V pairs), neighbours in memory
@@ -65,52 +72,65 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   const int turns = a.pairs / V, per_head = turns + (a.dim - 2 * a.pairs) / V;
   const int heads = a.x[0].heads + a.x[1].heads;
   const int per_token = heads * per_head;
-  for (int e = threadIdx.x; e < n_tokens * per_token; e += kRotaryThreads) {
-    const int t = e / per_token, th = e - t * per_token;
-    int head = th / per_head;
-    const int c = th - head * per_head;
-    const int which = head >= a.x[0].heads;
-    head -= which ? a.x[0].heads : 0;
-    const RotaryTensor& x = a.x[which];
-    const int64_t token = token0 + t;
-    const T* in = static_cast<const T*>(x.in) + token * x.token_stride + head * x.head_stride;
-    T* out = static_cast<T*>(x.out) + (token * x.heads + head) * a.dim;
-    if (c >= turns) {
-      const int i = 2 * a.pairs + (c - turns) * V;
-      *reinterpret_cast<Vec*>(out + i) = *reinterpret_cast<const Vec*>(in + i);
-      continue;
-    }
-    const int p = c * V;
-    const int i = a.adjacent ? 2 * p : p, j = a.adjacent ? 2 * p + V : p + a.pairs;
-    const Vec b0 = *reinterpret_cast<const Vec*>(in + i), b1 = *reinterpret_cast<const Vec*>(in + j);
-    T u[2 * V], y[2 * V];
+  // four items of a thread at a time, their loads first
+  constexpr int U = 4;
+  const int n = n_tokens * per_token;
+  for (int e0 = threadIdx.x; e0 < n; e0 += U * kRotaryThreads) {
+    Vec b0[U], b1[U];
+    T* to[U];
+    int at[U];  // first angle, or -1: copied elements
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      u[k] = b0[k];
-      u[V + k] = b1[k];
+    for (int q = 0; q < U; ++q) {
+      const int e = min(e0 + q * kRotaryThreads, n - 1);
+      const int t = e / per_token, th = e - t * per_token;
+      int head = th / per_head;
+      const int c = th - head * per_head;
+      const int which = head >= a.x[0].heads;
+      head -= which ? a.x[0].heads : 0;
+      const RotaryTensor& x = a.x[which];
+      const int64_t token = token0 + t;
+      const int p = c * V, i = c >= turns ? p + a.pairs : a.adjacent ? 2 * p : p;
+      const T* in = static_cast<const T*>(x.in) + token * x.token_stride + head * x.head_stride + i;
+      to[q] = static_cast<T*>(x.out) + (token * x.heads + head) * a.dim + i;
+      at[q] = c >= turns ? -1 : t * a.pairs + p;
+      b0[q] = *reinterpret_cast<const Vec*>(in);
+      b1[q] = c >= turns ? b0[q] : *reinterpret_cast<const Vec*>(in + (a.adjacent ? V : a.pairs));
     }
-    const float2* cs = table + t * a.pairs + p;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float f = static_cast<float>(a.adjacent ? u[2 * k] : u[k]);
-      const float w = static_cast<float>(a.adjacent ? u[2 * k + 1] : u[V + k]);
-      const T f1 = static_cast<T>(fmaf(f, cs[k].x, -(w * cs[k].y))), w1 = static_cast<T>(fmaf(f, cs[k].y, w * cs[k].x));
-      if (a.adjacent) {
-        y[2 * k] = f1;
-        y[2 * k + 1] = w1;
-      } else {
-        y[k] = f1;
-        y[V + k] = w1;
+    for (int q = 0; q < U; ++q) {
+      if (e0 + q * kRotaryThreads >= n) break;
+      if (at[q] < 0) {
+        *reinterpret_cast<Vec*>(to[q]) = b0[q];
+        continue;
       }
-    }
-    Vec y0, y1;
+      const float2* cs = table + at[q];
+      Vec y0, y1;
+      if (a.adjacent) {
+        T u[2 * V], y[2 * V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      y0[k] = y[k];
-      y1[k] = y[V + k];
+        for (int k = 0; k < V; ++k) {
+          u[k] = b0[q][k];
+          u[V + k] = b1[q][k];
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) rotate(u[2 * k], u[2 * k + 1], cs[k], &y[2 * k], &y[2 * k + 1]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          y0[k] = y[k];
+          y1[k] = y[V + k];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          T f, w;
+          rotate(static_cast<T>(b0[q][k]), static_cast<T>(b1[q][k]), cs[k], &f, &w);
+          y0[k] = f;
+          y1[k] = w;
+        }
+      }
+      *reinterpret_cast<Vec*>(to[q]) = y0;
+      *reinterpret_cast<Vec*>(to[q] + (a.adjacent ? V : a.pairs)) = y1;
     }
-    *reinterpret_cast<Vec*>(out + i) = y0;
-    *reinterpret_cast<Vec*>(out + j) = y1;
   }
 }
 
