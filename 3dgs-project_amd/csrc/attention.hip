@@ -173,6 +173,9 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
     for (int dt = 0; dt < DP / 32; ++dt) v[0][dt] = L::cols(lv, 32 * dt, 0, lane);
     keep_order<T>();
     softmax_step<T, MODE>(rule, s, o, st, k0 + kAttnKeys > wave_min, vis - k0, h);
+    // the wavefront that has its probabilities goes first: its products then run while the SIMD's other
+    // wavefront is at its exponentials, and not the two in step (584 -> 561 us at 8192 tokens, 16 heads of 128)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc) {
       if (kc < 3) {
@@ -184,6 +187,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], v[kc & 1][dt], p);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
   if (!live) return;
   const float m = st.m, l = half_sum(st.l);
