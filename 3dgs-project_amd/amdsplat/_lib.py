@@ -100,6 +100,7 @@ class GsAttention(C.Structure):
         ("k", C.c_void_p),
         ("v", C.c_void_p),
         ("out", C.c_void_p),
+        ("out_low", C.c_void_p),
         ("lse", C.c_void_p),
         ("q_offsets", C.c_void_p),
         ("k_offsets", C.c_void_p),

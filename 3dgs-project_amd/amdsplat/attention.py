@@ -33,14 +33,14 @@ def _readable(t: torch.Tensor, group: int = 0) -> torch.Tensor:
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
-def _args(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale) -> _lib.GsAttention:
+def _args(q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale) -> _lib.GsAttention:
     docs = 1 if offsets is None else offsets.numel() - 1
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     if not q.numel():
         qs = (0, 0, 1)
     if not k.numel():
         ks = vs = (0, 0, 1)
-    return _lib.GsAttention(ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(offsets), ptr(k_offsets), ptr(k_lengths),
+    return _lib.GsAttention(ptr(q), ptr(k), ptr(v), ptr(out), ptr(low), ptr(lse), ptr(offsets), ptr(k_offsets), ptr(k_lengths),
                             ptr(prefix), q.shape[0], k.shape[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], docs,
                             q.shape[1], k.shape[1], q.shape[2], _DTYPES[q.dtype][0], int(causal), softcap, scale)
 
@@ -50,10 +50,10 @@ def _workspace(name: str, args, device):
     return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
 
 
-def _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale):
+def _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale, low=None):
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    args = _args(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale)
+    args = _args(q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale)
     ws, n = _workspace("gs_attention_fwd_workspace_size", args, q.device)
     call("gs_attention_fwd", C.byref(args), ptr(ws), n, _lib.stream_handle(q.device))
     return out, lse
@@ -63,8 +63,10 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale):
         q, k, v = _readable(q, q.shape[1] // k.shape[1]), _readable(k), _readable(v)
-        out, lse = _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale)
-        ctx.save_for_backward(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix)
+        # what rounding takes off the output, for the gradient's row sums
+        low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q.dtype == torch.bfloat16 else None
+        out, lse = _forward(q, k, v, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale, low)
+        ctx.save_for_backward(q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix)
         ctx.rule = (causal, softcap, scale)
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -72,12 +74,12 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, _d_lse):
-        q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix = ctx.saved_tensors
+        q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix = ctx.saved_tensors
         d_out = d_out.contiguous()
         if d_out.numel() and d_out.data_ptr() % 16:
             d_out = d_out.clone()
         d_q, d_k, d_v = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        args = _args(q, k, v, out, lse, offsets, k_offsets, k_lengths, prefix, *ctx.rule)
+        args = _args(q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix, *ctx.rule)
         ws, n = _workspace("gs_attention_bwd_workspace_size", args, q.device)
         call("gs_attention_bwd", C.byref(args), ptr(d_out), ptr(d_q), ptr(d_k), ptr(d_v), ptr(ws), n,
              _lib.stream_handle(q.device))

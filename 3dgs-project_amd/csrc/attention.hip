@@ -92,6 +92,16 @@ __device__ __forceinline__ void softmax_step(const Rule& u, f32x16 (&s)[N], f32x
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
+// Four elements of a row of the output and, for a backward pass to come, what rounding took off them.
+template <typename T>
+__device__ __forceinline__ void store_out(const AttnArgs& a, int64_t at, f32x4 x) {
+  store4(static_cast<T*>(a.out) + at, x[0], x[1], x[2], x[3]);
+  if constexpr (sizeof(T) == 2) {
+    if (a.out_low)
+      store4(static_cast<T*>(a.out_low) + at, rounding_of(x[0]), rounding_of(x[1]), rounding_of(x[2]), rounding_of(x[3]));
+  }
+}
+
 // The query's sign takes the scale's, so that scores are scaled by |scale|.
 template <typename T>
 __device__ __forceinline__ Frag<T> load_query(const AttnArgs& a, const T* p, bool valid) {
@@ -115,11 +125,10 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
   __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = a.n_tiles - 1 - static_cast<int64_t>(blockIdx.x / a.kv_heads);
-  int64_t first;
-  const int di = find_stretch(a.q_offsets, a.q_tokens, a.docs, a.group, kAttnRows, tile, &first);
-  const Doc doc = doc_of(a, di);
+  const Found found = find_doc<false>(a, a.group, kAttnRows, tile);
+  const Doc& doc = found.doc;
   const int rows = static_cast<int>(doc.q_len) * a.group;
-  const int64_t base = (tile - first) * kAttnRows;
+  const int64_t base = (tile - found.first) * kAttnRows;
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
   const Piece piece = piece_of(a, visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group), blockIdx.y);
@@ -210,15 +219,16 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
     return;
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  T* op = static_cast<T*>(a.out) + ((doc.q0 + tok) * a.heads + head) * a.dim;
+  const int64_t at = (doc.q0 + tok) * a.heads + head;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * h;
-      if (d < a.dim) store4(op + d, o[dt][r] * inv, o[dt][r + 1] * inv, o[dt][r + 2] * inv, o[dt][r + 3] * inv);
+      if (d >= a.dim) continue;
+      store_out<T>(a, at * a.dim + d, f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]} * inv);
     }
-  if (h == 0) a.lse[(doc.q0 + tok) * a.heads + head] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (h == 0) a.lse[at] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
 // Few query rows (single tokens) against long keys: HBM-bound, so a workgroup's wavefronts each walk
@@ -237,11 +247,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
   __shared__ float l_m[kAttnWaves][32], l_l[kAttnWaves][32];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = static_cast<int64_t>(blockIdx.x / a.kv_heads);
-  int64_t first;
-  const int di = find_stretch(a.q_offsets, a.q_tokens, a.docs, a.group, 32, tile, &first);
-  const Doc doc = doc_of(a, di);
+  const Found found = find_doc<false>(a, a.group, 32, tile);
+  const Doc& doc = found.doc;
   const int rows = static_cast<int>(doc.q_len) * a.group;
-  const int64_t base = (tile - first) * 32;
+  const int64_t base = (tile - found.first) * 32;
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
   const int n_rows = min(32, rows - row0);
@@ -346,44 +355,56 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
       }
     } else {
       const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-      if (d < a.dim) store4(static_cast<T*>(a.out) + at * a.dim + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      if (d < a.dim) store_out<T>(a, at * a.dim + d, x * inv);
       if (d == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
     }
   }
 }
 
-// Joins the pieces of a (token, head), a wavefront each, in order. Rows outside every document have
-// no keys, hence one piece.
+// Joins the pieces of a (token, head), in order: 32 lanes take four elements each, and a piece's
+// statistics each. Rows outside every document have no keys, hence one piece.
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kAttnWaves + threadIdx.x / kWave;
+  constexpr int kLanes = 32;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * kAttnThreads + threadIdx.x) / kLanes;
   const int64_t all = a.q_tokens * a.heads;
   if (at >= all) return;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x % kLanes, d = 4 * lane;
   const int n = a.part_n[at];
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += kWave) top = fmaxf(top, a.part_stat[2 * (i * all + at)]);
+  float top = -INFINITY, sum = 0.0f;
+  f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < n; i0 += kLanes) {
+    const int64_t mine = (i0 + lane) * all + at;
+    const bool in = i0 + lane < n;
+    const float m = in ? a.part_stat[2 * mine] : -INFINITY;
+    const float l = in ? a.part_stat[2 * mine + 1] : 0.0f;
+    float up = fmaxf(top, m);
 #pragma unroll
-  for (int b = 1; b < kWave; b *= 2) top = fmaxf(top, __shfl_xor(top, b));
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, x0 = 0.0f, x1 = 0.0f;
-  const int d = 2 * lane;
-  for (int i = 0; i < n; ++i) {
-    const int64_t part = i * all + at;
-    const float f = exp2_hw(a.part_stat[2 * part] - ref);
-    sum += f * a.part_stat[2 * part + 1];
-    if (d < a.dim) {
-      const float2 v = *reinterpret_cast<const float2*>(a.part + part * a.dim + d);
-      x0 = fmaf(f, v.x, x0);
-      x1 = fmaf(f, v.y, x1);
+    for (int b = 1; b < kLanes; b *= 2) up = fmaxf(up, __shfl_xor(up, b, kLanes));
+    const float ref = up == -INFINITY ? 0.0f : up;
+    const float keep = exp2_hw(top - ref), w = exp2_hw(m - ref);
+    float part = w * l;
+#pragma unroll
+    for (int b = 1; b < kLanes; b *= 2) part += __shfl_xor(part, b, kLanes);
+    sum = sum * keep + part;
+    x *= keep;
+    top = up;
+    const int here = min(kLanes, n - i0);
+    for (int i = 0; i < here; i += 8) {  // eight pieces' loads at a time
+      f32x4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[k] = d < a.dim ? *reinterpret_cast<const f32x4*>(a.part + ((i0 + min(i + k, here - 1)) * all + at) * a.dim + d)
+                         : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float f = __shfl(w, min(i + k, kLanes - 1), kLanes);
+        if (i + k < here) x += f * v[k];
+      }
     }
   }
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  if (d < a.dim) {
-    T* out = static_cast<T*>(a.out) + at * a.dim + d;
-    out[0] = static_cast<T>(x0 * inv);
-    out[1] = static_cast<T>(x1 * inv);
-  }
+  if (d < a.dim) store_out<T>(a, at * a.dim + d, x * inv);
   if (lane == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
@@ -479,11 +500,10 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = a.n_tiles - 1 - static_cast<int64_t>(blockIdx.x / a.kv_heads);
-  int64_t first;
-  const int di = find_stretch(a.q_offsets, a.q_tokens, a.docs, a.group, kAttnRows, tile, &first);
-  const Doc doc = doc_of(a, di);
+  const Found found = find_doc<false>(a, a.group, kAttnRows, tile);
+  const Doc& doc = found.doc;
   const int rows = static_cast<int>(doc.q_len) * a.group;
-  const int64_t base = (tile - first) * kAttnRows;
+  const int64_t base = (tile - found.first) * kAttnRows;
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
   const int end = visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group);
@@ -506,6 +526,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   const int64_t at = ((doc.q0 + tok) * a.heads + head) * a.dim;
   const T* gp = static_cast<const T*>(a.d_out) + at;
   const T* op = static_cast<const T*>(a.out) + at;
+  const T* lp = static_cast<const T*>(a.out_low) + at;
   Frag<T> q[C], g[C];
   float delta = 0.0f;
 #pragma unroll
@@ -514,8 +535,10 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
     q[c] = load_query<T>(a, qp + 16 * c + 8 * h, in);
     g[c] = load_frag<T>(gp + 16 * c + 8 * h, in);
     const Frag<T> o = load_frag<T>(op + 16 * c + 8 * h, in);
+    const Frag<T> low = load_frag<T>(lp + 16 * c + 8 * h, in && a.out_low);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) delta = fmaf(static_cast<float>(g[c][j]), static_cast<float>(o[j]), delta);
+    for (int j = 0; j < 8; ++j)
+      delta = fmaf(static_cast<float>(g[c][j]), static_cast<float>(o[j]) + static_cast<float>(low[j]), delta);
   }
   delta = half_sum(delta);
   const int64_t stat = (doc.q0 + tok) * a.heads + head;
@@ -623,10 +646,9 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
   const auto& l_vis = sh.vis;
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = blockIdx.x / a.kv_heads;
-  int64_t first;
-  const int di = find_stretch(a.k_offsets, a.k_tokens, a.docs, 1, kAttnRows, tile, &first);
-  const Doc doc = doc_of(a, di);
-  const int64_t base = (tile - first) * kAttnRows;
+  const Found found = find_doc<true>(a, 1, kAttnRows, tile);
+  const Doc& doc = found.doc;
+  const int64_t base = (tile - found.first) * kAttnRows;
   if (base >= doc.k_cap) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int key0 = static_cast<int>(base), wkey = key0 + wave * 32;
@@ -860,12 +882,13 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
   GS_REQUIRE((64 / group + 2) * p->q_token_stride + group * p->q_head_stride < (int64_t(1) << 28), GS_ERR_ALIGN,
              "attention: q's strides are too large");
   GS_REQUIRE(aligned(p->q, 16) && aligned(p->k, 16) && aligned(p->v, 16) && aligned(p->out, 16) &&
-                 aligned(p->lse, 4), GS_ERR_ALIGN, "attention: tensors must be 16-byte aligned");
+                 aligned(p->out_low, 16) && aligned(p->lse, 4), GS_ERR_ALIGN, "attention: tensors must be 16-byte aligned");
   a = {};
   a.q = p->q;
   a.k = p->k;
   a.v = p->v;
   a.out = p->out;
+  a.out_low = p->dtype == GS_BFLOAT16 ? p->out_low : nullptr;
   a.lse = p->lse;
   a.q_offsets = p->q_offsets;
   a.k_offsets = p->k_offsets;
@@ -995,7 +1018,7 @@ extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t w
     launch_attn<FwdKernel>(a, p->dtype, f.tiles * a.kv_heads, a.splits, st);
   if (const int rc = check_launch("attention")) return rc;
   if (a.splits == 1) return GS_OK;
-  const dim3 grid(static_cast<unsigned>((rows + kAttnWaves - 1) / kAttnWaves)), block(kAttnThreads);
+  const dim3 grid(static_cast<unsigned>((rows * 32 + kAttnThreads - 1) / kAttnThreads)), block(kAttnThreads);
   if (p->dtype == GS_BFLOAT16)
     hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, block, 0, st, a);
   else
@@ -1023,7 +1046,7 @@ static BwdPlan plan_bwd(const AttnArgs& a, int dtype) {
   const int64_t blocks = (a.k_tokens + kAttnRows - 1) / kAttnRows * a.kv_heads * b.kv_roles;
   const int64_t rows = a.q_tokens * a.group / a.docs;
   const int64_t want = blocks > 0 ? (a.causal ? 4 : 2) * 512 / blocks : 1;
-  b.row_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, rows / 512, 8})));
+  b.row_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, rows / (dtype == GS_BFLOAT16 ? 256 : 128), 8})));
   b.delta = (static_cast<size_t>(a.q_tokens) * a.heads + 3) / 4 * 4;
   b.part = b.row_parts > 1 ? 2 * static_cast<size_t>(b.row_parts) * a.k_tokens * a.kv_heads * a.dim : 0;
   return b;

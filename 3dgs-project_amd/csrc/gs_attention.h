@@ -131,7 +131,7 @@ __device__ __forceinline__ Frag<T> load_frag(const T* p, bool valid) {
 
 struct AttnArgs {
   const void *q, *k, *v;
-  void* out;
+  void *out, *out_low;
   float* lse;
   const int32_t *q_offsets, *k_offsets, *k_lengths, *prefix;
   int64_t q_tokens, k_tokens;
@@ -261,6 +261,9 @@ __device__ __forceinline__ void store4(float* p, float a, float b, float c, floa
   *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d};
 }
 
+// What the rounding to bfloat16 took off, rounded to bfloat16 again: with it a row is known to 2^-17.
+__device__ __forceinline__ float rounding_of(float v) { return v - static_cast<float>(static_cast<__bf16>(v)); }
+
 // v of lane l and of lane l ^ 32, added (or the larger one): the two halves of a query's keys.
 __device__ __forceinline__ float half_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -320,49 +323,73 @@ struct Doc {
   int64_t k_cap;    // tokens of the key stretch
   int64_t k_len;    // of them valid
   int64_t prefix;
-  int64_t tile;     // tile within the document
 };
 
-// The stretch and the tile in it of tile t, where stretch i (of `per` rows a token) starts at tile
-// floor(edge(i) per / rows) + i: at least as many tiles as it needs, with no sums over the documents.
-// 64 stretches are looked at in one step (a load each), then 64 within the interval found.
-__device__ __forceinline__ int find_stretch(const int32_t* off, int64_t tokens, int docs, int64_t per, int rows,
-                                            int64_t t, int64_t* first) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int lo = 0, n = docs + 2;  // the answer is in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + kWave - 1) / kWave;
-    const int i = lo + lane * step;
-    const bool before = lane * step < n && edge(off, tokens, docs, i) * per / rows + i <= t;
-    const uint64_t b = __ballot(before);
-    const int last = b ? 63 - __builtin_clzll(b) : 0;
-    n = min(step, n - last * step);
-    lo += last * step;
-  }
-  *first = edge(off, tokens, docs, lo) * per / rows + lo;
-  return lo;
+// Finds the stretch and the tile in it of tile t, where stretch i (of `per` rows a token, by the offsets
+// `off` of the queries or the keys) starts at tile floor(edge(i) per / rows) + i: at least as many tiles
+// as it needs, with no sums over the documents. Up to 62 documents: a lane looks at one each and has
+// loaded all that describes it in the same round trip to memory. More: 64 probes a step over the
+// offsets, then the description.
+struct Found {
+  Doc doc;
+  int64_t first;  // the stretch's first tile
+};
+__device__ __forceinline__ int64_t pick(int64_t v, int lane) {
+  const int lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+  const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
 }
-
-__device__ __forceinline__ Doc doc_of(const AttnArgs& a, int i) {
-  Doc d;
-  d.q0 = edge(a.q_offsets, a.q_tokens, a.docs, i);
-  d.q_len = edge(a.q_offsets, a.q_tokens, a.docs, i + 1) - d.q0;
-  d.k0 = edge(a.k_offsets, a.k_tokens, a.docs, i);
-  d.k_cap = edge(a.k_offsets, a.k_tokens, a.docs, i + 1) - d.k0;
-  if (d.q_len < 0) d.q_len = 0;
-  if (d.k_cap < 0) d.k_cap = 0;
-  d.k_len = d.k_cap;
-  d.prefix = 0;
-  if (i < 1 || i > a.docs) {
-    d.k_len = 0;
+template <bool BY_KEYS>
+__device__ __forceinline__ Found find_doc(const AttnArgs& a, int64_t per, int rows, int64_t t) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const int32_t* off = BY_KEYS ? a.k_offsets : a.q_offsets;
+  const int64_t tokens = BY_KEYS ? a.k_tokens : a.q_tokens;
+  Found f;
+  Doc& d = f.doc;
+  int i;
+  int64_t q1, k1, len = INT32_MAX, prefix = 0;
+  if (a.docs + 2 <= kWave) {
+    const int64_t q = edge(a.q_offsets, a.q_tokens, a.docs, lane), k = edge(a.k_offsets, a.k_tokens, a.docs, lane);
+    const bool real = lane >= 1 && lane <= a.docs;
+    const int32_t n = real && a.k_lengths ? a.k_lengths[lane - 1] : INT32_MAX;
+    const int32_t p = real && a.prefix ? a.prefix[lane - 1] : 0;
+    const int64_t start = (BY_KEYS ? k : q) * per / rows + lane;
+    const uint64_t b = __ballot(lane < a.docs + 2 && start <= t);
+    i = b ? 63 - __builtin_clzll(b) : 0;
+    f.first = pick(start, i);
+    d.q0 = pick(q, i);
+    d.k0 = pick(k, i);
+    q1 = i + 1 < a.docs + 2 ? pick(q, i + 1) : a.q_tokens;
+    k1 = i + 1 < a.docs + 2 ? pick(k, i + 1) : a.k_tokens;
+    len = __builtin_amdgcn_readlane(n, i);
+    prefix = __builtin_amdgcn_readlane(p, i);
   } else {
-    if (a.k_lengths) {
-      const int64_t n = a.k_lengths[i - 1];
-      d.k_len = n < 0 ? 0 : (n < d.k_cap ? n : d.k_cap);
+    int lo = 0, n = a.docs + 2;  // the answer is in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + kWave - 1) / kWave;
+      const int at = lo + lane * step;
+      const bool before = lane * step < n && edge(off, tokens, a.docs, at) * per / rows + at <= t;
+      const uint64_t b = __ballot(before);
+      const int last = b ? 63 - __builtin_clzll(b) : 0;
+      n = min(step, n - last * step);
+      lo += last * step;
     }
-    if (a.prefix) d.prefix = a.prefix[i - 1];
+    i = lo;
+    f.first = edge(off, tokens, a.docs, i) * per / rows + i;
+    d.q0 = edge(a.q_offsets, a.q_tokens, a.docs, i);
+    d.k0 = edge(a.k_offsets, a.k_tokens, a.docs, i);
+    q1 = edge(a.q_offsets, a.q_tokens, a.docs, i + 1);
+    k1 = edge(a.k_offsets, a.k_tokens, a.docs, i + 1);
+    if (i >= 1 && i <= a.docs) {
+      if (a.k_lengths) len = a.k_lengths[i - 1];
+      if (a.prefix) prefix = a.prefix[i - 1];
+    }
   }
-  return d;
+  d.q_len = q1 > d.q0 ? q1 - d.q0 : 0;
+  d.k_cap = k1 > d.k0 ? k1 - d.k0 : 0;
+  d.k_len = i < 1 || i > a.docs || len < 0 ? 0 : (len < d.k_cap ? len : d.k_cap);
+  d.prefix = prefix;
+  return f;
 }
 
 // Keys that token t of the document sees: always the first so many.

@@ -633,14 +633,17 @@ int gs_rotary_axes(const gs_rotary* args, void* stream);
  * A query that sees nothing, and one outside every document, gets 0 and -infinity. Key tokens
  * outside the documents and their lengths are never used, whatever they hold. Offsets and lengths
  * outside the tensors are cut to them.
- * gs_attention_bwd takes out and lse of the forward and d_out [q_tokens, heads, dim], and writes
+ * out_low (may be NULL; bfloat16 only): like out, what rounding took off it, for a backward to come: the
+ * row sums dO.out of the softmax's gradient are then exact to 2^-17, where documents are short or few
+ * keys share the weight (without it the gradients of such rows are off by up to twice the type's rounding).
+ * gs_attention_bwd takes out, lse and out_low (as it was in the forward, or NULL) and d_out [q_tokens, heads, dim], and writes
  * d_q, d_k, d_v (contiguous, every element; keys that nothing sees get 0). No atomics: the same
  * inputs give the same bits.
  * ------------------------------------------------------------------------------------- */
 #define GS_ATTENTION_MAX_DIM 128
 typedef struct gs_attention {
   const void *q, *k, *v;
-  void* out;
+  void *out, *out_low;
   float* lse;
   const int32_t *q_offsets, *k_offsets, *k_lengths, *prefix;
   int64_t q_tokens, k_tokens;
