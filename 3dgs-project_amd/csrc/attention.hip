@@ -231,20 +231,25 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
   if (h == 0) a.lse[at] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
-// Few query rows (single tokens) against long keys: HBM-bound, so a workgroup's wavefronts each walk
+// Few query rows (single tokens) against long keys (24 documents of 16k keys, 32 heads on 8 of 128: 276
+// us, 5.8 TB/s; one of 777, 8 heads of 64: 7.7 us, 10.0 with four wavefronts): HBM-bound, so a workgroup's wavefronts each walk
 // over keys of their own, 32 at a time, for the same 32 rows, and join at the end. The next keys' and
 // values' loads (16 KB a wavefront at 128 elements of bfloat16) are in flight while the present ones are
 // multiplied; they pass through the wavefront's own LDS (rows to be read across and along), with no
 // barrier in the loop.
+// bfloat16: eight wavefronts, so that a short document is a few steps long. float32's tiles allow four.
+template <typename T>
+constexpr int kFewWaves = sizeof(T) == 2 ? 8 : 4;
 template <typename T, int DP, int MODE>
-__global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs a) {
+  constexpr int kWaves = kFewWaves<T>;
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
   constexpr int kLoads = 32 * L::kChunks / kWave;  // 16-byte loads a lane for 32 rows
   constexpr int kTileBytes = 32 * L::kRowBytes;
   static_assert(2 * kTileBytes >= 32 * DP * 4, "the join reuses the wavefront's tiles");
-  __shared__ __attribute__((aligned(16))) char lds[kAttnWaves * 2 * kTileBytes];
-  __shared__ float l_m[kAttnWaves][32], l_l[kAttnWaves][32];
+  __shared__ __attribute__((aligned(16))) char lds[kWaves * 2 * kTileBytes];
+  __shared__ float l_m[kWaves][32], l_l[kWaves][32];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = static_cast<int64_t>(blockIdx.x / a.kv_heads);
   const Found found = find_doc<false>(a, a.group, 32, tile);
@@ -292,7 +297,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
   Frag<T> q[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) q[c] = load_query<T>(a, qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
-  for (; k0 < piece.stop; k0 += kAttnWaves * 32) {
+  for (; k0 < piece.stop; k0 += kWaves * 32) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int e = i * kWave + lane;
@@ -300,7 +305,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
       *reinterpret_cast<f32x4*>(lv + L::at(e / L::kChunks, e % L::kChunks)) = pv[i];
     }
     wave_sync();
-    if (k0 + kAttnWaves * 32 < piece.stop) fetch(k0 + kAttnWaves * 32);
+    if (k0 + kWaves * 32 < piece.stop) fetch(k0 + kWaves * 32);
     f32x16 s[1] = {};
 #pragma unroll
     for (int c = 0; c < C; ++c) mma(s[0], L::rows(lk, 0, c, lane), q[c]);
@@ -329,16 +334,16 @@ __global__ __launch_bounds__(kAttnThreads) void attn_few_kernel(AttnArgs a) {
         store4(own + (lane & 31) * DP + 32 * dt + 2 * r + 4 * h, o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < n_rows * (DP / 4); e += kAttnThreads) {
+  for (int e = threadIdx.x; e < n_rows * (DP / 4); e += kWaves * kWave) {
     const int i = e / (DP / 4), d = e % (DP / 4) * 4;
     float top = l_m[0][i];
 #pragma unroll
-    for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, l_m[w][i]);
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, l_m[w][i]);
     const float ref = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       const float f = exp2_hw(l_m[w][i] - ref);
       sum += f * l_l[w][i];
       x += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 2 * kTileBytes) + i * DP + d);
@@ -936,19 +941,19 @@ static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts,
     else launch_mode<K, float, 64>(a, grid, st);
   }
 }
-#define GS_ATTN_KERNEL(NAME, KERNEL, FIXED)                                            \
+#define GS_ATTN_KERNEL(NAME, KERNEL, FIXED, THREADS)                                   \
   template <typename T, int DP, int MODE>                                              \
   struct NAME {                                                                        \
     static constexpr bool kFixed = FIXED;                                              \
     static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                 \
       constexpr int mode = !FIXED && MODE == kCapFixed ? static_cast<int>(kCap) : MODE; \
-      hipLaunchKernelGGL((KERNEL<T, DP, mode>), grid, dim3(kAttnThreads), 0, st, a);   \
+      hipLaunchKernelGGL((KERNEL<T, DP, mode>), grid, dim3(THREADS), 0, st, a);        \
     }                                                                                  \
   }
-GS_ATTN_KERNEL(FwdKernel, attn_fwd_kernel, true);
-GS_ATTN_KERNEL(FewKernel, attn_few_kernel, true);
-GS_ATTN_KERNEL(BwdQKernel, attn_bwd_q_kernel, false);
-GS_ATTN_KERNEL(BwdKvKernel, attn_bwd_kv_kernel, false);
+GS_ATTN_KERNEL(FwdKernel, attn_fwd_kernel, true, kAttnThreads);
+GS_ATTN_KERNEL(FewKernel, attn_few_kernel, true, kFewWaves<T> * kWave);
+GS_ATTN_KERNEL(BwdQKernel, attn_bwd_q_kernel, false, kAttnThreads);
+GS_ATTN_KERNEL(BwdKvKernel, attn_bwd_kv_kernel, false, kAttnThreads);
 #undef GS_ATTN_KERNEL
 
 // How a forward call is laid out, by sizes alone (so that the workspace can be asked for first).
@@ -957,8 +962,8 @@ struct FwdPlan {
   int64_t tiles;  // row tiles
   int splits;     // pieces of the keys
 };
-constexpr int kFewSplitKeys = 512, kTileSplitKeys = 256;
-constexpr int kFewBlocks = 2048, kTileBlocks = 512, kMaxSplits = 256;
+constexpr int kFewSplitKeys = 1024, kTileSplitKeys = 256;
+constexpr int kFewBlocks = 1024, kTileBlocks = 512, kMaxSplits = 256;
 
 static FwdPlan plan_fwd(const AttnArgs& a) {
   FwdPlan f;

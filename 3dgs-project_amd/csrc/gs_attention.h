@@ -301,7 +301,7 @@ struct Piece {
 __device__ __forceinline__ Piece piece_of(const AttnArgs& a, int end, int split) {
   if (a.splits == 1) return {0, end, 1};
   int per = (end + a.splits - 1) / a.splits;
-  per = max((per + 127) & ~127, a.split_keys);
+  per = max((per + 255) & ~255, a.split_keys);
   const int n = max(1, (end + per - 1) / per);
   return {min(split * per, end), min((split + 1) * per, end), n};
 }
