@@ -108,7 +108,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     if j <= i + Lk - Lq; prefix [docs] int32 (with causal): or if j < prefix[d]. softcap c > 0: scores
     s become c tanh(s / c). scale: of the scores before the cap (default 1 / sqrt(D)).
 
-    A query that sees no key gets 0 and -infinity. D up to 128 (padded to a multiple of 8 by a copy).
+    A query that sees no key gets 0 and -infinity. A key or value that is not finite reaches only the
+    queries that see it (the gradients of its document are not kept apart so). D up to 128 (padded to a multiple of 8 by a copy).
     Tensors are read through their strides where these and the addresses are multiples of 16 bytes
     and the last dimension is contiguous; otherwise they are copied first."""
     if not (q.dim() == k.dim() == v.dim() == 3):

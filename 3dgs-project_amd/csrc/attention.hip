@@ -117,7 +117,53 @@ __device__ __forceinline__ void keep_order() {
   if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 }
 
+// A masked key's probability is 0, but 0 times an infinity or a NaN among its values is not. Such values
+// reach the sums of queries that do not see them only under the causal mask, where some queries of a tile
+// see a key and others do not; they are then visible in the sums, which are formed again here over the
+// keys that each query sees, one by one. Finite values never come here.
+template <int M>
+__device__ __forceinline__ bool any_not_finite(const f32x16 (&o)[M]) {
+  float t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t = fmaf(o[i][r], 0.0f, t);
+  return __any(!(t == 0.0f));
+}
+// Keys begin .. begin + 31, then `step` further on, below `vis`.
 template <typename T, int DP, int MODE>
+__device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, const Frag<T> (&q)[DP / 16], const T* kp,
+                                             const T* vp, float m, int begin, int step, int vis, int h,
+                                             f32x16 (&o)[DP / 32]) {
+  const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
+  for (int k0 = begin; k0 < vis; k0 += step)
+    for (int key = k0; key < min(k0 + 32, vis); ++key) {
+      float s = 0.0f;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) {
+        const int d = 16 * c + 8 * h;
+        const Frag<T> k = load_frag<T>(kp + key * a.k_token + d, d < a.dim);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf(static_cast<float>(q[c][j]), static_cast<float>(k[j]), s);
+      }
+      s = exponent<T, MODE>(u, half_sum(s));
+      const float p = static_cast<float>(static_cast<T>(prob<MODE>(u, s, ref)));
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const int d = 32 * dt + 2 * r + 4 * h;
+          if (d >= a.dim) continue;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[dt][r + j] = fmaf(p, static_cast<float>(vp[key * a.v_token + d + j]), o[dt][r + j]);
+        }
+    }
+}
+
+template <typename T, int DP, int MODE, bool CAUSAL>
 __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd_kernel(AttnArgs a) {
   using L = Tile<T, DP>;
   constexpr int C = DP / 16;
@@ -198,6 +244,12 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
     }
     __builtin_amdgcn_s_setprio(0);
   }
+  // an instance of its own: the code costs registers (8192 causal tokens, 16 heads: 276 -> 278 us at 128
+  // elements, 251 -> 266 us at 64, capped)
+  if constexpr (CAUSAL) {
+    if (any_not_finite(o))
+      sums_of_seen<T, DP, MODE>(a, rule, q, kp, vp, st.m, piece.begin, 32, min(vis, piece.stop), h, o);
+  }
   if (!live) return;
   const float m = st.m, l = half_sum(st.l);
   if (a.splits > 1) {
@@ -218,7 +270,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
     }
     return;
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t at = (doc.q0 + tok) * a.heads + head;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -228,7 +280,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
       if (d >= a.dim) continue;
       store_out<T>(a, at * a.dim + d, f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]} * inv);
     }
-  if (h == 0) a.lse[at] = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // Few query rows (single tokens) against long keys (24 documents of 16k keys, 32 heads on 8 of 128: 276
@@ -240,7 +292,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_fwd
 // bfloat16: eight wavefronts, so that a short document is a few steps long. float32's tiles allow four.
 template <typename T>
 constexpr int kFewWaves = sizeof(T) == 2 ? 8 : 4;
-template <typename T, int DP, int MODE>
+template <typename T, int DP, int MODE, bool CAUSAL>
 __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs a) {
   constexpr int kWaves = kFewWaves<T>;
   using L = Tile<T, DP>;
@@ -318,6 +370,10 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
     }
     wave_sync();
   }
+  if constexpr (CAUSAL) {
+    if (any_not_finite(o))
+      sums_of_seen<T, DP, MODE>(a, rule, q, kp, vp, st.m, piece.begin + wave * 32, kWaves * 32, vis, h, o);
+  }
   // join: every wavefront leaves its rows, statistics and (in its own tiles) sums; then all threads
   // take the same rows' elements and add the wavefronts' in order
   const float m = st.m, l = half_sum(st.l);
@@ -359,9 +415,9 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
         if (blockIdx.y == 0) a.part_n[at] = piece.n;
       }
     } else {
-      const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
       if (d < a.dim) store_out<T>(a, at * a.dim + d, x * inv);
-      if (d == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      if (d == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
   }
 }
@@ -408,9 +464,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
       }
     }
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   if (d < a.dim) store_out<T>(a, at * a.dim + d, x * inv);
-  if (lane == 0) a.lse[at] = sum > 0.0f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  if (lane == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // Lays out the instructions since the last keep_order as M times one matrix instruction and V vector
@@ -941,20 +997,31 @@ static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts,
     else launch_mode<K, float, 64>(a, grid, st);
   }
 }
-#define GS_ATTN_KERNEL(NAME, KERNEL, FIXED, THREADS)                                   \
-  template <typename T, int DP, int MODE>                                              \
-  struct NAME {                                                                        \
-    static constexpr bool kFixed = FIXED;                                              \
-    static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                 \
-      constexpr int mode = !FIXED && MODE == kCapFixed ? static_cast<int>(kCap) : MODE; \
-      hipLaunchKernelGGL((KERNEL<T, DP, mode>), grid, dim3(THREADS), 0, st, a);        \
-    }                                                                                  \
+// Forward kernels have an instance for the fixed cap and one for the causal mask, the backward's do not.
+#define GS_ATTN_FORWARD(NAME, KERNEL, THREADS)                                                            \
+  template <typename T, int DP, int MODE>                                                                 \
+  struct NAME {                                                                                           \
+    static constexpr bool kFixed = true;                                                                  \
+    static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                                    \
+      if (a.causal) hipLaunchKernelGGL((KERNEL<T, DP, MODE, true>), grid, dim3(THREADS), 0, st, a);       \
+      else hipLaunchKernelGGL((KERNEL<T, DP, MODE, false>), grid, dim3(THREADS), 0, st, a);               \
+    }                                                                                                     \
   }
-GS_ATTN_KERNEL(FwdKernel, attn_fwd_kernel, true, kAttnThreads);
-GS_ATTN_KERNEL(FewKernel, attn_few_kernel, true, kFewWaves<T> * kWave);
-GS_ATTN_KERNEL(BwdQKernel, attn_bwd_q_kernel, false, kAttnThreads);
-GS_ATTN_KERNEL(BwdKvKernel, attn_bwd_kv_kernel, false, kAttnThreads);
-#undef GS_ATTN_KERNEL
+#define GS_ATTN_BACKWARD(NAME, KERNEL)                                                                    \
+  template <typename T, int DP, int MODE>                                                                 \
+  struct NAME {                                                                                           \
+    static constexpr bool kFixed = false;                                                                 \
+    static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                                    \
+      constexpr int mode = MODE == kPlain ? kPlain : kCap;                                                \
+      hipLaunchKernelGGL((KERNEL<T, DP, mode>), grid, dim3(kAttnThreads), 0, st, a);                      \
+    }                                                                                                     \
+  }
+GS_ATTN_FORWARD(FwdKernel, attn_fwd_kernel, kAttnThreads);
+GS_ATTN_FORWARD(FewKernel, attn_few_kernel, kFewWaves<T> * kWave);
+GS_ATTN_BACKWARD(BwdQKernel, attn_bwd_q_kernel);
+GS_ATTN_BACKWARD(BwdKvKernel, attn_bwd_kv_kernel);
+#undef GS_ATTN_FORWARD
+#undef GS_ATTN_BACKWARD
 
 // How a forward call is laid out, by sizes alone (so that the workspace can be asked for first).
 struct FwdPlan {

@@ -631,14 +631,16 @@ int gs_rotary_axes(const gs_rotary* args, void* stream);
  * softcap tanh(scale q.k / softcap).
  *   out [q_tokens, heads, dim] = sum_j softmax(s)_j v_j, lse [q_tokens, heads] float32 = ln sum_j e^s_j.
  * A query that sees nothing, and one outside every document, gets 0 and -infinity. Key tokens
- * outside the documents and their lengths are never used, whatever they hold. Offsets and lengths
- * outside the tensors are cut to them.
+ * outside the documents and their lengths are never used, whatever they hold, and a key or value that is
+ * not finite reaches the queries that see it only. Offsets and lengths outside the tensors are cut to
+ * them.
  * out_low (may be NULL; bfloat16 only): like out, what rounding took off it, for a backward to come: the
  * row sums dO.out of the softmax's gradient are then exact to 2^-17, where documents are short or few
  * keys share the weight (without it the gradients of such rows are off by up to twice the type's rounding).
  * gs_attention_bwd takes out, lse and out_low (as it was in the forward, or NULL) and d_out [q_tokens, heads, dim], and writes
- * d_q, d_k, d_v (contiguous, every element; keys that nothing sees get 0). No atomics: the same
- * inputs give the same bits.
+ * d_q, d_k, d_v (contiguous, every element; keys that nothing sees get 0). What is not finite
+ * among a document's own tokens may reach all of its gradients. No atomics: the same inputs give the same
+ * bits.
  * ------------------------------------------------------------------------------------- */
 #define GS_ATTENTION_MAX_DIM 128
 typedef struct gs_attention {

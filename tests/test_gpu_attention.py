@@ -328,3 +328,65 @@ def test_refusals():
         with pytest.raises(ValueError, match=text):
             attention(args.pop("q"), args.pop("k"), args.pop("v"), **args)
     assert attention(q, k, k).shape == q.shape
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_not_finite_reaches_only_what_sees_it(bad, softcap, dim, dtype):
+    # in order: queries before the token see nothing of it, the others all of it, element by element
+    for n, at, nq in ((150, 100, 150), (70, 69, 70), (300, 290, 20)):
+        q, k, v, _ = inputs(nq, n, 4, 2, dim, dtype, n)
+        want = A.attention(q, k, v, [0, nq], [0, n], causal=True, softcap=softcap)
+        v[at, :, 3::7] = bad
+        first = at - (n - nq)  # the first query that sees it
+        got = run(q, k, v, None, causal=True, softcap=softcap, offsets=ints([0, nq]), k_offsets=ints([0, n]))
+        check({"out": got["out"][:first]}, {"out": tuple(t[:first] for t in want["out"])})
+        check({"lse": got["lse"]}, want)
+        seen = got["out"][first:].cpu()
+        assert not bool(torch.isfinite(seen[..., 3::7]).any())
+        clean = [d for d in range(dim) if d % 7 != 3]
+        check({"out": seen[..., clean]}, {"out": tuple(t[first:, :, clean] for t in want["out"])})
+        # a key: its scores are not finite where it is seen
+        q, k, v, _ = inputs(nq, n, 4, 2, dim, dtype, n)
+        k[at] = float("nan")
+        got = run(q, k, v, None, causal=True, softcap=softcap, offsets=ints([0, nq]), k_offsets=ints([0, n]))
+        check({"out": got["out"][:first], "lse": got["lse"][:first]},
+              {name: tuple(t[:first] for t in want[name]) for name in ("out", "lse")})
+        assert bool(got["out"][first:].isnan().all()) and bool(got["lse"][first:].isnan().all())
+
+
+def test_captured_in_a_graph():
+    """Calls that take workspaces and several launches, replayed with other work between."""
+    from amdsplat import clip_grad_norm, rotary_axes
+
+    q, k, v, g = (t.to(DEV) for t in inputs(600, 600, 4, 1, 64, torch.bfloat16, 33))
+    one = q[:1].clone()
+    x = [torch.randn(5000, device=DEV), torch.randn(77, device=DEV).bfloat16()]
+    out = [torch.empty_like(t) for t in x]
+    pos = torch.arange(600, device=DEV, dtype=torch.float32)[:, None]
+
+    def work():
+        a, b = rotary_axes(q, k, pos, (32,))
+        r = run(a, b, v, g, causal=True)
+        long = attention(one, k.repeat(20, 1, 1), v.repeat(20, 1, 1), offsets=ints_one, k_offsets=ints_all)
+        return [*r.values(), long, clip_grad_norm(x, 1.0, out=out), *out]
+
+    ints_one, ints_all = ints([0, 1]), ints([0, 12000])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = work()
+    for i in range(4):
+        q.mul_(1.01)
+        x[0].add_(0.1)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in kept]
+        for a, b in zip(got, [t.clone() for t in work()]):
+            assert torch.equal(a, b), i
+        torch.empty(1 << 22, device=DEV).normal_()
