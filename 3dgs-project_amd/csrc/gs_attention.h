@@ -149,8 +149,10 @@ struct AttnArgs {
   float* part;        // [splits][q_tokens][heads][dim], unnormalised
   float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
   int32_t* part_n;    // [q_tokens][heads] pieces
-  // backward: query rows of a key tile cut into `row_parts`, each part's dK and dV in float32
-  int row_parts;
+  // backward: the rows of a key tile cut into `row_parts`, the keys of a row tile into `key_parts`, each
+  // part's gradients in float32
+  int row_parts, key_parts;
+  float* part_q;      // [key_parts][q_tokens][heads][dim]
   float* part_kv;     // [dK, dV][row_parts][k_tokens][kv_heads][dim]
 };
 
