@@ -70,12 +70,14 @@ __device__ __forceinline__ void adam_elem(const AdamGroupK& G, float g, float& p
 template <bool SCALED>
 __global__ __launch_bounds__(kAdamThreads) void adam_kernel(AdamArgs a) {
   const float scale = SCALED ? *a.scale : 1.0f;
+  // scaled: from the last block to the first, whose gradients the norm's pass has just read
+  const int64_t block = SCALED ? static_cast<int64_t>(gridDim.x) - 1 - blockIdx.x : blockIdx.x;
   int gi = 0;
 #pragma unroll
   for (int k = 1; k < GS_ADAM_MAX_GROUPS; ++k)
-    if (k < a.n_groups && static_cast<int64_t>(blockIdx.x) >= a.g[k].block0) gi = k;
+    if (k < a.n_groups && block >= a.g[k].block0) gi = k;
   const AdamGroupK& G = a.g[gi];
-  const int64_t e0 = (static_cast<int64_t>(blockIdx.x) - G.block0) * kAdamBlockElems +
+  const int64_t e0 = (block - G.block0) * kAdamBlockElems +
                      static_cast<int64_t>(threadIdx.x) * kAdamPerThread;
   if (e0 >= G.n) return;
   const int cnt = static_cast<int>(min<int64_t>(kAdamPerThread, G.n - e0));
