@@ -26,23 +26,26 @@ def _readable(t: torch.Tensor, group: int = 0) -> torch.Tensor:
     heads to a key head (q: 64 consecutive rows have to span less than 2^28 elements)."""
     per = _DTYPES[t.dtype][1]
     st, sh, sd = t.stride()
-    if t.numel() == 0:
+    if 0 in t.shape:
         return t
     ok = ((sd == 1 or t.shape[2] == 1) and 0 <= st < 1 << 22 and 0 <= sh < 1 << 40 and st % per == 0 and sh % per == 0
           and t.data_ptr() % 16 == 0 and (not group or (64 // group + 2) * st + group * sh < 1 << 28))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+def _at(t) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _args(q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix, causal, softcap, scale) -> _lib.GsAttention:
-    docs = 1 if offsets is None else offsets.numel() - 1
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    if not q.numel():
-        qs = (0, 0, 1)
-    if not k.numel():
-        ks = vs = (0, 0, 1)
-    return _lib.GsAttention(ptr(q), ptr(k), ptr(v), ptr(out), ptr(low), ptr(lse), ptr(offsets), ptr(k_offsets), ptr(k_lengths),
-                            ptr(prefix), q.shape[0], k.shape[0], qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], docs,
-                            q.shape[1], k.shape[1], q.shape[2], _DTYPES[q.dtype][0], int(causal), softcap, scale)
+    tq, heads, dim = q.shape
+    tk, kv_heads, _ = k.shape
+    q_token, q_head, _ = q.stride() if tq else (0, 0, 1)
+    (k_token, k_head, _), (v_token, v_head, _) = (k.stride(), v.stride()) if tk else ((0, 0, 1), (0, 0, 1))
+    return _lib.GsAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _at(low), lse.data_ptr(),
+                            _at(offsets), _at(k_offsets), _at(k_lengths), _at(prefix), tq, tk, q_token, q_head,
+                            k_token, k_head, v_token, v_head, 1 if offsets is None else offsets.shape[0] - 1, heads,
+                            kv_heads, dim, _DTYPES[q.dtype][0], causal, softcap, scale)
 
 
 def _workspace(name: str, args, device):
@@ -90,8 +93,8 @@ def _table(t, name: str, n: int, device) -> None:
     if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous()
             and t.device == device):
         raise ValueError(f"{name} must be a contiguous int32 tensor on the tensors' device")
-    if t.numel() != n:
-        raise ValueError(f"{name} must have {n} entries, got {t.numel()}")
+    if t.shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, got {t.shape[0]}")
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: torch.Tensor | None = None,
@@ -132,7 +135,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
         raise ValueError("k_offsets without offsets")
     docs = 1
     if offsets is not None:
-        docs = offsets.numel() - 1
+        docs = offsets.numel() - 1 if isinstance(offsets, torch.Tensor) else 0
         if docs < 1:
             raise ValueError("offsets must have at least 2 entries")
         _table(offsets, "offsets", docs + 1, device)

@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import call, ptr
+from ._lib import call
 
 MAX_AXES, MAX_PAIRS = 4, 256  # GS_ROTARY_MAX_AXES, GS_ROTARY_MAX_PAIRS
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
@@ -27,17 +27,18 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _turn(q, k, positions, sections, base: float, flags: int):
     q = _rows(q)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a = _lib.GsRotary(q=ptr(q), q_out=ptr(q_out), positions=ptr(positions), tokens=q.shape[0],
-                      q_token_stride=q.stride(0), q_head_stride=q.stride(1), base=base, q_heads=q.shape[1],
-                      dim=q.shape[2], axes=len(sections), dtype=_DTYPES[q.dtype], flags=flags)
-    a.sections[:len(sections)] = sections
-    k_out = None
+    tokens, heads, dim = q.shape
+    q_out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    q_token, q_head, _ = q.stride()
+    k_out, k_at, k_to, k_token, k_head, k_heads = None, None, None, 0, 0, 0
     if k is not None:
         k = _rows(k)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        a.k, a.k_out, a.k_heads = ptr(k), ptr(k_out), k.shape[1]
-        a.k_token_stride, a.k_head_stride = k.stride(0), k.stride(1)
+        k_heads = k.shape[1]
+        k_out = torch.empty((tokens, k_heads, dim), dtype=q.dtype, device=q.device)
+        k_at, k_to = k.data_ptr(), k_out.data_ptr()
+        k_token, k_head, _ = k.stride()
+    a = _lib.GsRotary(q.data_ptr(), k_at, q_out.data_ptr(), k_to, positions.data_ptr(), tokens, q_token, q_head, k_token,
+                      k_head, base, heads, k_heads, dim, len(sections), sections, _DTYPES[q.dtype], flags)
     call("gs_rotary_axes", C.byref(a), _lib.stream_handle(q.device))
     return q_out, k_out
 
