@@ -368,8 +368,19 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
       const Frag<T> p = acc_frag<T>(s[0], kc);
+      // Here the matrix unit has time to spare, so what rounding took off the probabilities is multiplied
+      // too: the output is off by its own rounding alone.
+      Frag<T> low = {};
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], L::cols(lv, 32 * dt, 16 * kc, lane), p);
+        for (int j = 0; j < 8; ++j) low[j] = static_cast<T>(s[0][8 * kc + j] - static_cast<float>(p[j]));
+      }
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) {
+        const Frag<T> v = L::cols(lv, 32 * dt, 16 * kc, lane);
+        mma(o[dt], v, p);
+        if constexpr (sizeof(T) == 2) mma(o[dt], v, low);
+      }
     }
     wave_sync();
   }
