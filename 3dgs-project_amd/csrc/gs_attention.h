@@ -58,15 +58,18 @@ __device__ __forceinline__ Frag<T> acc_frag(const f32x16& c, int k) {
 }
 
 // A tile in LDS: rows of DP elements, the 16-byte chunks of a row permuted by XOR with bits of the
-// row number so that both kinds of read below fall on distinct banks: eight consecutive rows at one
-// chunk, and four consecutive rows at a pair of chunks.
+// row number so that the reads below fall on distinct banks (256 bytes of them). Along a row: sixteen
+// consecutive rows at one chunk. Across, in bfloat16: four consecutive rows at four consecutive chunks
+// (32 lanes), so the lowest two row bits have to go to other chunk bits than the lowest two; in float32
+// rows 4 apart at eight consecutive chunks.
 template <typename T, int DP>
 struct Tile {
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kElemsPerChunk = 16 / static_cast<int>(sizeof(T));
   static __device__ __forceinline__ int swizzle(int row) {
-    if constexpr (kChunks == 8) return ((row & 6) | ((row >> 3) & 1));
+    if constexpr (kChunks == 8) return ((row & 2) << 1) | ((row & 4) >> 1) | ((row >> 3) & 1);  // (row & 1: by layout)
+    if constexpr (sizeof(T) == 2) return ((row & 3) << 2) | ((row & 4) >> 1) | ((row >> 3) & 1);
     return ((row << 1) & 14) | ((row >> 3) & 1);
   }
   static __device__ __forceinline__ int at(int row, int chunk) {
