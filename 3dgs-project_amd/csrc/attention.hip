@@ -20,20 +20,33 @@ struct Rule {
   float scale2;    // plain: scale log2 e
   float in_scale;  // capped: scale / cap
   float cap2;      // capped: cap log2 e
+  float twice;     // capped: 2 log2 e scale / cap
 };
+
+// Capped scores, s' = cap tanh x, x = scale s / cap. In bfloat16 tanh x = 1 - 2 r with r = 1 / (1 + e^2x)
+// from the hardware exponential and reciprocal (absolute error 2e-7, both ends saturate): s' - ref is then
+// one fma of r, and the slope 1 - tanh^2 = 4 r (1 - r). float32 takes the library's tanh, whose relative
+// error near zero is small too.
+__device__ __forceinline__ float cap_r(const Rule& u, float s) {
+  return __builtin_amdgcn_rcpf(1.0f + exp2_hw(s * u.twice));
+}
 template <int MODE>
 __device__ __forceinline__ Rule rule_of(const AttnArgs& a) {
   const float scale = fabsf(a.scale);
-  return {fmaxf(scale * kLog2e, 1e-30f), MODE == kPlain ? 0.0f : scale / a.softcap, a.softcap * kLog2e};
+  return {fmaxf(scale * kLog2e, 1e-30f), MODE == kPlain ? 0.0f : scale / a.softcap, a.softcap * kLog2e,
+          MODE == kPlain ? 0.0f : 2.0f * kLog2e * scale / a.softcap};
 }
 template <typename T, int MODE>
 __device__ __forceinline__ float exponent(const Rule& u, float s) {
   if constexpr (MODE == kPlain) return s;
-  return u.cap2 * tanh_of<T>(s * u.in_scale);
+  if constexpr (sizeof(T) == 2) return fmaf(-2.0f * u.cap2, cap_r(u, s), MODE == kCapFixed ? kFixedTop : u.cap2);
+  const float x = u.cap2 * tanhf(s * u.in_scale);
+  return MODE == kCapFixed ? x - (u.cap2 - kFixedTop) : x;
 }
 template <int MODE>
 __device__ __forceinline__ float prob(const Rule& u, float x, float ref) {
   if constexpr (MODE == kPlain) return exp2_hw(fmaf(x, u.scale2, -ref));
+  if constexpr (MODE == kCapFixed) return exp2_hw(x);  // relative to the fixed reference already
   return exp2_hw(x - ref);
 }
 
@@ -560,7 +573,12 @@ __device__ __forceinline__ void add_cols_times(const char* lds, int row0, int la
 template <typename T, int MODE>
 __device__ __forceinline__ float prob_of(const Rule& u, float s, float lse2, float* slope) {
   if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.scale2, -lse2));
-  const float t = tanh_of<T>(s * u.in_scale);
+  if constexpr (sizeof(T) == 2) {
+    const float r = cap_r(u, s), r4 = 4.0f * r;
+    *slope = fmaf(-r4, r, r4);
+    return exp2_hw(fmaf(-2.0f * u.cap2, r, u.cap2 - lse2));
+  }
+  const float t = tanhf(s * u.in_scale);
   *slope = fmaf(-t, t, 1.0f);
   return exp2_hw(fmaf(u.cap2, t, -lse2));
 }

@@ -289,16 +289,6 @@ enum { kPlain = 0, kCap = 1, kCapFixed = 2 };
 // stays below 2^90.
 constexpr float kFixedCap = 90.0f, kFixedTop = 60.0f;
 
-// tanh. bfloat16: 1 - 2 / (1 + e^2x) from the hardware exponential and reciprocal (absolute error
-// 2e-7; both ends saturate). float32: the library's, which keeps the relative error near zero.
-template <typename T>
-__device__ __forceinline__ float tanh_of(float x) {
-  if constexpr (sizeof(T) == 2)
-    return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + exp2_hw(2.0f * kLog2e * x)), 1.0f);
-  else
-    return tanhf(x);
-}
-
 // The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one).
 struct Piece {
   int begin, stop, n;
