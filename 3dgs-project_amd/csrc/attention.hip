@@ -570,17 +570,23 @@ __device__ __forceinline__ void add_cols_times(const char* lds, int row0, int la
 
 // Probability of a score, p = e^(s - lse), and (capped) the score's slope 1 - tanh^2. The raw score's
 // gradient is p slope (dp - delta).
+// `base` is the row's, from base_of its log-sum-exp.
 template <typename T, int MODE>
-__device__ __forceinline__ float prob_of(const Rule& u, float s, float lse2, float* slope) {
-  if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.scale2, -lse2));
+__device__ __forceinline__ float base_of(const Rule& u, float lse) {
+  const float lse2 = lse == -INFINITY ? 0.0f : lse * kLog2e;
+  return MODE != kPlain && sizeof(T) == 2 ? u.cap2 - lse2 : -lse2;
+}
+template <typename T, int MODE>
+__device__ __forceinline__ float prob_of(const Rule& u, float s, float base, float* slope) {
+  if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.scale2, base));
   if constexpr (sizeof(T) == 2) {
     const float r = cap_r(u, s), r4 = 4.0f * r;
     *slope = fmaf(-r4, r, r4);
-    return exp2_hw(fmaf(-2.0f * u.cap2, r, u.cap2 - lse2));
+    return exp2_hw(fmaf(-2.0f * u.cap2, r, base));
   }
   const float t = tanhf(s * u.in_scale);
   *slope = fmaf(-t, t, 1.0f);
-  return exp2_hw(fmaf(u.cap2, t, -lse2));
+  return exp2_hw(fmaf(u.cap2, t, base));
 }
 
 // Query gradients, and delta_i = dO_i . O_i for the key gradients. Like the forward, a lane owns a
@@ -642,11 +648,10 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   delta = half_sum(delta);
   const int64_t stat = (doc.q0 + tok) * a.heads + head;
   if (live && h == 0 && blockIdx.y == 0) a.delta[stat] = delta;
-  const float lse = a.lse[stat];
-  const float lse2 = lse == -INFINITY ? 0.0f : lse * kLog2e;
+  const Rule rule = rule_of<MODE>(a);
+  const float row_base = base_of<T, MODE>(rule, a.lse[stat]);
   const int vis = live ? visible(a, doc, tok) : 0;
   const int wave_min = wrow + 31 < rows ? visible(a, doc, wrow / a.group) : 0;
-  const Rule rule = rule_of<MODE>(a);
   f32x16 dq[DP / 32] = {};
   int buf = 0;
   for (int k0 = begin; k0 < end; k0 += kAttnKeys, buf ^= 1) {
@@ -663,7 +668,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float slope = 1.0f;
-            s[r] = prob_of<T, MODE>(rule, s[r], lse2, &slope);
+            s[r] = prob_of<T, MODE>(rule, s[r], row_base, &slope);
             if constexpr (MODE != kPlain) s[r] *= slope;
             if (masked.value && k0 + 32 * t + 8 * (r / 4) + 4 * h + r % 4 >= vis) s[r] = 0.0f;
           }
@@ -718,7 +723,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
 }
 
 // Key and value gradients: a lane owns one key, the workgroup walks over the query rows that see it,
-// 64 at a time. Rows past the document's end need no mask: their q, dO, lse and delta are zero, and so
+// 64 at a time. Rows past the document's end need no mask: their q, dO and delta are zero (and p finite), and so
 // is what they add. The lanes of keys past the valid length gather nothing that is kept.
 //
 // At 128 elements of bfloat16 both gradients' accumulators (128 registers beside K and V's 64) leave no
@@ -733,7 +738,7 @@ constexpr int kKvRows = 64;  // query rows of a tile
 template <typename T, int DP>
 struct KvShared {
   char tiles[4 * kKvRows * Tile<T, DP>::kRowBytes];
-  float lse[2][kKvRows], delta[2][kKvRows];
+  float base[2][kKvRows], delta[2][kKvRows];
   int vis[2][kKvRows];
 };
 
@@ -744,7 +749,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
   constexpr int R = kKvRows;
   constexpr int kTileBytes = R * L::kRowBytes;
   char* lds = sh.tiles;
-  const auto &l_lse = sh.lse, &l_delta = sh.delta;
+  const auto &l_base = sh.base, &l_delta = sh.delta;
   const auto& l_vis = sh.vis;
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
   const int64_t tile = blockIdx.x / a.kv_heads;
@@ -775,6 +780,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
   }
   const RowTileCopy<T, DP, R, kAttnThreads> copy_q = {a.q_token, a.q_head};
   const RowTileCopy<T, DP, R, kAttnThreads> copy_g = {static_cast<int64_t>(a.heads) * a.dim, a.dim};
+  const Rule rule = rule_of<MODE>(a);
   float n_lse = 0.0f, n_delta = 0.0f;
   int n_vis = 0;
   const auto fetch = [&](int r0, char* to) {
@@ -797,7 +803,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
   };
   const auto keep = [&](int b) {
     if (threadIdx.x < R) {
-      sh.lse[b][threadIdx.x] = n_lse == -INFINITY ? 0.0f : n_lse * kLog2e;
+      sh.base[b][threadIdx.x] = base_of<T, MODE>(rule, n_lse);
       sh.delta[b][threadIdx.x] = n_delta;
       sh.vis[b][threadIdx.x] = n_vis;
     }
@@ -813,7 +819,6 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
     if (a.scale < 0.0f) k[c] = -k[c];
     if constexpr (DK) v[c] = load_frag<T>(vp + 16 * c + 8 * h, in);
   }
-  const Rule rule = rule_of<MODE>(a);
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
   int buf = 0;
   for (int r0 = row_begin; r0 < row_end; r0 += R, buf ^= 1) {
@@ -833,12 +838,12 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int at = 32 * t + 8 * i + 4 * h;
-            const f32x4 lse2 = *reinterpret_cast<const f32x4*>(&l_lse[buf][at]);
+            const f32x4 base = *reinterpret_cast<const f32x4*>(&l_base[buf][at]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int r = 4 * i + j;
               float slope = 1.0f;
-              s[r] = prob_of<T, MODE>(rule, s[r], lse2[j], &slope);
+              s[r] = prob_of<T, MODE>(rule, s[r], base[j], &slope);
               if constexpr (MODE != kPlain && DV) sl[r] = slope;
               if constexpr (MODE != kPlain && !DV) s[r] *= slope;
               if (masked.value && key >= l_vis[buf][at + j]) s[r] = 0.0f;
