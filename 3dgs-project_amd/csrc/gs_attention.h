@@ -147,8 +147,9 @@ struct AttnArgs {
   void *d_q, *d_k, *d_v;
   float* delta;
   int n_tiles;
-  // keys of a row tile cut into up to `splits` pieces of at least split_keys, joined by a second launch
-  int splits, split_keys;
+  // keys of a row tile cut into up to `splits` pieces of at least split_keys, multiples of split_unit (what
+  // a workgroup takes in one step), joined by a second launch
+  int splits, split_keys, split_unit;
   float* part;        // [splits][q_tokens][heads][dim], unnormalised
   float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
   int32_t* part_n;    // [q_tokens][heads] pieces
@@ -296,7 +297,7 @@ struct Piece {
 __device__ __forceinline__ Piece piece_of(const AttnArgs& a, int end, int split) {
   if (a.splits == 1) return {0, end, 1};
   int per = (end + a.splits - 1) / a.splits;
-  per = max((per + 255) & ~255, a.split_keys);
+  per = max((per + a.split_unit - 1) / a.split_unit * a.split_unit, a.split_keys);
   const int n = max(1, (end + per - 1) / per);
   return {min(split * per, end), min((split + 1) * per, end), n};
 }
