@@ -193,7 +193,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
   const int64_t base = (tile - found.first) * kAttnRows;
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
-  const Piece piece = piece_of(a, visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group), blockIdx.y);
+  const Piece piece = piece_of(a, visible(a, doc, (min(row0 + kAttnRows, rows) - 1) / a.group), blockIdx.y, found.share);
   if (static_cast<int>(blockIdx.y) >= piece.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int wrow = row0 + wave * 32;
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
   if (base >= rows) return;
   const int row0 = static_cast<int>(base);
   const int n_rows = min(32, rows - row0);
-  const Piece piece = piece_of(a, visible(a, doc, (row0 + n_rows - 1) / a.group), blockIdx.y);
+  const Piece piece = piece_of(a, visible(a, doc, (row0 + n_rows - 1) / a.group), blockIdx.y, found.share);
   if (static_cast<int>(blockIdx.y) >= piece.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int row = row0 + (lane & 31);
@@ -730,7 +730,8 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
 // room for a second wavefront on the SIMD, and the compiler then moves operands between the register
 // files. There, workgroups with blockIdx.y = 0 gather dK (three products) and the others dV (S again, two
 // products): five products for four, but two wavefronts a SIMD that fill each other's gaps. Measured at
-// 8192 tokens, 16 heads of 128: 1663 us together, KVSPLIT us apart. Smaller heads keep both in one.
+// 8192 tokens, 16 heads of 128, the whole backward: 2199 us together with one wavefront a SIMD, 2008 apart; causal
+// 1263 and 1123. Smaller heads keep both in one.
 template <typename T, int DP>
 constexpr bool kSplitKv = sizeof(T) == 2 && DP == 128;
 
@@ -1077,9 +1078,12 @@ struct FwdPlan {
 };
 // Measured: pieces of the tile kernel for 512 workgroups against 1024: 181 queries on three caches of 5000
 // 38 us against 43, 300 on two of 16000 87 us against 83; of the few-row kernel for 1024 against 2048: one
-// token on 32k keys 39 us against 43, on 131k (2 key heads) 51 us against 70.
+// token on 32k keys 39 us against 43, on 131k (2 key heads) 51 us against 70. Pieces of one length for all
+// documents against as many pieces for each: 100 queries on caches of 9000 and seven of 500 40 us against
+// 48, on eight of 3000 33 against 31 (workgroups that find no piece); 300 on 16000 and 1000 69 against 84.
+// Provided for a document six times the average rather than twice: 41, 43 and 69 us.
 constexpr int kFewSplitKeys = 1024, kTileSplitKeys = 256;
-constexpr int kFewBlocks = 1024, kTileBlocks = 512, kMaxSplits = 256;
+constexpr int kFewBlocks = 1024, kTileBlocks = 512, kMaxSplits = 256, kLongest = 2;
 
 static FwdPlan plan_fwd(const AttnArgs& a) {
   FwdPlan f;
@@ -1087,12 +1091,14 @@ static FwdPlan plan_fwd(const AttnArgs& a) {
   // mostly padding and each workgroup's keys one long chain.
   f.few = a.q_tokens * a.group <= 32 * static_cast<int64_t>(a.docs);
   f.tiles = tiles_of(a.q_tokens, a.group, f.few ? 32 : kAttnRows, a.docs);
-  // Pieces until the chip has its workgroups, each of split_keys at least. Ragged documents: up to twice
-  // the average length is provided for; a longer one gets longer pieces.
+  // Pieces until the chip has its workgroups, each of split_keys at least. A document's part of them goes
+  // by its length, which is known on the device only: up to kLongest times the average is provided for, a
+  // longer one gets longer pieces.
   const int64_t work = (f.few ? std::max<int64_t>(a.docs, a.q_tokens * a.group / 32)
                               : a.q_tokens * a.group / kAttnRows + 1) * a.kv_heads;
-  const int64_t keys = a.docs == 1 ? a.k_tokens : 2 * (a.k_tokens / a.docs);
-  const int64_t want = (f.few ? kFewBlocks : kTileBlocks) / work;
+  const int64_t longest = std::min<int64_t>(a.docs, kLongest);
+  const int64_t keys = a.k_tokens / a.docs * longest;
+  const int64_t want = (f.few ? kFewBlocks : kTileBlocks) * longest / work;
   const int64_t most = keys / (f.few ? kFewSplitKeys : kTileSplitKeys);
   f.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
   return f;
@@ -1121,7 +1127,10 @@ extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t w
   if (const int rc = attn_setup(p, a)) return rc;
   if (p->q_tokens == 0) return GS_OK;
   const FwdPlan f = plan_fwd(a);
-  GS_REQUIRE(f.tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG, "attention: too many tokens, documents or heads");
+  // a launch holds fewer than 2^32 threads
+  const int64_t threads = f.few ? (p->dtype == GS_BFLOAT16 ? kFewWaves<__bf16> : kFewWaves<float>) * kWave : kAttnThreads;
+  GS_REQUIRE(f.tiles * a.kv_heads * threads < (int64_t(1) << 32), GS_ERR_ARG,
+             "attention: too many tokens, documents or heads");
   GS_REQUIRE(workspace_bytes >= fwd_workspace(a, f) && (workspace || f.splits == 1), GS_ERR_WORKSPACE,
              "attention: workspace too small");
   GS_REQUIRE(aligned(workspace, 16), GS_ERR_ALIGN, "attention: workspace must be 16-byte aligned");
@@ -1130,6 +1139,7 @@ extern "C" int gs_attention_fwd(const gs_attention* p, void* workspace, size_t w
   a.splits = f.splits;
   a.split_keys = f.few ? kFewSplitKeys : kTileSplitKeys;
   a.split_unit = f.few ? 8 * 32 : kAttnKeys;
+  a.split_blocks = f.few ? kFewBlocks : kTileBlocks;
   const int64_t rows = a.q_tokens * a.heads;
   a.part = static_cast<float*>(workspace);
   a.part_stat = a.part + rows * a.splits * a.dim;
@@ -1206,7 +1216,7 @@ extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* 
   GS_REQUIRE(workspace_bytes >= need && (workspace || need == 0), GS_ERR_WORKSPACE,
              "attention backward: workspace too small");
   GS_REQUIRE(aligned(workspace, 16), GS_ERR_ALIGN, "attention backward: workspace must be 16-byte aligned");
-  GS_REQUIRE(b.q_tiles * a.kv_heads < (int64_t(1) << 31) && b.k_tiles * a.kv_heads < (int64_t(1) << 31), GS_ERR_ARG,
+  GS_REQUIRE(std::max(b.q_tiles, b.k_tiles) * a.kv_heads * kAttnThreads < (int64_t(1) << 32), GS_ERR_ARG,
              "attention: too many tokens, documents or heads");
   a.d_out = d_out;
   a.d_q = d_q;

@@ -148,8 +148,8 @@ struct AttnArgs {
   float* delta;
   int n_tiles;
   // keys of a row tile cut into up to `splits` pieces of at least split_keys, multiples of split_unit (what
-  // a workgroup takes in one step), joined by a second launch
-  int splits, split_keys, split_unit;
+  // a workgroup takes in one step), for about split_blocks workgroups in all; joined by a second launch
+  int splits, split_keys, split_unit, split_blocks;
   float* part;        // [splits][q_tokens][heads][dim], unnormalised
   float* part_stat;   // [splits][q_tokens][heads][2]: maximum (base 2), sum
   int32_t* part_n;    // [q_tokens][heads] pieces
@@ -290,16 +290,17 @@ enum { kPlain = 0, kCap = 1, kCapFixed = 2 };
 // stays below 2^90.
 constexpr float kFixedCap = 90.0f, kFixedTop = 60.0f;
 
-// The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one).
+// The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one) of
+// at least `share`.
 struct Piece {
   int begin, stop, n;
 };
-__device__ __forceinline__ Piece piece_of(const AttnArgs& a, int end, int split) {
+__device__ __forceinline__ Piece piece_of(const AttnArgs& a, int end, int split, int share) {
   if (a.splits == 1) return {0, end, 1};
-  int per = (end + a.splits - 1) / a.splits;
-  per = max((per + a.split_unit - 1) / a.split_unit * a.split_unit, a.split_keys);
+  const int per = (max((end + a.splits - 1) / a.splits, share) + a.split_unit - 1) / a.split_unit * a.split_unit;
   const int n = max(1, (end + per - 1) / per);
-  return {min(split * per, end), min((split + 1) * per, end), n};
+  const int begin = split < n ? split * per : end;
+  return {begin, begin + min(per, end - begin), n};
 }
 
 // The tokens in order belong to docs + 2 stretches: those before the first document's offset, the
@@ -329,6 +330,7 @@ struct Doc {
 struct Found {
   Doc doc;
   int64_t first;  // the stretch's first tile
+  int share;      // with splits: keys of a piece, the same for all documents
 };
 __device__ __forceinline__ int64_t pick(int64_t v, int lane) {
   const int lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
@@ -342,6 +344,7 @@ __device__ __forceinline__ Found find_doc(const AttnArgs& a, int64_t per, int ro
   const int64_t tokens = BY_KEYS ? a.k_tokens : a.q_tokens;
   Found f;
   Doc& d = f.doc;
+  f.share = a.split_keys;
   int i;
   int64_t q1, k1, len = INT32_MAX, prefix = 0;
   if (a.docs + 2 <= kWave) {
@@ -359,6 +362,16 @@ __device__ __forceinline__ Found find_doc(const AttnArgs& a, int64_t per, int ro
     k1 = i + 1 < a.docs + 2 ? pick(k, i + 1) : a.k_tokens;
     len = __builtin_amdgcn_readlane(n, i);
     prefix = __builtin_amdgcn_readlane(p, i);
+    if (!BY_KEYS && a.splits > 1) {
+      // pieces of a length that gives all row tiles' keys together split_blocks workgroups
+      const int64_t q_next = edge(a.q_offsets, a.q_tokens, a.docs, lane + 1);
+      const int64_t k_next = edge(a.k_offsets, a.k_tokens, a.docs, lane + 1);
+      const float tiles = static_cast<float>((max<int64_t>(q_next - q, 0) * per + rows - 1) / rows);
+      float work = real ? tiles * static_cast<float>(max<int64_t>(min<int64_t>(k_next - k, n), 0)) : 0.0f;
+#pragma unroll
+      for (int b = 1; b < kWave; b *= 2) work += __shfl_xor(work, b);
+      f.share = uniform(max(f.share, static_cast<int>(fminf(work * a.kv_heads / a.split_blocks, 1e9f))));
+    }
   } else {
     int lo = 0, n = a.docs + 2;  // the answer is in [lo, lo + n)
     while (n > 1) {

@@ -197,7 +197,9 @@ extern "C" int gs_rotary_axes(const gs_rotary* p, void* stream) {
   int64_t per = (8 * kRotaryThreads + items - 1) / items;
   per = std::min<int64_t>({per, kRotaryTable / a.pairs, (p->tokens + 1023) / 1024});
   a.tokens_per_block = static_cast<int>(std::max<int64_t>(1, per));
-  const dim3 grid(static_cast<unsigned>((p->tokens + a.tokens_per_block - 1) / a.tokens_per_block));
+  const int64_t blocks = (p->tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+  GS_REQUIRE(blocks * kRotaryThreads < (int64_t(1) << 32), GS_ERR_ARG, "rotary: too many tokens");
+  const dim3 grid(static_cast<unsigned>(blocks));
   const dim3 block(kRotaryThreads);
   const hipStream_t st = as_stream(stream);
   if (p->dtype == GS_BFLOAT16) {
