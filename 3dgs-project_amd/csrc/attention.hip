@@ -226,6 +226,9 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
     copies_done();
     __syncthreads();
     if (k0 + kAttnKeys < piece.stop) fetch(k0 + kAttnKeys, lds + (buf ^ 1) * 2 * kTileBytes);
+    // a wavefront past the last row only copies: its SIMD is the other workgroup's (8192 causal tokens, 16
+    // heads of 64: 201 -> 175 us, where registers count too; in the gradients' kernels it gains nothing)
+    if (uniform(wrow) >= rows) continue;
     f32x16 s[2] = {};
     {
       Frag<T> ka[C], kb[C];
