@@ -52,12 +52,16 @@ __device__ __forceinline__ void rotate(T u, T w, float2 cs, T* u1, T* w1) {
 // HBM-bound: every element is read and written once, in vectors of V. A workgroup takes a few tokens:
 // it forms their angles' cos and sin once, in LDS, for all heads of both tensors (a sincos costs as much
 // as moving some 30 elements), then its threads run over (token, head, V pairs), neighbours in memory
-// next to each other. V is 16 bytes' worth where the pairs, the copied rest, the strides and the
-// addresses are multiples of it, else one element. 32771 tokens, 16 + 16 heads of 64 bfloat16 out of a
+// next to each other. V is 16 bytes' worth at whatever address (the memory system splits an access that
+// crosses a line), less only where a head has fewer pairs or copied elements than that. The last vector of
+// the pairs and of the rest ends where they end: where V does not divide them it overlaps the one before,
+// and two threads write the same values to the same place. (One element a thread wherever 16 bytes do not
+// divide all: 30000 tokens, 24 bfloat16 heads of 96 with 45 pairs 147 us, so 84; 16 + 4 heads of 64 with 31
+// pairs 69 us, so 46; 4099 tokens, 9 float32 heads of 72 with 31 pairs 10.9 us, so 8.1.) 32771 tokens, 16 + 16 heads of 64 bfloat16 out of a
 // packed projection: 61 us, 4.4 TB/s (171 us with the angles formed per head and one element a thread).
 template <typename T, int V>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
-  using Vec = T __attribute__((ext_vector_type(V)));
+  typedef T Vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   __shared__ float2 table[kRotaryTable];
   const int64_t token0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block;
   const int n_tokens = static_cast<int>(min<int64_t>(a.tokens_per_block, a.tokens - token0));
@@ -70,7 +74,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
     table[e] = cs;
   }
   __syncthreads();
-  const int turns = a.pairs / V, per_head = turns + (a.dim - 2 * a.pairs) / V;
+  const int turns = (a.pairs + V - 1) / V, rest = a.dim - 2 * a.pairs, per_head = turns + (rest + V - 1) / V;
   const int heads = a.x[0].heads + a.x[1].heads;
   const int per_token = heads * per_head;
   // four items of a thread at a time, their loads first
@@ -90,7 +94,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
       head -= which ? a.x[0].heads : 0;
       const RotaryTensor& x = a.x[which];
       const int64_t token = token0 + t;
-      const int p = c * V, i = c >= turns ? p + a.pairs : a.adjacent ? 2 * p : p;
+      const int p = min(c * V, a.pairs - V);
+      const int i = c >= turns ? 2 * a.pairs + min((c - turns) * V, rest - V) : a.adjacent ? 2 * p : p;
       const T* in = static_cast<const T*>(x.in) + token * x.token_stride + head * x.head_stride + i;
       to[q] = static_cast<T*>(x.out) + (token * x.heads + head) * a.dim + i;
       at[q] = c >= turns ? -1 : t * a.pairs + p;
@@ -183,16 +188,12 @@ extern "C" int gs_rotary_axes(const gs_rotary* p, void* stream) {
       a.freq_hi[i] = static_cast<float>(f);
       a.freq_lo[i] = static_cast<float>(f - a.freq_hi[i]);
     }
-  const auto fits = [&](int v) {
-    bool ok = a.pairs % v == 0 && p->dim % v == 0;
-    for (const RotaryTensor& x : a.x)
-      ok = ok && (x.heads == 0 || (x.token_stride % v == 0 && x.head_stride % v == 0 && aligned(x.in, v * es) &&
-                                   aligned(x.out, v * es)));
-    return ok;
-  };
-  const int v = fits(static_cast<int>(16 / es)) ? static_cast<int>(16 / es) : 1;
+  // the widest vector that fits into the pairs and into the rest
+  const int rest = p->dim - 2 * a.pairs;
+  int v = static_cast<int>(16 / es);
+  while (v > 1 && (a.pairs < v || (rest > 0 && rest < v))) v /= 2;
   // Tokens of a workgroup: eight items a thread, if that leaves workgroups for the whole chip.
-  const int64_t items = static_cast<int64_t>(p->q_heads + p->k_heads) * ((p->dim - a.pairs) / v);
+  const int64_t items = static_cast<int64_t>(p->q_heads + p->k_heads) * ((a.pairs + v - 1) / v + (rest + v - 1) / v);
   GS_REQUIRE(items < (1 << 26), GS_ERR_ARG, "rotary: too many heads");
   int64_t per = (8 * kRotaryThreads + items - 1) / items;
   per = std::min<int64_t>({per, kRotaryTable / a.pairs, (p->tokens + 1023) / 1024});
@@ -202,12 +203,16 @@ extern "C" int gs_rotary_axes(const gs_rotary* p, void* stream) {
   const dim3 grid(static_cast<unsigned>(blocks));
   const dim3 block(kRotaryThreads);
   const hipStream_t st = as_stream(stream);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, a); };
   if (p->dtype == GS_BFLOAT16) {
-    if (v == 8) hipLaunchKernelGGL((rotary_kernel<__bf16, 8>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((rotary_kernel<__bf16, 1>), grid, block, 0, st, a);
+    if (v == 8) launch(rotary_kernel<__bf16, 8>);
+    else if (v == 4) launch(rotary_kernel<__bf16, 4>);
+    else if (v == 2) launch(rotary_kernel<__bf16, 2>);
+    else launch(rotary_kernel<__bf16, 1>);
   } else {
-    if (v == 4) hipLaunchKernelGGL((rotary_kernel<float, 4>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((rotary_kernel<float, 1>), grid, block, 0, st, a);
+    if (v == 4) launch(rotary_kernel<float, 4>);
+    else if (v == 2) launch(rotary_kernel<float, 2>);
+    else launch(rotary_kernel<float, 1>);
   }
   return check_launch("rotary");
 }

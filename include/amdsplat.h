@@ -599,7 +599,8 @@ int gs_grad_scale(const void* const* grads, void* const* out, const int64_t* siz
  * on the elements (p, p + P), or with GS_ROTARY_ADJACENT (2 p, 2 p + 1); the elements from 2 P on
  * are copied. GS_ROTARY_INVERSE negates the angle (the gradient). q [tokens, q_heads, dim] and k
  * [tokens, k_heads, dim] (k_heads 0: none) are read through their strides (elements; the last
- * dimension is contiguous) and written contiguously. positions: [tokens, axes] float32.
+ * dimension is contiguous) and written contiguously, to memory that overlaps no input. positions:
+ * [tokens, axes] float32.
  * ------------------------------------------------------------------------------------- */
 #define GS_ROTARY_MAX_AXES 4
 #define GS_ROTARY_MAX_PAIRS 256

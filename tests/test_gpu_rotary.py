@@ -156,3 +156,18 @@ def test_refusals():
     ]:
         with pytest.raises(ValueError, match=text):
             rotary_axes(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("pairing", ["half", "adjacent"])
+@pytest.mark.parametrize("dim,pairs", [(8, 1), (9, 1), (11, 4), (17, 8), (18, 8), (20, 8), (24, 8), (25, 8), (45, 17),
+                                       (64, 31), (70, 32), (31, 15), (16, 3), (22, 7)])
+def test_pairs_and_rest_beside_the_vector(dim, pairs, pairing, dtype):
+    """Pair counts and copied rests that fill no vector, one vector, or one and a part, out of a packed
+    projection at an odd element."""
+    rows, pos = data(53, 5, dim + 3, dtype, dim, 1)
+    for x in (rows[:, :, :dim], rows[:, 1:, 3:]):
+        got, other = rotary_axes(x, rows[:, :2, 1:dim + 1], pos, (pairs,), pairing=pairing)
+        check(got, formula(x, pos, (pairs,), 10000.0, pairing, "axis"))
+        check(other, formula(rows[:, :2, 1:dim + 1], pos, (pairs,), 10000.0, pairing, "axis"))
+        assert torch.equal(got[..., 2 * pairs:], x[..., 2 * pairs:])
