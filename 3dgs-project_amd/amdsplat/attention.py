@@ -72,11 +72,14 @@ class _Attention(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix)
         ctx.rule = (causal, softcap, scale)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)  # (a zero gradient for lse would be a launch that nothing reads)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, _d_lse):
+        if d_out is None:
+            return (None,) * 10
         q, k, v, out, low, lse, offsets, k_offsets, k_lengths, prefix = ctx.saved_tensors
         d_out = d_out.contiguous()
         if d_out.numel() and d_out.data_ptr() % 16:
