@@ -152,7 +152,7 @@ class FusedAdam(torch.optim.Adam):
         norm = scale = None
         if max_norm is not None:
             if not grads:
-                return torch.zeros(())
+                return torch.zeros((), device=self.param_groups[0]["params"][0].device)
             norm, scale = clip_coefficient(grads, max_norm)
         for (n_prim, _, device), (vis, groups) in batches.items():
             _launch(groups, n_prim, _visibility(vis, n_prim), device, scale)
