@@ -14,6 +14,13 @@ constexpr int kAttnThreads = kAttnWaves * kWave;
 constexpr int kAttnRows = kAttnWaves * 32;  // query rows (or keys, in the key gradients) of a workgroup
 constexpr int kAttnKeys = 64;               // keys (or query rows) of a tile in LDS
 
+// Kernels are instances for heads of up to DU = 32, 64, 96 or 128 elements: what they multiply and hold in
+// registers. A row of a tile in LDS is a power of two, so that its chunks can be permuted.
+// With instances for 64 and 128 alone, forward and backward: 8192 bfloat16 tokens, 16 heads of 96 513 and 2007
+// us, so 457 and 1765; of 32 323 and 933 us, so 265 and 740; 2500 float32 tokens, 16 heads of 96, causal, 368
+// and 1731 us, so 284 and 942. 64 and 128 are the same either way.
+constexpr int row_of(int du) { return du > 64 ? 128 : 64; }
+
 // Base-2 exponent of a score, up to the reference that p = 2^(x - ref) takes off. Plain scores stay as
 // they come (monotone in x: the scale is positive) and are scaled in the same fma that subtracts.
 struct Rule {
@@ -144,18 +151,18 @@ __device__ __forceinline__ bool any_not_finite(const f32x16 (&o)[M]) {
   return __any(!(t == 0.0f));
 }
 // Keys begin .. begin + 31, then `step` further on, below `vis`.
-template <typename T, int DP, int MODE>
-__device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, const Frag<T> (&q)[DP / 16], const T* kp,
+template <typename T, int DU, int MODE>
+__device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, const Frag<T> (&q)[DU / 16], const T* kp,
                                              const T* vp, float m, int begin, int step, int vis, int h,
-                                             f32x16 (&o)[DP / 32]) {
+                                             f32x16 (&o)[DU / 32]) {
   const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) o[i] = f32x16{};
+  for (int i = 0; i < DU / 32; ++i) o[i] = f32x16{};
   for (int k0 = begin; k0 < vis; k0 += step)
     for (int key = k0; key < min(k0 + 32, vis); ++key) {
       float s = 0.0f;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
+      for (int c = 0; c < DU / 16; ++c) {
         const int d = 16 * c + 8 * h;
         const Frag<T> k = load_frag<T>(kp + key * a.k_token + d, d < a.dim);
 #pragma unroll
@@ -164,7 +171,7 @@ __device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, c
       s = exponent<T, MODE>(u, half_sum(s));
       const float p = static_cast<float>(static_cast<T>(prob<MODE>(u, s, ref)));
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
+      for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
           const int d = 32 * dt + 2 * r + 4 * h;
@@ -180,10 +187,10 @@ __device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, c
 // shorter (8203 tokens in 4 documents, 16 heads: 112 -> 102 us; 8192 in one, four full rounds, 315 either
 // way). The causal instance would spill a little: 8192 tokens 179 -> 170 us plain, but 220 -> 225 capped, and
 // 100 queries on eight caches of 3000 30 -> 32.
-template <typename T, int DP, int MODE, bool CAUSAL>
-__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
-  using L = Tile<T, DP>;
-  constexpr int C = DP / 16;
+template <typename T, int DU, int MODE, bool CAUSAL>
+__global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DU <= 64 && !CAUSAL ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
+  using L = Tile<T, row_of(DU)>;
+  constexpr int C = DU / 16;
   constexpr int kTileBytes = kAttnKeys * L::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
@@ -209,11 +216,11 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
   const int vis = visible(a, doc, tok);
   const int wave_min = visible(a, doc, min(wrow, rows - 1) / a.group);
   const Rule rule = rule_of<MODE>(a);
-  f32x16 o[DP / 32] = {};
+  f32x16 o[DU / 32] = {};
   Softmax st;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
-  const TileCopy<T, DP, kAttnKeys, kAttnThreads> copy_k(a.k_token, a.dim), copy_v(a.v_token, a.dim);
+  const TileCopy<T, row_of(DU), kAttnKeys, kAttnThreads> copy_k(a.k_token, a.dim), copy_v(a.v_token, a.dim);
   const auto fetch = [&](int k0, char* to) {
     const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
     copy_k(to, row_buffer(kp + k0 * a.k_token, a.k_token, valid, a.dim));
@@ -243,9 +250,9 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
 #pragma unroll
       for (int c = 0; c < C; ++c) mma(s[1], kb[c], q[c]);
     }
-    Frag<T> v[2][DP / 32];
+    Frag<T> v[2][DU / 32];
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) v[0][dt] = L::cols(lv, 32 * dt, 0, lane);
+    for (int dt = 0; dt < DU / 32; ++dt) v[0][dt] = L::cols(lv, 32 * dt, 0, lane);
     keep_order<T>();
     softmax_step<T, MODE>(rule, s, o, st, k0 + kAttnKeys > wave_min, vis - k0, h);
     // the wavefront that has its probabilities goes first: its products then run while the SIMD's other
@@ -255,12 +262,12 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
     for (int kc = 0; kc < 4; ++kc) {
       if (kc < 3) {
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) v[(kc + 1) & 1][dt] = L::cols(lv, 32 * dt, 16 * (kc + 1), lane);
+        for (int dt = 0; dt < DU / 32; ++dt) v[(kc + 1) & 1][dt] = L::cols(lv, 32 * dt, 16 * (kc + 1), lane);
         keep_order<T>();
       }
       const Frag<T> p = acc_frag<T>(s[kc / 2], kc % 2);
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) mma(o[dt], v[kc & 1][dt], p);
+      for (int dt = 0; dt < DU / 32; ++dt) mma(o[dt], v[kc & 1][dt], p);
     }
     __builtin_amdgcn_s_setprio(0);
   }
@@ -268,7 +275,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
   // elements, 251 -> 266 us at 64, capped)
   if constexpr (CAUSAL) {
     if (any_not_finite(o))
-      sums_of_seen<T, DP, MODE>(a, rule, q, kp, vp, st.m, piece.begin, 32, min(vis, piece.stop), h, o);
+      sums_of_seen<T, DU, MODE>(a, rule, q, kp, vp, st.m, piece.begin, 32, min(vis, piece.stop), h, o);
   }
   if (!live) return;
   const float m = st.m, l = half_sum(st.l);
@@ -277,7 +284,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
     const int64_t part = blockIdx.y * a.q_tokens * a.heads + at;
     float* pp = a.part + part * a.dim;
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const int d = 32 * dt + 2 * r + 4 * h;
@@ -293,7 +300,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t at = (doc.q0 + tok) * a.heads + head;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * h;
@@ -312,14 +319,14 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DP == 64 && !CAUSAL
 // bfloat16: eight wavefronts, so that a short document is a few steps long. float32's tiles allow four.
 template <typename T>
 constexpr int kFewWaves = sizeof(T) == 2 ? 8 : 4;
-template <typename T, int DP, int MODE, bool CAUSAL>
+template <typename T, int DU, int MODE, bool CAUSAL>
 __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs a) {
   constexpr int kWaves = kFewWaves<T>;
-  using L = Tile<T, DP>;
-  constexpr int C = DP / 16;
+  using L = Tile<T, row_of(DU)>;
+  constexpr int C = DU / 16;
   constexpr int kLoads = 32 * L::kChunks / kWave;  // 16-byte loads a lane for 32 rows
   constexpr int kTileBytes = 32 * L::kRowBytes;
-  static_assert(2 * kTileBytes >= 32 * DP * 4, "the join reuses the wavefront's tiles");
+  static_assert(2 * kTileBytes >= 32 * DU * 4, "the join reuses the wavefront's tiles");
   __shared__ __attribute__((aligned(16))) char lds[kWaves * 2 * kTileBytes];
   __shared__ float l_m[kWaves][32], l_l[kWaves][32];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
@@ -342,7 +349,7 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
   const int vis = min(visible(a, doc, tok), piece.stop);
   const int all_min = min(visible(a, doc, row0 / a.group), piece.stop);
   const Rule rule = rule_of<MODE>(a);
-  f32x16 o[DP / 32] = {};
+  f32x16 o[DU / 32] = {};
   Softmax st;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
@@ -393,7 +400,7 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
         for (int j = 0; j < 8; ++j) low[j] = static_cast<T>(s[0][8 * kc + j] - static_cast<float>(p[j]));
       }
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
+      for (int dt = 0; dt < DU / 32; ++dt) {
         const Frag<T> v = L::cols(lv, 32 * dt, 16 * kc, lane);
         mma(o[dt], v, p);
         if constexpr (sizeof(T) == 2) mma(o[dt], v, low);
@@ -403,7 +410,7 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
   }
   if constexpr (CAUSAL) {
     if (any_not_finite(o))
-      sums_of_seen<T, DP, MODE>(a, rule, q, kp, vp, st.m, piece.begin + wave * 32, kWaves * 32, vis, h, o);
+      sums_of_seen<T, DU, MODE>(a, rule, q, kp, vp, st.m, piece.begin + wave * 32, kWaves * 32, vis, h, o);
   }
   // join: every wavefront leaves its rows, statistics and (in its own tiles) sums; then all threads
   // take the same rows' elements and add the wavefronts' in order
@@ -415,14 +422,14 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
       l_l[wave][lane & 31] = l;
     }
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
       for (int r = 0; r < 16; r += 4)
-        store4(own + (lane & 31) * DP + 32 * dt + 2 * r + 4 * h, o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
+        store4(own + (lane & 31) * DU + 32 * dt + 2 * r + 4 * h, o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < n_rows * (DP / 4); e += kWaves * kWave) {
-    const int i = e / (DP / 4), d = e % (DP / 4) * 4;
+  for (int e = threadIdx.x; e < n_rows * (DU / 4); e += kWaves * kWave) {
+    const int i = e / (DU / 4), d = e % (DU / 4) * 4;
     float top = l_m[0][i];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) top = fmaxf(top, l_m[w][i]);
@@ -433,7 +440,7 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
     for (int w = 0; w < kWaves; ++w) {
       const float f = exp2_hw(l_m[w][i] - ref);
       sum += f * l_l[w][i];
-      x += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 2 * kTileBytes) + i * DP + d);
+      x += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * 2 * kTileBytes) + i * DU + d);
     }
     const int t = (row0 + i) / a.group;
     const int64_t at = (doc.q0 + t) * a.heads + hk * a.group + row0 + i - t * a.group;
@@ -513,33 +520,33 @@ __device__ __forceinline__ void interleave() {
 }
 
 // The fragments of 32 rows of a tile, along (rows) and across (cols).
-template <typename T, int DP>
+template <typename T, int DU>
 struct Rows {
-  Frag<T> f[DP / 16];
+  Frag<T> f[DU / 16];
   __device__ __forceinline__ void read(const char* lds, int row0, int lane) {
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) f[c] = Tile<T, DP>::rows(lds, row0, c, lane);
+    for (int c = 0; c < DU / 16; ++c) f[c] = Tile<T, row_of(DU)>::rows(lds, row0, c, lane);
   }
-  __device__ __forceinline__ void times(const Frag<T> (&b)[DP / 16], f32x16& acc) const {
+  __device__ __forceinline__ void times(const Frag<T> (&b)[DU / 16], f32x16& acc) const {
     acc = f32x16{};
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) mma(acc, f[c], b[c]);
+    for (int c = 0; c < DU / 16; ++c) mma(acc, f[c], b[c]);
   }
 };
-template <typename T, int DP>
+template <typename T, int DU>
 struct Cols {
-  Frag<T> f[2][DP / 32];
+  Frag<T> f[2][DU / 32];
   __device__ __forceinline__ void read(const char* lds, int row0, int lane) {
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) f[kc][dt] = Tile<T, DP>::cols(lds, 32 * dt, row0 + 16 * kc, lane);
+      for (int dt = 0; dt < DU / 32; ++dt) f[kc][dt] = Tile<T, row_of(DU)>::cols(lds, 32 * dt, row0 + 16 * kc, lane);
   }
-  __device__ __forceinline__ void add_times(const Frag<T> (&p)[2], f32x16 (&acc)[DP / 32]) const {
+  __device__ __forceinline__ void add_times(const Frag<T> (&p)[2], f32x16 (&acc)[DU / 32]) const {
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) mma(acc[dt], f[kc][dt], p[kc]);
+      for (int dt = 0; dt < DU / 32; ++dt) mma(acc[dt], f[kc][dt], p[kc]);
   }
 };
 template <typename T>
@@ -549,24 +556,24 @@ __device__ __forceinline__ void acc_frags(const f32x16& c, Frag<T> (&f)[2]) {
 }
 
 // The same products in float32, whose fragments are twice as large: read as they are used.
-template <int DP>
-__device__ __forceinline__ void rows_times(const char* lds, int row0, int lane, const f32x8 (&b)[DP / 16], f32x16& acc) {
+template <int DU>
+__device__ __forceinline__ void rows_times(const char* lds, int row0, int lane, const f32x8 (&b)[DU / 16], f32x16& acc) {
   acc = f32x16{};
 #pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    mma(acc, Tile<float, DP>::rows(lds, row0, c, lane), b[c]);
+  for (int c = 0; c < DU / 16; ++c) {
+    mma(acc, Tile<float, row_of(DU)>::rows(lds, row0, c, lane), b[c]);
     if (c % 2) __builtin_amdgcn_sched_barrier(0);
   }
 }
-template <int DP>
+template <int DU>
 __device__ __forceinline__ void add_cols_times(const char* lds, int row0, int lane, const f32x16& p,
-                                               f32x16 (&acc)[DP / 32]) {
+                                               f32x16 (&acc)[DU / 32]) {
 #pragma unroll
   for (int kc = 0; kc < 2; ++kc) {
     const f32x8 f = acc_frag<float>(p, kc);
 #pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) {
-      mma(acc[dt], Tile<float, DP>::cols(lds, 32 * dt, row0 + 16 * kc, lane), f);
+    for (int dt = 0; dt < DU / 32; ++dt) {
+      mma(acc[dt], Tile<float, row_of(DU)>::cols(lds, 32 * dt, row0 + 16 * kc, lane), f);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -595,10 +602,10 @@ __device__ __forceinline__ float prob_of(const Rule& u, float s, float base, flo
 
 // Query gradients, and delta_i = dO_i . O_i for the key gradients. Like the forward, a lane owns a
 // query; its score gradients are the B operand of dQ = dS K.
-template <typename T, int DP, int MODE>
+template <typename T, int DU, int MODE>
 __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd_q_kernel(AttnArgs a) {
-  using L = Tile<T, DP>;
-  constexpr int C = DP / 16;
+  using L = Tile<T, row_of(DU)>;
+  constexpr int C = DU / 16;
   constexpr int kTileBytes = kAttnKeys * L::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTileBytes];
   const int hk = static_cast<int>(blockIdx.x % a.kv_heads);
@@ -624,7 +631,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   const int tok = rc / a.group, head = hk * a.group + rc - tok * a.group;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
   const T* vp = static_cast<const T*>(a.v) + doc.k0 * a.v_token + hk * a.v_head;
-  const TileCopy<T, DP, kAttnKeys, kAttnThreads> copy_k(a.k_token, a.dim), copy_v(a.v_token, a.dim);
+  const TileCopy<T, row_of(DU), kAttnKeys, kAttnThreads> copy_k(a.k_token, a.dim), copy_v(a.v_token, a.dim);
   const auto fetch = [&](int k0, char* to) {
     const int valid = min(kAttnKeys, static_cast<int>(doc.k_len) - k0);
     copy_k(to, row_buffer(kp + k0 * a.k_token, a.k_token, valid, a.dim));
@@ -656,7 +663,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   const float row_base = base_of<T, MODE>(rule, a.lse[stat]);
   const int vis = live ? visible(a, doc, tok) : 0;
   const int wave_min = wrow + 31 < rows ? visible(a, doc, wrow / a.group) : 0;
-  f32x16 dq[DP / 32] = {};
+  f32x16 dq[DU / 32] = {};
   int buf = 0;
   for (int k0 = begin; k0 < end; k0 += kAttnKeys, buf ^= 1) {
     const char* lk = lds + buf * 2 * kTileBytes;
@@ -682,8 +689,8 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
           for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
         };
         if constexpr (sizeof(T) == 2) {
-          Rows<T, DP> x, y;
-          Cols<T, DP> z;
+          Rows<T, DU> x, y;
+          Cols<T, DU> z;
           Frag<T> f[2];
           x.read(lk, 32 * t, lane);
           y.read(lv, 32 * t, lane);
@@ -699,11 +706,11 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
           z.add_times(f, dq);
           keep_order<T>();
         } else {
-          rows_times<DP>(lk, 32 * t, lane, q, s);
-          rows_times<DP>(lv, 32 * t, lane, g, dp);
+          rows_times<DU>(lk, 32 * t, lane, q, s);
+          rows_times<DU>(lv, 32 * t, lane, g, dp);
           probs();
           grads();
-          add_cols_times<DP>(lk, 32 * t, lane, s, dq);
+          add_cols_times<DU>(lk, 32 * t, lane, s, dq);
         }
       }
     };
@@ -713,7 +720,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   if (!live) return;
   T* to = static_cast<T*>(a.d_q) + at;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * h;
@@ -736,21 +743,21 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
 // products): five products for four, but two wavefronts a SIMD that fill each other's gaps. Measured at
 // 8192 tokens, 16 heads of 128, the whole backward: 2199 us together with one wavefront a SIMD, 2008 apart; causal
 // 1263 and 1123. Smaller heads keep both in one.
-template <typename T, int DP>
-constexpr bool kSplitKv = sizeof(T) == 2 && DP == 128;
+template <typename T, int DU>
+constexpr bool kSplitKv = sizeof(T) == 2 && DU > 64;
 
 constexpr int kKvRows = 64;  // query rows of a tile
-template <typename T, int DP>
+template <typename T, int DU>
 struct KvShared {
-  char tiles[4 * kKvRows * Tile<T, DP>::kRowBytes];
+  char tiles[4 * kKvRows * Tile<T, row_of(DU)>::kRowBytes];
   float base[2][kKvRows], delta[2][kKvRows];
   int vis[2][kKvRows];
 };
 
-template <typename T, int DP, int MODE, bool DK, bool DV>
-__device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& sh) {
-  using L = Tile<T, DP>;
-  constexpr int C = DP / 16;
+template <typename T, int DU, int MODE, bool DK, bool DV>
+__device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DU>& sh) {
+  using L = Tile<T, row_of(DU)>;
+  constexpr int C = DU / 16;
   constexpr int R = kKvRows;
   constexpr int kTileBytes = R * L::kRowBytes;
   char* lds = sh.tiles;
@@ -783,8 +790,8 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
     row_begin += from;
     row_end = min(row_begin + per, rows);
   }
-  const RowTileCopy<T, DP, R, kAttnThreads> copy_q = {a.q_token, a.q_head};
-  const RowTileCopy<T, DP, R, kAttnThreads> copy_g = {static_cast<int64_t>(a.heads) * a.dim, a.dim};
+  const RowTileCopy<T, row_of(DU), R, kAttnThreads> copy_q = {a.q_token, a.q_head};
+  const RowTileCopy<T, row_of(DU), R, kAttnThreads> copy_g = {static_cast<int64_t>(a.heads) * a.dim, a.dim};
   const Rule rule = rule_of<MODE>(a);
   float n_lse = 0.0f, n_delta = 0.0f;
   int n_vis = 0;
@@ -824,7 +831,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
     if (a.scale < 0.0f) k[c] = -k[c];
     if constexpr (DK) v[c] = load_frag<T>(vp + 16 * c + 8 * h, in);
   }
-  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+  f32x16 dk[DU / 32] = {}, dv[DU / 32] = {};
   int buf = 0;
   for (int r0 = row_begin; r0 < row_end; r0 += R, buf ^= 1) {
     const char* lq = lds + buf * 2 * kTileBytes;
@@ -870,8 +877,8 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
         if constexpr (sizeof(T) == 2) {
           // products of C matrix instructions; the probabilities are formed in the second's shadow, the
           // score gradients in the third's, and an operand is read during the product before its own
-          Rows<T, DP> x, y;
-          Cols<T, DP> zg, zq;
+          Rows<T, DU> x, y;
+          Cols<T, DU> zg, zq;
           Frag<T> f[2], e[2];
           x.read(lq, 32 * t, lane);
           if constexpr (DK && DV) y.read(lg, 32 * t, lane);
@@ -898,12 +905,12 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
           }
           keep_order<T>();
         } else {
-          rows_times<DP>(lq, 32 * t, lane, k, s);
-          rows_times<DP>(lg, 32 * t, lane, v, dp);
+          rows_times<DU>(lq, 32 * t, lane, k, s);
+          rows_times<DU>(lg, 32 * t, lane, v, dp);
           probs();
           grads();
-          add_cols_times<DP>(lg, 32 * t, lane, s, dv);
-          add_cols_times<DP>(lq, 32 * t, lane, dp, dk);
+          add_cols_times<DU>(lg, 32 * t, lane, s, dv);
+          add_cols_times<DU>(lq, 32 * t, lane, dp, dk);
         }
       }
     };
@@ -915,7 +922,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
   T* dkp = static_cast<T*>(a.d_k) + at;
   T* dvp = static_cast<T*>(a.d_v) + at;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       const int d = 32 * dt + 2 * r + 4 * h;
@@ -937,12 +944,12 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DP>& 
     }
 }
 
-template <typename T, int DP, int MODE>
+template <typename T, int DU, int MODE>
 __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kv_kernel(AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) KvShared<T, DP> sh;
-  if constexpr (!kSplitKv<T, DP>) attn_bwd_kv<T, DP, MODE, true, true>(a, sh);
-  else if (blockIdx.y == 0) attn_bwd_kv<T, DP, MODE, true, false>(a, sh);
-  else attn_bwd_kv<T, DP, MODE, false, true>(a, sh);
+  __shared__ __attribute__((aligned(16))) KvShared<T, DU> sh;
+  if constexpr (!kSplitKv<T, DU>) attn_bwd_kv<T, DU, MODE, true, true>(a, sh);
+  else if (blockIdx.y == 0) attn_bwd_kv<T, DU, MODE, true, false>(a, sh);
+  else attn_bwd_kv<T, DU, MODE, false, true>(a, sh);
 }
 
 // Adds parts' gradients, in order, four elements a thread: blockIdx.y picks the first or the second.
@@ -1031,40 +1038,41 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
 // Tiles of `rows` rows that `tokens` tokens of `per` rows in docs + 2 stretches can take.
 static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { return tokens * per / rows + docs + 2; }
 
-template <template <typename, int, int> class K, typename T, int DP>
+template <template <typename, int, int> class K, typename T, int DU>
 static void launch_mode(const AttnArgs& a, dim3 grid, hipStream_t st) {
-  if (a.softcap == 0.0f) K<T, DP, kPlain>::launch(a, grid, st);
-  else if (K<T, DP, kCap>::kFixed && a.softcap * kLog2e <= kFixedCap) K<T, DP, kCapFixed>::launch(a, grid, st);
-  else K<T, DP, kCap>::launch(a, grid, st);
+  if (a.softcap == 0.0f) K<T, DU, kPlain>::launch(a, grid, st);
+  else if (K<T, DU, kCap>::kFixed && a.softcap * kLog2e <= kFixedCap) K<T, DU, kCapFixed>::launch(a, grid, st);
+  else K<T, DU, kCap>::launch(a, grid, st);
 }
 template <template <typename, int, int> class K>
 static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts, hipStream_t st) {
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(parts), static_cast<unsigned>(a.row_parts));
-  if (dtype == GS_BFLOAT16) {
-    if (a.dim > 64) launch_mode<K, __bf16, 128>(a, grid, st);
-    else launch_mode<K, __bf16, 64>(a, grid, st);
-  } else {
-    if (a.dim > 64) launch_mode<K, float, 128>(a, grid, st);
-    else launch_mode<K, float, 64>(a, grid, st);
-  }
+  const auto by_type = [&](auto du) {
+    if (dtype == GS_BFLOAT16) launch_mode<K, __bf16, du.value>(a, grid, st);
+    else launch_mode<K, float, du.value>(a, grid, st);
+  };
+  if (a.dim > 96) by_type(std::integral_constant<int, 128>{});
+  else if (a.dim > 64) by_type(std::integral_constant<int, 96>{});
+  else if (a.dim > 32) by_type(std::integral_constant<int, 64>{});
+  else by_type(std::integral_constant<int, 32>{});
 }
 // Forward kernels have an instance for the fixed cap and one for the causal mask, the backward's do not.
 #define GS_ATTN_FORWARD(NAME, KERNEL, THREADS)                                                            \
-  template <typename T, int DP, int MODE>                                                                 \
+  template <typename T, int DU, int MODE>                                                                 \
   struct NAME {                                                                                           \
     static constexpr bool kFixed = true;                                                                  \
     static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                                    \
-      if (a.causal) hipLaunchKernelGGL((KERNEL<T, DP, MODE, true>), grid, dim3(THREADS), 0, st, a);       \
-      else hipLaunchKernelGGL((KERNEL<T, DP, MODE, false>), grid, dim3(THREADS), 0, st, a);               \
+      if (a.causal) hipLaunchKernelGGL((KERNEL<T, DU, MODE, true>), grid, dim3(THREADS), 0, st, a);       \
+      else hipLaunchKernelGGL((KERNEL<T, DU, MODE, false>), grid, dim3(THREADS), 0, st, a);               \
     }                                                                                                     \
   }
 #define GS_ATTN_BACKWARD(NAME, KERNEL)                                                                    \
-  template <typename T, int DP, int MODE>                                                                 \
+  template <typename T, int DU, int MODE>                                                                 \
   struct NAME {                                                                                           \
     static constexpr bool kFixed = false;                                                                 \
     static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                                    \
       constexpr int mode = MODE == kPlain ? kPlain : kCap;                                                \
-      hipLaunchKernelGGL((KERNEL<T, DP, mode>), grid, dim3(kAttnThreads), 0, st, a);                      \
+      hipLaunchKernelGGL((KERNEL<T, DU, mode>), grid, dim3(kAttnThreads), 0, st, a);                      \
     }                                                                                                     \
   }
 GS_ATTN_FORWARD(FwdKernel, attn_fwd_kernel, kAttnThreads);
