@@ -737,14 +737,17 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
 // 64 at a time. Rows past the document's end need no mask: their q, dO and delta are zero (and p finite), and so
 // is what they add. The lanes of keys past the valid length gather nothing that is kept.
 //
-// At 128 elements of bfloat16 both gradients' accumulators (128 registers beside K and V's 64) leave no
+// At 96 and 128 elements of bfloat16 both gradients' accumulators (128 registers beside K and V's 64) leave no
 // room for a second wavefront on the SIMD, and the compiler then moves operands between the register
 // files. There, workgroups with blockIdx.y = 0 gather dK (three products) and the others dV (S again, two
 // products): five products for four, but two wavefronts a SIMD that fill each other's gaps. Measured at
 // 8192 tokens, 16 heads of 128, the whole backward: 2199 us together with one wavefront a SIMD, 2008 apart; causal
-// 1263 and 1123. Smaller heads keep both in one.
+// 1263 and 1123. In float32 it is 128 elements at which both do not fit one wavefront's 512 registers: 2500
+// tokens, 16 heads, causal, the whole backward 1804 us together (115 registers spilled) and 1428 apart, capped 2079
+// and 1568; without the mask, whose code spills most, 2669 and 2713. Smaller heads keep both in one.
+constexpr bool split_kv(bool bf16, int dim) { return dim > (bf16 ? 64 : 96); }
 template <typename T, int DU>
-constexpr bool kSplitKv = sizeof(T) == 2 && DU > 64;
+constexpr bool kSplitKv = split_kv(sizeof(T) == 2, DU);
 
 constexpr int kKvRows = 64;  // query rows of a tile
 template <typename T, int DU>
@@ -906,11 +909,11 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DU>& 
           keep_order<T>();
         } else {
           rows_times<DU>(lq, 32 * t, lane, k, s);
-          rows_times<DU>(lg, 32 * t, lane, v, dp);
+          if constexpr (DK) rows_times<DU>(lg, 32 * t, lane, v, dp);
           probs();
-          grads();
-          add_cols_times<DU>(lg, 32 * t, lane, s, dv);
-          add_cols_times<DU>(lq, 32 * t, lane, dp, dk);
+          if constexpr (DK) grads();
+          if constexpr (DV) add_cols_times<DU>(lg, 32 * t, lane, s, dv);
+          if constexpr (DK) add_cols_times<DU>(lq, 32 * t, lane, dp, dk);
         }
       }
     };
@@ -1186,7 +1189,7 @@ static BwdPlan plan_bwd(const AttnArgs& a, int dtype) {
   BwdPlan b;
   b.q_tiles = tiles_of(a.q_tokens, a.group, kAttnRows, a.docs);
   b.k_tiles = tiles_of(a.k_tokens, 1, kAttnRows, a.docs);
-  b.kv_roles = dtype == GS_BFLOAT16 && kSplitKv<__bf16, 128> && a.dim > 64 ? 2 : 1;
+  b.kv_roles = split_kv(dtype == GS_BFLOAT16, a.dim) ? 2 : 1;
   const int64_t blocks = (a.k_tokens + kAttnRows - 1) / kAttnRows * a.kv_heads * b.kv_roles;
   const int64_t rows = a.q_tokens * a.group / a.docs;
   const int64_t want = blocks > 0 ? (a.causal ? 4 : 2) * 512 / blocks : 1;
