@@ -190,11 +190,11 @@ __device__ __forceinline__ f32x4 load16(__amdgpu_buffer_rsrc_t b, uint32_t offse
 // wavefront's own, a barrier after it for the others'. The LDS side is linear in the lanes, so it is
 // the global side that a lane permutes: it fetches the chunk that belongs to its place in the tile.
 // The instruction is written out because the compiler, given its builtin, waits for every copy under
-// way before each transposed LDS read. It has no output registers; M0 (the LDS base), a register that
-// the compiler keeps nothing in from one instruction to the next, needs one wait state before its use. The
-// resource comes from v_readfirstlane, and a vector-memory instruction may read a scalar register five wait
-// states after a vector instruction wrote it at the earliest: the hardware does not wait, and the compiler adds
-// none inside the block. The move to M0 is one, s_nop 3 the other four.
+// way before each transposed LDS read. It has no output registers. The LDS base is an
+// input in M0, so that the compiler, which uses that register too, knows what it holds. The resource comes from
+// v_readfirstlane, and a vector-memory instruction may read a scalar register five wait states after a vector
+// instruction wrote it at the earliest (M0: one after any write): the hardware does not wait, and the compiler
+// adds none inside the block. s_nop 4 is five.
 template <typename T, int DP, int ROWS, int THREADS>
 struct TileCopy {
   using L = Tile<T, DP>;
@@ -218,8 +218,8 @@ struct TileCopy {
 #pragma unroll
     for (int i = 0; i < ROWS / kRowsPerStep; ++i) {
       const uint32_t from = kOneOffset ? offset + i * step : at(threadIdx.x / L::kChunks + i * kRowsPerStep);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(to + i * (THREADS * 16)), "v"(from), "s"(src) : "memory");
+      asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "{m0}"(to + i * (THREADS * 16)), "v"(from), "s"(src) : "memory");
     }
   }
 };
@@ -254,8 +254,8 @@ struct RowTileCopy {
       const uint32_t at = t * static_cast<uint32_t>(token_stride) +
                           (n - t * a.group) * static_cast<uint32_t>(head_stride) + c;
       const uint32_t from = row < valid && c < a.dim ? at * static_cast<uint32_t>(sizeof(T)) : kNowhere;
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                   :: "s"(to + i * (THREADS * 16)), "v"(from), "s"(src) : "memory");
+      asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :: "{m0}"(to + i * (THREADS * 16)), "v"(from), "s"(src) : "memory");
     }
   }
 };

@@ -64,6 +64,17 @@ def test_short_waits_are_found():
     assert [x[1:] for x in short_waits(["v_add_co_u32_e64 v1, s[42:43], v1, v2", load])] == [(42, 0), (43, 0)]
 
 
+def test_assembly_leaves_m0_to_the_compiler():
+    """The compiler keeps LDS bases and indexes in M0 and may reuse what it put there: a block that needs a
+    value in M0 takes it as an input and writes nothing to it."""
+    blocks = []
+    for path in sorted((Path(_lib.__file__).resolve().parent.parent / "csrc").iterdir()):
+        blocks += re.findall(r"asm volatile\((.*?)\);", path.read_text(), re.S)
+    copies = [b for b in blocks if re.search(r" lds\"", b)]
+    assert len(copies) == 2 and all('"{m0}"(' in b for b in copies), copies
+    assert not [b for b in blocks if re.search(r"\bm0\s*,", b)]
+
+
 @pytest.mark.skipif(TOOL is None, reason="no llvm-objdump")
 def test_kernels_wait_for_their_scalars(tmp_path):
     lib = tmp_path / "lib.so"
