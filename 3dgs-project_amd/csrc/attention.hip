@@ -21,40 +21,39 @@ constexpr int kAttnKeys = 64;               // keys (or query rows) of a tile in
 // and 1731 us, so 284 and 942. 64 and 128 are the same either way.
 constexpr int row_of(int du) { return du > 64 ? 128 : 64; }
 
-// Base-2 exponent of a score, up to the reference that p = 2^(x - ref) takes off. Plain scores stay as
-// they come (monotone in x: the scale is positive) and are scaled in the same fma that subtracts.
+// Scores as base-2 exponents, x = gain z + bias: z is what tiles of scores are kept as (monotone in the score,
+// -infinity where masked), so that maxima are taken of z and a probability is p = 2^(gain z + (bias - m)),
+// one fma and one exponential.
 struct Rule {
-  float scale2;    // plain: scale log2 e
+  float gain, bias;
   float in_scale;  // capped: scale / cap
   float cap2;      // capped: cap log2 e
   float twice;     // capped: 2 log2 e scale / cap
 };
 
 // Capped scores, s' = cap tanh x, x = scale s / cap. In bfloat16 tanh x = 1 - 2 r with r = 1 / (1 + e^2x)
-// from the hardware exponential and reciprocal (absolute error 2e-7, both ends saturate): s' - ref is then
-// one fma of r, and the slope 1 - tanh^2 = 4 r (1 - r). float32 takes the library's tanh, whose relative
-// error near zero is small too.
+// from the hardware exponential and reciprocal (absolute error 2e-7, both ends saturate), and z = -r; the
+// slope is 1 - tanh^2 = 4 r (1 - r). float32 takes the library's tanh, whose relative error near zero is
+// small too, as z.
 __device__ __forceinline__ float cap_r(const Rule& u, float s) {
   return __builtin_amdgcn_rcpf(1.0f + exp2_hw(s * u.twice));
 }
-template <int MODE>
+template <typename T, int MODE>
 __device__ __forceinline__ Rule rule_of(const AttnArgs& a) {
   const float scale = fabsf(a.scale);
-  return {fmaxf(scale * kLog2e, 1e-30f), MODE == kPlain ? 0.0f : scale / a.softcap, a.softcap * kLog2e,
-          MODE == kPlain ? 0.0f : 2.0f * kLog2e * scale / a.softcap};
+  if constexpr (MODE == kPlain) return {fmaxf(scale * kLog2e, 1e-30f), 0.0f, 0.0f, 0.0f, 0.0f};
+  const float cap2 = a.softcap * kLog2e;
+  const bool r = sizeof(T) == 2;
+  return {r ? 2.0f * cap2 : cap2, r ? cap2 : 0.0f, scale / a.softcap, cap2, 2.0f * kLog2e * scale / a.softcap};
 }
 template <typename T, int MODE>
-__device__ __forceinline__ float exponent(const Rule& u, float s) {
+__device__ __forceinline__ float z_of(const Rule& u, float s) {
   if constexpr (MODE == kPlain) return s;
-  if constexpr (sizeof(T) == 2) return fmaf(-2.0f * u.cap2, cap_r(u, s), MODE == kCapFixed ? kFixedTop : u.cap2);
-  const float x = u.cap2 * tanhf(s * u.in_scale);
-  return MODE == kCapFixed ? x - (u.cap2 - kFixedTop) : x;
+  if constexpr (sizeof(T) == 2) return -cap_r(u, s);
+  return tanhf(s * u.in_scale);
 }
-template <int MODE>
-__device__ __forceinline__ float prob(const Rule& u, float x, float ref) {
-  if constexpr (MODE == kPlain) return exp2_hw(fmaf(x, u.scale2, -ref));
-  if constexpr (MODE == kCapFixed) return exp2_hw(x);  // relative to the fixed reference already
-  return exp2_hw(x - ref);
+__device__ __forceinline__ float prob(const Rule& u, float z, float m) {
+  return exp2_hw(fmaf(z, u.gain, u.bias - m));
 }
 
 // Softmax state of a lane's query: running maximum of the exponents (kept within 2^8 of the true one:
@@ -72,7 +71,7 @@ __device__ __forceinline__ void softmax_step(const Rule& u, f32x16 (&s)[N], f32x
 #pragma unroll
   for (int t = 0; t < N; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[t][r] = exponent<T, MODE>(u, s[t][r]);
+    for (int r = 0; r < 16; ++r) s[t][r] = z_of<T, MODE>(u, s[t][r]);
   if (mask) {
 #pragma unroll
     for (int t = 0; t < N; ++t)
@@ -80,33 +79,26 @@ __device__ __forceinline__ void softmax_step(const Rule& u, f32x16 (&s)[N], f32x
       for (int r = 0; r < 16; ++r)
         if (32 * t + 8 * (r / 4) + 4 * h + r % 4 >= vis) s[t][r] = -INFINITY;
   }
-  float ref;
-  if constexpr (MODE == kCapFixed) {
-    ref = u.cap2 - kFixedTop;
-    st.m = ref;
-  } else {
 #pragma unroll
-    for (int t = 0; t < N; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) top[r % 4] = fmaxf(top[r % 4], s[t][r]);
-    float x = half_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-    if constexpr (MODE == kPlain) x *= u.scale2;
-    if (__any(x > st.m + 8.0f)) {
-      const float m = fmaxf(st.m, x);
-      const float f = exp2_hw(st.m - (m == -INFINITY ? 0.0f : m));
-      st.m = m;
-      st.l *= f;
+    for (int r = 0; r < 16; ++r) top[r % 4] = fmaxf(top[r % 4], s[t][r]);
+  const float x = fmaf(half_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), u.gain, u.bias);
+  if (__any(x > st.m + 8.0f)) {
+    const float m = fmaxf(st.m, x);
+    const float f = exp2_hw(st.m - (m == -INFINITY ? 0.0f : m));
+    st.m = m;
+    st.l *= f;
 #pragma unroll
-      for (int i = 0; i < M; ++i) o[i] *= f;
-    }
-    ref = st.m == -INFINITY ? 0.0f : st.m;
+    for (int i = 0; i < M; ++i) o[i] *= f;
   }
+  const float ref = st.m == -INFINITY ? 0.0f : st.m;
   float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[t][r] = prob<MODE>(u, s[t][r], ref);
+      s[t][r] = prob(u, s[t][r], ref);
       sum[r % 4] += s[t][r];
     }
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -168,8 +160,7 @@ __device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, c
 #pragma unroll
         for (int j = 0; j < 8; ++j) s = fmaf(static_cast<float>(q[c][j]), static_cast<float>(k[j]), s);
       }
-      s = exponent<T, MODE>(u, half_sum(s));
-      const float p = static_cast<float>(static_cast<T>(prob<MODE>(u, s, ref)));
+      const float p = static_cast<float>(static_cast<T>(prob(u, z_of<T, MODE>(u, half_sum(s)), ref)));
 #pragma unroll
       for (int dt = 0; dt < DU / 32; ++dt)
 #pragma unroll
@@ -215,7 +206,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DU <= 64 && !CAUSAL
   for (int c = 0; c < C; ++c) q[c] = load_query<T>(a, qp + 16 * c + 8 * h, 16 * c + 8 * h < a.dim);
   const int vis = visible(a, doc, tok);
   const int wave_min = visible(a, doc, min(wrow, rows - 1) / a.group);
-  const Rule rule = rule_of<MODE>(a);
+  const Rule rule = rule_of<T, MODE>(a);
   f32x16 o[DU / 32] = {};
   Softmax st;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
@@ -348,7 +339,7 @@ __global__ __launch_bounds__(kFewWaves<T> * kWave) void attn_few_kernel(AttnArgs
   const T* qp = static_cast<const T*>(a.q) + (doc.q0 + tok) * a.q_token + head * a.q_head;
   const int vis = min(visible(a, doc, tok), piece.stop);
   const int all_min = min(visible(a, doc, row0 / a.group), piece.stop);
-  const Rule rule = rule_of<MODE>(a);
+  const Rule rule = rule_of<T, MODE>(a);
   f32x16 o[DU / 32] = {};
   Softmax st;
   const T* kp = static_cast<const T*>(a.k) + doc.k0 * a.k_token + hk * a.k_head;
@@ -589,7 +580,7 @@ __device__ __forceinline__ float base_of(const Rule& u, float lse) {
 }
 template <typename T, int MODE>
 __device__ __forceinline__ float prob_of(const Rule& u, float s, float base, float* slope) {
-  if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.scale2, base));
+  if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.gain, base));
   if constexpr (sizeof(T) == 2) {
     const float r = cap_r(u, s), r4 = 4.0f * r;
     *slope = fmaf(-r4, r, r4);
@@ -659,7 +650,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
   delta = half_sum(delta);
   const int64_t stat = (doc.q0 + tok) * a.heads + head;
   if (live && h == 0 && blockIdx.y == 0) a.delta[stat] = delta;
-  const Rule rule = rule_of<MODE>(a);
+  const Rule rule = rule_of<T, MODE>(a);
   const float row_base = base_of<T, MODE>(rule, a.lse[stat]);
   const int vis = live ? visible(a, doc, tok) : 0;
   const int wave_min = wrow + 31 < rows ? visible(a, doc, wrow / a.group) : 0;
@@ -795,7 +786,7 @@ __device__ __forceinline__ void attn_bwd_kv(const AttnArgs& a, KvShared<T, DU>& 
   }
   const RowTileCopy<T, row_of(DU), R, kAttnThreads> copy_q = {a.q_token, a.q_head};
   const RowTileCopy<T, row_of(DU), R, kAttnThreads> copy_g = {static_cast<int64_t>(a.heads) * a.dim, a.dim};
-  const Rule rule = rule_of<MODE>(a);
+  const Rule rule = rule_of<T, MODE>(a);
   float n_lse = 0.0f, n_delta = 0.0f;
   int n_vis = 0;
   const auto fetch = [&](int r0, char* to) {
@@ -1044,7 +1035,6 @@ static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { retur
 template <template <typename, int, int> class K, typename T, int DU>
 static void launch_mode(const AttnArgs& a, dim3 grid, hipStream_t st) {
   if (a.softcap == 0.0f) K<T, DU, kPlain>::launch(a, grid, st);
-  else if (K<T, DU, kCap>::kFixed && a.softcap * kLog2e <= kFixedCap) K<T, DU, kCapFixed>::launch(a, grid, st);
   else K<T, DU, kCap>::launch(a, grid, st);
 }
 template <template <typename, int, int> class K>
@@ -1059,11 +1049,10 @@ static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts,
   else if (a.dim > 32) by_type(std::integral_constant<int, 64>{});
   else by_type(std::integral_constant<int, 32>{});
 }
-// Forward kernels have an instance for the fixed cap and one for the causal mask, the backward's do not.
+// Forward kernels have an instance for the causal mask, the backward's do not.
 #define GS_ATTN_FORWARD(NAME, KERNEL, THREADS)                                                            \
   template <typename T, int DU, int MODE>                                                                 \
   struct NAME {                                                                                           \
-    static constexpr bool kFixed = true;                                                                  \
     static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                                    \
       if (a.causal) hipLaunchKernelGGL((KERNEL<T, DU, MODE, true>), grid, dim3(THREADS), 0, st, a);       \
       else hipLaunchKernelGGL((KERNEL<T, DU, MODE, false>), grid, dim3(THREADS), 0, st, a);               \
@@ -1072,10 +1061,8 @@ static void launch_attn(const AttnArgs& a, int dtype, int64_t blocks, int parts,
 #define GS_ATTN_BACKWARD(NAME, KERNEL)                                                                    \
   template <typename T, int DU, int MODE>                                                                 \
   struct NAME {                                                                                           \
-    static constexpr bool kFixed = false;                                                                 \
     static void launch(const AttnArgs& a, dim3 grid, hipStream_t st) {                                    \
-      constexpr int mode = MODE == kPlain ? kPlain : kCap;                                                \
-      hipLaunchKernelGGL((KERNEL<T, DU, mode>), grid, dim3(kAttnThreads), 0, st, a);                      \
+      hipLaunchKernelGGL((KERNEL<T, DU, MODE>), grid, dim3(kAttnThreads), 0, st, a);                      \
     }                                                                                                     \
   }
 GS_ATTN_FORWARD(FwdKernel, attn_fwd_kernel, kAttnThreads);

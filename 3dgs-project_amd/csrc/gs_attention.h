@@ -287,11 +287,7 @@ __device__ __forceinline__ float half_max(float v) {
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // How scores become base-2 exponents.
-enum { kPlain = 0, kCap = 1, kCapFixed = 2 };
-// kCapFixed: scores capped at cap2 (base 2) <= kFixedCap need no running maximum: relative to cap2 -
-// 60 every exponent lies in [-120, 60], so no probability under- or overflows and a sum over 2^30 keys
-// stays below 2^90.
-constexpr float kFixedCap = 90.0f, kFixedTop = 60.0f;
+enum { kPlain = 0, kCap = 1 };
 
 // The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one) of
 // at least `share`.

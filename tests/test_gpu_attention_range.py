@@ -1,0 +1,46 @@
+"""GPU parity of amdsplat.attention at the ends of what its arguments may be: large and small values under
+capped scores, large and small caps and scales. Values and bounds are the float64 oracle's
+(oracle/attention_ref.py)."""
+import pytest
+import torch
+
+import attention_ref as A
+from test_gpu_attention import DT, check, ints, run
+
+pytestmark = pytest.mark.gpu
+
+
+def aligned(nq, nk, signs, size, dtype, seed, dim=64, heads=4, kv_heads=2):
+    """Queries and keys whose scores before the cap are near signs[j] * size: each is a fixed pattern of +-1 with
+    an eighth of noise."""
+    g = torch.Generator().manual_seed(seed)
+    pattern = torch.randint(0, 2, (dim,), generator=g) * 2.0 - 1.0
+    a = (size / dim ** 0.5) ** 0.5  # a^2 dim / sqrt(dim) = size
+    noise = lambda *s: 1.0 + 0.125 * torch.randn(*s, generator=g)  # noqa: E731
+    q = (a * pattern * noise(nq, heads, dim)).to(dtype)
+    k = (a * signs[:, None, None] * pattern * noise(nk, kv_heads, dim)).to(dtype)
+    return q, k, torch.randn(nk, kv_heads, dim, generator=g)
+
+
+SIGNS = {
+    "top": lambda n: torch.ones(n),
+    "bottom": lambda n: -torch.ones(n),
+    "rising": lambda n: torch.where(torch.arange(n) < n - n // 3, -1.0, 1.0),
+    "falling": lambda n: torch.where(torch.arange(n) < n // 3, 1.0, -1.0),
+}
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("signs", SIGNS)
+@pytest.mark.parametrize("softcap", [15.0, 30.0, 50.0, 62.0, 100.0])
+@pytest.mark.parametrize("gain", [1e30, 1e-25])
+@pytest.mark.parametrize("nq,nk,causal", [(150, 150, True), (150, 150, False), (1, 9000, False), (3, 4000, True),
+                                          (181, 5000, True)])
+def test_values_of_every_size_under_a_cap(nq, nk, causal, gain, softcap, signs, dtype):
+    """Saturated scores at either end of the cap: the output is a mean of the values whatever their size. The
+    sums stay in float32's range (1e30 times 2^8 times 9000 keys)."""
+    q, k, v = aligned(nq, nk, SIGNS[signs](nk), 10 * softcap, dtype, nk + nq)
+    v = (gain * v).to(dtype)
+    got = run(q, k, v, None, causal=causal, softcap=softcap, offsets=ints([0, nq]), k_offsets=ints([0, nk]))
+    check(got, A.attention(q, k, v, [0, nq], [0, nk], causal=causal, softcap=softcap))
+    assert bool(got["out"].any())
