@@ -33,8 +33,8 @@ struct Rule {
 
 // Capped scores, s' = cap tanh x, x = scale s / cap. In bfloat16 tanh x = 1 - 2 r with r = 1 / (1 + e^2x)
 // from the hardware exponential and reciprocal (absolute error 2e-7, both ends saturate), and z = -r; the
-// slope is 1 - tanh^2 = 4 r (1 - r). float32 takes the library's tanh, whose relative error near zero is
-// small too, as z.
+// slope is 1 - tanh^2 = 4 r (1 - r). float32, and bfloat16 under far caps, take the library's tanh, whose relative
+// error near zero is small too, as z.
 __device__ __forceinline__ float cap_r(const Rule& u, float s) {
   return __builtin_amdgcn_rcpf(1.0f + exp2_hw(s * u.twice));
 }
@@ -43,13 +43,13 @@ __device__ __forceinline__ Rule rule_of(const AttnArgs& a) {
   const float scale = fabsf(a.scale);
   if constexpr (MODE == kPlain) return {fmaxf(scale * kLog2e, 1e-30f), 0.0f, 0.0f, 0.0f, 0.0f};
   const float cap2 = a.softcap * kLog2e;
-  const bool r = sizeof(T) == 2;
+  const bool r = kByExp<T, MODE>;
   return {r ? 2.0f * cap2 : cap2, r ? cap2 : 0.0f, scale / a.softcap, cap2, 2.0f * kLog2e * scale / a.softcap};
 }
 template <typename T, int MODE>
 __device__ __forceinline__ float z_of(const Rule& u, float s) {
   if constexpr (MODE == kPlain) return s;
-  if constexpr (sizeof(T) == 2) return -cap_r(u, s);
+  if constexpr (kByExp<T, MODE>) return -cap_r(u, s);
   return tanhf(s * u.in_scale);
 }
 __device__ __forceinline__ float prob(const Rule& u, float z, float m) {
@@ -576,12 +576,12 @@ __device__ __forceinline__ void add_cols_times(const char* lds, int row0, int la
 template <typename T, int MODE>
 __device__ __forceinline__ float base_of(const Rule& u, float lse) {
   const float lse2 = lse == -INFINITY ? 0.0f : lse * kLog2e;
-  return MODE != kPlain && sizeof(T) == 2 ? u.cap2 - lse2 : -lse2;
+  return kByExp<T, MODE> ? u.cap2 - lse2 : -lse2;
 }
 template <typename T, int MODE>
 __device__ __forceinline__ float prob_of(const Rule& u, float s, float base, float* slope) {
   if constexpr (MODE == kPlain) return exp2_hw(fmaf(s, u.gain, base));
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (kByExp<T, MODE>) {
     const float r = cap_r(u, s), r4 = 4.0f * r;
     *slope = fmaf(-r4, r, r4);
     return exp2_hw(fmaf(-2.0f * u.cap2, r, base));
@@ -1035,6 +1035,7 @@ static int64_t tiles_of(int64_t tokens, int64_t per, int rows, int docs) { retur
 template <template <typename, int, int> class K, typename T, int DU>
 static void launch_mode(const AttnArgs& a, dim3 grid, hipStream_t st) {
   if (a.softcap == 0.0f) K<T, DU, kPlain>::launch(a, grid, st);
+  else if (sizeof(T) == 2 && a.softcap > kFarCap) K<T, DU, sizeof(T) == 2 ? kCapFar : kCap>::launch(a, grid, st);
   else K<T, DU, kCap>::launch(a, grid, st);
 }
 template <template <typename, int, int> class K>

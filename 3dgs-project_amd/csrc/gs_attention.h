@@ -287,7 +287,14 @@ __device__ __forceinline__ float half_max(float v) {
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // How scores become base-2 exponents.
-enum { kPlain = 0, kCap = 1 };
+enum { kPlain = 0, kCap = 1, kCapFar = 2 };
+// bfloat16, capped: kCap's tanh has an absolute error of 2e-7, so the score is off by that much of the cap: 6e-5 at
+// kFarCap, beside the 4e-3 of a probability's rounding. Larger caps take the library's tanh, whose error is
+// relative (8192 tokens, 16 heads of 64, cap 300: forward 428 us by the exponential, 602 by the library; backward 1301 and
+// 1585).
+constexpr float kFarCap = 256.0f;
+template <typename T, int MODE>
+constexpr bool kByExp = sizeof(T) == 2 && MODE == kCap;
 
 // The piece of [0, end) that workgroup `split` takes: keys [begin, stop) of `n` pieces (at least one) of
 // at least `share`.

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import attention_ref as A
-from test_gpu_attention import DT, check, ints, run
+from test_gpu_attention import DT, check, inputs, ints, run
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,21 @@ def test_values_of_every_size_under_a_cap(nq, nk, causal, gain, softcap, signs, 
     got = run(q, k, v, None, causal=causal, softcap=softcap, offsets=ints([0, nq]), k_offsets=ints([0, nk]))
     check(got, A.attention(q, k, v, [0, nq], [0, nk], causal=causal, softcap=softcap))
     assert bool(got["out"].any())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("softcap", [257.0, 300.0, 1e4, 1e6, 1e8])
+@pytest.mark.parametrize("nq,nk,causal,train", [(150, 150, True, True), (97, 97, False, True), (1, 3000, False, False),
+                                                (130, 4000, True, False)])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_scores_far_below_the_cap(dim, nq, nk, causal, train, softcap, dtype):
+    """A cap far above the scores changes them little, and its size is no error of theirs. The bound is the one
+    of uncapped scores, with 4 units of 2^-23 of the scores more for the tanh (two operations beside the D + 4 of the
+    product): (D + 8) / (D + 4) of it."""
+    q, k, v, g = inputs(nq, nk, 4, 2, dim, dtype, dim + nk)
+    at = ([0, nq], [0, nk])
+    d_out = g if train else None
+    got = run(q, k, v, d_out, causal=causal, softcap=softcap, offsets=ints(at[0]), k_offsets=ints(at[1]))
+    want = A.attention(q, k, v, *at, causal=causal, softcap=softcap, d_out=d_out)
+    near = A.attention(q, k, v, *at, causal=causal, d_out=d_out)
+    check(got, {n: (want[n][0], near[n][1] * (dim + 8) / (dim + 4)) for n in want})
