@@ -111,8 +111,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     (None: one document of all tokens). k_offsets: the same for the keys (None: as the queries).
     k_lengths [docs] int32: of a document's key tokens only the first so many are there (a cache);
     the rest may hold anything. causal: query i of a document of Lq queries and Lk keys sees key j
-    if j <= i + Lk - Lq; prefix [docs] int32 (with causal): or if j < prefix[d]. softcap c > 0: scores
-    s become c tanh(s / c). scale: of the scores before the cap (default 1 / sqrt(D)).
+    if j <= i + Lk - Lq; prefix [docs] int32 (with causal): or if j < prefix[d]. softcap c (0, or 2^-96 to 2^96):
+    scores s become c tanh(s / c). scale: of the scores before the cap (default 1 / sqrt(D)).
 
     A query that sees no key gets 0 and -infinity. A key or value that is not finite reaches only the
     queries that see it (the gradients of its document are not kept apart so). D up to 128 (padded to a multiple of 8 by a copy).
@@ -155,11 +155,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
             raise ValueError("a prefix needs causal=True")
         _table(prefix, "prefix", docs, device)
     softcap = float(softcap)
-    if not (softcap >= 0.0 and math.isfinite(softcap)):
-        raise ValueError("softcap must be finite and >= 0")
+    if softcap != 0.0 and not 2.0 ** -96 <= softcap <= 2.0 ** 96:
+        raise ValueError("softcap must be 0 or between 2^-96 and 2^96")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    if softcap and scale and not 2.0 ** -126 <= abs(scale) / softcap <= 2.0 ** 125:
+        raise ValueError("scale / softcap must be between 2^-126 and 2^125")
     if d % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, -d % 8)) for t in (q, k, v))
     rest = (offsets, k_offsets, k_lengths, prefix, bool(causal), softcap, scale)

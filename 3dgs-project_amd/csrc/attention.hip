@@ -978,9 +978,14 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
                  p->docs < (1 << 26), GS_ERR_ARG, "attention: too many tokens or documents");
   GS_REQUIRE(group <= 512, GS_ERR_ARG, "attention: at most 512 heads share a key head");
   GS_REQUIRE(p->prefix == nullptr || p->causal, GS_ERR_ARG, "attention: a prefix needs the causal mask");
-  GS_REQUIRE(p->scale == p->scale && p->softcap >= 0.0f && p->softcap <= FLT_MAX &&
-                 p->scale <= FLT_MAX && p->scale >= -FLT_MAX, GS_ERR_ARG,
-             "attention: scale must be finite, softcap finite and >= 0");
+  GS_REQUIRE(p->scale == p->scale && p->scale <= FLT_MAX && p->scale >= -FLT_MAX, GS_ERR_ARG,
+             "attention: scale must be finite");
+  // in float32, and so that scores over the cap neither over- nor underflow where they count
+  const float per_cap = p->softcap != 0.0f && p->scale != 0.0f ? fabsf(p->scale) / p->softcap : 1.0f;
+  GS_REQUIRE(p->softcap == 0.0f || (p->softcap >= 0x1p-96f && p->softcap <= 0x1p96f), GS_ERR_ARG,
+             "attention: softcap must be 0 or between 2^-96 and 2^96");
+  GS_REQUIRE(per_cap >= FLT_MIN && per_cap <= 0x1p125f, GS_ERR_ARG,
+             "attention: scale / softcap must be between 2^-126 and 2^125");
   const bool has_q = p->q_tokens > 0, has_k = p->k_tokens > 0;
   GS_REQUIRE((!has_q || (p->q && p->out && p->lse)) && (!has_k || (p->k && p->v)), GS_ERR_ARG,
              "attention: null pointer");

@@ -62,3 +62,19 @@ def test_scores_far_below_the_cap(dim, nq, nk, causal, train, softcap, dtype):
     want = A.attention(q, k, v, *at, causal=causal, softcap=softcap, d_out=d_out)
     near = A.attention(q, k, v, *at, causal=causal, d_out=d_out)
     check(got, {n: (want[n][0], near[n][1] * (dim + 8) / (dim + 4)) for n in want})
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("softcap", [2.0 ** -96, 1e-20, 1e-3, 2.0 ** 96])
+def test_caps_at_their_ends(softcap, dtype):
+    """Under a cap of next to nothing every key counts the same and the scores have next to no gradient (a slope times
+    the scale); under one far above the scores nothing is capped. A key of zeros has a score of 0."""
+    nq = nk = 150
+    q, k, v, g = inputs(nq, nk, 4, 2, 64, dtype, 41)
+    k[7] = 0.0
+    at = ([0, nq], [0, nk])
+    got = run(q, k, v, g, causal=True, softcap=softcap, offsets=ints(at[0]), k_offsets=ints(at[1]))
+    want = A.attention(q, k, v, *at, causal=True, softcap=softcap, d_out=g)
+    near = A.attention(q, k, v, *at, causal=True, d_out=g)
+    check(got, {n: (want[n][0], torch.maximum(want[n][1], near[n][1] * 72 / 68) if softcap < 1 else near[n][1] * 72 / 68)
+                for n in want})
