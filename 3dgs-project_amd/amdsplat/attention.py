@@ -158,8 +158,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     if softcap != 0.0 and not 2.0 ** -96 <= softcap <= 2.0 ** 96:
         raise ValueError("softcap must be 0 or between 2^-96 and 2^96")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if scale != 0.0 and not 2.0 ** -126 <= abs(scale) <= 2.0 ** 126:
+        raise ValueError("scale must be finite, 0 or between 2^-126 and 2^126 in size")
     if softcap and scale and not 2.0 ** -126 <= abs(scale) / softcap <= 2.0 ** 125:
         raise ValueError("scale / softcap must be between 2^-126 and 2^125")
     if d % 8:

@@ -41,7 +41,8 @@ __device__ __forceinline__ float cap_r(const Rule& u, float s) {
 template <typename T, int MODE>
 __device__ __forceinline__ Rule rule_of(const AttnArgs& a) {
   const float scale = fabsf(a.scale);
-  if constexpr (MODE == kPlain) return {fmaxf(scale * kLog2e, 1e-30f), 0.0f, 0.0f, 0.0f, 0.0f};
+  // (a scale of 0 becomes the smallest that takes a masked -infinity along)
+  if constexpr (MODE == kPlain) return {fmaxf(scale * kLog2e, FLT_MIN), 0.0f, 0.0f, 0.0f, 0.0f};
   const float cap2 = a.softcap * kLog2e;
   const bool r = kByExp<T, MODE>;
   return {r ? 2.0f * cap2 : cap2, r ? cap2 : 0.0f, scale / a.softcap, cap2, 2.0f * kLog2e * scale / a.softcap};
@@ -978,8 +979,8 @@ static int attn_setup(const gs_attention* p, AttnArgs& a) {
                  p->docs < (1 << 26), GS_ERR_ARG, "attention: too many tokens or documents");
   GS_REQUIRE(group <= 512, GS_ERR_ARG, "attention: at most 512 heads share a key head");
   GS_REQUIRE(p->prefix == nullptr || p->causal, GS_ERR_ARG, "attention: a prefix needs the causal mask");
-  GS_REQUIRE(p->scale == p->scale && p->scale <= FLT_MAX && p->scale >= -FLT_MAX, GS_ERR_ARG,
-             "attention: scale must be finite");
+  GS_REQUIRE(p->scale == 0.0f || (fabsf(p->scale) >= FLT_MIN && fabsf(p->scale) <= 0x1p126f), GS_ERR_ARG,
+             "attention: scale must be finite, 0 or between 2^-126 and 2^126 in size");
   // in float32, and so that scores over the cap neither over- nor underflow where they count
   const float per_cap = p->softcap != 0.0f && p->scale != 0.0f ? fabsf(p->scale) / p->softcap : 1.0f;
   GS_REQUIRE(p->softcap == 0.0f || (p->softcap >= 0x1p-96f && p->softcap <= 0x1p96f), GS_ERR_ARG,

@@ -628,8 +628,8 @@ int gs_rotary_axes(const gs_rotary* args, void* stream);
  * the key tokens k_offsets[d] .. k_offsets[d + 1] the first k_lengths[d] (NULL: all): device int32,
  * offsets non-decreasing, docs + 1 of them (NULL for one document: all tokens). With Lq, Lk the
  * document's counts, query i sees key j < Lk if not causal, or j <= i + Lk - Lq, or j < prefix[d]
- * (device int32, may be NULL; only with causal). Scores s = scale q.k, or with a softcap
- * (0: none; 2^-96 to 2^96, and scale / softcap 2^-126 to 2^125) softcap tanh(scale q.k / softcap).
+ * (device int32, may be NULL; only with causal). Scores s = scale q.k (a scale of 0, or
+ * 2^-126 to 2^126 in size), or with a softcap (0: none; 2^-96 to 2^96, and scale / softcap 2^-126 to 2^125) softcap tanh(scale q.k / softcap).
  *   out [q_tokens, heads, dim] = sum_j softmax(s)_j v_j, lse [q_tokens, heads] float32 = ln sum_j e^s_j.
  * A query that sees nothing, and one outside every document, gets 0 and -infinity. Key tokens
  * outside the documents and their lengths are never used, whatever they hold, and a key or value that is

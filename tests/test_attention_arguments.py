@@ -45,7 +45,15 @@ def test_scales_far_from_the_cap(scale, softcap):
     python("scale / softcap", scale=scale, softcap=softcap)
 
 
+@pytest.mark.parametrize("scale", [1e-46, 1e-39, -1e-39, 2.0 ** 127, -(2.0 ** 127), 1e300])
+def test_scales_out_of_range(scale):
+    if 0.0 < abs(C.c_float(scale).value) < float("inf"):
+        refused("scale", scale=scale)
+    python("scale", scale=scale)
+
+
 def test_the_ends_are_accepted():
     for softcap, scale in ((2.0 ** -96, 2.0 ** 29), (2.0 ** -96, 0.125), (2.0 ** 96, 2.0 ** -30), (2.0 ** 96, -8.0),
-                           (2.0 ** -96, 0.0), (0.0, 0.0), (30.0, 0.0)):
+                           (2.0 ** -96, 0.0), (0.0, 0.0), (30.0, 0.0),
+                           (0.0, 2.0 ** -126), (0.0, -(2.0 ** 126))):
         accepted(softcap=softcap, scale=scale)

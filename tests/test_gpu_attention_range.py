@@ -78,3 +78,17 @@ def test_caps_at_their_ends(softcap, dtype):
     near = A.attention(q, k, v, *at, causal=True, d_out=g)
     check(got, {n: (want[n][0], torch.maximum(want[n][1], near[n][1] * 72 / 68) if softcap < 1 else near[n][1] * 72 / 68)
                 for n in want})
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** -50, 2.0 ** 50, 2.0 ** 61])
+def test_scales_of_every_size(size, causal, dtype):
+    """Queries and keys of one size, and the scale that takes it off again: the scores are those of size 1, since a
+    power of two changes no rounding. Gradients are then of the other size, hence of the oracle's as well."""
+    for nq, nk in ((150, 150), (1, 700)):
+        q, k, v, g = inputs(nq, nk, 4, 2, 64, dtype, 43)
+        at, scale = ([0, nq], [0, nk]), 0.125 / size ** 2
+        d_out = g if nq > 1 else None
+        got = run(q * size, k * size, v, d_out, causal=causal, scale=scale, offsets=ints(at[0]), k_offsets=ints(at[1]))
+        check(got, A.attention(q * size, k * size, v, *at, causal=causal, scale=scale, d_out=d_out))
