@@ -15,6 +15,7 @@ import math
 import torch
 
 from . import _lib
+from ._grad import tracked
 from ._lib import call, ptr
 
 MAX_DIM = 128  # GS_ATTENTION_MAX_DIM
@@ -165,7 +166,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     if d % 8:
         q, k, v = (torch.nn.functional.pad(t, (0, -d % 8)) for t in (q, k, v))
     rest = (offsets, k_offsets, k_lengths, prefix, bool(causal), softcap, scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if tracked(q, k, v):
         out, lse = _Attention.apply(q, k, v, *rest)
     else:
         out, lse = _forward(_readable(q, heads // kv_heads), _readable(k), _readable(v), *rest)

@@ -14,6 +14,7 @@ import math
 import torch
 
 from . import _lib
+from ._grad import tracked
 from ._lib import call
 
 MAX_AXES, MAX_PAIRS = 4, 256  # GS_ROTARY_MAX_AXES, GS_ROTARY_MAX_PAIRS
@@ -98,7 +99,7 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     if positions.dtype != torch.float32 or not positions.is_contiguous():
         positions = positions.to(torch.float32).contiguous()
     flags = _FLAGS[pairing] | _FLAGS[spectrum]
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if tracked(q, k):
         q2, k2 = _Rotary.apply(q, k, positions, sections, base, flags)
     else:
         q2, k2 = _turn(q, k, positions, sections, base, flags)
