@@ -12,6 +12,7 @@ from array import array
 import torch
 
 from . import _lib
+from ._grad import refuse_tangents
 from ._lib import call
 
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
@@ -45,6 +46,7 @@ def _list(grads, what: str):
         raise ValueError(f"{what}: no tensors")
     if any(not isinstance(t, torch.Tensor) or t.layout != torch.strided for t in grads):
         raise ValueError(f"{what} must be dense tensors")
+    refuse_tangents(grads, what)
     return grads
 
 
