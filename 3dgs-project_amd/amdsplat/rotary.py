@@ -67,7 +67,8 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
 
     pairing "half": pair p is the elements (p, p + P); "adjacent": (2 p, 2 p + 1). The angle is
     position * base^-x: spectrum "axis" runs x over [0, 1) within each section, "shared" over all
-    P pairs. The angle is formed to float32's last place whatever the position."""
+    P pairs. The angle is formed to float32's last place for positions up to 2^30 (2^28
+    turns). Integer positions are taken as float32, which holds them exactly up to 2^24."""
     if q.dim() != 3 or (k is not None and k.dim() != 3):
         raise ValueError("q and k must be [tokens, heads, D]")
     if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):

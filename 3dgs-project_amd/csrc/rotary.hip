@@ -24,21 +24,20 @@ struct RotaryArgs {
   int tokens_per_block;
   int section_end[GS_ROTARY_MAX_AXES];
   float sign;
-  // frequency in turns, as the sum of two floats
-  float freq_hi[GS_ROTARY_MAX_PAIRS], freq_lo[GS_ROTARY_MAX_PAIRS];
+  double freq[GS_ROTARY_MAX_PAIRS];  // in turns
 };
 
 constexpr int kRotaryThreads = 256;
 constexpr int kRotaryTable = 1024;  // (token, pair) angles of a workgroup
 
-// cos and sin of 2 pi pos f. The product is formed to about 48 bits and reduced to a turn before
-// anything is rounded, so the angle's error does not grow with the position.
-__device__ __forceinline__ float2 turn(float pos, float hi, float lo) {
-  const float ph = pos * hi;
-  const float pl = fmaf(pos, lo, fmaf(pos, hi, -ph));
-  const float f = (ph - rintf(ph)) + pl;
+// cos and sin of 2 pi pos f. The product is formed in float64 and reduced to a turn before it is rounded to
+// float32, so the angle's error does not grow with the position until the product's own rounding counts: n
+// turns are known to about n 2^-52 of a turn, less than float32's 2^-24 up to 2^28 turns, a position of 2^30 at a
+// frequency of 1.
+__device__ __forceinline__ float2 turn(float pos, double f) {
+  const double t = static_cast<double>(pos) * f;
   float2 r;
-  sincospif(2.0f * f, &r.y, &r.x);
+  sincospif(2.0f * static_cast<float>(t - rint(t)), &r.y, &r.x);
   return r;
 }
 
@@ -69,7 +68,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
     const int t = e / a.pairs, p = e - t * a.pairs;
     int axis = 0;
     while (axis + 1 < a.axes && p >= a.section_end[axis]) ++axis;
-    float2 cs = turn(a.positions[(token0 + t) * a.axes + axis], a.freq_hi[p], a.freq_lo[p]);
+    float2 cs = turn(a.positions[(token0 + t) * a.axes + axis], a.freq[p]);
     cs.y *= a.sign;
     table[e] = cs;
   }
@@ -184,9 +183,7 @@ extern "C" int gs_rotary_axes(const gs_rotary* p, void* stream) {
     for (int j = 0; j < p->sections[axis]; ++j, ++i) {
       const double x = p->flags & GS_ROTARY_SHARED ? static_cast<double>(i) / a.pairs
                                                    : static_cast<double>(j) / p->sections[axis];
-      const double f = exp(-x * ln) * 0.15915494309189533577;  // turns
-      a.freq_hi[i] = static_cast<float>(f);
-      a.freq_lo[i] = static_cast<float>(f - a.freq_hi[i]);
+      a.freq[i] = exp(-x * ln) * 0.15915494309189533577;
     }
   // the widest vector that fits into the pairs and into the rest
   const int rest = p->dim - 2 * a.pairs;

@@ -600,7 +600,7 @@ int gs_grad_scale(const void* const* grads, void* const* out, const int64_t* siz
  * are copied. GS_ROTARY_INVERSE negates the angle (the gradient). q [tokens, q_heads, dim] and k
  * [tokens, k_heads, dim] (k_heads 0: none) are read through their strides (elements; the last
  * dimension is contiguous) and written contiguously, to memory that overlaps no input. positions:
- * [tokens, axes] float32.
+ * [tokens, axes] float32; angles are exact to float32's last place up to 2^28 turns.
  * ------------------------------------------------------------------------------------- */
 #define GS_ROTARY_MAX_AXES 4
 #define GS_ROTARY_MAX_PAIRS 256
