@@ -118,8 +118,9 @@ class FusedAdam(torch.optim.Adam):
             visibility = None
         elif visibility is None:
             visibility = _Rasterize3D.last_visibility
-        batches: dict = {}
-        grads = []
+        # everything that can be refused comes before the first state that changes
+        todo = []
+        fallbacks = 0
         for group in self.param_groups:
             assert len(group["params"]) == 1, "more than one tensor in group"
             param = group["params"][0]
@@ -127,33 +128,36 @@ class FusedAdam(torch.optim.Adam):
                 continue
             lowp = group.get("name") in self.lowp_moment_groups
             moment_dtype = torch.bfloat16 if lowp else param.dtype
-            state = self.state[param]
-            if len(state) == 0:
-                state["step"] = 0
-                state["exp_avg"] = torch.zeros_like(param, dtype=moment_dtype)
-                state["exp_avg_sq"] = torch.zeros_like(param, dtype=moment_dtype)
-            elif state["exp_avg"].dtype != moment_dtype:
-                state["exp_avg"] = state["exp_avg"].to(moment_dtype)
-                state["exp_avg_sq"] = state["exp_avg_sq"].to(moment_dtype)
-            state["step"] += 1
             grad = param.grad.contiguous()
-            _check(param, grad, state["exp_avg"], state["exp_avg_sq"])
-            grads.append(grad)
+            state = self.state.get(param)
+            if state:
+                m, v = state["exp_avg"], state["exp_avg_sq"]
+                if m.dtype != moment_dtype:
+                    m, v = m.to(moment_dtype), v.to(moment_dtype)
+            else:
+                m, v = (torch.zeros_like(param, dtype=moment_dtype) for _ in "mv")
+            _check(param, grad, m, v)
             n_prim = param.shape[0]
             vis = visibility
             if vis is not None and vis.numel() != n_prim:
                 vis = None  # a mask of another model size: update this group densely
-                self.n_dense_fallbacks += 1
+                fallbacks += 1
+            todo.append((group, param, grad, m, v, n_prim, _visibility(vis, n_prim)))
+        norm = scale = None
+        if max_norm is not None:
+            if not todo:
+                return torch.zeros((), device=self.param_groups[0]["params"][0].device)
+            norm, scale = clip_coefficient([t[2] for t in todo], max_norm)
+        self.n_dense_fallbacks += fallbacks
+        batches: dict = {}
+        for group, param, grad, m, v, n_prim, vis in todo:
+            state = self.state[param]
+            state["step"] = state.get("step", 0) + 1
+            state["exp_avg"], state["exp_avg_sq"] = m, v
             key = (n_prim, None if vis is None else vis.data_ptr(), param.device)
             b1, b2 = group["betas"]
             batches.setdefault(key, (vis, []))[1].append(
-                _group(grad, param, state["exp_avg"], state["exp_avg_sq"], state["step"], group["lr"], b1, b2,
-                       group["eps"]))
-        norm = scale = None
-        if max_norm is not None:
-            if not grads:
-                return torch.zeros((), device=self.param_groups[0]["params"][0].device)
-            norm, scale = clip_coefficient(grads, max_norm)
+                _group(grad, param, m, v, state["step"], group["lr"], b1, b2, group["eps"]))
         for (n_prim, _, device), (vis, groups) in batches.items():
-            _launch(groups, n_prim, _visibility(vis, n_prim), device, scale)
+            _launch(groups, n_prim, vis, device, scale)
         return norm
