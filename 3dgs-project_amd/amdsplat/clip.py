@@ -78,7 +78,7 @@ def grad_norm(grads) -> torch.Tensor:
 @torch.no_grad()
 def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     """Scales the gradients by min(1, max_norm / (norm + 1e-6)), in place or into the tensors `out`
-    (same shapes and dtypes, not overlapping the gradients), and returns the norm before clipping (a
+    (of the gradients' shapes or flat, of their dtypes, not overlapping them), and returns the norm before clipping (a
     0-dim float32 device tensor). A norm that is infinite or NaN leaves no gradient usable, as the
     product says; the caller checks the returned norm."""
     grads = _list(grads, "gradients")
@@ -94,8 +94,9 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
         if any(not o.is_contiguous() for o in out):
             raise ValueError("out must be contiguous")
         to = _Tensors(out, "out")
-        if to.sizes != t.sizes or to.dtypes != t.dtypes or to.device != t.device:
-            raise ValueError("out must have the gradients' shapes and dtypes, on their device")
+        if (any(o.shape != g.shape and (o.dim() != 1 or o.numel() != g.numel()) for o, g in zip(out, grads))
+                or to.dtypes != t.dtypes or to.device != t.device):
+            raise ValueError("out must have the gradients' shapes (or be flat) and dtypes, on their device")
     norm, coef = _norm(t, max_norm)
     call("gs_grad_scale", _at(t.ptrs), _at(to.ptrs), _at(t.sizes), _at(t.dtypes), t.n, coef.data_ptr(),
          _lib.stream_handle(t.device))
