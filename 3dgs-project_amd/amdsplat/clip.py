@@ -100,6 +100,7 @@ def clip_grad_norm(grads, max_norm: float, out=None) -> torch.Tensor:
     norm, coef = _norm(t, max_norm)
     call("gs_grad_scale", _at(t.ptrs), _at(to.ptrs), _at(t.sizes), _at(t.dtypes), t.n, coef.data_ptr(),
          _lib.stream_handle(t.device))
+    torch.autograd.graph.increment_version(to.keep)  # autograd sees the writes
     return norm
 
 
