@@ -1220,6 +1220,9 @@ extern "C" int gs_attention_bwd(const gs_attention* p, const void* d_out, void* 
              "attention backward: null pointer");
   GS_REQUIRE(aligned(d_out, 16) && aligned(d_q, 16) && aligned(d_k, 16) && aligned(d_v, 16), GS_ERR_ALIGN,
              "attention backward: tensors must be 16-byte aligned");
+  // d_out is contiguous, whatever q's strides: 64 of its rows, like those of q
+  GS_REQUIRE((64 / a.group + 2) * static_cast<int64_t>(a.heads) * a.dim < (int64_t(1) << 28), GS_ERR_ARG,
+             "attention backward: too many heads");
   const BwdPlan b = plan_bwd(a, p->dtype);
   const size_t need = (b.delta + b.part_q + b.part_kv) * sizeof(float);
   GS_REQUIRE(workspace_bytes >= need && (workspace || need == 0), GS_ERR_WORKSPACE,

@@ -57,3 +57,13 @@ def test_the_ends_are_accepted():
                            (2.0 ** -96, 0.0), (0.0, 0.0), (30.0, 0.0),
                            (0.0, 2.0 ** -126), (0.0, -(2.0 ** 126))):
         accepted(softcap=softcap, scale=scale)
+
+
+def test_rows_of_the_output_gradient():
+    """The key gradients address 64 rows of d_out with 32 bits. Its tokens are heads * dim apart even where q's are
+    not (a broadcast q), so that q's strides do not bound them."""
+    wide = dict(q_token_stride=0, q_head_stride=0, k_token_stride=0, k_head_stride=0, v_token_stride=0, v_head_stride=0)
+    for heads, kv_heads, dim in ((1 << 16, 1 << 16, 64), (1 << 15, 1 << 15, 128), (1 << 26, 1 << 18, 128)):
+        a = attention_args(heads=heads, kv_heads=kv_heads, dim=dim, **wide)
+        expect(_lib.lib().gs_attention_bwd(C.byref(a), 256, 256, 256, 256, None, 0, None), ARG, "too many heads")
+    accepted(heads=31000, kv_heads=31000, dim=128, **wide)
