@@ -109,7 +109,9 @@ class FusedAdam(torch.optim.Adam):
         """visibility: int32 [n_primitives] (> 0 = update), e.g. aux["visibility"] of the view's
         forward; None takes the last differentiable forward's (sparse only). max_norm: the update
         uses the gradients clipped to this global norm (of all groups' rows, visible or not), which
-        the call returns as a 0-dim device tensor; the gradients themselves are left unscaled."""
+        the call returns as a 0-dim device tensor; the gradients themselves are left unscaled. Such a
+        step weights the new value by 1 - beta rounded from float64, the plain one, like the reference,
+        by 1 - float32(beta): their exp_avg_sq differ by 1.3e-5 of it. A refused call changes nothing."""
         from .raster3d import _Rasterize3D
 
         if max_norm is not None:

@@ -116,9 +116,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: tor
     scores s become c tanh(s / c). scale: of the scores before the cap (default 1 / sqrt(D)).
 
     A query that sees no key gets 0 and -infinity. A key or value that is not finite reaches only the
-    queries that see it (the gradients of its document are not kept apart so). D up to 128 (padded to a multiple of 8 by a copy).
-    Tensors are read through their strides where these and the addresses are multiples of 16 bytes
-    and the last dimension is contiguous; otherwise they are copied first."""
+    queries that see it (the gradients of its document are not kept apart so). Sums are float32: 2^8
+    times the sum of |v| over a query's keys has to be finite there. No forward-mode derivative. D up to
+    128 (padded to a multiple of 8 by a copy). Tensors are read through their strides where these and the
+    addresses are multiples of 16 bytes and the last dimension is contiguous; otherwise they are copied
+    first."""
     if not (q.dim() == k.dim() == v.dim() == 3):
         raise ValueError("q, k and v must be [tokens, heads, D]")
     if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:

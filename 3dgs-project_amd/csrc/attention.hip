@@ -175,10 +175,11 @@ __device__ __forceinline__ void sums_of_seen(const AttnArgs& a, const Rule& u, c
     }
 }
 
-// Three workgroups a CU for 64 elements without the causal mask: a packed batch's last round is then
-// shorter (8203 tokens in 4 documents, 16 heads: 112 -> 102 us; 8192 in one, four full rounds, 315 either
-// way). The causal instance would spill a little: 8192 tokens 179 -> 170 us plain, but 220 -> 225 capped, and
-// 100 queries on eight caches of 3000 30 -> 32.
+// Three workgroups a CU for up to 64 elements without the causal mask: a packed batch's last round is then
+// shorter (8203 tokens in 4 documents, 16 heads of 64: 115 -> 104 us, capped 151 -> 144; 8192 in one 344 -> 336),
+// for a register spilled at 64. The causal instance, of 178 registers, gains plain (8192 tokens 182 -> 174 us) but
+// loses capped (245 -> 251) and over caches (100 queries on eight of 3000 30 -> 32, capped 37 -> 42). Of the
+// instances with two workgroups those for 128 elements under the causal mask spill one to three of 256.
 template <typename T, int DU, int MODE, bool CAUSAL>
 __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DU <= 64 && !CAUSAL ? 3 : 2) : 1) void attn_fwd_kernel(AttnArgs a) {
   using L = Tile<T, row_of(DU)>;
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DU <= 64 && !CAUSAL
     __syncthreads();
     if (k0 + kAttnKeys < piece.stop) fetch(k0 + kAttnKeys, lds + (buf ^ 1) * 2 * kTileBytes);
     // a wavefront past the last row only copies: its SIMD is the other workgroup's (8192 causal tokens, 16
-    // heads of 64: 201 -> 175 us, where registers count too; in the gradients' kernels it gains nothing)
+    // heads of 64: 209 -> 182 us, of 128 297 -> 286; in the gradients' kernels it gains nothing)
     if (uniform(wrow) >= rows) continue;
     f32x16 s[2] = {};
     {
@@ -248,7 +249,8 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DU <= 64 && !CAUSAL
     keep_order<T>();
     softmax_step<T, MODE>(rule, s, o, st, k0 + kAttnKeys > wave_min, vis - k0, h);
     // the wavefront that has its probabilities goes first: its products then run while the SIMD's other
-    // wavefront is at its exponentials, and not the two in step (584 -> 561 us at 8192 tokens, 16 heads of 128)
+    // wavefront is at its exponentials, and not the two in step (8192 tokens, 16 heads of 128: 562 -> 547 us,
+    // causal 311 -> 286, capped 689 -> 669; both together lose a little, 365 -> 370)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int kc = 0; kc < 4; ++kc) {
@@ -263,8 +265,8 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? (DU <= 64 && !CAUSAL
     }
     __builtin_amdgcn_s_setprio(0);
   }
-  // an instance of its own: the code costs registers (8192 causal tokens, 16 heads: 276 -> 278 us at 128
-  // elements, 251 -> 266 us at 64, capped)
+  // only where queries of a tile see different keys (8192 causal tokens, 16 heads of 128, with and without this
+  // code 286 and 287 us; of 64, capped, 245 and 246)
   if constexpr (CAUSAL) {
     if (any_not_finite(o))
       sums_of_seen<T, DU, MODE>(a, rule, q, kp, vp, st.m, piece.begin, 32, min(vis, piece.stop), h, o);
@@ -734,9 +736,11 @@ __global__ __launch_bounds__(kAttnThreads, sizeof(T) == 2 ? 2 : 1) void attn_bwd
 // files. There, workgroups with blockIdx.y = 0 gather dK (three products) and the others dV (S again, two
 // products): five products for four, but two wavefronts a SIMD that fill each other's gaps. Measured at
 // 8192 tokens, 16 heads of 128, the whole backward: 2199 us together with one wavefront a SIMD, 2008 apart; causal
-// 1263 and 1123. In float32 it is 128 elements at which both do not fit one wavefront's 512 registers: 2500
-// tokens, 16 heads, causal, the whole backward 1804 us together (115 registers spilled) and 1428 apart, capped 2079
-// and 1568; without the mask, whose code spills most, 2669 and 2713. Smaller heads keep both in one.
+// 1263 and 1123. In float32 it is 128 elements at which both do not fit one wavefront's 512 registers (115
+// spilled). The whole backward together and apart, 16 heads: 700 tokens 337 and 283 us, causal 257 and 225; 2500
+// tokens 2680 and 2711, causal 1789 and 1430, capped 3348 and 3009, both 2074 and 1576; 6000 tokens 11319 and 11662,
+// causal 7305 and 6179, capped 16734 and 12871. Apart loses 1 to 3% in long plain documents without the mask and
+// gains elsewhere, so it is taken throughout. Smaller heads keep both in one.
 constexpr bool split_kv(bool bf16, int dim) { return dim > (bf16 ? 64 : 96); }
 template <typename T, int DU>
 constexpr bool kSplitKv = split_kv(sizeof(T) == 2, DU);
@@ -1173,7 +1177,7 @@ namespace gs {
 // heads of its group: with few key heads that is one long chain on a part of the chip. The rows are then
 // cut into parts, until the longest chain is about half of what each of the chip's 512 workgroups has to
 // do on average (a causal tile has half the rows on average); the parts' sums are joined in float32.
-// Measured at 8192 causal tokens, 16 heads on 4 of 128, capped: backward 1998 us in one part, 1532 us in 4.
+// Measured at 8192 causal tokens, 16 heads on 4 of 128, capped: backward 1983 us in one part, 1509 us in 4.
 struct BwdPlan {
   int64_t q_tiles, k_tiles;
   int kv_roles, row_parts, key_parts;

@@ -631,7 +631,8 @@ int gs_rotary_axes(const gs_rotary* args, void* stream);
  * (device int32, may be NULL; only with causal). Scores s = scale q.k (a scale of 0, or
  * 2^-126 to 2^126 in size), or with a softcap (0: none; 2^-96 to 2^96, and scale / softcap 2^-126 to 2^125) softcap tanh(scale q.k / softcap).
  *   out [q_tokens, heads, dim] = sum_j softmax(s)_j v_j, lse [q_tokens, heads] float32 = ln sum_j e^s_j.
- * A query that sees nothing, and one outside every document, gets 0 and -infinity. Key tokens
+ * Sums are float32 and divided at the end: of a row, 2^8 times the sum of |v| over the keys it sees has to be
+ * finite in float32. A query that sees nothing, and one outside every document, gets 0 and -infinity. Key tokens
  * outside the documents and their lengths are never used, whatever they hold, and a key or value that is
  * not finite reaches the queries that see it only. Offsets and lengths outside the tensors are cut to
  * them.
