@@ -9,10 +9,14 @@ Gaussians from images there are `attention`, `rotary_axes`, and `grad_norm` / `c
 from .adam import FusedAdam, adam_step, adam_step_sparse
 from .attention import attention
 from .clip import clip_grad_norm, grad_norm
+from .dropout import dropout
 from .loss import fused_ssim, l1_ssim_loss
+from .norm import norm, residual_norm
 from .raster3d import (Camera, backward_pass, densification_stats, forward_pass, pruning_scores, rasterize,
                        rasterize_inference)
 from .rotary import rotary_axes
+from .scan import gated_scan
 
 __all__ = ["Camera", "rasterize", "rasterize_inference", "pruning_scores", "forward_pass", "backward_pass", "densification_stats", "FusedAdam", "adam_step", "adam_step_sparse",
-           "l1_ssim_loss", "fused_ssim", "attention", "rotary_axes", "grad_norm", "clip_grad_norm"]
+           "l1_ssim_loss", "fused_ssim", "attention", "rotary_axes", "grad_norm", "clip_grad_norm",
+           "norm", "residual_norm", "dropout", "gated_scan"]

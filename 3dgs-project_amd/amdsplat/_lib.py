@@ -125,6 +125,59 @@ class GsAttention(C.Structure):
     ]
 
 
+class GsResidualNorm(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("y", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("post_weight", C.c_void_p),
+        ("post_bias", C.c_void_p),
+        ("gate", C.c_void_p),
+        ("h", C.c_void_p),
+        ("n", C.c_void_p),
+        ("stats", C.c_void_p),
+        ("seed_at", C.c_void_p),
+        ("seed", C.c_uint64),
+        ("draw", C.c_uint64),
+        ("rows", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("y_stride", C.c_int64),
+        ("gate_stride", C.c_int64),
+        ("dropout", C.c_double),
+        ("eps", C.c_float),
+        ("scale", C.c_float),
+        ("width", C.c_int32),
+        ("x_dtype", C.c_int32),
+        ("y_dtype", C.c_int32),
+        ("weight_dtype", C.c_int32),
+        ("gate_dtype", C.c_int32),
+        ("gate_rows", C.c_int32),
+        ("layer", C.c_int32),
+    ]
+
+
+class GsGatedScan(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("forget", C.c_void_p),
+        ("gate", C.c_void_p),
+        ("initial", C.c_void_p),
+        ("y", C.c_void_p),
+        ("state", C.c_void_p),
+        ("carry", C.c_void_p),
+        ("offsets", C.c_void_p),
+        ("tokens", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("forget_stride", C.c_int64),
+        ("gate_stride", C.c_int64),
+        ("docs", C.c_int32),
+        ("width", C.c_int32),
+        ("dtype", C.c_int32),
+        ("reverse", C.c_int32),
+    ]
+
+
 class AmdSplatError(RuntimeError):
     pass
 
@@ -181,6 +234,14 @@ _SIGS = {
     "gs_attention_fwd": (_i32, [_vp, _vp, _sz, _vp]),
     "gs_attention_bwd_workspace_size": (_sz, [_vp]),
     "gs_attention_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gs_residual_norm_fwd": (_i32, [_vp, _vp]),
+    "gs_residual_norm_bwd_workspace_size": (_sz, [_vp]),
+    "gs_residual_norm_bwd": (_i32, [_vp] * 11 + [_sz, _vp]),
+    "gs_dropout": (_i32, [_vp, _vp, _i64, _i64, _i32, _i32, C.c_double, _vp, C.c_uint64, C.c_uint64, _vp]),
+    "gs_gated_scan_chunks": (_i64, [_i64]),
+    "gs_gated_scan_workspace_size": (_sz, [_i64, _i32]),
+    "gs_gated_scan_fwd": (_i32, [_vp, _vp, _sz, _vp]),
+    "gs_gated_scan_bwd": (_i32, [_vp] * 8 + [_sz, _vp]),
     "gs_densification_stats": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp]),
     "gs_l1_ssim_workspace_size": (_sz, [_i32, _i32, _i32]),
     "gs_l1_ssim_fwd": (_i32, [_vp, _vp, _i32, _i32, _i32, C.c_float, _vp, _vp, _vp, _sz, _vp]),

@@ -20,7 +20,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 OUT = HERE / "amdsplat" / "libamdsplat.so"
 SOURCES = ["capi.hip", "preprocess.hip", "binning.hip", "blend.hip", "view.hip", "raster2d.hip", "adam.hip", "loss.hip",
-           "attention.hip", "rotary.hip", "clip.hip", "probe.hip"]
+           "attention.hip", "rotary.hip", "clip.hip", "norm.hip",
+           "scan.hip", "probe.hip"]
 
 HIPCC_FLAGS = [
     "-O3",

@@ -1,0 +1,64 @@
+// Rows of float32 or bfloat16 in vectors of eight elements, at any address and stride (the memory system splits
+// an access that crosses a line), the last vector of a row cut short.
+#pragma once
+
+#include "gs_host.h"
+
+namespace gs {
+
+template <typename T>
+struct Raw8 {
+  typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+  static constexpr int kParts = sizeof(T) / 2;  // 16-byte accesses
+  static constexpr int kPer = 16 / sizeof(T);
+};
+
+// Elements p[0 .. n) of eight as float, the others zero. n >= 8: one or two 16-byte loads.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
+  using R = Raw8<T>;
+  if (n >= 8) {
+#pragma unroll
+    for (int i = 0; i < R::kParts; ++i) {
+      const auto a = *reinterpret_cast<const typename R::Vec*>(p + i * R::kPer);
+#pragma unroll
+      for (int j = 0; j < R::kPer; ++j) v[i * R::kPer + j] = static_cast<float>(a[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? static_cast<float>(p[j]) : 0.0f;
+  }
+}
+// The same of a tensor whose type is known at run time.
+__device__ __forceinline__ void load8(const void* p, bool bf16, int64_t at, int n, float (&v)[8]) {
+  if (bf16) load8(static_cast<const __bf16*>(p) + at, n, v);
+  else load8(static_cast<const float*>(p) + at, n, v);
+}
+
+// Rounded once, to nearest.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {
+  using R = Raw8<T>;
+  if (n >= 8) {
+#pragma unroll
+    for (int i = 0; i < R::kParts; ++i) {
+      typename R::Vec a;
+#pragma unroll
+      for (int j = 0; j < R::kPer; ++j) a[j] = static_cast<T>(v[i * R::kPer + j]);
+      *reinterpret_cast<typename R::Vec*>(p + i * R::kPer) = a;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = static_cast<T>(v[j]);
+  }
+}
+__device__ __forceinline__ void store8(void* p, bool bf16, int64_t at, int n, const float (&v)[8]) {
+  if (bf16) store8(static_cast<__bf16*>(p) + at, n, v);
+  else store8(static_cast<float*>(p) + at, n, v);
+}
+
+inline bool row_type(int dtype) { return dtype == GS_FLOAT32 || dtype == GS_BFLOAT16; }
+inline size_t row_type_bytes(int dtype) { return dtype == GS_BFLOAT16 ? 2 : 4; }
+
+}  // namespace gs

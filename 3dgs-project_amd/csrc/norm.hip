@@ -1,0 +1,553 @@
+// Norms before and after a block, fused with what lies between them, forward and backward:
+//
+//   b = y, or post(y) = w' y^ + b'        y^ = (y - mean) / sqrt(var + eps), or without a mean y / sqrt(mean y^2 + eps)
+//   h = x + scale gate k b                k: the dropout's factors, formed from the counter (gs_philox.h)
+//   n = w h^ + b                          h^: h standardised in the same way
+//
+// and dropout alone. A row is held in the registers of 64 to 1024 lanes from its one reading to its one writing;
+// deviations are taken from the mean, not from the sum of squares. The backward pass forms h and its
+// standardised rows again from x, y and four saved statistics a row, so that nothing else is kept:
+//
+//   t = dn w;  D = dh + (t - h^ mean(t h^) [- mean t]) / dev        dx = D
+//   dgate = sum or each of scale D k b;   v = scale D gate k;   dw' = sum v y^, db' = sum v;  dw = sum dn h^, db = sum dn
+//   q = v w';  dy = (q - y^ mean(q y^) [- mean q]) / dev'
+//
+// Column sums are kept in registers over the rows of a workgroup, joined in LDS, written as one part a workgroup
+// and summed in a fixed order: no atomics, the same inputs give the same bits.
+#include <algorithm>
+
+#include "gs_philox.h"
+#include "gs_rows.h"
+
+namespace gs {
+
+struct NormArgs {
+  const void *x, *y, *weight, *bias, *post_weight, *post_bias, *gate;
+  void *h, *n;
+  float* stats;  // [rows][4]: mean and 1 / deviation of h, of y
+  int64_t rows, x_stride, y_stride, gate_stride;
+  int width;
+  bool layer, post, weights_bf16, gate_bf16;
+  float eps, scale, inv_width;
+  DropRule drop;
+  // backward
+  const void *d_h, *d_n;
+  void *d_x, *d_y, *d_gate_rows;
+  float* parts;      // [workgroups][sums][width]
+  int sums;          // of the five column sums
+  int8_t slot[5];    // where they are among these, -1: not wanted
+};
+enum { kSumWeight = 0, kSumBias, kSumPostWeight, kSumPostBias, kSumGate };
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 1; o < kWave; o *= 2) v += __shfl_xor(v, o);
+  return v;
+}
+
+// Sums of two values over the G lanes of a row; `turn` alternates between two sets of LDS words, so that one barrier
+// a sum is enough.
+template <int G, int GROUPS>
+struct RowSum {
+  float2 (*lds)[GROUPS][G / kWave];
+  int turn = 0;
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (G > kWave) {
+      const int group = threadIdx.x / G, wave = threadIdx.x % G / kWave;
+      if (threadIdx.x % kWave == 0) lds[turn][group][wave] = make_float2(a, b);
+      __syncthreads();
+      a = b = 0.0f;
+#pragma unroll
+      for (int i = 0; i < G / kWave; ++i) {
+        a += lds[turn][group][i].x;
+        b += lds[turn][group][i].y;
+      }
+      turn ^= 1;
+    }
+    return make_float2(a, b);
+  }
+};
+
+// Mean and 1 / deviation of a row held in registers (elements past the width are zero).
+template <int NV, typename S>
+__device__ __forceinline__ float2 row_stats(const NormArgs& a, const float (&v)[NV][8], const int (&left)[NV], S& sum) {
+  float mean = 0.0f;
+  if (a.layer) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[i][j];
+    mean = sum(s, 0.0f).x * a.inv_width;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = j < left[i] ? v[i][j] - mean : 0.0f;
+      q = fmaf(d, d, q);
+    }
+  const float var = sum(q, 0.0f).x * a.inv_width;
+  return make_float2(mean, 1.0f / sqrtf(var + a.eps));
+}
+
+// k b of eight elements from y (given standardised as `hat`).
+__device__ __forceinline__ void branch8(const NormArgs& a, uint64_t seed, int64_t row, int col, int n,
+                                        const float (&hat)[8], float (&keep)[8], float (&u)[8]) {
+  float w[8], b[8];
+  if (a.post) {
+    load8(a.post_weight, a.weights_bf16, col, n, w);
+    if (a.post_bias) load8(a.post_bias, a.weights_bf16, col, n, b);
+  }
+  if (a.drop.threshold) keep8(a.drop, seed, static_cast<uint32_t>(row), col / 8, keep);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    u[j] = hat[j];
+    if (a.post) u[j] = a.post_bias ? fmaf(hat[j], w[j], b[j]) : hat[j] * w[j];
+    if (a.drop.threshold) u[j] = keep[j] != 0.0f ? u[j] * keep[j] : 0.0f;
+    else keep[j] = 1.0f;
+  }
+}
+
+// G lanes a row, each NV vectors of eight: vector i of lane l begins at 8 (l + G i).
+template <typename X, typename Y, int G, int NV>
+__global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a) {
+  constexpr int kGroups = G > 256 ? 1 : 256 / G;
+  __shared__ float2 lds[2][kGroups][G / kWave];
+  RowSum<G, kGroups> sum{lds};
+  const int lane = threadIdx.x % G;
+  const int64_t row_at = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
+  // (groups past the last row repeat it without writing: every lane meets every barrier)
+  const bool mine = row_at < a.rows;
+  const int64_t row = mine ? row_at : a.rows - 1;
+  float h[NV][8], b[NV][8];
+  int left[NV];
+  const X* x = static_cast<const X*>(a.x) + row * a.x_stride;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = 8 * (lane + G * i);
+    left[i] = a.width - col;
+    load8(x + col, left[i], h[i]);
+  }
+  if (a.y) {
+    const Y* y = static_cast<const Y*>(a.y) + row * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load8(y + 8 * (lane + G * i), left[i], b[i]);
+    float2 st = {0.0f, 1.0f};
+    if (a.post) st = row_stats(a, b, left, sum);
+    if (mine && lane == 0 && a.stats) {
+      a.stats[4 * row + 2] = st.x;
+      a.stats[4 * row + 3] = st.y;
+    }
+    const uint64_t seed = a.drop.threshold ? seed_of(a.drop) : 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (left[i] <= 0) continue;
+      const int col = 8 * (lane + G * i);
+      float keep[8], u[8], g[8], hat[8];
+      if (a.gate) load8(a.gate, a.gate_bf16, row * a.gate_stride + col, left[i], g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hat[j] = a.post ? (b[i][j] - st.x) * st.y : b[i][j];
+      branch8(a, seed, row, col, left[i], hat, keep, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = a.gate ? a.scale * g[j] : a.scale;
+        h[i][j] = j < left[i] ? fmaf(w, u[j], h[i][j]) : 0.0f;
+      }
+      if (mine) store8(static_cast<X*>(a.h) + row * a.width + col, left[i], h[i]);
+    }
+  }
+  const float2 st = row_stats(a, h, left, sum);
+  if (mine && lane == 0 && a.stats) {
+    a.stats[4 * row] = st.x;
+    a.stats[4 * row + 1] = st.y;
+  }
+  if (!mine) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (left[i] <= 0) continue;
+    const int col = 8 * (lane + G * i);
+    float w[8], c[8], n[8];
+    if (a.weight) load8(a.weight, a.weights_bf16, col, left[i], w);
+    if (a.bias) load8(a.bias, a.weights_bf16, col, left[i], c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      n[j] = (h[i][j] - st.x) * st.y;
+      if (a.weight) n[j] *= w[j];
+      if (a.bias) n[j] += c[j];
+    }
+    store8(static_cast<Y*>(a.n) + row * a.width + col, left[i], n);
+  }
+}
+
+template <typename X, typename Y, int G, int NV>
+__global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a) {
+  constexpr int kGroups = G > 256 ? 1 : 256 / G;
+  constexpr int kWidth = 8 * G * NV;
+  __shared__ float2 lds[2][kGroups][G / kWave];
+  __shared__ float join[kGroups > 1 ? kGroups * kWidth : 1];
+  RowSum<G, kGroups> sum{lds};
+  const int lane = threadIdx.x % G;
+  float col_sum[5][NV][8] = {};
+  int left[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) left[i] = a.width - 8 * (lane + G * i);
+  const uint64_t seed = a.drop.threshold ? seed_of(a.drop) : 0;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  // (the groups of a workgroup take as many turns as its first one: barriers are met by all)
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows; first += step) {
+    const int64_t row_at = first + threadIdx.x / G;
+    const bool mine = row_at < a.rows;
+    const int64_t row = mine ? row_at : a.rows - 1;
+    float hat[NV][8], t[NV][8], d[NV][8], b[NV][8], u[NV][8], keep[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
+      load8(static_cast<const X*>(a.x) + row * a.x_stride + col, n, hat[i]);
+      if (a.y) load8(static_cast<const Y*>(a.y) + row * a.y_stride + col, n, b[i]);
+      load8(static_cast<const Y*>(a.d_n) + row * a.width + col, a.d_n ? n : 0, t[i]);
+      load8(static_cast<const X*>(a.d_h) + row * a.width + col, a.d_h ? n : 0, d[i]);
+    }
+    const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
+      float w[8];
+      if (a.weight && n > 0) load8(a.weight, a.weights_bf16, col, n, w);
+      if (a.y && n > 0) {
+        float g[8];
+        if (a.gate) load8(a.gate, a.gate_bf16, row * a.gate_stride + col, n, g);
+        if (a.post) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) b[i][j] = (b[i][j] - st.z) * st.w;
+        }
+        branch8(a, seed, row, col, n, b[i], keep[i], u[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float f = a.gate ? a.scale * g[j] : a.scale;
+          hat[i][j] = fmaf(f, u[i][j], hat[i][j]);
+          keep[i][j] *= f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        hat[i][j] = j < n ? (hat[i][j] - st.x) * st.y : 0.0f;
+        col_sum[kSumWeight][i][j] = fmaf(t[i][j], hat[i][j], col_sum[kSumWeight][i][j]);
+        col_sum[kSumBias][i][j] += t[i][j];
+        if (a.weight) t[i][j] = j < n ? t[i][j] * w[j] : 0.0f;
+        s1 = fmaf(t[i][j], hat[i][j], s1);
+        s2 += t[i][j];
+      }
+    }
+    const float2 m = sum(s1, s2);
+    const float m1 = m.x * a.inv_width, m2 = a.layer ? m.y * a.inv_width : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[i][j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
+      if (a.d_x && n > 0) store8(static_cast<X*>(a.d_x) + row * a.width + col, n, d[i]);
+    }
+    if (!a.y) continue;
+    s1 = s2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
+      float e[8], w[8];
+      if (a.post && n > 0) load8(a.post_weight, a.weights_bf16, col, n, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = j < n ? a.scale * d[i][j] * u[i][j] : 0.0f;  // of the gate
+        col_sum[kSumGate][i][j] += e[j];
+        const float v = j < n ? d[i][j] * keep[i][j] : 0.0f;
+        if (a.post) {
+          if (j >= n) b[i][j] = 0.0f;
+          col_sum[kSumPostWeight][i][j] = fmaf(v, b[i][j], col_sum[kSumPostWeight][i][j]);
+          col_sum[kSumPostBias][i][j] += v;
+          t[i][j] = j < n ? v * w[j] : 0.0f;
+          s1 = fmaf(t[i][j], b[i][j], s1);
+          s2 += t[i][j];
+        } else {
+          t[i][j] = v;
+        }
+      }
+      if (a.d_gate_rows && n > 0) store8(a.d_gate_rows, a.gate_bf16, row * a.width + col, n, e);
+    }
+    if (a.post) {
+      const float2 p = sum(s1, s2);
+      const float p1 = p.x * a.inv_width, p2 = a.layer ? p.y * a.inv_width : 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[i][j] = st.w * (t[i][j] - fmaf(b[i][j], p1, p2));
+    }
+    if (a.d_y) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (mine && left[i] > 0) store8(static_cast<Y*>(a.d_y) + row * a.width + 8 * (lane + G * i), left[i], t[i]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 5; ++k) {
+    if (a.slot[k] < 0) continue;
+    float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * a.sums + a.slot[k]) * a.width;
+    if constexpr (kGroups == 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (left[i] > 0) store8(part + 8 * (lane + G * i), left[i], col_sum[k][i]);
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) join[(threadIdx.x / G) * kWidth + 8 * (lane + G * i) + j] = col_sum[k][i][j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.width; c += 256) {
+        float s = join[c];
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) s += join[g * kWidth + c];
+        part[c] = s;
+      }
+    }
+  }
+}
+
+// Sums the workgroups' parts, column by column in a fixed order: 64 columns of one sum a workgroup, its wavefronts
+// take the parts in turn.
+constexpr int kPartThreads = 1024;
+struct NormSums {
+  const float* parts;
+  int n, sums, width;
+  void* out[5];
+  bool bf16[5];
+};
+__global__ __launch_bounds__(kPartThreads) void norm_sums_kernel(NormSums a) {
+  __shared__ float part[kPartThreads];
+  const int k = blockIdx.y, c = blockIdx.x * kWave + threadIdx.x % kWave, w = threadIdx.x / kWave;
+  float s[4] = {};
+  if (c < a.width) {
+    constexpr int kStep = kPartThreads / kWave;
+    int p = w;
+    const auto at = [&](int i) { return a.parts[(static_cast<int64_t>(i) * a.sums + k) * a.width + c]; };
+    for (; p + 3 * kStep < a.n; p += 4 * kStep) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += at(p + i * kStep);
+    }
+    for (; p < a.n; p += kStep) s[0] += at(p);
+  }
+  part[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (w == 0 && c < a.width) {
+    float t = 0.0f;
+    for (int i = 0; i < kPartThreads / kWave; ++i) t += part[i * kWave + threadIdx.x];
+    if (a.bf16[k]) static_cast<__bf16*>(a.out[k])[c] = static_cast<__bf16>(t);
+    else static_cast<float*>(a.out[k])[c] = t;
+  }
+}
+
+// Dropout alone: a vector of eight a thread.
+constexpr int kDropThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* x, T* out, int64_t rows, int64_t stride,
+                                                               int width, int groups, DropRule drop) {
+  const uint64_t seed = seed_of(drop);
+  const int64_t all = rows * groups;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x;
+  if (i >= all) return;
+  const int64_t row = i / groups;
+  const int group = static_cast<int>(i - row * groups), n = width - 8 * group;
+  float v[8], keep[8];
+  load8(x + row * stride + 8 * group, n, v);
+  keep8(drop, seed, static_cast<uint32_t>(row), group, keep);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = keep[j] != 0.0f ? v[j] * keep[j] : 0.0f;
+  store8(out + row * width + 8 * group, n, v);
+}
+
+// Workgroups of the backward pass: two a CU, so that the parts stay small beside the rows (at 1024 columns and
+// three sums 6 MB written and read).
+constexpr int64_t kNormParts = 512;
+static int64_t norm_parts(int64_t rows) { return std::min<int64_t>(kNormParts, rows); }
+
+static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
+  GS_REQUIRE(p, GS_ERR_ARG, "residual norm: args is NULL");
+  GS_REQUIRE(row_type(p->x_dtype) && row_type(p->y_dtype), GS_ERR_ARG,
+             "residual norm: dtypes must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(p->x_dtype == GS_FLOAT32 || p->y_dtype == GS_BFLOAT16, GS_ERR_ARG,
+             "residual norm: a bfloat16 stream takes a bfloat16 branch and norm");
+  GS_REQUIRE((!p->weight && !p->bias && !p->post_weight && !p->post_bias) || row_type(p->weight_dtype), GS_ERR_ARG,
+             "residual norm: weight dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(!p->gate || row_type(p->gate_dtype), GS_ERR_ARG, "residual norm: gate dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(p->rows >= 0 && p->rows < (int64_t(1) << 31), GS_ERR_ARG, "residual norm: invalid row count");
+  GS_REQUIRE(p->width >= 1 && p->width <= GS_NORM_MAX_WIDTH, GS_ERR_ARG, "residual norm: width %d: 1 to %d are provided",
+             p->width, GS_NORM_MAX_WIDTH);
+  GS_REQUIRE(p->eps > 0.0f && p->eps <= 1e30f, GS_ERR_ARG, "residual norm: eps must be positive and finite");
+  GS_REQUIRE(p->scale - p->scale == 0.0f, GS_ERR_ARG, "residual norm: scale must be finite");
+  GS_REQUIRE(p->dropout >= 0.0 && p->dropout < 1.0, GS_ERR_ARG, "residual norm: dropout must be at least 0 and below 1");
+  GS_REQUIRE(p->y || (!p->gate && !p->post_weight && !p->post_bias && p->dropout == 0.0), GS_ERR_ARG,
+             "residual norm: a gate, a post norm or dropout needs y");
+  GS_REQUIRE(!p->post_bias || p->post_weight, GS_ERR_ARG, "residual norm: a post bias needs a post weight");
+  GS_REQUIRE(p->rows == 0 || (p->x && (backward || (p->n && (!p->y || p->h)))), GS_ERR_ARG, "residual norm: null pointer");
+  const size_t xs = row_type_bytes(p->x_dtype), ys = row_type_bytes(p->y_dtype), ws = row_type_bytes(p->weight_dtype);
+  GS_REQUIRE(aligned(p->x, xs) && aligned(p->h, xs) && aligned(p->y, ys) && aligned(p->n, ys) && aligned(p->weight, ws) &&
+                 aligned(p->bias, ws) && aligned(p->post_weight, ws) && aligned(p->post_bias, ws) &&
+                 aligned(p->gate, row_type_bytes(p->gate_dtype)) && aligned(p->stats, 16) && aligned(p->seed_at, 8),
+             GS_ERR_ALIGN, "residual norm: misaligned tensor");
+  *a = {};
+  a->x = p->x;
+  a->y = p->y;
+  a->weight = p->weight;
+  a->bias = p->bias;
+  a->post_weight = p->post_weight;
+  a->post_bias = p->post_bias;
+  a->gate = p->gate;
+  a->h = p->h;
+  a->n = p->n;
+  a->stats = p->stats;
+  a->rows = p->rows;
+  a->x_stride = p->x_stride;
+  a->y_stride = p->y_stride;
+  a->gate_stride = p->gate_rows ? p->gate_stride : 0;
+  a->width = p->width;
+  a->layer = p->layer != 0;
+  a->post = p->post_weight != nullptr;
+  a->weights_bf16 = p->weight_dtype == GS_BFLOAT16;
+  a->gate_bf16 = p->gate_dtype == GS_BFLOAT16;
+  a->eps = p->eps;
+  a->scale = p->scale;
+  a->inv_width = static_cast<float>(1.0 / p->width);
+  a->drop = drop_rule(p->dropout, p->seed_at, p->seed, p->draw);
+  return GS_OK;
+}
+
+// Calls f(kernel, lanes a row) with the instance for a width: a wavefront a row where eight or sixteen elements a
+// lane do, more wavefronts above.
+template <typename X, typename Y, typename F>
+static int with_fwd(int width, F f) {
+  if (width <= 512) return f(norm_fwd_kernel<X, Y, 64, 1>, 64);
+  if (width <= 1024) return f(norm_fwd_kernel<X, Y, 64, 2>, 64);
+  if (width <= 2048) return f(norm_fwd_kernel<X, Y, 64, 4>, 64);
+  if (width <= 4096) return f(norm_fwd_kernel<X, Y, 256, 2>, 256);
+  if (width <= 8192) return f(norm_fwd_kernel<X, Y, 512, 2>, 512);
+  return f(norm_fwd_kernel<X, Y, 1024, 2>, 1024);
+}
+template <typename X, typename Y, typename F>
+static int with_bwd(int width, F f) {
+  if (width <= 512) return f(norm_bwd_kernel<X, Y, 64, 1>, 64);
+  if (width <= 1024) return f(norm_bwd_kernel<X, Y, 64, 2>, 64);
+  if (width <= 2048) return f(norm_bwd_kernel<X, Y, 256, 1>, 256);
+  if (width <= 4096) return f(norm_bwd_kernel<X, Y, 256, 2>, 256);
+  if (width <= 8192) return f(norm_bwd_kernel<X, Y, 512, 2>, 512);
+  return f(norm_bwd_kernel<X, Y, 1024, 2>, 1024);
+}
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int gs_residual_norm_fwd(const gs_residual_norm* p, void* stream) {
+  clear_error();
+  NormArgs a;
+  if (const int rc = check_norm(p, false, &a)) return rc;
+  if (a.rows == 0) return GS_OK;
+  const auto run = [&](auto kernel, int lanes) {
+    const int groups = std::max(1, 256 / lanes);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)), dim3(std::max(256, lanes)), 0,
+                       as_stream(stream), a);
+    return check_launch("residual norm");
+  };
+  if (p->x_dtype == GS_BFLOAT16) return with_fwd<__bf16, __bf16>(a.width, run);
+  if (p->y_dtype == GS_BFLOAT16) return with_fwd<float, __bf16>(a.width, run);
+  return with_fwd<float, float>(a.width, run);
+}
+
+extern "C" size_t gs_residual_norm_bwd_workspace_size(const gs_residual_norm* p) {
+  clear_error();
+  if (!p || p->rows <= 0 || p->width <= 0) return 0;
+  return static_cast<size_t>(norm_parts(p->rows)) * 5 * static_cast<size_t>(p->width) * sizeof(float);
+}
+
+extern "C" int gs_residual_norm_bwd(const gs_residual_norm* p, const void* d_h, const void* d_n, void* d_x, void* d_y,
+                                    void* d_weight, void* d_bias, void* d_post_weight, void* d_post_bias, void* d_gate,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  NormArgs a;
+  if (const int rc = check_norm(p, true, &a)) return rc;
+  GS_REQUIRE(a.rows == 0 || a.stats, GS_ERR_ARG, "residual norm: the backward pass needs the statistics");
+  GS_REQUIRE(a.y || (!d_y && !d_gate && !d_post_weight && !d_post_bias && !d_h), GS_ERR_ARG,
+             "residual norm: gradients of a branch that is not there");
+  GS_REQUIRE((a.gate || !d_gate) && (a.post || (!d_post_weight && !d_post_bias)), GS_ERR_ARG,
+             "residual norm: gradients of a gate or post norm that is not there");
+  GS_REQUIRE(workspace_bytes >= gs_residual_norm_bwd_workspace_size(p) && (workspace || a.rows == 0), GS_ERR_WORKSPACE,
+             "residual norm: workspace too small");
+  const size_t xs = row_type_bytes(p->x_dtype), ys = row_type_bytes(p->y_dtype), ws = row_type_bytes(p->weight_dtype);
+  GS_REQUIRE(aligned(d_h, xs) && aligned(d_x, xs) && aligned(d_n, ys) && aligned(d_y, ys) && aligned(d_weight, ws) &&
+                 aligned(d_bias, ws) && aligned(d_post_weight, ws) && aligned(d_post_bias, ws) &&
+                 aligned(d_gate, row_type_bytes(p->gate_dtype)) && aligned(workspace, 16),
+             GS_ERR_ALIGN, "residual norm: misaligned gradient or workspace");
+  a.d_h = d_h;
+  a.d_n = d_n;
+  a.d_x = d_x;
+  a.d_y = d_y;
+  const bool gate_column = p->gate_rows == 0;
+  a.d_gate_rows = gate_column ? nullptr : d_gate;
+  void* const outs[5] = {d_weight, d_bias, d_post_weight, d_post_bias, gate_column ? d_gate : nullptr};
+  NormSums s = {};
+  for (int k = 0; k < 5; ++k) {
+    a.slot[k] = outs[k] ? static_cast<int8_t>(a.sums) : int8_t(-1);
+    if (!outs[k]) continue;
+    s.out[a.sums] = outs[k];
+    s.bf16[a.sums++] = k == kSumGate ? a.gate_bf16 : a.weights_bf16;
+  }
+  a.parts = static_cast<float*>(workspace);
+  const hipStream_t st = as_stream(stream);
+  int64_t blocks = 0;
+  if (a.rows > 0) {
+    const auto run = [&](auto kernel, int lanes) {
+      const int groups = std::max(1, 256 / lanes);
+      blocks = std::min<int64_t>(norm_parts(a.rows), (a.rows + groups - 1) / groups);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(std::max(256, lanes)), 0, st, a);
+      return check_launch("residual norm backward");
+    };
+    const int rc = p->x_dtype == GS_BFLOAT16 ? with_bwd<__bf16, __bf16>(a.width, run)
+                   : p->y_dtype == GS_BFLOAT16 ? with_bwd<float, __bf16>(a.width, run)
+                                               : with_bwd<float, float>(a.width, run);
+    if (rc) return rc;
+  }
+  if (a.sums == 0) return GS_OK;
+  s.parts = a.parts;
+  s.n = static_cast<int>(blocks);  // (no rows: the sums are zero)
+  s.sums = a.sums;
+  s.width = a.width;
+  hipLaunchKernelGGL(norm_sums_kernel, dim3((a.width + kWave - 1) / kWave, a.sums), dim3(kPartThreads), 0, st, s);
+  return check_launch("residual norm backward (sums)");
+}
+
+extern "C" int gs_dropout(const void* x, void* out, int64_t rows, int64_t stride, int width, int dtype, double p,
+                          const int64_t* seed_at, uint64_t seed, uint64_t draw, void* stream) {
+  clear_error();
+  GS_REQUIRE(row_type(dtype), GS_ERR_ARG, "dropout: dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(rows >= 0 && rows < (int64_t(1) << 32) && width >= 0, GS_ERR_ARG, "dropout: invalid size");
+  GS_REQUIRE(p >= 0.0 && p < 1.0, GS_ERR_ARG, "dropout: p must be at least 0 and below 1");
+  GS_REQUIRE(rows == 0 || width == 0 || (x && out), GS_ERR_ARG, "dropout: null pointer");
+  const size_t es = row_type_bytes(dtype);
+  GS_REQUIRE(aligned(x, es) && aligned(out, es) && aligned(seed_at, 8), GS_ERR_ALIGN, "dropout: misaligned tensor");
+  const int64_t groups = (static_cast<int64_t>(width) + 7) / 8, all = rows * groups;
+  const int64_t blocks = (all + kDropThreads - 1) / kDropThreads;
+  GS_REQUIRE(blocks * kDropThreads < (int64_t(1) << 32), GS_ERR_ARG, "dropout: too many elements");
+  if (all == 0) return GS_OK;
+  const DropRule d = drop_rule(p, seed_at, seed, draw);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(kDropThreads);
+  if (dtype == GS_BFLOAT16) {
+    hipLaunchKernelGGL(dropout_kernel<__bf16>, grid, block, 0, as_stream(stream), static_cast<const __bf16*>(x),
+                       static_cast<__bf16*>(out), rows, stride, width, static_cast<int>(groups), d);
+  } else {
+    hipLaunchKernelGGL(dropout_kernel<float>, grid, block, 0, as_stream(stream), static_cast<const float*>(x),
+                       static_cast<float*>(out), rows, stride, width, static_cast<int>(groups), d);
+  }
+  return check_launch("dropout");
+}

@@ -1,0 +1,570 @@
+// A gated linear recurrence over packed documents, forward and backward:
+//
+//   a = sigmoid(f);  h_t = a_t h_(t-1) + (1 - a_t) x_t;  y_t = h_t, or h_t silu(o_t)
+//   l_t = dy_t silu(o_t) + a_(t+1) l_(t+1)   (at a document's last token the state's gradient in place of the second term)
+//   dx = (1 - a) l;  df = l (h_(t-1) - x) a (1 - a);  do = dy h silu'(o);  dinitial = a l at the first token
+//
+// A step is the map h -> E + P h, and maps compose, so the tokens are cut into chunks of 16 that a wavefront walks, a
+// lane holding four channels: scan_sums_kernel forms every chunk's map and, in LDS, the maps from the start of
+// a part (some chunks of one workgroup) to each of its chunks; scan_apply_kernel joins the parts before its own, which gives every
+// chunk its state, and walks the tokens again with it. The inputs are so read twice, the second time from the last-level
+// cache as far as it holds them. (One pass that waits for the workgroups before it would read them once, but
+// needs them to be running; nothing here waits for another workgroup.)
+//
+// A document's first token replaces the state, so P = 0 there, and a map with P = 0 drops what came before it whatever
+// that was: documents do not see each other's infinities and NaN.
+//
+// Accuracy: long memories have a near 1, where 1 - a is what counts. The smaller of a and 1 - a is formed
+// directly, s = e / (1 + e) with e = exp(-|f|), and steps are taken as h + s (x - h) or x + s (h - x). A chunk's P is
+// kept as 1 - P while that is the smaller one; a chunk's sum starts at zero, so its rounding is relative to what
+// the chunk adds; chunks are joined in float64. Rounding so does not pile up over the length of the sequence.
+#include <algorithm>
+
+#include "gs_attention.h"
+#include "gs_rows.h"
+
+namespace gs {
+
+constexpr int kScanChunk = 16;                           // tokens of a chunk
+constexpr int kScanWaves = 8;
+constexpr int kScanThreads = kScanWaves * kWave;
+constexpr int kScanVec = 4;                              // channels of a lane
+constexpr int kScanGroup = kWave * kScanVec;             // channels of a workgroup
+constexpr int kScanParts = 256;
+constexpr int kScanBatch = 8;                            // tokens whose loads are in flight together
+
+struct ScanArgs {
+  const void *x, *f, *o;
+  const float* initial;
+  void* y;
+  float *state, *carry;  // carry [chunks][width]: the state before every chunk
+  const int32_t* offsets;
+  int64_t tokens, x_stride, f_stride, o_stride;
+  int docs, width, reverse;
+  int chunks, parts, blocks;  // blocks: of a part
+  int serial;                 // one wavefront walks all chunks
+  float2* prefix;             // [chunks][width]: the map from the part's start to the chunk
+  double2* part;              // [parts][width]: the map of a part
+  // backward
+  const void* d_y;
+  const float* d_state;
+  void *d_x, *d_f, *d_o;
+  float* d_initial;
+};
+
+// Elements p[0 .. n) of four as float, the others zero.
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int n, float (&v)[4]) {
+  typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= 4) {
+    const Vec a = *reinterpret_cast<const Vec*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(a[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? static_cast<float>(p[j]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* p, int n, const float (&v)[4]) {
+  typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  if (n >= 4) {
+    Vec a;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = static_cast<T>(v[j]);
+    *reinterpret_cast<Vec*>(p) = a;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = static_cast<T>(v[j]);
+  }
+}
+
+// sigmoid(v): the larger of it and its complement, and the smaller.
+struct Sigmoid {
+  float large, small;
+  bool up;  // the larger one is sigmoid(v)
+  __device__ __forceinline__ explicit Sigmoid(float v) {
+    const float e = exp2_hw(-fabsf(v) * kLog2e);
+    large = __builtin_amdgcn_rcpf(1.0f + e);
+    small = e * large;
+    up = v >= 0.0f;
+  }
+  __device__ __forceinline__ float value() const { return up ? large : small; }
+  __device__ __forceinline__ float rest() const { return up ? small : large; }
+  __device__ __forceinline__ float step(float h, float x) const {
+    const float from = up ? h : x, to = up ? x : h;
+    return fmaf(small, to - from, from);
+  }
+  __device__ __forceinline__ float times(float v) const { return up ? fmaf(-small, v, v) : small * v; }
+};
+
+// The factor P of a chunk: its product, and 1 minus it from sums of its own.
+struct Factor {
+  float p = 1.0f, q = 0.0f;
+  __device__ __forceinline__ void by(const Sigmoid& a) {
+    const float rest = 1.0f - q;
+    q = a.up ? fmaf(a.small, rest, q) : fmaf(-a.small, rest, 1.0f);
+    p *= a.up ? 1.0f - a.small : a.small;
+  }
+  __device__ __forceinline__ void drop() {
+    p = 0.0f;
+    q = 1.0f;
+  }
+};
+// One word for it: 1 - P where that is at most a half, -P otherwise (the sign tells them apart, -0 too).
+__device__ __forceinline__ float packed(float p, float q) { return q <= 0.5f ? q : -p; }
+__device__ __forceinline__ double factor_of(float w) {
+  return __float_as_uint(w) >> 31 ? -static_cast<double>(w) : 1.0 - static_cast<double>(w);
+}
+__device__ __forceinline__ float packed(double p) {
+  return p >= 0.5 ? fabsf(static_cast<float>(1.0 - p)) : -static_cast<float>(p);
+}
+// E + P h where P = 0 drops h.
+__device__ __forceinline__ double mapped(double e, double p, double h) { return p == 0.0 ? e : fma(p, h, e); }
+
+// Place i of the documents' edges in walking order: from the front, or from the back when reversed.
+__device__ __forceinline__ int64_t scan_edge(const ScanArgs& a, int i) {
+  const int k = a.reverse ? a.docs - i : i;
+  int64_t v = a.offsets ? a.offsets[k] : (k ? a.tokens : 0);
+  v = v < 0 ? 0 : (v > a.tokens ? a.tokens : v);
+  return a.reverse ? a.tokens - v : v;
+}
+__device__ __forceinline__ int doc_at(const ScanArgs& a, int i) { return a.reverse ? a.docs - 1 - i : i; }
+__device__ __forceinline__ int64_t token_at(const ScanArgs& a, int64_t p) { return a.reverse ? a.tokens - 1 - p : p; }
+
+// What the tokens of a chunk at places p0 .. p0 + 15 are: bits for those inside a document, its first, its last; and
+// in lane k the document of token k.
+struct Places {
+  uint32_t inside, first, last;
+  int doc;
+  __device__ __forceinline__ Places(const ScanArgs& a, int64_t p0) {
+    const int lane = threadIdx.x % kWave;
+    const int64_t p = p0 + lane;
+    const bool mine = lane < kScanChunk && p < a.tokens;
+    // i: the last edge at or before p, so that empty documents are passed over
+    int i = -1;
+    int64_t at = -1, next = -1;
+    if (a.docs < kWave) {
+      const int64_t e = scan_edge(a, min(lane, a.docs));
+#pragma unroll
+      for (int k = 0; k < kScanChunk; ++k) {
+        const uint64_t b = __ballot(lane <= a.docs && e <= p0 + k);
+        if (lane == k) i = static_cast<int>(__popcll(b)) - 1;
+      }
+      at = __shfl(e, max(i, 0));
+      next = __shfl(e, min(i + 1, a.docs));
+    } else if (mine) {
+      int lo = 0, hi = a.docs + 1;  // edges before lo are at or before p, those from hi on are not
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (scan_edge(a, mid) <= p) lo = mid + 1;
+        else hi = mid;
+      }
+      i = lo - 1;
+      at = scan_edge(a, max(i, 0));
+      next = scan_edge(a, min(i + 1, a.docs));
+    }
+    const bool in = mine && i >= 0 && i < a.docs;
+    doc = in ? doc_at(a, i) : 0;
+    inside = static_cast<uint32_t>(__ballot(in));
+    first = static_cast<uint32_t>(__ballot(in && at == p));
+    last = static_cast<uint32_t>(__ballot(in && next == p + 1));
+  }
+  __device__ __forceinline__ int doc_of(int k) const { return __builtin_amdgcn_readlane(doc, k); }
+};
+
+// A lane's channels.
+struct Channels {
+  int at, n;
+  __device__ __forceinline__ explicit Channels(const ScanArgs& a)
+      : at((blockIdx.x * kWave + threadIdx.x % kWave) * kScanVec), n(a.width - at) {}
+};
+
+// Rows of tokens k0 .. k0 + 7 of a chunk; rows outside documents are zero.
+template <typename T>
+__device__ __forceinline__ void load_batch(const ScanArgs& a, const void* p, int64_t stride, const Places& pl, int64_t p0,
+                                           int k0, const Channels& c, float (&v)[kScanBatch][4]) {
+#pragma unroll
+  for (int k = 0; k < kScanBatch; ++k)
+    load4(static_cast<const T*>(p) + token_at(a, p0 + k0 + k) * stride + c.at, (pl.inside >> (k0 + k)) & 1 ? c.n : 0, v[k]);
+}
+template <typename T>
+__device__ __forceinline__ void put_row(T* p, const Channels& c, const float (&v)[4]) {
+  if (c.n > 0) put4(p + c.at, c.n, v);
+}
+
+// ---- the maps of chunks and parts --------------------------------------------------------------------
+// BACK: of l, whose walk starts at a chunk's last token.
+
+template <typename T, bool BACK>
+__global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
+  __shared__ float2 maps[kScanWaves][kScanGroup];
+  const Channels c(a);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  // the running map of the part, of one channel a thread (the first four wavefronts)
+  double e_run = 0.0, p_run = 1.0;
+  const int own = blockIdx.x * kScanGroup + threadIdx.x;
+  for (int block = 0; block < a.blocks; ++block) {
+    const int n0 = (blockIdx.y * a.blocks + block) * kScanWaves;  // in walking order
+    if (n0 >= a.chunks) break;
+    const int n = n0 + wave;
+    float e[4] = {};
+    Factor f[4];
+    if (n < a.chunks) {
+      const int64_t p0 = static_cast<int64_t>(BACK ? a.chunks - 1 - n : n) * kScanChunk;
+      const Places pl(a, p0);
+#pragma unroll
+      for (int b = 0; b < kScanChunk / kScanBatch; ++b) {
+        const int k0 = (BACK ? kScanChunk / kScanBatch - 1 - b : b) * kScanBatch;
+        float vf[kScanBatch][4], vx[kScanBatch][4], vo[kScanBatch][4];
+        load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
+        if constexpr (BACK) {
+          load_batch<T>(a, a.d_y, a.width, pl, p0, k0, c, vx);
+          if (a.o) load_batch<T>(a, a.o, a.o_stride, pl, p0, k0, c, vo);
+        } else {
+          load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
+        }
+#pragma unroll
+        for (int i = 0; i < kScanBatch; ++i) {
+          const int k = BACK ? k0 + kScanBatch - 1 - i : k0 + i, r = k - k0;
+          if (!((pl.inside >> k) & 1)) continue;
+          if (((BACK ? pl.last : pl.first) >> k) & 1) {
+            const float* from = BACK ? a.d_state : a.initial;
+            load4(from + static_cast<int64_t>(pl.doc_of(k)) * a.width + c.at, from ? c.n : 0, e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j].drop();
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Sigmoid s(vf[r][j]);
+            if constexpr (BACK) e[j] = s.times(e[j] + (a.o ? vx[r][j] * (vo[r][j] * Sigmoid(vo[r][j]).value()) : vx[r][j]));
+            else e[j] = s.step(e[j], vx[r][j]);
+            f[j].by(s);
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) maps[wave][(threadIdx.x % kWave) * kScanVec + j] = make_float2(e[j], packed(f[j].p, f[j].q));
+    __syncthreads();
+    if (threadIdx.x < kScanGroup && own < a.width) {
+      for (int w = 0; w < kScanWaves && n0 + w < a.chunks; ++w) {
+        a.prefix[static_cast<int64_t>(n0 + w) * a.width + own] = make_float2(static_cast<float>(e_run), packed(p_run));
+        const float2 m = maps[w][threadIdx.x];
+        const double p = factor_of(m.y);
+        e_run = mapped(m.x, p, e_run);
+        p_run = p == 0.0 ? 0.0 : p_run * p;
+      }
+    }
+  }
+  if (a.parts > 1 && threadIdx.x < kScanGroup && own < a.width)
+    a.part[static_cast<int64_t>(blockIdx.y) * a.width + own] = make_double2(e_run, p_run);
+}
+
+// The map of all parts before `part`, of zero: the state that a part starts with. A wavefront joins an eighth of them;
+// the result is in LDS for the workgroup's channels.
+struct PartState {
+  double2 maps[kScanWaves][kScanGroup];
+  double state[kScanGroup];
+};
+__device__ __forceinline__ void join_parts(const ScanArgs& a, int part, PartState& s) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int per = (part + kScanWaves - 1) / kScanWaves;
+  const int from = min(wave * per, part), to = min(from + per, part);
+#pragma unroll
+  for (int j = 0; j < kScanVec; ++j) {
+    const int ch = lane + j * kWave, at = blockIdx.x * kScanGroup + ch;
+    double e = 0.0, p = 1.0;
+    if (at < a.width) {
+#pragma unroll 4
+      for (int i = from; i < to; ++i) {
+        const double2 m = a.part[static_cast<int64_t>(i) * a.width + at];
+        e = mapped(m.x, m.y, e);
+        p = m.y == 0.0 ? 0.0 : p * m.y;
+      }
+    }
+    s.maps[wave][ch] = make_double2(e, p);
+  }
+  __syncthreads();
+  if (threadIdx.x < kScanGroup) {
+    double h = 0.0;
+    for (int w = 0; w < kScanWaves; ++w) h = mapped(s.maps[w][threadIdx.x].x, s.maps[w][threadIdx.x].y, h);
+    s.state[threadIdx.x] = h;
+  }
+  __syncthreads();
+}
+
+// The state that chunk n (in walking order) starts with.
+__device__ __forceinline__ void state_before(const ScanArgs& a, int n, const Channels& c, const PartState& s, float (&h)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= c.n) continue;
+    const float2 m = a.prefix[static_cast<int64_t>(n) * a.width + c.at + j];
+    const double from = a.parts > 1 ? s.state[(threadIdx.x % kWave) * kScanVec + j] : 0.0;
+    h[j] = static_cast<float>(mapped(m.x, factor_of(m.y), from));
+  }
+}
+
+// Documents without tokens: their state goes through as it is, and so does its gradient.
+__device__ __forceinline__ void pass_empty(const ScanArgs& a, const Channels& c, const float* from, float* to) {
+  if (to == nullptr) return;
+  const int waves = blockDim.x / kWave;
+  for (int d = blockIdx.y * waves + threadIdx.x / kWave; d < a.docs; d += gridDim.y * waves) {
+    if (scan_edge(a, d) < scan_edge(a, d + 1)) continue;
+    float v[4];
+    const int64_t at = static_cast<int64_t>(doc_at(a, d)) * a.width;
+    load4(from + at + c.at, from ? c.n : 0, v);
+    put_row(to + at, c, v);
+  }
+}
+
+// ---- the walk ----------------------------------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void scan_apply_kernel(ScanArgs a) {
+  __shared__ PartState join;
+  const Channels c(a);
+  // the last part first: what the sums' kernel read last is still in the cache
+  const int part = gridDim.y - 1 - blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  pass_empty(a, c, a.initial, a.state);
+  if (a.parts > 1) join_parts(a, part, join);
+  float h[4] = {};
+  const int step = a.serial ? 1 : kScanWaves;
+  const int end = min((part + 1) * a.blocks * step, a.chunks);
+  for (int n = part * a.blocks * step + wave; n < end; n += step) {
+    const int64_t p0 = static_cast<int64_t>(n) * kScanChunk;
+    if (!a.serial) state_before(a, n, c, join, h);
+    if (a.carry) put_row(a.carry + static_cast<int64_t>(n) * a.width, c, h);
+    const Places pl(a, p0);
+#pragma unroll
+    for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
+      if (p0 + k0 >= a.tokens) break;
+      float vf[kScanBatch][4], vx[kScanBatch][4], vo[kScanBatch][4], first[kScanBatch][4];
+      load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
+      load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
+      if (a.o) load_batch<T>(a, a.o, a.o_stride, pl, p0, k0, c, vo);
+      if ((pl.first >> k0) & ((1u << kScanBatch) - 1)) {
+#pragma unroll
+        for (int k = 0; k < kScanBatch; ++k)
+          if ((pl.first >> (k0 + k)) & 1)
+            load4(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0, first[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kScanBatch; ++k) {
+        const int64_t p = p0 + k0 + k;
+        if (p >= a.tokens) break;
+        float y[4] = {};
+        if ((pl.inside >> (k0 + k)) & 1) {
+          const bool fresh = (pl.first >> (k0 + k)) & 1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            h[j] = Sigmoid(vf[k][j]).step(fresh ? first[k][j] : h[j], vx[k][j]);
+            y[j] = a.o ? h[j] * (vo[k][j] * Sigmoid(vo[k][j]).value()) : h[j];
+          }
+          if (a.state && ((pl.last >> (k0 + k)) & 1)) put_row(a.state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width, c, h);
+        }
+        put_row(static_cast<T*>(a.y) + token_at(a, p) * a.width, c, y);
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
+  __shared__ PartState join;
+  const Channels c(a);
+  const int part = gridDim.y - 1 - blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  pass_empty(a, c, a.d_state, a.d_initial);
+  if (a.parts > 1) join_parts(a, part, join);
+  float l[4] = {};  // a l of the token after
+  const int step = a.serial ? 1 : kScanWaves;
+  const int end = min((part + 1) * a.blocks * step, a.chunks);
+  for (int n = part * a.blocks * step + wave; n < end; n += step) {
+    const int chunk = a.chunks - 1 - n;
+    const int64_t p0 = static_cast<int64_t>(chunk) * kScanChunk;
+    if (!a.serial) state_before(a, n, c, join, l);
+    const Places pl(a, p0);
+    // the states before each token
+    float before[kScanChunk][4], h[4];
+    load4(a.carry + static_cast<int64_t>(chunk) * a.width + c.at, c.n, h);
+#pragma unroll
+    for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
+      float vf[kScanBatch][4], vx[kScanBatch][4];
+      load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
+      load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
+#pragma unroll
+      for (int k = 0; k < kScanBatch; ++k) {
+        if ((pl.first >> (k0 + k)) & 1)
+          load4(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0, h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          before[k0 + k][j] = h[j];
+          h[j] = Sigmoid(vf[k][j]).step(h[j], vx[k][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int k0 = kScanChunk - kScanBatch; k0 >= 0; k0 -= kScanBatch) {
+      float vf[kScanBatch][4], vx[kScanBatch][4], vo[kScanBatch][4], vd[kScanBatch][4];
+      load_batch<T>(a, a.d_y, a.width, pl, p0, k0, c, vd);
+      if (a.o) load_batch<T>(a, a.o, a.o_stride, pl, p0, k0, c, vo);
+      load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
+      load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
+#pragma unroll
+      for (int k = kScanBatch - 1; k >= 0; --k) {
+        const int64_t p = p0 + k0 + k;
+        if (p >= a.tokens) continue;
+        float dx[4] = {}, df[4] = {}, dg[4] = {};
+        if ((pl.inside >> (k0 + k)) & 1) {
+          if ((pl.last >> (k0 + k)) & 1)
+            load4(a.d_state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.d_state ? c.n : 0, l);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Sigmoid s(vf[k][j]);
+            const float was = before[k0 + k][j];
+            float d = vd[k][j];
+            if (a.o) {
+              const Sigmoid g(vo[k][j]);
+              const float open = vo[k][j] * g.value();
+              dg[j] = d * s.step(was, vx[k][j]) * fmaf(vo[k][j], g.large * g.small, g.value());
+              d *= open;
+            }
+            const float whole = d + l[j];
+            dx[j] = whole * s.rest();
+            df[j] = whole * (was - vx[k][j]) * (s.large * s.small);
+            l[j] = s.times(whole);
+          }
+          if (a.d_initial && ((pl.first >> (k0 + k)) & 1))
+            put_row(a.d_initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width, c, l);
+        }
+        const int64_t at = token_at(a, p) * a.width;
+        if (a.d_x) put_row(static_cast<T*>(a.d_x) + at, c, dx);
+        if (a.d_f) put_row(static_cast<T*>(a.d_f) + at, c, df);
+        if (a.d_o) put_row(static_cast<T*>(a.d_o) + at, c, dg);
+      }
+    }
+  }
+}
+
+// Up to so many tokens one wavefront a channel group walks them all, in one launch.
+constexpr int kScanSerial = 32;
+
+struct ScanPlan {
+  int chunks, parts, blocks, serial;
+  size_t prefix, part;  // bytes
+};
+static ScanPlan scan_plan(int64_t tokens, int width) {
+  ScanPlan s = {};
+  s.chunks = static_cast<int>((tokens + kScanChunk - 1) / kScanChunk);
+  s.serial = tokens <= kScanSerial;
+  if (s.serial) {
+    s.parts = 1;
+    s.blocks = s.chunks;
+    return s;
+  }
+  const int all = (s.chunks + kScanWaves - 1) / kScanWaves;
+  s.blocks = (all + kScanParts - 1) / kScanParts;
+  s.parts = (all + s.blocks - 1) / s.blocks;
+  s.prefix = (static_cast<size_t>(s.chunks) * width * sizeof(float2) + 15) / 16 * 16;
+  s.part = s.parts > 1 ? static_cast<size_t>(s.parts) * width * sizeof(double2) : 0;
+  return s;
+}
+
+static int check_scan(const gs_gated_scan* p, void* workspace, size_t workspace_bytes, ScanArgs* a) {
+  GS_REQUIRE(p, GS_ERR_ARG, "gated scan: args is NULL");
+  GS_REQUIRE(row_type(p->dtype), GS_ERR_ARG, "gated scan: dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(p->tokens >= 0 && p->tokens < (int64_t(1) << 31), GS_ERR_ARG, "gated scan: invalid token count");
+  GS_REQUIRE(p->width >= 1 && p->width <= GS_SCAN_MAX_WIDTH, GS_ERR_ARG, "gated scan: width %d: 1 to %d are provided",
+             p->width, GS_SCAN_MAX_WIDTH);
+  GS_REQUIRE(p->docs >= 1 && p->docs < (1 << 30) && (p->offsets || p->docs == 1), GS_ERR_ARG,
+             "gated scan: at least one document, and offsets for more than one");
+  GS_REQUIRE(p->tokens == 0 || (p->x && p->forget), GS_ERR_ARG, "gated scan: null pointer");
+  const size_t es = row_type_bytes(p->dtype);
+  GS_REQUIRE(aligned(p->x, es) && aligned(p->forget, es) && aligned(p->gate, es) && aligned(p->y, es) &&
+                 aligned(p->initial, 4) && aligned(p->state, 4) && aligned(p->carry, 4) && aligned(p->offsets, 4) &&
+                 aligned(workspace, 16), GS_ERR_ALIGN, "gated scan: misaligned tensor or workspace");
+  const ScanPlan s = scan_plan(p->tokens, p->width);
+  GS_REQUIRE(workspace_bytes >= s.prefix + s.part && (workspace || s.prefix == 0), GS_ERR_WORKSPACE,
+             "gated scan: workspace too small");
+  *a = {};
+  a->x = p->x;
+  a->f = p->forget;
+  a->o = p->gate;
+  a->initial = p->initial;
+  a->y = p->y;
+  a->state = p->state;
+  a->carry = p->carry;
+  a->offsets = p->offsets;
+  a->tokens = p->tokens;
+  a->x_stride = p->x_stride;
+  a->f_stride = p->forget_stride;
+  a->o_stride = p->gate_stride;
+  a->docs = p->docs;
+  a->width = p->width;
+  a->reverse = p->reverse != 0;
+  a->chunks = s.chunks;
+  a->parts = s.parts;
+  a->blocks = s.blocks;
+  a->serial = s.serial;
+  a->prefix = static_cast<float2*>(workspace);
+  a->part = reinterpret_cast<double2*>(static_cast<char*>(workspace) + s.prefix);
+  return GS_OK;
+}
+
+template <typename T, bool BACK>
+static int run_scan(const ScanArgs& a, hipStream_t st) {
+  const dim3 grid((a.width + kScanGroup - 1) / kScanGroup, a.parts), block(a.serial ? kWave : kScanThreads);
+  if (!a.serial) {
+    hipLaunchKernelGGL((scan_sums_kernel<T, BACK>), grid, block, 0, st, a);
+    if (const int rc = check_launch("gated scan (sums)")) return rc;
+  }
+  if constexpr (BACK) hipLaunchKernelGGL(scan_bwd_kernel<T>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(scan_apply_kernel<T>, grid, block, 0, st, a);
+  return check_launch("gated scan");
+}
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" int64_t gs_gated_scan_chunks(int64_t tokens) { return tokens <= 0 ? 0 : (tokens + kScanChunk - 1) / kScanChunk; }
+
+extern "C" size_t gs_gated_scan_workspace_size(int64_t tokens, int width) {
+  clear_error();
+  if (tokens <= 0 || width <= 0) return 0;
+  const ScanPlan s = scan_plan(tokens, width);
+  return s.prefix + s.part;
+}
+
+extern "C" int gs_gated_scan_fwd(const gs_gated_scan* p, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  ScanArgs a;
+  if (const int rc = check_scan(p, workspace, workspace_bytes, &a)) return rc;
+  GS_REQUIRE(a.tokens == 0 || a.y, GS_ERR_ARG, "gated scan: null pointer");
+  if (a.tokens == 0 && a.state == nullptr) return GS_OK;
+  return p->dtype == GS_BFLOAT16 ? run_scan<__bf16, false>(a, as_stream(stream)) : run_scan<float, false>(a, as_stream(stream));
+}
+
+extern "C" int gs_gated_scan_bwd(const gs_gated_scan* p, const void* d_y, const float* d_state, void* d_x, void* d_forget,
+                                 void* d_gate, float* d_initial, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  ScanArgs a;
+  if (const int rc = check_scan(p, workspace, workspace_bytes, &a)) return rc;
+  GS_REQUIRE(a.tokens == 0 || (a.carry && d_y), GS_ERR_ARG, "gated scan: the backward pass needs the carried states and d_y");
+  GS_REQUIRE(a.o || !d_gate, GS_ERR_ARG, "gated scan: the gradient of a gate that is not there");
+  const size_t es = row_type_bytes(p->dtype);
+  GS_REQUIRE(aligned(d_y, es) && aligned(d_x, es) && aligned(d_forget, es) && aligned(d_gate, es) && aligned(d_state, 4) &&
+                 aligned(d_initial, 4), GS_ERR_ALIGN, "gated scan: misaligned gradient");
+  a.d_y = d_y;
+  a.d_state = d_state;
+  a.d_x = d_x;
+  a.d_f = d_forget;
+  a.d_o = d_gate;
+  a.d_initial = d_initial;
+  if (a.tokens == 0 && d_initial == nullptr) return GS_OK;
+  return p->dtype == GS_BFLOAT16 ? run_scan<__bf16, true>(a, as_stream(stream)) : run_scan<float, true>(a, as_stream(stream));
+}

@@ -662,6 +662,87 @@ size_t gs_attention_bwd_workspace_size(const gs_attention* args);
 int gs_attention_bwd(const gs_attention* args, const void* d_out, void* d_q, void* d_k, void* d_v,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Norms before and after a block, fused with what lies between them. x [rows, width] is the residual stream, y
+ * [rows, width] the block's output (NULL: none, then n is the norm of x alone and h is not written):
+ *   b = y, or with post_weight  post_weight y^ + post_bias
+ *   h = x + scale gate k b,     n = weight h^ + bias
+ * v^ = v / sqrt(mean of v^2 + eps), or with `layer` (v - mean) / sqrt(variance + eps), over a row; weight, bias,
+ * post_bias and gate may be NULL; gate is [width], or with gate_rows [rows, width]. k is the dropout's factors (see
+ * gs_dropout; dropout 0: one). x and h are of x_dtype, y and n of y_dtype (float32 streams take either,
+ * bfloat16 streams bfloat16), the weights and biases of weight_dtype. x, y and gate are read through row
+ * strides (elements); the rest is contiguous, at an element's alignment. Sums are float32: the mean of a row's squares
+ * has to be finite there. stats (float32 [rows, 4], 16-byte aligned; NULL if no backward pass follows): the
+ * rows' mean and 1 / deviation of h and of y.
+ *
+ * gs_residual_norm_bwd takes the same arguments (h and n are not used), d_h of x_dtype and d_n of y_dtype (either may be
+ * NULL: zero) and writes those of d_x, d_y, d_weight, d_bias, d_post_weight, d_post_bias, d_gate that are not
+ * NULL, each in its tensor's type and shape. Sums over rows are float32 in a fixed order: the same inputs
+ * give the same bits.
+ * ------------------------------------------------------------------------------------- */
+#define GS_NORM_MAX_WIDTH 16384
+typedef struct gs_residual_norm {
+  const void *x, *y, *weight, *bias, *post_weight, *post_bias, *gate;
+  void *h, *n;
+  float* stats;
+  const int64_t* seed_at; /* device; NULL: seed */
+  uint64_t seed, draw;
+  int64_t rows, x_stride, y_stride, gate_stride;
+  double dropout;
+  float eps, scale;
+  int32_t width, x_dtype, y_dtype, weight_dtype, gate_dtype, gate_rows, layer;
+} gs_residual_norm;
+int gs_residual_norm_fwd(const gs_residual_norm* args, void* stream);
+size_t gs_residual_norm_bwd_workspace_size(const gs_residual_norm* args);
+int gs_residual_norm_bwd(const gs_residual_norm* args, const void* d_h, const void* d_n, void* d_x, void* d_y,
+                         void* d_weight, void* d_bias, void* d_post_weight, void* d_post_bias, void* d_gate,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Dropout whose mask is a function of the seed: out = k x, k = 0 or 2^16 / (2^16 - t), t = p 2^16 rounded to the
+ * nearest integer (at most 2^16 - 1). Element (row, column) is dropped where 16 bits of Philox4x32-10 are below t: key = the
+ * seed, counter = (column / 8, row, draw mod 2^32, draw / 2^32), of word column % 8 / 2 the low half for even
+ * columns, the high half for odd ones. The gradient is the same call on the output's gradient. seed_at (device
+ * int64, may be NULL) takes the place of seed, so that a captured graph can be replayed with other seeds. x
+ * [rows, width] is read through its row stride (elements), out is contiguous and may be x where x is. What is
+ * dropped is 0 whatever x holds.
+ * ------------------------------------------------------------------------------------- */
+int gs_dropout(const void* x, void* out, int64_t rows, int64_t stride, int width, int dtype, double p,
+               const int64_t* seed_at, uint64_t seed, uint64_t draw, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * A gated linear recurrence over packed documents: with a = sigmoid(forget),
+ *   h_t = a_t h_(t-1) + (1 - a_t) x_t,   y_t = h_t, or with a gate h_t silu(gate_t),
+ * from a document's first token (its last, with reverse), where h_(t-1) is initial [docs, width] (float32; NULL:
+ * zero), to its last, where h is written to state [docs, width] (float32; may be NULL). x, forget, gate and y
+ * [tokens, width] are of dtype, the inputs read through row strides (elements) at an element's alignment, y contiguous.
+ * Document d owns the tokens offsets[d] .. offsets[d + 1] (device int32, non-decreasing, docs + 1 of them; NULL for one
+ * document of all tokens; values outside the tensors are cut to them). An empty document's state is its initial
+ * one. Tokens outside the documents give y = 0. h is float32, and the states of long sequences are joined in
+ * float64; differences x - h have to be finite in float32. Documents do not reach each other, whatever they hold.
+ * carry (float32 [gs_gated_scan_chunks(tokens), width]; NULL if no backward pass follows) is written by the
+ * forward and read by the backward.
+ *
+ * gs_gated_scan_bwd takes the same arguments (y and state are not used), d_y of dtype and d_state (float32; NULL: zero), and
+ * writes those of d_x, d_forget, d_gate (contiguous, dtype) and d_initial (float32) that are not NULL, zero for tokens
+ * outside the documents. No atomics: the same inputs give the same bits.
+ * ------------------------------------------------------------------------------------- */
+#define GS_SCAN_MAX_WIDTH (1 << 20)
+typedef struct gs_gated_scan {
+  const void *x, *forget, *gate;
+  const float* initial;
+  void* y;
+  float *state, *carry;
+  const int32_t* offsets;
+  int64_t tokens, x_stride, forget_stride, gate_stride;
+  int32_t docs, width, dtype, reverse;
+} gs_gated_scan;
+int64_t gs_gated_scan_chunks(int64_t tokens);
+size_t gs_gated_scan_workspace_size(int64_t tokens, int width);
+int gs_gated_scan_fwd(const gs_gated_scan* args, void* workspace, size_t workspace_bytes, void* stream);
+int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d_state, void* d_x, void* d_forget,
+                      void* d_gate, float* d_initial, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
