@@ -10,6 +10,7 @@ from .adam import FusedAdam, adam_step, adam_step_sparse
 from .attention import attention
 from .clip import clip_grad_norm, grad_norm
 from .dropout import dropout
+from .linear import linear
 from .loss import fused_ssim, l1_ssim_loss
 from .norm import norm, residual_norm
 from .raster3d import (Camera, backward_pass, densification_stats, forward_pass, pruning_scores, rasterize,
@@ -19,4 +20,4 @@ from .scan import gated_scan
 
 __all__ = ["Camera", "rasterize", "rasterize_inference", "pruning_scores", "forward_pass", "backward_pass", "densification_stats", "FusedAdam", "adam_step", "adam_step_sparse",
            "l1_ssim_loss", "fused_ssim", "attention", "rotary_axes", "grad_norm", "clip_grad_norm",
-           "norm", "residual_norm", "dropout", "gated_scan"]
+           "norm", "residual_norm", "dropout", "gated_scan", "linear"]

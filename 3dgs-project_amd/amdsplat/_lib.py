@@ -178,6 +178,28 @@ class GsGatedScan(C.Structure):
     ]
 
 
+class GsLinear(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("weight", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("out", C.c_void_p),
+        ("z", C.c_void_p),
+        ("rows", C.c_int64),
+        ("x_stride", C.c_int64),
+        ("weight_stride", C.c_int64),
+        ("residual_stride", C.c_int64),
+        ("inputs", C.c_int32),
+        ("outputs", C.c_int32),
+        ("dtype", C.c_int32),
+        ("out_dtype", C.c_int32),
+        ("z_dtype", C.c_int32),
+        ("bias_dtype", C.c_int32),
+        ("activation", C.c_int32),
+    ]
+
+
 class AmdSplatError(RuntimeError):
     pass
 
@@ -242,6 +264,10 @@ _SIGS = {
     "gs_gated_scan_workspace_size": (_sz, [_i64, _i32]),
     "gs_gated_scan_fwd": (_i32, [_vp, _vp, _sz, _vp]),
     "gs_gated_scan_bwd": (_i32, [_vp] * 8 + [_sz, _vp]),
+    "gs_linear_fwd_workspace_size": (_sz, [_vp]),
+    "gs_linear_fwd": (_i32, [_vp, _vp, _sz, _vp]),
+    "gs_linear_bwd_workspace_size": (_sz, [_vp]),
+    "gs_linear_bwd": (_i32, [_vp] * 6 + [_sz, _vp]),
     "gs_densification_stats": (_i32, [_vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp]),
     "gs_l1_ssim_workspace_size": (_sz, [_i32, _i32, _i32]),
     "gs_l1_ssim_fwd": (_i32, [_vp, _vp, _i32, _i32, _i32, C.c_float, _vp, _vp, _vp, _sz, _vp]),

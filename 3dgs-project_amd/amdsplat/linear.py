@@ -1,0 +1,123 @@
+"""Projections with their epilogue on the GPU (gs_linear_fwd / gs_linear_bwd).
+
+`linear(x, weight, bias, activation=..., residual=...)` is act(x W^T + b) + residual in one pass over the result: the
+halves of a transformer block's MLP and the projections beside attention. bfloat16 products may be added to a
+float32 residual stream without being rounded first.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._grad import tracked
+from ._lib import call, ptr
+
+MAX_WIDTH = 1 << 19  # GS_LINEAR_MAX_WIDTH
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # GS_ACT_*
+_DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8)}
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """t itself if the kernels can read it through its row stride, otherwise a contiguous copy."""
+    per = _DTYPES[t.dtype][1]
+    s = t.stride(0)
+    ok = t.stride(1) == 1 and 0 <= s < 1 << 20 and s % per == 0 and t.data_ptr() % 16 == 0
+    return t if ok or t.shape[0] == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows(t):
+    return t if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= 0) else t.contiguous()
+
+
+def _args(x, weight, bias, residual, out, z, out_dtype, activation) -> _lib.GsLinear:
+    rows = x.shape[0]
+    return _lib.GsLinear(x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                         None if residual is None else residual.data_ptr(), ptr(out), ptr(z), rows,
+                         x.stride(0) if rows else 0, weight.stride(0), 0 if residual is None else residual.stride(0),
+                         x.shape[1], weight.shape[0], _DTYPES[x.dtype][0], _DTYPES[out_dtype][0],
+                         0 if z is None else _DTYPES[z.dtype][0], 0 if bias is None else _DTYPES[bias.dtype][0], activation)
+
+
+def _workspace(name: str, a, device):
+    n = _lib.size_call(name, C.byref(a))
+    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
+
+
+def _forward(x, weight, bias, residual, activation, out_dtype, keep: bool):
+    out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype, device=x.device)
+    z = None
+    if keep and activation:  # float32 where a bias' gradient sums its slopes; the products round them anyway
+        z = torch.empty(out.shape, dtype=x.dtype if bias is None else torch.float32, device=x.device)
+    a = _args(x, weight, bias, residual, out, z, out_dtype, activation)
+    ws, n = _workspace("gs_linear_fwd_workspace_size", a, x.device)
+    call("gs_linear_fwd", C.byref(a), ptr(ws), n, _lib.stream_handle(x.device))
+    return out, z
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, out_dtype):
+        x, weight = _readable(x), _readable(weight)
+        out, z = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, z)
+        ctx.rule = (out_dtype, activation)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        x, weight, bias, z = ctx.saved_tensors
+        grads = [None, None, None]
+        if any(ctx.needs_input_grad[:3]):
+            d = d_out.contiguous()
+            if d.data_ptr() % 16:
+                d = d.clone()
+            grads = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if t is not None and need else None
+                     for t, need in zip((x, weight, bias), ctx.needs_input_grad)]
+            a = _args(x, weight, bias, None, None, z, *ctx.rule)
+            ws, n = _workspace("gs_linear_bwd_workspace_size", a, x.device)
+            call("gs_linear_bwd", C.byref(a), ptr(d), *map(ptr, grads), ptr(ws), n, _lib.stream_handle(x.device))
+        return (*grads, d_out if ctx.needs_input_grad[3] else None, None, None)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual, [T, N], of x [T, K] and weight [N, K] (one dtype, bfloat16 or float32), bias [N]
+    (either) and residual [T, N] (x's dtype, or float32); differentiable in all of them. activation: "none", "relu",
+    "gelu" (z Phi(z)), "gelu_tanh" or "silu". The result has the residual's dtype, without one x's. Products and
+    epilogue are float32 and rounded once; in the backward pass the output's gradient times act' is rounded to
+    x's dtype as an operand of the products (not in the bias' gradient), and act' is taken at z = x weight^T + bias, which the forward
+    keeps: in float32, or without a bias in x's dtype. No forward-mode derivative.
+
+    x and weight are read through their row strides where these, the addresses and K are multiples of 16 bytes;
+    otherwise they are copied first (for K: padded with zeros, at every call)."""
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"x must be [tokens, inputs] and weight [outputs, inputs], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dtype not in _DTYPES or weight.dtype != x.dtype:
+        raise ValueError(f"x and weight must share a dtype, float32 or bfloat16: got {x.dtype}, {weight.dtype}")
+    device = x.device
+    if not x.is_cuda or weight.device != device:
+        raise ValueError("x and weight must be on one GPU")
+    n = weight.shape[0]
+    if not (1 <= x.shape[1] <= MAX_WIDTH and 1 <= n <= MAX_WIDTH):
+        raise ValueError(f"{x.shape[1]} inputs and {n} outputs: 1 to {MAX_WIDTH} are provided")
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype not in _DTYPES or bias.device != device:
+            raise ValueError(f"bias must be [{n}], float32 or bfloat16, on x's device")
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+    out_dtype = x.dtype
+    if residual is not None:
+        if residual.shape != (x.shape[0], n) or residual.device != device or residual.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"residual must be [{x.shape[0]}, {n}], float32 or x's dtype, on x's device")
+        out_dtype, residual = residual.dtype, _rows(residual)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    per = _DTYPES[x.dtype][1]
+    if x.shape[1] % per:
+        x, weight = (torch.nn.functional.pad(t, (0, -t.shape[1] % per)) for t in (x, weight))
+    rest = (bias, residual, ACTIVATIONS[activation], out_dtype)
+    if tracked(x, weight, bias, residual):
+        return _Linear.apply(x, weight, *rest)
+    return _forward(_readable(x), _readable(weight), *rest, False)[0]

@@ -21,7 +21,7 @@ CSRC = HERE / "csrc"
 OUT = HERE / "amdsplat" / "libamdsplat.so"
 SOURCES = ["capi.hip", "preprocess.hip", "binning.hip", "blend.hip", "view.hip", "raster2d.hip", "adam.hip", "loss.hip",
            "attention.hip", "rotary.hip", "clip.hip", "norm.hip",
-           "scan.hip", "probe.hip"]
+           "scan.hip", "linear.hip", "probe.hip"]
 
 HIPCC_FLAGS = [
     "-O3",

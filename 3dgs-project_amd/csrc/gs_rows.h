@@ -58,6 +58,43 @@ __device__ __forceinline__ void store8(void* p, bool bf16, int64_t at, int n, co
   else store8(static_cast<float*>(p) + at, n, v);
 }
 
+// Sums of parts, column by column in a fixed order: out[k][c] = sum over p of parts[p][k][c]. 64 columns of one sum a
+// workgroup, its wavefronts take the parts in turn.
+constexpr int kSumThreads = 1024;
+struct ColumnSums {
+  const float* parts;
+  int n, sums, width;
+  void* out[5];
+  bool bf16[5];
+};
+static __global__ __launch_bounds__(kSumThreads) void column_sums_kernel(ColumnSums a) {
+  __shared__ float part[kSumThreads];
+  const int k = blockIdx.y, c = blockIdx.x * kWave + threadIdx.x % kWave, w = threadIdx.x / kWave;
+  constexpr int kStep = kSumThreads / kWave;
+  float s[4] = {};
+  if (c < a.width) {
+    const auto at = [&](int i) { return a.parts[(static_cast<int64_t>(i) * a.sums + k) * a.width + c]; };
+    int p = w;
+    for (; p + 3 * kStep < a.n; p += 4 * kStep) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += at(p + i * kStep);
+    }
+    for (; p < a.n; p += kStep) s[0] += at(p);
+  }
+  part[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (w == 0 && c < a.width) {
+    float t = 0.0f;
+    for (int i = 0; i < kStep; ++i) t += part[i * kWave + threadIdx.x];
+    if (a.bf16[k]) static_cast<__bf16*>(a.out[k])[c] = static_cast<__bf16>(t);
+    else static_cast<float*>(a.out[k])[c] = t;
+  }
+}
+inline int column_sums(const ColumnSums& a, const char* what, hipStream_t st) {
+  hipLaunchKernelGGL(column_sums_kernel, dim3((a.width + kWave - 1) / kWave, a.sums), dim3(kSumThreads), 0, st, a);
+  return check_launch(what);
+}
+
 inline bool row_type(int dtype) { return dtype == GS_FLOAT32 || dtype == GS_BFLOAT16; }
 inline size_t row_type_bytes(int dtype) { return dtype == GS_BFLOAT16 ? 2 : 4; }
 

@@ -1,0 +1,643 @@
+// Projections with their epilogue, out = act(x W^T + b) + residual, and their gradients
+//
+//   dz = dout act'(z);   dx = dz W;   dW = dz^T x;   db = sum over rows of dz
+//
+// on the matrix cores. One tile kernel makes all three products: each of its operands is a matrix whose rows or whose
+// columns run along the contraction. Both sides of a tile are copied to LDS straight from memory (gs_attention.h), 128
+// bytes of contraction at a time, one stage ahead of the products; operands whose rows run along the
+// contraction are read as they lie, the others through the LDS unit's transpose (bfloat16) or word by word (float32).
+// Products accumulate in float32 (v_mfma_f32_32x32x16_bf16, or v_mfma_f32_32x32x2_f32 in float32). The result goes
+// through LDS once, so that bias, activation, residual and stores see eight neighbouring columns a lane, and is
+// rounded once. Tiles that would leave CUs idle are cut along the contraction into float32 parts, which a second
+// launch sums in order and finishes.
+//
+// Few rows are bound by reading W once: linear_few_kernel streams it past the matrix unit without LDS.
+#include <algorithm>
+
+#include "gs_attention.h"
+#include "gs_rows.h"
+
+namespace gs {
+
+enum { kActNone = GS_ACT_NONE, kActRelu = GS_ACT_RELU, kActGelu = GS_ACT_GELU, kActGeluTanh = GS_ACT_GELU_TANH,
+       kActSilu = GS_ACT_SILU, kActs };
+
+// ---- activations -------------------------------------------------------------------------------------
+
+// exp(v), v <= 0: in bfloat16 by the hardware's exponential, off by 2^-23 |v| of itself.
+template <typename T>
+__device__ __forceinline__ float exp_down(float v) {
+  if constexpr (sizeof(T) == 2) return exp2_hw(v * kLog2e);
+  return expf(v);
+}
+template <typename T>
+__device__ __forceinline__ float recip(float v) {
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(v);
+  return 1.0f / v;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float v) {
+  const float e = exp_down<T>(-fabsf(v));
+  const float r = recip<T>(1.0f + e);
+  return v >= 0.0f ? r : e * r;
+}
+// The normal distribution function, and exp(-z^2 / 2). float32: the library's erfc. bfloat16: Phi(-u) = exp(-u^2 / 2)
+// t P(t), t = 1 / (1 + 0.27 u), P of degree six fitted to erfcx(u / sqrt 2) / 2 over t by reweighted least squares:
+// off by 1.6e-6 of itself at most, so the tail is as exact as the middle (8203 x 4096 outputs: 9 us less than erfc).
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float z, float& bell) {
+  bell = exp_down<T>(-0.5f * z * z);
+  if constexpr (sizeof(T) != 2) {
+    return 0.5f * erfcf(z * -0.70710678118654752f);
+  } else {
+    const float u = fabsf(z), t = recip<T>(fmaf(0.27f, u, 1.0f));
+    float p = -0.06105639412999153f;
+    p = fmaf(p, t, 0.15936046838760376f);
+    p = fmaf(p, t, -0.025581030175089836f);
+    p = fmaf(p, t, 0.11871293932199478f);
+    p = fmaf(p, t, 0.09232588112354279f);
+    p = fmaf(p, t, 0.10856088250875473f);
+    p = fmaf(p, t, 0.10767664760351181f);
+    const float q = bell * (p * t);
+    return z >= 0.0f ? 1.0f - q : q;
+  }
+}
+constexpr float kTanhOuter = 1.5957691216057308f, kTanhInner = 0.044715f;  // 2 sqrt(2 / pi)
+
+// Beyond 100 in size the exponentials are below float32's smallest number: values and slopes are taken there, so that
+// their products do not become infinity times zero.
+constexpr float kFar = 100.0f;
+
+template <typename T>
+__device__ __forceinline__ float act_value(int act, float z) {
+  float bell;
+  if (act >= kActGelu) z = z < -kFar ? -kFar : z;  // NaN stays
+  switch (act) {
+    case kActRelu: return z < 0.0f ? 0.0f : z;
+    case kActGelu: return z * normal_cdf<T>(z, bell);
+    case kActGeluTanh: return z * sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
+    case kActSilu: return z * sigmoid<T>(z);
+    default: return z;
+  }
+}
+template <typename T>
+__device__ __forceinline__ float act_slope(int act, float z) {
+  if (act >= kActGelu) z = z < -kFar ? -kFar : (z > kFar ? kFar : z);
+  switch (act) {
+    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+    case kActGelu: {
+      float bell;
+      const float p = normal_cdf<T>(z, bell);
+      return fmaf(z * 0.3989422804014327f, bell, p);
+    }
+    case kActGeluTanh: {
+      const float p = sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
+      return fmaf(z * p * (1.0f - p), kTanhOuter * fmaf(3.0f * kTanhInner * z, z, 1.0f), p);
+    }
+    case kActSilu: {
+      const float p = sigmoid<T>(z);
+      return fmaf(z * p, 1.0f - p, p);
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---- the tile kernel ---------------------------------------------------------------------------------
+
+// A product out[m][n] = sum over k of a(m, k) b(n, k) and its epilogue.
+struct GemmArgs {
+  const void *a, *b;
+  int64_t lda, ldb;  // strides in elements: of rows m, n, or where these are columns of rows k
+  int64_t m, k;
+  int n;
+  int act;
+  const void *bias, *residual;
+  int64_t residual_stride;
+  void *out, *z;     // [m][n], contiguous; z: before the activation (NULL: not wanted)
+  bool bias_bf16, residual_bf16, out_bf16, z_bf16;
+  int tiles_m, tiles_n, splits;
+  int64_t split_k;   // contraction of a part, a multiple of a stage's
+  float* part;       // [splits][m][n] where splits > 1
+};
+
+// Bias, activation, residual and store of columns col .. col + 7 of a row (the first n of them).
+template <typename T>
+__device__ __forceinline__ void finish8(const GemmArgs& g, int64_t row, int col, int n, float (&v)[8]) {
+  if (g.bias) {
+    float b[8];
+    load8(g.bias, g.bias_bf16, col, n, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += b[j];
+  }
+  if (g.z) store8(g.z, g.z_bf16, row * g.n + col, n, v);
+  if (g.act != kActNone) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act_value<T>(g.act, v[j]);
+  }
+  if (g.residual) {
+    float r[8];
+    load8(g.residual, g.residual_bf16, row * g.residual_stride + col, n, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+  }
+  store8(g.out, g.out_bf16, row * g.n + col, n, v);
+}
+
+template <typename T>
+constexpr int kStage = 128 / static_cast<int>(sizeof(T));  // contraction of a stage
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+// One side of a tile: ROWS rows (or columns) of an operand, a stage of them in LDS. ALONG: the operand's rows run
+// along the contraction.
+template <typename T, bool ALONG, int ROWS, int THREADS>
+struct Side {
+  static constexpr int kWidth = ALONG ? kStage<T> : (ROWS * static_cast<int>(sizeof(T)) < 256 ? ROWS : 256 / static_cast<int>(sizeof(T)));
+  static constexpr int kSubs = ALONG ? 1 : ROWS / kWidth;
+  static constexpr int kBytes = ROWS * 128;
+  using L = Tile<T, kWidth>;
+  using Copy = TileCopy<T, kWidth, ALONG ? ROWS : kStage<T>, THREADS>;
+  const T* base;
+  int64_t ld;
+  int rows;  // there are from the tile's first on
+  __device__ __forceinline__ Side(const void* p, int64_t ld_, int64_t row0, int64_t all)
+      : base(static_cast<const T*>(p) + row0 * (ALONG ? ld_ : 1)), ld(ld_),
+        rows(static_cast<int>(all - row0 < ROWS ? all - row0 : ROWS)) {}
+  // Contraction k0 .. of `left` more; what is past the operand's end is zero. Rows are there to a whole vector: where
+  // they run along the contraction its rest is zero in one operand at least, where columns are copied it
+  // ends in results that are not stored.
+  __device__ __forceinline__ void stage(char* lds, int64_t k0, int64_t left) const {
+    const int n = left < kStage<T> ? static_cast<int>(left) : kStage<T>;
+    if constexpr (ALONG) {
+      const int whole = (n + kVec<T> - 1) / kVec<T> * kVec<T>;
+      Copy(ld, whole)(lds, row_buffer(base + k0, ld, rows, whole));
+    } else {
+#pragma unroll
+      for (int s = 0; s < kSubs; ++s) {
+        const int cols = (rows + kVec<T> - 1) / kVec<T> * kVec<T> - s * kWidth;
+        const int dim = cols < 0 ? 0 : (cols < kWidth ? cols : kWidth);
+        Copy(ld, dim)(lds + s * kStage<T> * L::kRowBytes, row_buffer(base + k0 * ld + s * kWidth, ld, dim ? n : 0, dim));
+      }
+    }
+  }
+  // Rows row0 + l % 32, contraction slots of group c of sixteen: both sides list them in the same order.
+  static __device__ __forceinline__ Frag<T> frag(const char* lds, int row0, int c, int lane) {
+    if constexpr (ALONG && sizeof(T) == 2) {
+      return L::rows(lds, row0, c, lane);
+    } else if constexpr (ALONG) {
+      const int row = row0 + (lane & 31), h = lane >> 5;
+      const f32x4 a = *reinterpret_cast<const f32x4*>(lds + L::at(row, 4 * c + h));
+      const f32x4 b = *reinterpret_cast<const f32x4*>(lds + L::at(row, 4 * c + 2 + h));
+      return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+      lds += row0 / kWidth * (kStage<T> * L::kRowBytes);
+      row0 %= kWidth;
+      if constexpr (sizeof(T) == 4) {
+        return L::cols(lds, row0, 16 * c, lane);
+      } else {
+        typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+        const int i = lane & 15, col = row0 + (lane & 16) + 4 * (i & 3), r = 16 * c + 8 * (lane >> 5) + (i >> 2);
+        const int in = (col & 7) * 2;
+        const i16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + L::at(r, col >> 3) + in));
+        const i16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(lds + L::at(r + 4, col >> 3) + in));
+        using i16x8 = short __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(bf16x8, i16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+      }
+    }
+  }
+};
+
+// Tiles are taken in groups of eight rows of them, down a group's columns, and an XCD has a contiguous share of
+// that order: what its CUs work on together is a block of some eight by four tiles.
+constexpr int kTileGroup = 8;
+
+// BM x BN results by WM x WN wavefronts.
+template <typename T, int BM, int BN, int WM, int WN, bool A_ALONG, bool B_ALONG>
+__global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
+  constexpr int kThreads = WM * WN * kWave;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 results of a wavefront
+  constexpr int kStageBytes = (BM + BN) * 128;
+  constexpr int kRowFloats = TN * 32 + 4;  // of the epilogue's rows, padded against bank conflicts
+  constexpr int kOutBytes = WM * WN * 32 * kRowFloats * 4;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStageBytes > kOutBytes ? 2 * kStageBytes : kOutBytes];
+  using A = Side<T, A_ALONG, BM, kThreads>;
+  using B = Side<T, B_ALONG, BN, kThreads>;
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int at = xcd_tile(blockIdx.x, gridDim.x);
+  const int split = at / tiles, t = at - split * tiles;
+  const int group = t / (kTileGroup * g.tiles_n), first = group * kTileGroup;
+  const int high = min(kTileGroup, g.tiles_m - first), in = t - first * g.tiles_n;
+  const int64_t m0 = static_cast<int64_t>(first + in % high) * BM;
+  const int n0 = in / high * BN;
+  const int64_t k_begin = split * g.split_k, k_end = g.k - k_begin < g.split_k ? g.k : k_begin + g.split_k;
+  const A a(g.a, g.lda, m0, g.m);
+  const B b(g.b, g.ldb, n0, g.n);
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  f32x16 acc[TM][TN] = {};
+  char *now = lds, *next = lds + kStageBytes;
+  if (k_begin < k_end) {
+    a.stage(now, k_begin, k_end - k_begin);
+    b.stage(now + A::kBytes, k_begin, k_end - k_begin);
+  }
+  for (int64_t k0 = k_begin; k0 < k_end; k0 += kStage<T>) {
+    copies_done();
+    __syncthreads();  // everyone's copies are there, and everyone has left the other stage
+    if (k0 + kStage<T> < k_end) {
+      a.stage(next, k0 + kStage<T>, k_end - k0 - kStage<T>);
+      b.stage(next + A::kBytes, k0 + kStage<T>, k_end - k0 - kStage<T>);
+    }
+#pragma unroll
+    for (int c = 0; c < kStage<T> / 16; ++c) {
+      Frag<T> fa[TM], fb[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = A::frag(now, wm + 32 * i, c, lane);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = B::frag(now + A::kBytes, wn + 32 * j, c, lane);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) mma(acc[i][j], fb[j], fa[i]);
+    }
+    char* s = now;
+    now = next;
+    next = s;
+  }
+  __syncthreads();
+  // A lane holds row l % 32 and of every 32 columns 8 (r / 4) + 4 (l / 32) + r % 4: 32 rows at a time through the
+  // wavefront's own LDS, then eight neighbouring columns a lane.
+  constexpr int kLanes = TN * 4;  // of a row
+  float* own = reinterpret_cast<float*>(lds) + wave * 32 * kRowFloats;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4)
+        store4(own + (lane & 31) * kRowFloats + 32 * j + 2 * r + 4 * (lane >> 5), acc[i][j][r], acc[i][j][r + 1],
+               acc[i][j][r + 2], acc[i][j][r + 3]);
+    wave_sync();
+#pragma unroll
+    for (int r = 0; r < 32; r += kWave / kLanes) {
+      const int row = r + lane / kLanes, c = lane % kLanes * 8;
+      const int64_t m = m0 + wm + 32 * i + row;
+      const int col = n0 + wn + c, n = m < g.m ? g.n - col : 0;
+      if (n <= 0) continue;
+      float v[8];
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(own + row * kRowFloats + c);
+      const f32x4 hi = *reinterpret_cast<const f32x4*>(own + row * kRowFloats + c + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+      if (g.splits > 1) store8(g.part + (split * g.m + m) * g.n + col, n, v);
+      else finish8<T>(g, m, col, n, v);
+    }
+  }
+}
+
+// Sums the parts of the contraction in order and finishes.
+constexpr int kFinishThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kFinishThreads) void gemm_finish_kernel(GemmArgs g) {
+  const int vecs = (g.n + 7) / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kFinishThreads + threadIdx.x;
+  if (i >= g.m * vecs) return;
+  const int64_t row = i / vecs;
+  const int col = static_cast<int>(i - row * vecs) * 8, n = g.n - col;
+  float v[8];
+  load8(g.part + row * g.n + col, n, v);
+  for (int s = 1; s < g.splits; ++s) {
+    float p[8];
+    load8(g.part + (s * g.m + row) * g.n + col, n, p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += p[j];
+  }
+  finish8<T>(g, row, col, n, v);
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------
+
+// Sixteen columns a workgroup, all rows (16 MT of them): its wavefronts take the contraction in turn, straight from
+// memory into the matrix instruction's operands, and are joined in LDS.
+constexpr int kFewWaves = 8;
+template <typename T, int MT>
+__global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g) {
+  constexpr int kGroup = 64 / static_cast<int>(sizeof(T));  // contraction of one load: 4 x 16 bytes a row
+  __shared__ __attribute__((aligned(16))) float join[kFewWaves][MT * 16][16 + 4];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, row = lane % 16;
+  const int n0 = blockIdx.x * 16, k_lane = lane / 16 * kVec<T>;
+  const bool in_n = n0 + row < g.n;
+  const T* w = static_cast<const T*>(g.b) + (n0 + row) * g.ldb + k_lane;
+  const T* x = static_cast<const T*>(g.a) + row * g.lda + k_lane;
+  f32x4 acc[MT] = {};
+#pragma unroll 4
+  for (int64_t k = wave * kGroup; k < g.k; k += kFewWaves * kGroup) {
+    using Raw = uint32_t __attribute__((ext_vector_type(4)));
+    const bool in_k = k + k_lane < g.k;
+    const Raw zero = {0, 0, 0, 0};
+    const Raw fw = in_n && in_k ? *reinterpret_cast<const Raw*>(w + k) : zero;
+    Raw fx[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      fx[i] = 16 * i + row < g.m && in_k ? *reinterpret_cast<const Raw*>(x + 16 * i * g.lda + k) : zero;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fw), __builtin_bit_cast(bf16x8, fx[i]),
+                                                         acc[i], 0, 0, 0);
+      } else {
+        const f32x4 a = __builtin_bit_cast(f32x4, fw), b = __builtin_bit_cast(f32x4, fx[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc[i], 0, 0, 0);
+      }
+    }
+  }
+  // a lane holds row l % 16 and columns 4 (l / 16) .. + 3
+#pragma unroll
+  for (int i = 0; i < MT; ++i) store4(&join[wave][16 * i + row][lane / 16 * 4], acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+  __syncthreads();
+  for (int e = threadIdx.x; e < MT * 16 * 2; e += kFewWaves * kWave) {
+    const int r = e / 2, c = e % 2 * 8, n = g.n - n0 - c;
+    if (r >= g.m || n <= 0) continue;
+    float v[8] = {};
+#pragma unroll
+    for (int s = 0; s < kFewWaves; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += join[s][r][c + j];
+    finish8<T>(g, r, n0 + c, n, v);
+  }
+}
+
+// ---- the activation's gradient -----------------------------------------------------------------------
+
+// dz = dout act'(z) in the operands' type, rows padded with zeros to a multiple of 16 bytes, and the column sums of
+// the unrounded dz over a workgroup's rows.
+constexpr int kSlopeThreads = 256, kSlopeRows = 64;
+struct SlopeArgs {
+  const void *d_out, *z;
+  void* dz;       // NULL: only sums
+  float* parts;   // [workgroups down][n], NULL: no sums
+  int64_t m, ld;
+  int n, act;
+  bool z_bf16;
+};
+template <typename T, typename O>
+__global__ __launch_bounds__(kSlopeThreads) void slope_kernel(SlopeArgs a) {
+  constexpr int kGroups = kSlopeThreads / kWave;
+  __shared__ float join[kGroups][kWave * 8 + 4];
+  const int lane = threadIdx.x % kWave, col = (blockIdx.y * kWave + lane) * 8, n = a.n - col;
+  float sum[8] = {};
+  const int64_t end = a.m < (blockIdx.x + int64_t(1)) * kSlopeRows ? a.m : (blockIdx.x + int64_t(1)) * kSlopeRows;
+  for (int64_t row = blockIdx.x * static_cast<int64_t>(kSlopeRows) + threadIdx.x / kWave; row < end; row += kGroups) {
+    float d[8], z[8];
+    load8(static_cast<const O*>(a.d_out) + row * a.n + col, n, d);
+    if (a.act != kActNone) {
+      load8(a.z, a.z_bf16, row * a.n + col, n, z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] *= act_slope<T>(a.act, z[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] += d[j];
+    if (a.dz && col < a.ld) store8(static_cast<T*>(a.dz) + row * a.ld + col, static_cast<int>(a.ld - col), d);
+  }
+  if (a.parts == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) join[threadIdx.x / kWave][lane * 8 + j] = sum[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < kWave * 8; c += kSlopeThreads) {
+    const int at = blockIdx.y * kWave * 8 + c;
+    if (at >= a.n) continue;
+    float s = join[0][c];
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) s += join[i][c];
+    a.parts[static_cast<int64_t>(blockIdx.x) * a.n + at] = s;
+  }
+}
+
+// ---- plans and launches ------------------------------------------------------------------------------
+
+constexpr int kCus = 256;
+constexpr int kFewRows = 32;
+
+struct GemmPlan {
+  int tile;          // side: 256, 128 or 64
+  int tiles_m, tiles_n, splits;
+  int64_t split_k;
+  size_t part;       // bytes
+};
+static GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, size_t es) {
+  GemmPlan p = {};
+  const int64_t stage = 128 / static_cast<int64_t>(es);
+  const auto count = [&](int64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
+  p.tile = count(256) >= kCus / 2 ? 256 : (count(128) >= kCus / 2 ? 128 : 64);
+  p.tiles_m = static_cast<int>((m + p.tile - 1) / p.tile);
+  p.tiles_n = static_cast<int>((n + p.tile - 1) / p.tile);
+  const int64_t stages = std::max<int64_t>(1, (k + stage - 1) / stage);
+  const int64_t want = std::max<int64_t>(1, kCus / std::max<int64_t>(1, count(p.tile)));
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(want, stages / 8));
+  p.split_k = (stages + splits - 1) / splits * stage;
+  p.splits = std::max(1, static_cast<int>((k + p.split_k - 1) / p.split_k));
+  p.part = p.splits > 1 ? static_cast<size_t>(p.splits) * m * n * sizeof(float) : 0;
+  return p;
+}
+
+template <typename T, bool A_ALONG, bool B_ALONG>
+static int run_gemm(GemmArgs g, void* workspace, const char* what, hipStream_t st) {
+  const GemmPlan p = gemm_plan(g.m, g.n, g.k, sizeof(T));
+  g.tiles_m = p.tiles_m;
+  g.tiles_n = p.tiles_n;
+  g.splits = p.splits;
+  g.split_k = p.split_k;
+  g.part = static_cast<float*>(workspace);
+  const dim3 grid(static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits);
+  if (p.tile == 256)
+    hipLaunchKernelGGL((gemm_kernel<T, 256, 256, 2, 4, A_ALONG, B_ALONG>), grid, dim3(512), 0, st, g);
+  else if (p.tile == 128)
+    hipLaunchKernelGGL((gemm_kernel<T, 128, 128, 2, 2, A_ALONG, B_ALONG>), grid, dim3(256), 0, st, g);
+  else
+    hipLaunchKernelGGL((gemm_kernel<T, 64, 64, 2, 2, A_ALONG, B_ALONG>), grid, dim3(256), 0, st, g);
+  if (const int rc = check_launch(what)) return rc;
+  if (p.splits == 1) return GS_OK;
+  const int64_t blocks = (g.m * ((g.n + 7) / 8) + kFinishThreads - 1) / kFinishThreads;
+  hipLaunchKernelGGL(gemm_finish_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kFinishThreads), 0, st, g);
+  return check_launch(what);
+}
+
+template <typename T>
+static int run_forward(const GemmArgs& g, void* workspace, hipStream_t st) {
+  const dim3 grid((g.n + 15) / 16), block(kFewWaves * kWave);
+  if (g.m <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, block, 0, st, g);
+  else if (g.m <= kFewRows) hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, st, g);
+  else return run_gemm<T, true, true>(g, workspace, "linear", st);
+  return check_launch("linear");
+}
+
+static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Workspace of the backward pass: dz, the bias gradient's parts, the products' parts (one after the other).
+struct BackPlan {
+  bool make_dz;
+  int64_t ld;
+  int down;  // workgroups down a column
+  size_t dz, parts, product;
+};
+static BackPlan back_plan(const gs_linear* p, bool bias) {
+  BackPlan b = {};
+  const size_t es = row_type_bytes(p->dtype);
+  const int64_t per = 16 / static_cast<int64_t>(es);
+  // the output's gradient is the product's operand as it is where there is no activation, no rounding and no padding
+  b.make_dz = p->activation != kActNone || p->out_dtype != p->dtype || p->outputs % per != 0;
+  b.ld = (p->outputs + per - 1) / per * per;
+  b.down = static_cast<int>((p->rows + kSlopeRows - 1) / kSlopeRows);
+  b.dz = b.make_dz ? round16(static_cast<size_t>(p->rows) * b.ld * es) : 0;
+  b.parts = bias ? round16(static_cast<size_t>(b.down) * p->outputs * sizeof(float)) : 0;
+  b.product = std::max(gemm_plan(p->rows, p->inputs, p->outputs, es).part, gemm_plan(p->outputs, p->inputs, p->rows, es).part);
+  return b;
+}
+
+static int check_linear(const gs_linear* p, bool backward) {
+  GS_REQUIRE(p, GS_ERR_ARG, "linear: args is NULL");
+  GS_REQUIRE(row_type(p->dtype) && row_type(p->out_dtype), GS_ERR_ARG, "linear: dtypes must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(p->dtype == GS_BFLOAT16 || p->out_dtype == GS_FLOAT32, GS_ERR_ARG,
+             "linear: float32 products have a float32 result");
+  GS_REQUIRE(!p->bias || row_type(p->bias_dtype), GS_ERR_ARG, "linear: bias dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(!p->z || (row_type(p->z_dtype) && (p->dtype == GS_BFLOAT16 || p->z_dtype == GS_FLOAT32)), GS_ERR_ARG,
+             "linear: z must be GS_FLOAT32, or GS_BFLOAT16 of bfloat16 products");
+  GS_REQUIRE(p->activation >= 0 && p->activation < kActs, GS_ERR_ARG, "linear: unknown activation");
+  GS_REQUIRE(p->rows >= 0 && p->rows < (int64_t(1) << 31), GS_ERR_ARG, "linear: invalid row count");
+  GS_REQUIRE(p->inputs >= 1 && p->inputs <= GS_LINEAR_MAX_WIDTH && p->outputs >= 1 && p->outputs <= GS_LINEAR_MAX_WIDTH,
+             GS_ERR_ARG, "linear: %d inputs and %d outputs: 1 to %d are provided", p->inputs, p->outputs, GS_LINEAR_MAX_WIDTH);
+  const size_t es = row_type_bytes(p->dtype);
+  const int per = static_cast<int>(16 / es);
+  GS_REQUIRE(p->inputs % per == 0, GS_ERR_ALIGN, "linear: inputs must be a multiple of %d", per);
+  GS_REQUIRE(p->rows == 0 || (p->x && p->weight && (backward || p->out)), GS_ERR_ARG, "linear: null pointer");
+  for (const int64_t s : {p->x_stride, p->weight_stride})
+    GS_REQUIRE(s >= 0 && s % per == 0 && s < GS_LINEAR_MAX_STRIDE, GS_ERR_ALIGN,
+               "linear: row strides must be multiples of 16 bytes below %d elements", GS_LINEAR_MAX_STRIDE);
+  const size_t os = row_type_bytes(p->out_dtype);
+  GS_REQUIRE(aligned(p->x, 16) && aligned(p->weight, 16) && aligned(p->z, row_type_bytes(p->z_dtype)) &&
+                 aligned(p->bias, row_type_bytes(p->bias_dtype)) && aligned(p->residual, os) && aligned(p->out, os),
+             GS_ERR_ALIGN, "linear: misaligned tensor (x and weight: 16 bytes)");
+  // grids of a dimension below 2^32 threads; results indexed below 2^62
+  const int64_t m = p->rows, n = p->outputs, k = p->inputs;
+  GS_REQUIRE((m + 63) / 64 * ((std::max(n, k) + 63) / 64) < (int64_t(1) << 23) && m * ((std::max(n, k) + 7) / 8) < (int64_t(1) << 32),
+             GS_ERR_ARG, "linear: too many results");
+  return GS_OK;
+}
+
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" size_t gs_linear_fwd_workspace_size(const gs_linear* p) {
+  clear_error();
+  if (!p || p->rows <= kFewRows || p->inputs <= 0 || p->outputs <= 0 || !row_type(p->dtype)) return 0;
+  return gemm_plan(p->rows, p->outputs, p->inputs, row_type_bytes(p->dtype)).part;
+}
+
+extern "C" int gs_linear_fwd(const gs_linear* p, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (const int rc = check_linear(p, false)) return rc;
+  const size_t need = gs_linear_fwd_workspace_size(p);
+  GS_REQUIRE(workspace_bytes >= need && (workspace || need == 0), GS_ERR_WORKSPACE, "linear: workspace too small");
+  GS_REQUIRE(aligned(workspace, 16), GS_ERR_ALIGN, "linear: misaligned workspace");
+  if (p->rows == 0) return GS_OK;
+  GemmArgs g = {};
+  g.a = p->x;
+  g.b = p->weight;
+  g.lda = p->x_stride;
+  g.ldb = p->weight_stride;
+  g.m = p->rows;
+  g.n = p->outputs;
+  g.k = p->inputs;
+  g.act = p->activation;
+  g.bias = p->bias;
+  g.bias_bf16 = p->bias_dtype == GS_BFLOAT16;
+  g.residual = p->residual;
+  g.residual_stride = p->residual_stride;
+  g.residual_bf16 = g.out_bf16 = p->out_dtype == GS_BFLOAT16;
+  g.out = p->out;
+  g.z = p->z;
+  g.z_bf16 = p->z_dtype == GS_BFLOAT16;
+  return p->dtype == GS_BFLOAT16 ? run_forward<__bf16>(g, workspace, as_stream(stream))
+                                 : run_forward<float>(g, workspace, as_stream(stream));
+}
+
+extern "C" size_t gs_linear_bwd_workspace_size(const gs_linear* p) {
+  clear_error();
+  if (!p || p->rows <= 0 || p->inputs <= 0 || p->outputs <= 0 || !row_type(p->dtype)) return 0;
+  const BackPlan b = back_plan(p, true);
+  return b.dz + b.parts + b.product;
+}
+
+template <typename T>
+static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* d_weight, void* d_bias, void* workspace,
+                        hipStream_t st) {
+  const BackPlan b = back_plan(p, true);
+  char* ws = static_cast<char*>(workspace);
+  float* parts = reinterpret_cast<float*>(ws + b.dz);
+  void* product = ws + b.dz + b.parts;
+  const bool make_dz = b.make_dz && (d_x || d_weight);
+  if ((make_dz || d_bias) && p->rows > 0) {
+    const SlopeArgs s = {d_out, p->z, make_dz ? ws : nullptr, d_bias ? parts : nullptr, p->rows, b.ld, p->outputs, p->activation,
+                         p->z_dtype == GS_BFLOAT16};
+    const dim3 grid(b.down, (p->outputs + kWave * 8 - 1) / (kWave * 8)), block(kSlopeThreads);
+    if (p->out_dtype == GS_FLOAT32) hipLaunchKernelGGL((slope_kernel<T, float>), grid, block, 0, st, s);
+    else hipLaunchKernelGGL((slope_kernel<T, __bf16>), grid, block, 0, st, s);
+    if (const int rc = check_launch("linear backward (activation)")) return rc;
+  }
+  if (d_bias) {
+    ColumnSums s = {};
+    s.parts = parts;
+    s.n = b.down;
+    s.sums = 1;
+    s.width = p->outputs;
+    s.out[0] = d_bias;
+    s.bf16[0] = p->bias_dtype == GS_BFLOAT16;
+    if (const int rc = column_sums(s, "linear backward (bias)", st)) return rc;
+  }
+  GemmArgs g = {};
+  g.out_bf16 = sizeof(T) == 2;
+  const void* dz = make_dz ? static_cast<const void*>(ws) : d_out;
+  const int64_t ld = make_dz ? b.ld : p->outputs;
+  if (d_x && p->rows > 0) {
+    g.a = dz;
+    g.lda = ld;
+    g.b = p->weight;
+    g.ldb = p->weight_stride;
+    g.m = p->rows;
+    g.n = p->inputs;
+    g.k = p->outputs;
+    g.out = d_x;
+    if (const int rc = run_gemm<T, true, false>(g, product, "linear backward (input)", st)) return rc;
+  }
+  if (d_weight) {
+    g.a = dz;
+    g.lda = ld;
+    g.b = p->x;
+    g.ldb = p->x_stride;
+    g.m = p->outputs;
+    g.n = p->inputs;
+    g.k = p->rows;
+    g.out = d_weight;
+    if (const int rc = run_gemm<T, false, false>(g, product, "linear backward (weight)", st)) return rc;
+  }
+  return GS_OK;
+}
+
+extern "C" int gs_linear_bwd(const gs_linear* p, const void* d_out, void* d_x, void* d_weight, void* d_bias,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  if (const int rc = check_linear(p, true)) return rc;
+  GS_REQUIRE(p->rows == 0 || d_out, GS_ERR_ARG, "linear: null gradient");
+  GS_REQUIRE(p->rows == 0 || p->activation == kActNone || p->z, GS_ERR_ARG, "linear: the activation's gradient needs z");
+  const size_t need = gs_linear_bwd_workspace_size(p), es = row_type_bytes(p->dtype);
+  GS_REQUIRE(workspace_bytes >= need && (workspace || need == 0), GS_ERR_WORKSPACE, "linear: workspace too small");
+  GS_REQUIRE(aligned(workspace, 16) && aligned(d_out, 16) && aligned(d_x, es) &&
+                 aligned(d_weight, es) && aligned(d_bias, row_type_bytes(p->bias_dtype)),
+             GS_ERR_ALIGN, "linear: misaligned gradient or workspace");
+  const hipStream_t st = as_stream(stream);
+  return p->dtype == GS_BFLOAT16 ? run_backward<__bf16>(p, d_out, d_x, d_weight, d_bias, workspace, st)
+                                 : run_backward<float>(p, d_out, d_x, d_weight, d_bias, workspace, st);
+}

@@ -316,39 +316,6 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
   }
 }
 
-// Sums the workgroups' parts, column by column in a fixed order: 64 columns of one sum a workgroup, its wavefronts
-// take the parts in turn.
-constexpr int kPartThreads = 1024;
-struct NormSums {
-  const float* parts;
-  int n, sums, width;
-  void* out[5];
-  bool bf16[5];
-};
-__global__ __launch_bounds__(kPartThreads) void norm_sums_kernel(NormSums a) {
-  __shared__ float part[kPartThreads];
-  const int k = blockIdx.y, c = blockIdx.x * kWave + threadIdx.x % kWave, w = threadIdx.x / kWave;
-  float s[4] = {};
-  if (c < a.width) {
-    constexpr int kStep = kPartThreads / kWave;
-    int p = w;
-    const auto at = [&](int i) { return a.parts[(static_cast<int64_t>(i) * a.sums + k) * a.width + c]; };
-    for (; p + 3 * kStep < a.n; p += 4 * kStep) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] += at(p + i * kStep);
-    }
-    for (; p < a.n; p += kStep) s[0] += at(p);
-  }
-  part[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
-  __syncthreads();
-  if (w == 0 && c < a.width) {
-    float t = 0.0f;
-    for (int i = 0; i < kPartThreads / kWave; ++i) t += part[i * kWave + threadIdx.x];
-    if (a.bf16[k]) static_cast<__bf16*>(a.out[k])[c] = static_cast<__bf16>(t);
-    else static_cast<float*>(a.out[k])[c] = t;
-  }
-}
-
 // Dropout alone: a vector of eight a thread.
 constexpr int kDropThreads = 256;
 template <typename T>
@@ -496,7 +463,7 @@ extern "C" int gs_residual_norm_bwd(const gs_residual_norm* p, const void* d_h, 
   const bool gate_column = p->gate_rows == 0;
   a.d_gate_rows = gate_column ? nullptr : d_gate;
   void* const outs[5] = {d_weight, d_bias, d_post_weight, d_post_bias, gate_column ? d_gate : nullptr};
-  NormSums s = {};
+  ColumnSums s = {};
   for (int k = 0; k < 5; ++k) {
     a.slot[k] = outs[k] ? static_cast<int8_t>(a.sums) : int8_t(-1);
     if (!outs[k]) continue;
@@ -523,8 +490,7 @@ extern "C" int gs_residual_norm_bwd(const gs_residual_norm* p, const void* d_h, 
   s.n = static_cast<int>(blocks);  // (no rows: the sums are zero)
   s.sums = a.sums;
   s.width = a.width;
-  hipLaunchKernelGGL(norm_sums_kernel, dim3((a.width + kWave - 1) / kWave, a.sums), dim3(kPartThreads), 0, st, s);
-  return check_launch("residual norm backward (sums)");
+  return column_sums(s, "residual norm backward (sums)", st);
 }
 
 extern "C" int gs_dropout(const void* x, void* out, int64_t rows, int64_t stride, int width, int dtype, double p,

@@ -743,6 +743,39 @@ int gs_gated_scan_fwd(const gs_gated_scan* args, void* workspace, size_t workspa
 int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d_state, void* d_x, void* d_forget,
                       void* d_gate, float* d_initial, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * out [rows, outputs] = act(x weight^T + bias) + residual, x [rows, inputs] and weight [outputs, inputs] of dtype, read
+ * through row strides (multiples of 16 bytes below GS_LINEAR_MAX_STRIDE elements, pointers 16-byte aligned, inputs a multiple
+ * of 16 bytes; rows of a stride of 0 are one row). bias [outputs] of bias_dtype and residual [rows, outputs] of out_dtype (row
+ * stride residual_stride) may be NULL. out is of out_dtype: dtype, or GS_FLOAT32 for bfloat16 products. Products and the
+ * epilogue are float32, rounded once. z (of z_dtype: GS_FLOAT32, or dtype; may be NULL): x weight^T + bias, for the backward
+ * of an activation, whose slopes are taken there (a float32 d_bias needs a float32 z).
+ * Activations: relu, gelu z Phi(z), its tanh form, silu z sigmoid(z).
+ *
+ * gs_linear_bwd takes the same arguments (out and residual are not used, z is needed but for GS_ACT_NONE) and d_out [rows,
+ * outputs] of out_dtype (16-byte aligned), and writes those of d_x [rows, inputs], d_weight (dtype) and d_bias (bias_dtype) that are not NULL;
+ * the residual's gradient is d_out. d_out act'(z) is rounded to dtype as an operand.
+ * No atomics: the same inputs give the same bits.
+ * ------------------------------------------------------------------------------------- */
+#define GS_LINEAR_MAX_WIDTH (1 << 19)
+#define GS_LINEAR_MAX_STRIDE (1 << 20)
+#define GS_ACT_NONE 0
+#define GS_ACT_RELU 1
+#define GS_ACT_GELU 2
+#define GS_ACT_GELU_TANH 3
+#define GS_ACT_SILU 4
+typedef struct gs_linear {
+  const void *x, *weight, *bias, *residual;
+  void *out, *z;
+  int64_t rows, x_stride, weight_stride, residual_stride;
+  int32_t inputs, outputs, dtype, out_dtype, z_dtype, bias_dtype, activation;
+} gs_linear;
+size_t gs_linear_fwd_workspace_size(const gs_linear* args);
+int gs_linear_fwd(const gs_linear* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t gs_linear_bwd_workspace_size(const gs_linear* args);
+int gs_linear_bwd(const gs_linear* args, const void* d_out, void* d_x, void* d_weight, void* d_bias, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

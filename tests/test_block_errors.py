@@ -125,9 +125,56 @@ def test_scan_calls():
     expect(back(a, ds=258), ALIGN, "misaligned")
 
 
+def linear_args(**kw):
+    a = dict(x=256, weight=256, bias=256, residual=256, out=256, z=256, rows=100, x_stride=64, weight_stride=64,
+             residual_stride=40, inputs=64, outputs=40, activation=2)
+    a.update(kw)
+    return _lib.GsLinear(**a)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(dtype=1), ARG, "dtypes"), (dict(out_dtype=1), ARG, "dtypes"), (dict(out_dtype=BF), ARG, "float32 products"),
+    (dict(bias_dtype=1), ARG, "bias dtype"), (dict(z_dtype=1), ARG, "z must"), (dict(z_dtype=BF), ARG, "z must"),
+    (dict(activation=-1), ARG, "activation"), (dict(activation=5), ARG, "activation"), (dict(rows=-1), ARG, "row count"),
+    (dict(rows=1 << 31), ARG, "row count"), (dict(inputs=0), ARG, "inputs"), (dict(inputs=(1 << 19) + 4), ARG, "inputs"),
+    (dict(outputs=0), ARG, "outputs"), (dict(x=None), ARG, "null"), (dict(weight=None), ARG, "null"),
+    (dict(x_stride=66), ALIGN, "strides"), (dict(weight_stride=-64), ALIGN, "strides"), (dict(x_stride=1 << 20), ALIGN, "strides"),
+    (dict(x=260), ALIGN, "misaligned"), (dict(weight=264), ALIGN, "misaligned"), (dict(bias=258), ALIGN, "misaligned"),
+    (dict(rows=(1 << 31) - 1, outputs=1 << 19), ARG, "too many"),
+])
+def test_linear_arguments(kw, code, text):
+    L = _lib.lib()
+    a = linear_args(**kw)
+    expect(L.gs_linear_fwd(C.byref(a), 256, 1 << 62, None), code, text)
+    expect(L.gs_linear_bwd(C.byref(a), 256, 256, 256, 256, 256, 1 << 62, None), code, text)
+
+
+def test_linear_calls():
+    L = _lib.lib()
+    a = linear_args()
+    need = L.gs_linear_bwd_workspace_size(C.byref(a))
+    assert need > 0 and L.gs_linear_bwd_workspace_size(None) == 0 and L.gs_linear_fwd_workspace_size(None) == 0
+    back = lambda a, d=256, dx=256, ws=256, n=need: L.gs_linear_bwd(C.byref(a), d, dx, 256, 256, ws, n, None)  # noqa: E731
+    expect(L.gs_linear_fwd(None, None, 0, None), ARG, "NULL")
+    expect(L.gs_linear_fwd(C.byref(linear_args(out=None)), 256, 1 << 40, None), ARG, "null")
+    expect(L.gs_linear_fwd(C.byref(linear_args(out=258)), 256, 1 << 40, None), ALIGN, "misaligned")
+    expect(back(a, d=None), ARG, "null")
+    expect(back(linear_args(z=None)), ARG, "needs z")
+    expect(back(a, n=need - 1), WORKSPACE, "workspace")
+    expect(back(a, ws=None), WORKSPACE, "workspace")
+    expect(back(a, ws=264), ALIGN, "misaligned")
+    expect(back(a, d=264), ALIGN, "misaligned")
+    expect(back(a, dx=258), ALIGN, "misaligned")
+    split = linear_args(rows=64, inputs=8192, outputs=64, x_stride=8192, weight_stride=8192)
+    need = L.gs_linear_fwd_workspace_size(C.byref(split))
+    assert need > 0
+    expect(L.gs_linear_fwd(C.byref(split), 256, need - 1, None), WORKSPACE, "workspace")
+    expect(L.gs_linear_fwd(C.byref(split), 264, need, None), ALIGN, "misaligned")
+
+
 def test_tensors_off_the_gpu_are_refused():
     x = torch.zeros(4, 16)
     for call in (lambda: amdsplat.norm(x), lambda: amdsplat.residual_norm(x, x), lambda: amdsplat.dropout(x, 0.5, 1),
-                 lambda: amdsplat.gated_scan(x, x)):
+                 lambda: amdsplat.gated_scan(x, x), lambda: amdsplat.linear(x, x)):
         with pytest.raises(ValueError, match="GPU"):
             call()
