@@ -14,21 +14,35 @@ from . import _lib
 from ._grad import tracked
 from ._lib import call, ptr
 
-MAX_WIDTH = 1 << 19  # GS_LINEAR_MAX_WIDTH
+MAX_WIDTH, FEW_ROWS = 1 << 19, 32  # GS_LINEAR_MAX_WIDTH, GS_LINEAR_FEW_ROWS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # GS_ACT_*
 _DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8)}
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """t itself if the kernels can read it through its row stride, otherwise a contiguous copy."""
-    per = _DTYPES[t.dtype][1]
-    s = t.stride(0)
-    ok = t.stride(1) == 1 and 0 <= s < 1 << 20 and s % per == 0 and t.data_ptr() % 16 == 0
-    return t if ok or t.shape[0] == 0 else t.clone(memory_format=torch.contiguous_format)
-
-
 def _rows(t):
+    """t, or a copy whose last dimension is contiguous."""
     return t if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= 0) else t.contiguous()
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """Rows of t as the tile kernels read them: t itself where its address, its row stride and its row length are multiples of
+    16 bytes, otherwise a copy with zeros behind the rows, of which this is a view."""
+    code, per = _DTYPES[t.dtype]
+    rows, cols = t.shape
+    s = t.stride(0)
+    if rows == 0 or (cols % per == 0 and t.stride(1) == 1 and 0 <= s < 1 << 20 and s % per == 0 and t.data_ptr() % 16 == 0):
+        return t
+    t = _rows(t)
+    wide = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)
+    call("gs_rows_pack", t.data_ptr(), rows, cols, t.stride(0), wide.data_ptr(), wide.shape[1], code,
+         _lib.stream_handle(t.device))
+    return wide[:, :cols]
+
+
+def _operands(x, weight):
+    if x.shape[0] <= FEW_ROWS and weight.stride(0) < 1 << 20 and x.stride(0) < 1 << 20:
+        return _rows(x), _rows(weight)
+    return _packed(x), _packed(weight)
 
 
 def _args(x, weight, bias, residual, out, z, out_dtype, activation) -> _lib.GsLinear:
@@ -36,7 +50,7 @@ def _args(x, weight, bias, residual, out, z, out_dtype, activation) -> _lib.GsLi
     return _lib.GsLinear(x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
                          None if residual is None else residual.data_ptr(), ptr(out), ptr(z), rows,
                          x.stride(0) if rows else 0, weight.stride(0), 0 if residual is None else residual.stride(0),
-                         x.shape[1], weight.shape[0], _DTYPES[x.dtype][0], _DTYPES[out_dtype][0],
+                         weight.shape[1], weight.shape[0], _DTYPES[x.dtype][0], _DTYPES[out_dtype][0],
                          0 if z is None else _DTYPES[z.dtype][0], 0 if bias is None else _DTYPES[bias.dtype][0], activation)
 
 
@@ -59,7 +73,7 @@ def _forward(x, weight, bias, residual, activation, out_dtype, keep: bool):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, out_dtype):
-        x, weight = _readable(x), _readable(weight)
+        x, weight = _operands(x, weight)
         out, z = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, bias, z)
         ctx.rule = (out_dtype, activation)
@@ -71,7 +85,7 @@ class _Linear(torch.autograd.Function):
         x, weight, bias, z = ctx.saved_tensors
         grads = [None, None, None]
         if any(ctx.needs_input_grad[:3]):
-            d = d_out.contiguous()
+            x, weight, d = _packed(x), _packed(weight), d_out.contiguous()
             if d.data_ptr() % 16:
                 d = d.clone()
             grads = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if t is not None and need else None
@@ -91,8 +105,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     x's dtype as an operand of the products (not in the bias' gradient), and act' is taken at z = x weight^T + bias, which the forward
     keeps: in float32, or without a bias in x's dtype. No forward-mode derivative.
 
-    x and weight are read through their row strides where these, the addresses and K are multiples of 16 bytes;
-    otherwise they are copied first (for K: padded with zeros, at every call)."""
+    x and weight are read through their row strides where these, the addresses and K are multiples of 16 bytes, and in a
+    forward of up to 32 rows wherever the last dimension is contiguous; otherwise they are copied first, at every call."""
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"x must be [tokens, inputs] and weight [outputs, inputs], got {tuple(x.shape)} and {tuple(weight.shape)}")
     if x.dtype not in _DTYPES or weight.dtype != x.dtype:
@@ -114,10 +128,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         out_dtype, residual = residual.dtype, _rows(residual)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
-    per = _DTYPES[x.dtype][1]
-    if x.shape[1] % per:
-        x, weight = (torch.nn.functional.pad(t, (0, -t.shape[1] % per)) for t in (x, weight))
     rest = (bias, residual, ACTIVATIONS[activation], out_dtype)
     if tracked(x, weight, bias, residual):
         return _Linear.apply(x, weight, *rest)
-    return _forward(_readable(x), _readable(weight), *rest, False)[0]
+    return _forward(*_operands(x, weight), *rest, False)[0]

@@ -6,28 +6,42 @@
 
 namespace gs {
 
-template <typename T>
-struct Raw8 {
-  typedef T Vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-  static constexpr int kParts = sizeof(T) / 2;  // 16-byte accesses
-  static constexpr int kPer = 16 / sizeof(T);
+// N elements as they lie in memory. Loads leave them so: turned to float inside the branch that loads them, every load
+// would be waited for before the next is sent.
+template <typename T, int N>
+struct RawN {
+  static constexpr int kPer = N * sizeof(T) > 16 ? 16 / sizeof(T) : N, kParts = N / kPer;
+  typedef T Vec __attribute__((ext_vector_type(kPer), aligned(sizeof(T))));
+  Vec part[kParts];
+  // Elements p[0 .. n) of N, the others zero.
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= N) {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) part[i] = *reinterpret_cast<const Vec*>(p + i * kPer);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) part[i] = 0;
+      if (n > 0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (j < n) part[j / kPer][j % kPer] = p[j];
+      }
+    }
+  }
+  __device__ __forceinline__ void to(float (&v)[N]) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = static_cast<float>(part[j / kPer][j % kPer]);
+  }
 };
+template <typename T>
+using Raw8 = RawN<T, 8>;
 
-// Elements p[0 .. n) of eight as float, the others zero. n >= 8: one or two 16-byte loads.
+// Elements p[0 .. n) of eight as float, the others zero.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-  using R = Raw8<T>;
-  if (n >= 8) {
-#pragma unroll
-    for (int i = 0; i < R::kParts; ++i) {
-      const auto a = *reinterpret_cast<const typename R::Vec*>(p + i * R::kPer);
-#pragma unroll
-      for (int j = 0; j < R::kPer; ++j) v[i * R::kPer + j] = static_cast<float>(a[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? static_cast<float>(p[j]) : 0.0f;
-  }
+  Raw8<T> r;
+  r.load(p, n);
+  r.to(v);
 }
 // The same of a tensor whose type is known at run time.
 __device__ __forceinline__ void load8(const void* p, bool bf16, int64_t at, int n, float (&v)[8]) {

@@ -8,8 +8,8 @@
 // contraction are read as they lie, the others through the LDS unit's transpose (bfloat16) or word by word (float32).
 // Products accumulate in float32 (v_mfma_f32_32x32x16_bf16, or v_mfma_f32_32x32x2_f32 in float32). The result goes
 // through LDS once, so that bias, activation, residual and stores see eight neighbouring columns a lane, and is
-// rounded once. Tiles that would leave CUs idle are cut along the contraction into float32 parts, which a second
-// launch sums in order and finishes.
+// rounded once. The last tiles, which would leave CUs idle, are cut along the contraction into float32 parts, which a
+// second launch sums in order and finishes (gemm_plan).
 //
 // Few rows are bound by reading W once: linear_few_kernel streams it past the matrix unit without LDS.
 #include <algorithm>
@@ -68,37 +68,62 @@ constexpr float kTanhOuter = 1.5957691216057308f, kTanhInner = 0.044715f;  // 2 
 // their products do not become infinity times zero.
 constexpr float kFar = 100.0f;
 
-template <typename T>
-__device__ __forceinline__ float act_value(int act, float z) {
-  float bell;
-  if (act >= kActGelu) z = z < -kFar ? -kFar : z;  // NaN stays
-  switch (act) {
-    case kActRelu: return z < 0.0f ? 0.0f : z;
-    case kActGelu: return z * normal_cdf<T>(z, bell);
-    case kActGeluTanh: return z * sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
-    case kActSilu: return z * sigmoid<T>(z);
-    default: return z;
-  }
+// Eight values, the kind chosen once for all of them.
+template <typename F>
+__device__ __forceinline__ void each8(float (&v)[8], F f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = f(v[j]);
 }
 template <typename T>
-__device__ __forceinline__ float act_slope(int act, float z) {
-  if (act >= kActGelu) z = z < -kFar ? -kFar : (z > kFar ? kFar : z);
+__device__ __forceinline__ void activate8(int act, float (&v)[8]) {
+  const auto near = [](float z) { return z < -kFar ? -kFar : z; };  // NaN stays
   switch (act) {
-    case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
-    case kActGelu: {
-      float bell;
-      const float p = normal_cdf<T>(z, bell);
-      return fmaf(z * 0.3989422804014327f, bell, p);
-    }
-    case kActGeluTanh: {
-      const float p = sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
-      return fmaf(z * p * (1.0f - p), kTanhOuter * fmaf(3.0f * kTanhInner * z, z, 1.0f), p);
-    }
-    case kActSilu: {
-      const float p = sigmoid<T>(z);
-      return fmaf(z * p, 1.0f - p, p);
-    }
-    default: return 1.0f;
+    case kActRelu: return each8(v, [](float z) { return z < 0.0f ? 0.0f : z; });
+    case kActGelu:
+      return each8(v, [&](float z) {
+        float bell;
+        z = near(z);
+        return z * normal_cdf<T>(z, bell);
+      });
+    case kActGeluTanh:
+      return each8(v, [&](float z) {
+        z = near(z);
+        return z * sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
+      });
+    case kActSilu:
+      return each8(v, [&](float z) {
+        z = near(z);
+        return z * sigmoid<T>(z);
+      });
+    default: return;
+  }
+}
+// act'(z) in place of z.
+template <typename T>
+__device__ __forceinline__ void slope8(int act, float (&v)[8]) {
+  const auto near = [](float z) { return z < -kFar ? -kFar : (z > kFar ? kFar : z); };
+  switch (act) {
+    case kActRelu: return each8(v, [](float z) { return z > 0.0f ? 1.0f : 0.0f; });
+    case kActGelu:
+      return each8(v, [&](float z) {
+        float bell;
+        z = near(z);
+        const float p = normal_cdf<T>(z, bell);
+        return fmaf(z * 0.3989422804014327f, bell, p);
+      });
+    case kActGeluTanh:
+      return each8(v, [&](float z) {
+        z = near(z);
+        const float p = sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
+        return fmaf(z * p * (1.0f - p), kTanhOuter * fmaf(3.0f * kTanhInner * z, z, 1.0f), p);
+      });
+    case kActSilu:
+      return each8(v, [&](float z) {
+        z = near(z);
+        const float p = sigmoid<T>(z);
+        return fmaf(z * p, 1.0f - p, p);
+      });
+    default: return each8(v, [](float) { return 1.0f; });
   }
 }
 
@@ -115,9 +140,24 @@ struct GemmArgs {
   int64_t residual_stride;
   void *out, *z;     // [m][n], contiguous; z: before the activation (NULL: not wanted)
   bool bias_bf16, residual_bf16, out_bf16, z_bf16;
-  int tiles_m, tiles_n, splits;
+  int tiles_m, tiles_n;
+  int whole, splits; // tiles that one workgroup makes; parts of each of the others
   int64_t split_k;   // contraction of a part, a multiple of a stage's
-  float* part;       // [splits][m][n] where splits > 1
+  float* part;       // [other tiles][splits][rows of a tile][columns of a tile]
+};
+
+// The first row and column of tile t. Tiles are taken in groups of eight rows of them, down a group's columns, and an XCD has a
+// contiguous share of that order: what its CUs work on together is a block of some eight by four tiles.
+constexpr int kTileGroup = 8;
+struct TileAt {
+  int64_t m0;
+  int n0;
+  __device__ __forceinline__ TileAt(const GemmArgs& g, int t, int bm, int bn) {
+    const int group = t / (kTileGroup * g.tiles_n), first = group * kTileGroup;
+    const int high = min(kTileGroup, g.tiles_m - first), in = t - first * g.tiles_n;
+    m0 = static_cast<int64_t>(first + in % high) * bm;
+    n0 = in / high * bn;
+  }
 };
 
 // Bias, activation, residual and store of columns col .. col + 7 of a row (the first n of them).
@@ -130,10 +170,7 @@ __device__ __forceinline__ void finish8(const GemmArgs& g, int64_t row, int col,
     for (int j = 0; j < 8; ++j) v[j] += b[j];
   }
   if (g.z) store8(g.z, g.z_bf16, row * g.n + col, n, v);
-  if (g.act != kActNone) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = act_value<T>(g.act, v[j]);
-  }
+  if (g.act != kActNone) activate8<T>(g.act, v);
   if (g.residual) {
     float r[8];
     load8(g.residual, g.residual_bf16, row * g.residual_stride + col, n, r);
@@ -207,10 +244,6 @@ struct Side {
   }
 };
 
-// Tiles are taken in groups of eight rows of them, down a group's columns, and an XCD has a contiguous share of
-// that order: what its CUs work on together is a block of some eight by four tiles.
-constexpr int kTileGroup = 8;
-
 // BM x BN results by WM x WN wavefronts.
 template <typename T, int BM, int BN, int WM, int WN, bool A_ALONG, bool B_ALONG>
 __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
@@ -222,14 +255,13 @@ __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[2 * kStageBytes > kOutBytes ? 2 * kStageBytes : kOutBytes];
   using A = Side<T, A_ALONG, BM, kThreads>;
   using B = Side<T, B_ALONG, BN, kThreads>;
-  const int tiles = g.tiles_m * g.tiles_n;
-  const int at = xcd_tile(blockIdx.x, gridDim.x);
-  const int split = at / tiles, t = at - split * tiles;
-  const int group = t / (kTileGroup * g.tiles_n), first = group * kTileGroup;
-  const int high = min(kTileGroup, g.tiles_m - first), in = t - first * g.tiles_n;
-  const int64_t m0 = static_cast<int64_t>(first + in % high) * BM;
-  const int n0 = in / high * BN;
-  const int64_t k_begin = split * g.split_k, k_end = g.k - k_begin < g.split_k ? g.k : k_begin + g.split_k;
+  const bool whole = static_cast<int>(blockIdx.x) < g.whole;
+  const int other = whole ? 0 : xcd_tile(blockIdx.x - g.whole, gridDim.x - g.whole), split = other % g.splits;
+  const TileAt at(g, whole ? xcd_tile(blockIdx.x, g.whole) : g.whole + other / g.splits, BM, BN);
+  const int64_t m0 = at.m0;
+  const int n0 = at.n0;
+  const int64_t k_begin = whole ? 0 : split * g.split_k;
+  const int64_t k_end = whole || g.k - k_begin < g.split_k ? g.k : k_begin + g.split_k;
   const A a(g.a, g.lda, m0, g.m);
   const B b(g.b, g.ldb, n0, g.n);
   const int lane = threadIdx.x % kWave;
@@ -255,10 +287,20 @@ __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
       for (int i = 0; i < TM; ++i) fa[i] = A::frag(now, wm + 32 * i, c, lane);
 #pragma unroll
       for (int j = 0; j < TN; ++j) fb[j] = B::frag(now + A::kBytes, wn + 32 * j, c, lane);
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) mma(acc[i][j], fb[j], fa[i]);
+          for (int j = 0; j < TN; ++j) mma(acc[i][j], fb[j], fa[i]);
+      } else {  // one pair of slots over all results, then the next: no product waits for the one before it
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+          for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][s], fa[i][s], acc[i][j], 0, 0, 0);
+      }
     }
     char* s = now;
     now = next;
@@ -284,74 +326,86 @@ __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
       const int row = r + lane / kLanes, c = lane % kLanes * 8;
       const int64_t m = m0 + wm + 32 * i + row;
       const int col = n0 + wn + c, n = m < g.m ? g.n - col : 0;
-      if (n <= 0) continue;
       float v[8];
       const f32x4 lo = *reinterpret_cast<const f32x4*>(own + row * kRowFloats + c);
       const f32x4 hi = *reinterpret_cast<const f32x4*>(own + row * kRowFloats + c + 4);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
-      if (g.splits > 1) store8(g.part + (split * g.m + m) * g.n + col, n, v);
-      else finish8<T>(g, m, col, n, v);
+      if (!whole) store8(g.part + (static_cast<int64_t>(other) * BM + wm + 32 * i + row) * BN + wn + c, 8, v);
+      else if (n > 0) finish8<T>(g, m, col, n, v);
     }
   }
 }
 
-// Sums the parts of the contraction in order and finishes.
+// Sums the parts of the tiles after the whole ones in order and finishes them: eight columns a thread.
 constexpr int kFinishThreads = 256;
-template <typename T>
+template <typename T, int TILE>
 __global__ __launch_bounds__(kFinishThreads) void gemm_finish_kernel(GemmArgs g) {
-  const int vecs = (g.n + 7) / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kFinishThreads + threadIdx.x;
-  if (i >= g.m * vecs) return;
-  const int64_t row = i / vecs;
-  const int col = static_cast<int>(i - row * vecs) * 8, n = g.n - col;
-  float v[8];
-  load8(g.part + row * g.n + col, n, v);
-  for (int s = 1; s < g.splits; ++s) {
-    float p[8];
-    load8(g.part + (s * g.m + row) * g.n + col, n, p);
+  constexpr int kBlocks = TILE * TILE / 8 / kFinishThreads;  // of a tile
+  const int other = blockIdx.x / kBlocks, i = blockIdx.x % kBlocks * kFinishThreads + threadIdx.x;
+  const TileAt at(g, g.whole + other, TILE, TILE);
+  const int row = i / (TILE / 8), c = i % (TILE / 8) * 8;
+  const int n = at.m0 + row < g.m ? g.n - at.n0 - c : 0;
+  if (n <= 0) return;
+  const float* p = g.part + (static_cast<int64_t>(other) * g.splits * TILE + row) * TILE + c;
+  float v[8] = {};
+  for (int s = 0; s < g.splits; ++s, p += TILE * TILE) {
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += p[j];
+    for (int j = 0; j < 4; ++j) v[j] += lo[j], v[4 + j] += hi[j];
   }
-  finish8<T>(g, row, col, n, v);
+  finish8<T>(g, at.m0 + row, at.n0 + c, n, v);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------
 
 // Sixteen columns a workgroup, all rows (16 MT of them): its wavefronts take the contraction in turn, straight from
-// memory into the matrix instruction's operands, and are joined in LDS.
-constexpr int kFewWaves = 8;
+// memory into the matrix instruction's operands, four loads of W in flight each, and are joined in LDS. Rows at any address
+// and stride: loads are of an element's alignment, and the contraction's last vector is read element by element.
+constexpr int kFewWaves = 8, kFewUnroll = 4;
 template <typename T, int MT>
 __global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g) {
   constexpr int kGroup = 64 / static_cast<int>(sizeof(T));  // contraction of one load: 4 x 16 bytes a row
+  constexpr int kTurn = kFewWaves * kGroup;
   __shared__ __attribute__((aligned(16))) float join[kFewWaves][MT * 16][16 + 4];
+  typedef T Vec __attribute__((ext_vector_type(kVec<T>), aligned(sizeof(T))));
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, row = lane % 16;
-  const int n0 = blockIdx.x * 16, k_lane = lane / 16 * kVec<T>;
-  const bool in_n = n0 + row < g.n;
+  const int n0 = blockIdx.x * 16, k_lane = wave * kGroup + lane / 16 * kVec<T>;
   const T* w = static_cast<const T*>(g.b) + (n0 + row) * g.ldb + k_lane;
   const T* x = static_cast<const T*>(g.a) + row * g.lda + k_lane;
-  f32x4 acc[MT] = {};
-#pragma unroll 4
-  for (int64_t k = wave * kGroup; k < g.k; k += kFewWaves * kGroup) {
-    using Raw = uint32_t __attribute__((ext_vector_type(4)));
-    const bool in_k = k + k_lane < g.k;
-    const Raw zero = {0, 0, 0, 0};
-    const Raw fw = in_n && in_k ? *reinterpret_cast<const Raw*>(w + k) : zero;
-    Raw fx[MT];
+  const int rows_n = n0 + row < g.n ? static_cast<int>(g.k) : 0;
+  const auto fetch = [](const T* p, int left) {
+    Vec v;
+    if (left >= kVec<T>) {
+      v = *reinterpret_cast<const Vec*>(p);
+    } else {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-      fx[i] = 16 * i + row < g.m && in_k ? *reinterpret_cast<const Raw*>(x + 16 * i * g.lda + k) : zero;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fw), __builtin_bit_cast(bf16x8, fx[i]),
-                                                         acc[i], 0, 0, 0);
-      } else {
-        const f32x4 a = __builtin_bit_cast(f32x4, fw), b = __builtin_bit_cast(f32x4, fx[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc[i], 0, 0, 0);
-      }
+      for (int j = 0; j < kVec<T>; ++j) v[j] = j < left ? p[j] : static_cast<T>(0.0f);
     }
+    return v;
+  };
+  f32x4 acc[MT] = {};
+  for (int k = 0; k < g.k; k += kFewUnroll * kTurn) {
+    Vec fw[kFewUnroll], fx[kFewUnroll][MT];
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) fw[u] = fetch(w + k + u * kTurn, rows_n - k_lane - k - u * kTurn);
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        fx[u][i] = fetch(x + 16 * i * g.lda + k + u * kTurn,
+                         16 * i + row < g.m ? static_cast<int>(g.k) - k_lane - k - u * kTurn : 0);
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (sizeof(T) == 2) {
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u], fx[u][i], acc[i], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[u][j], fx[u][i][j], acc[i], 0, 0, 0);
+        }
+      }
   }
   // a lane holds row l % 16 and columns 4 (l / 16) .. + 3
 #pragma unroll
@@ -373,13 +427,13 @@ __global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g
 
 // dz = dout act'(z) in the operands' type, rows padded with zeros to a multiple of 16 bytes, and the column sums of
 // the unrounded dz over a workgroup's rows.
-constexpr int kSlopeThreads = 256, kSlopeRows = 64;
+constexpr int kSlopeThreads = 256;
 struct SlopeArgs {
   const void *d_out, *z;
   void* dz;       // NULL: only sums
   float* parts;   // [workgroups down][n], NULL: no sums
   int64_t m, ld;
-  int n, act;
+  int n, act, rows;  // rows: of a workgroup
   bool z_bf16;
 };
 template <typename T, typename O>
@@ -388,14 +442,15 @@ __global__ __launch_bounds__(kSlopeThreads) void slope_kernel(SlopeArgs a) {
   __shared__ float join[kGroups][kWave * 8 + 4];
   const int lane = threadIdx.x % kWave, col = (blockIdx.y * kWave + lane) * 8, n = a.n - col;
   float sum[8] = {};
-  const int64_t end = a.m < (blockIdx.x + int64_t(1)) * kSlopeRows ? a.m : (blockIdx.x + int64_t(1)) * kSlopeRows;
-  for (int64_t row = blockIdx.x * static_cast<int64_t>(kSlopeRows) + threadIdx.x / kWave; row < end; row += kGroups) {
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * a.rows, end = a.m - from < a.rows ? a.m : from + a.rows;
+  for (int64_t row = from + threadIdx.x / kWave; row < end; row += kGroups) {
     float d[8], z[8];
     load8(static_cast<const O*>(a.d_out) + row * a.n + col, n, d);
     if (a.act != kActNone) {
       load8(a.z, a.z_bf16, row * a.n + col, n, z);
+      slope8<T>(a.act, z);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] *= act_slope<T>(a.act, z[j]);
+      for (int j = 0; j < 8; ++j) d[j] *= z[j];
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] += d[j];
@@ -415,61 +470,126 @@ __global__ __launch_bounds__(kSlopeThreads) void slope_kernel(SlopeArgs a) {
   }
 }
 
+// Rows copied to rows of a multiple of eight elements, the rest zero.
+template <typename T>
+__global__ __launch_bounds__(kFinishThreads) void pack_kernel(const T* src, int64_t rows, int64_t cols, int64_t stride, T* dst,
+                                                              int vecs) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kFinishThreads + threadIdx.x, row = i / vecs;
+  if (row >= rows) return;
+  const int64_t c = (i - row * vecs) * 8, left = cols - c;
+  float v[8];  // (float32 holds both types exactly)
+  load8(src + row * stride + c, left < 8 ? static_cast<int>(left) : 8, v);
+  store8(dst + i * 8, 8, v);
+}
+
 // ---- plans and launches ------------------------------------------------------------------------------
 
 constexpr int kCus = 256;
-constexpr int kFewRows = 32;
+constexpr int kFewRows = GS_LINEAR_FEW_ROWS;
 
 struct GemmPlan {
   int tile;          // side: 256, 128 or 64
-  int tiles_m, tiles_n, splits;
+  int tiles_m, tiles_n, whole, splits;
   int64_t split_k;
   size_t part;       // bytes
 };
-static GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, size_t es) {
-  GemmPlan p = {};
+// What a stage of 128 bytes of contraction takes a tile in us: of a CU's time where enough workgroups share it, and at
+// least, where there are few. bfloat16: 8192 x 4096 x 4096 in tiles of 256, 128, 64 takes 225, 258 and 371 us; 256 tiles of
+// 128 over 129 stages, one a CU, 87 us; 48 tiles of 64 over 16 stages 8 us. float32 (tiles of 256 have no
+// registers left for it): 4096 x 4096 x 4096 in tiles of 128 and 64 takes 1006 and 1052 us; 256 tiles of 128 over 32 stages,
+// one a CU, 77 us; 44 tiles of 64 over 18 stages 16 us.
+struct TileCost {
+  int side, share;  // workgroups that share a CU
+  float busy, alone;
+};
+constexpr TileCost kTileCost[2][3] = {{{128, 2, 1.96f, 2.4f}, {64, 4, 0.51f, 0.75f}, {0, 1, 0.0f, 0.0f}},
+                                      {{256, 1, 1.76f, 1.76f}, {128, 2, 0.48f, 0.67f}, {64, 4, 0.18f, 0.4f}}};
+// Chooses the side of the tiles and how many of them are made whole, one workgroup each: all; or as many as fill
+// every CU alike, where a few are left over; or none, where there are too few. The others are cut into parts of at least four
+// stages, which costs a second launch, and the parts written and read. 8203 rows are 65 tiles of 128, so that 512 of 65 x 8
+// tiles fill the chip and the other eight would take half as long again: 8203 x 1024 results over 4096 take 103 us
+// whole, 77 us with those eight in sixteen parts each; 4096 x 1024 over 8203 88 us in 256 tiles, 73 us in 2 x 256 parts.
+static GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, size_t es, size_t result) {
+  GemmPlan best = {};
+  float least = FLT_MAX;
   const int64_t stage = 128 / static_cast<int64_t>(es);
-  const auto count = [&](int64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
-  p.tile = count(256) >= kCus / 2 ? 256 : (count(128) >= kCus / 2 ? 128 : 64);
-  p.tiles_m = static_cast<int>((m + p.tile - 1) / p.tile);
-  p.tiles_n = static_cast<int>((n + p.tile - 1) / p.tile);
-  const int64_t stages = std::max<int64_t>(1, (k + stage - 1) / stage);
-  const int64_t want = std::max<int64_t>(1, kCus / std::max<int64_t>(1, count(p.tile)));
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(want, stages / 8));
-  p.split_k = (stages + splits - 1) / splits * stage;
-  p.splits = std::max(1, static_cast<int>((k + p.split_k - 1) / p.split_k));
-  p.part = p.splits > 1 ? static_cast<size_t>(p.splits) * m * n * sizeof(float) : 0;
-  return p;
+  const int stages = static_cast<int>(std::max<int64_t>(1, (k + stage - 1) / stage));
+  for (const TileCost& c : kTileCost[es == 2]) {
+    if (c.side == 0) continue;
+    const int64_t tiles_m = (m + c.side - 1) / c.side, tiles_n = (n + c.side - 1) / c.side;
+    const int tiles = static_cast<int>(tiles_m * tiles_n);
+    const float area = static_cast<float>(c.side) * c.side;
+    const float store = area * result / 19500.0f;  // through a CU's share of the memory, bytes a us
+    const auto take = [&](int others, int len) {
+      const int whole = tiles - others, parts = (stages + len - 1) / len;
+      const int turns = (whole + kCus - 1) / kCus, more = (others * parts + kCus - 1) / kCus;
+      float t = std::max((static_cast<float>(turns) * stages + static_cast<float>(more) * len) * c.busy,
+                         (turns ? stages : len) * c.alone) + turns * store;
+      if (turns > 1 && turns % c.share == 1) t += stages * (c.alone - c.busy);  // the last ones have a CU each
+      if (others) t += 6.0f + others * parts * 8.0f * area / 6e6f;
+      if (t >= least) return;
+      least = t;
+      best = {c.side, static_cast<int>(tiles_m), static_cast<int>(tiles_n), whole, parts, len * stage,
+              static_cast<size_t>(others) * parts * c.side * c.side * sizeof(float)};
+    };
+    take(0, stages);
+    const int others = tiles <= kCus ? tiles : tiles % kCus;
+    if (others == 0 || (tiles > kCus && others > kCus / 2)) continue;
+    for (const int p : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (stages < 4 * p) break;
+      take(others, (stages + p - 1) / p);
+    }
+  }
+  return best;
 }
 
+template <typename T, int TILE, int WM, int WN, bool A_ALONG, bool B_ALONG>
+static int launch_gemm(const GemmArgs& g, const char* what, hipStream_t st) {
+  const unsigned others = static_cast<unsigned>(g.tiles_m) * g.tiles_n - g.whole;
+  hipLaunchKernelGGL((gemm_kernel<T, TILE, TILE, WM, WN, A_ALONG, B_ALONG>), dim3(g.whole + others * g.splits),
+                     dim3(WM * WN * kWave), 0, st, g);
+  if (const int rc = check_launch(what)) return rc;
+  if (others == 0) return GS_OK;
+  hipLaunchKernelGGL((gemm_finish_kernel<T, TILE>), dim3(others * (TILE * TILE / 8 / kFinishThreads)), dim3(kFinishThreads), 0,
+                     st, g);
+  return check_launch(what);
+}
 template <typename T, bool A_ALONG, bool B_ALONG>
-static int run_gemm(GemmArgs g, void* workspace, const char* what, hipStream_t st) {
-  const GemmPlan p = gemm_plan(g.m, g.n, g.k, sizeof(T));
+static int run_gemm(GemmArgs g, const GemmPlan& p, void* workspace, const char* what, hipStream_t st) {
   g.tiles_m = p.tiles_m;
   g.tiles_n = p.tiles_n;
+  g.whole = p.whole;
   g.splits = p.splits;
   g.split_k = p.split_k;
   g.part = static_cast<float*>(workspace);
-  const dim3 grid(static_cast<unsigned>(p.tiles_m) * p.tiles_n * p.splits);
-  if (p.tile == 256)
-    hipLaunchKernelGGL((gemm_kernel<T, 256, 256, 2, 4, A_ALONG, B_ALONG>), grid, dim3(512), 0, st, g);
-  else if (p.tile == 128)
-    hipLaunchKernelGGL((gemm_kernel<T, 128, 128, 2, 2, A_ALONG, B_ALONG>), grid, dim3(256), 0, st, g);
-  else
-    hipLaunchKernelGGL((gemm_kernel<T, 64, 64, 2, 2, A_ALONG, B_ALONG>), grid, dim3(256), 0, st, g);
-  if (const int rc = check_launch(what)) return rc;
-  if (p.splits == 1) return GS_OK;
-  const int64_t blocks = (g.m * ((g.n + 7) / 8) + kFinishThreads - 1) / kFinishThreads;
-  hipLaunchKernelGGL(gemm_finish_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kFinishThreads), 0, st, g);
-  return check_launch(what);
+  if constexpr (sizeof(T) == 2) {
+    if (p.tile == 256) return launch_gemm<T, 256, 2, 4, A_ALONG, B_ALONG>(g, what, st);
+  }
+  if (p.tile == 128) return launch_gemm<T, 128, 2, 2, A_ALONG, B_ALONG>(g, what, st);
+  return launch_gemm<T, 64, 2, 2, A_ALONG, B_ALONG>(g, what, st);
+}
+static size_t result_bytes(const gs_linear* p) {
+  return row_type_bytes(p->out_dtype) + (p->z ? row_type_bytes(p->z_dtype) : 0) + (p->residual ? row_type_bytes(p->out_dtype) : 0);
+}
+static GemmPlan forward_plan(const gs_linear* p) {
+  return gemm_plan(p->rows, p->outputs, p->inputs, row_type_bytes(p->dtype), result_bytes(p));
+}
+// of d_x and of d_weight
+static GemmPlan input_plan(const gs_linear* p) {
+  const size_t es = row_type_bytes(p->dtype);
+  return gemm_plan(p->rows, p->inputs, p->outputs, es, es);
+}
+static GemmPlan weight_plan(const gs_linear* p) {
+  const size_t es = row_type_bytes(p->dtype);
+  return gemm_plan(p->outputs, p->inputs, p->rows, es, es);
 }
 
 template <typename T>
-static int run_forward(const GemmArgs& g, void* workspace, hipStream_t st) {
+static int run_forward(const gs_linear* p, const GemmArgs& g, void* workspace, hipStream_t st) {
   const dim3 grid((g.n + 15) / 16), block(kFewWaves * kWave);
   if (g.m <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, block, 0, st, g);
   else if (g.m <= kFewRows) hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, st, g);
-  else return run_gemm<T, true, true>(g, workspace, "linear", st);
+  else return run_gemm<T, true, true>(g, forward_plan(p), workspace, "linear", st);
   return check_launch("linear");
 }
 
@@ -479,7 +599,7 @@ static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 struct BackPlan {
   bool make_dz;
   int64_t ld;
-  int down;  // workgroups down a column
+  int rows, down;  // of a workgroup of the slope kernel, and workgroups down a column
   size_t dz, parts, product;
 };
 static BackPlan back_plan(const gs_linear* p, bool bias) {
@@ -489,10 +609,13 @@ static BackPlan back_plan(const gs_linear* p, bool bias) {
   // the output's gradient is the product's operand as it is where there is no activation, no rounding and no padding
   b.make_dz = p->activation != kActNone || p->out_dtype != p->dtype || p->outputs % per != 0;
   b.ld = (p->outputs + per - 1) / per * per;
-  b.down = static_cast<int>((p->rows + kSlopeRows - 1) / kSlopeRows);
+  // some thousand workgroups, of at most 64 rows, of one for each wavefront at least
+  const int64_t across = (p->outputs + kWave * 8 - 1) / (kWave * 8);
+  b.rows = static_cast<int>(std::max<int64_t>(4, std::min<int64_t>(64, p->rows * across / 1024 / 4 * 4)));
+  b.down = static_cast<int>((p->rows + b.rows - 1) / b.rows);
   b.dz = b.make_dz ? round16(static_cast<size_t>(p->rows) * b.ld * es) : 0;
   b.parts = bias ? round16(static_cast<size_t>(b.down) * p->outputs * sizeof(float)) : 0;
-  b.product = std::max(gemm_plan(p->rows, p->inputs, p->outputs, es).part, gemm_plan(p->outputs, p->inputs, p->rows, es).part);
+  b.product = std::max(input_plan(p).part, weight_plan(p).part);
   return b;
 }
 
@@ -510,13 +633,13 @@ static int check_linear(const gs_linear* p, bool backward) {
              GS_ERR_ARG, "linear: %d inputs and %d outputs: 1 to %d are provided", p->inputs, p->outputs, GS_LINEAR_MAX_WIDTH);
   const size_t es = row_type_bytes(p->dtype);
   const int per = static_cast<int>(16 / es);
-  GS_REQUIRE(p->inputs % per == 0, GS_ERR_ALIGN, "linear: inputs must be a multiple of %d", per);
   GS_REQUIRE(p->rows == 0 || (p->x && p->weight && (backward || p->out)), GS_ERR_ARG, "linear: null pointer");
-  for (const int64_t s : {p->x_stride, p->weight_stride})
-    GS_REQUIRE(s >= 0 && s % per == 0 && s < GS_LINEAR_MAX_STRIDE, GS_ERR_ALIGN,
-               "linear: row strides must be multiples of 16 bytes below %d elements", GS_LINEAR_MAX_STRIDE);
   const size_t os = row_type_bytes(p->out_dtype);
-  GS_REQUIRE(aligned(p->x, 16) && aligned(p->weight, 16) && aligned(p->z, row_type_bytes(p->z_dtype)) &&
+  const bool few = !backward && p->rows <= kFewRows;  // rows are read at any address and stride
+  for (const int64_t s : {p->x_stride, p->weight_stride})
+    GS_REQUIRE(s >= 0 && s < GS_LINEAR_MAX_STRIDE && (few || s % per == 0), GS_ERR_ALIGN,
+               "linear: row strides must be multiples of 16 bytes below %d elements", GS_LINEAR_MAX_STRIDE);
+  GS_REQUIRE(aligned(p->x, few ? es : 16) && aligned(p->weight, few ? es : 16) && aligned(p->z, row_type_bytes(p->z_dtype)) &&
                  aligned(p->bias, row_type_bytes(p->bias_dtype)) && aligned(p->residual, os) && aligned(p->out, os),
              GS_ERR_ALIGN, "linear: misaligned tensor (x and weight: 16 bytes)");
   // grids of a dimension below 2^32 threads; results indexed below 2^62
@@ -530,10 +653,32 @@ static int check_linear(const gs_linear* p, bool backward) {
 
 using namespace gs;
 
+extern "C" int gs_rows_pack(const void* src, int64_t rows, int64_t cols, int64_t stride, void* dst, int64_t dst_stride,
+                            int dtype, void* stream) {
+  clear_error();
+  GS_REQUIRE(row_type(dtype), GS_ERR_ARG, "row pack: dtype must be GS_FLOAT32 or GS_BFLOAT16");
+  GS_REQUIRE(rows >= 0 && cols >= 0 && dst_stride >= cols && dst_stride % 8 == 0, GS_ERR_ARG, "row pack: invalid size");
+  const int64_t vecs = dst_stride / 8;
+  GS_REQUIRE(rows < (int64_t(1) << 32) && vecs < (int64_t(1) << 31) && rows * vecs < (int64_t(1) << 32) - kFinishThreads,
+             GS_ERR_ARG, "row pack: too many elements");
+  GS_REQUIRE(rows * vecs == 0 || (src && dst), GS_ERR_ARG, "row pack: null pointer");
+  GS_REQUIRE(aligned(src, row_type_bytes(dtype)) && aligned(dst, 16), GS_ERR_ALIGN, "row pack: misaligned tensor");
+  if (rows * vecs == 0) return GS_OK;
+  const dim3 grid(static_cast<unsigned>((rows * vecs + kFinishThreads - 1) / kFinishThreads)), block(kFinishThreads);
+  if (dtype == GS_BFLOAT16) {
+    hipLaunchKernelGGL(pack_kernel<__bf16>, grid, block, 0, as_stream(stream), static_cast<const __bf16*>(src), rows, cols,
+                       stride, static_cast<__bf16*>(dst), static_cast<int>(vecs));
+  } else {
+    hipLaunchKernelGGL(pack_kernel<float>, grid, block, 0, as_stream(stream), static_cast<const float*>(src), rows, cols,
+                       stride, static_cast<float*>(dst), static_cast<int>(vecs));
+  }
+  return check_launch("row pack");
+}
+
 extern "C" size_t gs_linear_fwd_workspace_size(const gs_linear* p) {
   clear_error();
   if (!p || p->rows <= kFewRows || p->inputs <= 0 || p->outputs <= 0 || !row_type(p->dtype)) return 0;
-  return gemm_plan(p->rows, p->outputs, p->inputs, row_type_bytes(p->dtype)).part;
+  return forward_plan(p).part;
 }
 
 extern "C" int gs_linear_fwd(const gs_linear* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -560,8 +705,8 @@ extern "C" int gs_linear_fwd(const gs_linear* p, void* workspace, size_t workspa
   g.out = p->out;
   g.z = p->z;
   g.z_bf16 = p->z_dtype == GS_BFLOAT16;
-  return p->dtype == GS_BFLOAT16 ? run_forward<__bf16>(g, workspace, as_stream(stream))
-                                 : run_forward<float>(g, workspace, as_stream(stream));
+  return p->dtype == GS_BFLOAT16 ? run_forward<__bf16>(p, g, workspace, as_stream(stream))
+                                 : run_forward<float>(p, g, workspace, as_stream(stream));
 }
 
 extern "C" size_t gs_linear_bwd_workspace_size(const gs_linear* p) {
@@ -580,7 +725,7 @@ static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* 
   void* product = ws + b.dz + b.parts;
   const bool make_dz = b.make_dz && (d_x || d_weight);
   if ((make_dz || d_bias) && p->rows > 0) {
-    const SlopeArgs s = {d_out, p->z, make_dz ? ws : nullptr, d_bias ? parts : nullptr, p->rows, b.ld, p->outputs, p->activation,
+    const SlopeArgs s = {d_out, p->z, make_dz ? ws : nullptr, d_bias ? parts : nullptr, p->rows, b.ld, p->outputs, p->activation, b.rows,
                          p->z_dtype == GS_BFLOAT16};
     const dim3 grid(b.down, (p->outputs + kWave * 8 - 1) / (kWave * 8)), block(kSlopeThreads);
     if (p->out_dtype == GS_FLOAT32) hipLaunchKernelGGL((slope_kernel<T, float>), grid, block, 0, st, s);
@@ -610,7 +755,7 @@ static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* 
     g.n = p->inputs;
     g.k = p->outputs;
     g.out = d_x;
-    if (const int rc = run_gemm<T, true, false>(g, product, "linear backward (input)", st)) return rc;
+    if (const int rc = run_gemm<T, true, false>(g, input_plan(p), product, "linear backward (input)", st)) return rc;
   }
   if (d_weight) {
     g.a = dz;
@@ -621,7 +766,7 @@ static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* 
     g.n = p->inputs;
     g.k = p->rows;
     g.out = d_weight;
-    if (const int rc = run_gemm<T, false, false>(g, product, "linear backward (weight)", st)) return rc;
+    if (const int rc = run_gemm<T, false, false>(g, weight_plan(p), product, "linear backward (weight)", st)) return rc;
   }
   return GS_OK;
 }

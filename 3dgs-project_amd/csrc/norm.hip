@@ -125,17 +125,20 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
   const int64_t row = mine ? row_at : a.rows - 1;
   float h[NV][8], b[NV][8];
   int left[NV];
-  const X* x = static_cast<const X*>(a.x) + row * a.x_stride;
+  Raw8<X> rx[NV];
+  Raw8<Y> ry[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = 8 * (lane + G * i);
     left[i] = a.width - col;
-    load8(x + col, left[i], h[i]);
+    rx[i].load(static_cast<const X*>(a.x) + row * a.x_stride + col, left[i]);
+    if (a.y) ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, left[i]);
   }
-  if (a.y) {
-    const Y* y = static_cast<const Y*>(a.y) + row * a.y_stride;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8(y + 8 * (lane + G * i), left[i], b[i]);
+  for (int i = 0; i < NV; ++i) rx[i].to(h[i]);
+  if (a.y) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) ry[i].to(b[i]);
     float2 st = {0.0f, 1.0f};
     if (a.post) st = row_stats(a, b, left, sum);
     if (mine && lane == 0 && a.stats) {
@@ -203,13 +206,22 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
     const bool mine = row_at < a.rows;
     const int64_t row = mine ? row_at : a.rows - 1;
     float hat[NV][8], t[NV][8], d[NV][8], b[NV][8], u[NV][8], keep[NV][8];
+    Raw8<X> rx[NV], rdh[NV];
+    Raw8<Y> ry[NV], rdn[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
-      load8(static_cast<const X*>(a.x) + row * a.x_stride + col, n, hat[i]);
-      if (a.y) load8(static_cast<const Y*>(a.y) + row * a.y_stride + col, n, b[i]);
-      load8(static_cast<const Y*>(a.d_n) + row * a.width + col, a.d_n ? n : 0, t[i]);
-      load8(static_cast<const X*>(a.d_h) + row * a.width + col, a.d_h ? n : 0, d[i]);
+      rx[i].load(static_cast<const X*>(a.x) + row * a.x_stride + col, n);
+      ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, a.y ? n : 0);
+      rdn[i].load(static_cast<const Y*>(a.d_n) + row * a.width + col, a.d_n ? n : 0);
+      rdh[i].load(static_cast<const X*>(a.d_h) + row * a.width + col, a.d_h ? n : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      rx[i].to(hat[i]);
+      ry[i].to(b[i]);
+      rdn[i].to(t[i]);
+      rdh[i].to(d[i]);
     }
     const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
     float s1 = 0.0f, s2 = 0.0f;

@@ -52,18 +52,13 @@ struct ScanArgs {
   float* d_initial;
 };
 
-// Elements p[0 .. n) of four as float, the others zero.
+template <typename T>
+using Raw4 = RawN<T, 4>;
 template <typename T>
 __device__ __forceinline__ void load4(const T* p, int n, float (&v)[4]) {
-  typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  if (n >= 4) {
-    const Vec a = *reinterpret_cast<const Vec*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(a[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = j < n ? static_cast<float>(p[j]) : 0.0f;
-  }
+  Raw4<T> r;
+  r.load(p, n);
+  r.to(v);
 }
 template <typename T>
 __device__ __forceinline__ void put4(T* p, int n, const float (&v)[4]) {
@@ -181,14 +176,17 @@ struct Channels {
       : at((blockIdx.x * kWave + threadIdx.x % kWave) * kScanVec), n(a.width - at) {}
 };
 
-// Rows of tokens k0 .. k0 + 7 of a chunk; rows outside documents are zero.
+// Rows of the tokens at places p0 .. p0 + 7, whatever they belong to (so that no load waits for the documents); past the last
+// token zeros.
 template <typename T>
-__device__ __forceinline__ void load_batch(const ScanArgs& a, const void* p, int64_t stride, const Places& pl, int64_t p0,
-                                           int k0, const Channels& c, float (&v)[kScanBatch][4]) {
+struct Batch {
+  Raw4<T> row[kScanBatch];
+  __device__ __forceinline__ void load(const ScanArgs& a, const void* p, int64_t stride, int64_t p0, const Channels& c) {
 #pragma unroll
-  for (int k = 0; k < kScanBatch; ++k)
-    load4(static_cast<const T*>(p) + token_at(a, p0 + k0 + k) * stride + c.at, (pl.inside >> (k0 + k)) & 1 ? c.n : 0, v[k]);
-}
+    for (int k = 0; k < kScanBatch; ++k)
+      row[k].load(static_cast<const T*>(p) + token_at(a, p0 + k) * stride + c.at, p0 + k < a.tokens ? c.n : 0);
+  }
+};
 template <typename T>
 __device__ __forceinline__ void put_row(T* p, const Channels& c, const float (&v)[4]) {
   if (c.n > 0) put4(p + c.at, c.n, v);
@@ -217,14 +215,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
 #pragma unroll
       for (int b = 0; b < kScanChunk / kScanBatch; ++b) {
         const int k0 = (BACK ? kScanChunk / kScanBatch - 1 - b : b) * kScanBatch;
-        float vf[kScanBatch][4], vx[kScanBatch][4], vo[kScanBatch][4];
-        load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
-        if constexpr (BACK) {
-          load_batch<T>(a, a.d_y, a.width, pl, p0, k0, c, vx);
-          if (a.o) load_batch<T>(a, a.o, a.o_stride, pl, p0, k0, c, vo);
-        } else {
-          load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
-        }
+        Batch<T> bf, bx, bo;
+        bf.load(a, a.f, a.f_stride, p0 + k0, c);
+        bx.load(a, BACK ? a.d_y : a.x, BACK ? a.width : a.x_stride, p0 + k0, c);
+        if (BACK && a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
 #pragma unroll
         for (int i = 0; i < kScanBatch; ++i) {
           const int k = BACK ? k0 + kScanBatch - 1 - i : k0 + i, r = k - k0;
@@ -235,11 +229,19 @@ __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j].drop();
           }
+          float vf[4], vx[4], vo[4];
+          bf.row[r].to(vf);
+          bx.row[r].to(vx);
+          if (BACK && a.o) {
+            bo.row[r].to(vo);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vx[j] *= vo[j] * Sigmoid(vo[j]).value();
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const Sigmoid s(vf[r][j]);
-            if constexpr (BACK) e[j] = s.times(e[j] + (a.o ? vx[r][j] * (vo[r][j] * Sigmoid(vo[r][j]).value()) : vx[r][j]));
-            else e[j] = s.step(e[j], vx[r][j]);
+            const Sigmoid s(vf[j]);
+            if constexpr (BACK) e[j] = s.times(e[j] + vx[j]);
+            else e[j] = s.step(e[j], vx[j]);
             f[j].by(s);
           }
         }
@@ -310,13 +312,16 @@ __device__ __forceinline__ void state_before(const ScanArgs& a, int n, const Cha
 // Documents without tokens: their state goes through as it is, and so does its gradient.
 __device__ __forceinline__ void pass_empty(const ScanArgs& a, const Channels& c, const float* from, float* to) {
   if (to == nullptr) return;
-  const int waves = blockDim.x / kWave;
-  for (int d = blockIdx.y * waves + threadIdx.x / kWave; d < a.docs; d += gridDim.y * waves) {
-    if (scan_edge(a, d) < scan_edge(a, d + 1)) continue;
-    float v[4];
-    const int64_t at = static_cast<int64_t>(doc_at(a, d)) * a.width;
-    load4(from + at + c.at, from ? c.n : 0, v);
-    put_row(to + at, c, v);
+  const int waves = blockDim.x / kWave, lane = threadIdx.x % kWave;
+  for (int d0 = (blockIdx.y * waves + threadIdx.x / kWave) * kWave; d0 < a.docs; d0 += gridDim.y * waves * kWave) {
+    const int d = min(d0 + lane, a.docs - 1);
+    uint64_t empty = __ballot(d0 + lane < a.docs && scan_edge(a, d) >= scan_edge(a, d + 1));
+    for (; empty; empty &= empty - 1) {
+      const int64_t at = static_cast<int64_t>(doc_at(a, d0 + __builtin_ctzll(empty))) * a.width;
+      float v[4];
+      load4(from + at + c.at, from ? c.n : 0, v);
+      put_row(to + at, c, v);
+    }
   }
 }
 
@@ -342,15 +347,16 @@ __global__ __launch_bounds__(kScanThreads) void scan_apply_kernel(ScanArgs a) {
 #pragma unroll
     for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
       if (p0 + k0 >= a.tokens) break;
-      float vf[kScanBatch][4], vx[kScanBatch][4], vo[kScanBatch][4], first[kScanBatch][4];
-      load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
-      load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
-      if (a.o) load_batch<T>(a, a.o, a.o_stride, pl, p0, k0, c, vo);
+      Batch<T> bf, bx, bo;
+      bf.load(a, a.f, a.f_stride, p0 + k0, c);
+      bx.load(a, a.x, a.x_stride, p0 + k0, c);
+      if (a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
+      Raw4<float> first[kScanBatch];
       if ((pl.first >> k0) & ((1u << kScanBatch) - 1)) {
 #pragma unroll
         for (int k = 0; k < kScanBatch; ++k)
           if ((pl.first >> (k0 + k)) & 1)
-            load4(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0, first[k]);
+            first[k].load(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0);
       }
 #pragma unroll
       for (int k = 0; k < kScanBatch; ++k) {
@@ -358,11 +364,16 @@ __global__ __launch_bounds__(kScanThreads) void scan_apply_kernel(ScanArgs a) {
         if (p >= a.tokens) break;
         float y[4] = {};
         if ((pl.inside >> (k0 + k)) & 1) {
-          const bool fresh = (pl.first >> (k0 + k)) & 1;
+          if ((pl.first >> (k0 + k)) & 1) first[k].to(h);
+          float vf[4], vx[4], vo[4];
+          bf.row[k].to(vf);
+          bx.row[k].to(vx);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            h[j] = Sigmoid(vf[k][j]).step(fresh ? first[k][j] : h[j], vx[k][j]);
-            y[j] = a.o ? h[j] * (vo[k][j] * Sigmoid(vo[k][j]).value()) : h[j];
+          for (int j = 0; j < 4; ++j) y[j] = h[j] = Sigmoid(vf[j]).step(h[j], vx[j]);
+          if (a.o) {
+            bo.row[k].to(vo);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] *= vo[j] * Sigmoid(vo[j]).value();
           }
           if (a.state && ((pl.last >> (k0 + k)) & 1)) put_row(a.state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width, c, h);
         }
@@ -393,27 +404,30 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
     load4(a.carry + static_cast<int64_t>(chunk) * a.width + c.at, c.n, h);
 #pragma unroll
     for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
-      float vf[kScanBatch][4], vx[kScanBatch][4];
-      load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
-      load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
+      Batch<T> bf, bx;
+      bf.load(a, a.f, a.f_stride, p0 + k0, c);
+      bx.load(a, a.x, a.x_stride, p0 + k0, c);
 #pragma unroll
       for (int k = 0; k < kScanBatch; ++k) {
         if ((pl.first >> (k0 + k)) & 1)
           load4(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0, h);
+        float vf[4], vx[4];
+        bf.row[k].to(vf);
+        bx.row[k].to(vx);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           before[k0 + k][j] = h[j];
-          h[j] = Sigmoid(vf[k][j]).step(h[j], vx[k][j]);
+          h[j] = Sigmoid(vf[j]).step(h[j], vx[j]);
         }
       }
     }
 #pragma unroll
     for (int k0 = kScanChunk - kScanBatch; k0 >= 0; k0 -= kScanBatch) {
-      float vf[kScanBatch][4], vx[kScanBatch][4], vo[kScanBatch][4], vd[kScanBatch][4];
-      load_batch<T>(a, a.d_y, a.width, pl, p0, k0, c, vd);
-      if (a.o) load_batch<T>(a, a.o, a.o_stride, pl, p0, k0, c, vo);
-      load_batch<T>(a, a.f, a.f_stride, pl, p0, k0, c, vf);
-      load_batch<T>(a, a.x, a.x_stride, pl, p0, k0, c, vx);
+      Batch<T> bd, bo, bf, bx;
+      bd.load(a, a.d_y, a.width, p0 + k0, c);
+      if (a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
+      bf.load(a, a.f, a.f_stride, p0 + k0, c);
+      bx.load(a, a.x, a.x_stride, p0 + k0, c);
 #pragma unroll
       for (int k = kScanBatch - 1; k >= 0; --k) {
         const int64_t p = p0 + k0 + k;
@@ -422,20 +436,25 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
         if ((pl.inside >> (k0 + k)) & 1) {
           if ((pl.last >> (k0 + k)) & 1)
             load4(a.d_state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.d_state ? c.n : 0, l);
+          float vf[4], vx[4], vo[4], vd[4];
+          bf.row[k].to(vf);
+          bx.row[k].to(vx);
+          bd.row[k].to(vd);
+          if (a.o) bo.row[k].to(vo);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const Sigmoid s(vf[k][j]);
+            const Sigmoid s(vf[j]);
             const float was = before[k0 + k][j];
-            float d = vd[k][j];
+            float d = vd[j];
             if (a.o) {
-              const Sigmoid g(vo[k][j]);
-              const float open = vo[k][j] * g.value();
-              dg[j] = d * s.step(was, vx[k][j]) * fmaf(vo[k][j], g.large * g.small, g.value());
+              const Sigmoid g(vo[j]);
+              const float open = vo[j] * g.value();
+              dg[j] = d * s.step(was, vx[j]) * fmaf(vo[j], g.large * g.small, g.value());
               d *= open;
             }
             const float whole = d + l[j];
             dx[j] = whole * s.rest();
-            df[j] = whole * (was - vx[k][j]) * (s.large * s.small);
+            df[j] = whole * (was - vx[j]) * (s.large * s.small);
             l[j] = s.times(whole);
           }
           if (a.d_initial && ((pl.first >> (k0 + k)) & 1))

@@ -745,8 +745,9 @@ int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d
 
 /* ---------------------------------------------------------------------------------------
  * out [rows, outputs] = act(x weight^T + bias) + residual, x [rows, inputs] and weight [outputs, inputs] of dtype, read
- * through row strides (multiples of 16 bytes below GS_LINEAR_MAX_STRIDE elements, pointers 16-byte aligned, inputs a multiple
- * of 16 bytes; rows of a stride of 0 are one row). bias [outputs] of bias_dtype and residual [rows, outputs] of out_dtype (row
+ * through row strides (multiples of 16 bytes below GS_LINEAR_MAX_STRIDE elements, pointers 16-byte aligned; a stride of 0
+ * repeats one row). Where inputs is no multiple of 16 bytes, rows go on to the next one with zeros (gs_rows_pack makes such rows). A
+ * forward of up to GS_LINEAR_FEW_ROWS rows reads x and weight at any element's address and row stride, and no further than inputs. bias [outputs] of bias_dtype and residual [rows, outputs] of out_dtype (row
  * stride residual_stride) may be NULL. out is of out_dtype: dtype, or GS_FLOAT32 for bfloat16 products. Products and the
  * epilogue are float32, rounded once. z (of z_dtype: GS_FLOAT32, or dtype; may be NULL): x weight^T + bias, for the backward
  * of an activation, whose slopes are taken there (a float32 d_bias needs a float32 z).
@@ -759,6 +760,7 @@ int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d
  * ------------------------------------------------------------------------------------- */
 #define GS_LINEAR_MAX_WIDTH (1 << 19)
 #define GS_LINEAR_MAX_STRIDE (1 << 20)
+#define GS_LINEAR_FEW_ROWS 32
 #define GS_ACT_NONE 0
 #define GS_ACT_RELU 1
 #define GS_ACT_GELU 2
@@ -770,6 +772,10 @@ typedef struct gs_linear {
   int64_t rows, x_stride, weight_stride, residual_stride;
   int32_t inputs, outputs, dtype, out_dtype, z_dtype, bias_dtype, activation;
 } gs_linear;
+/* Copies rows [rows, cols] of a row stride (elements) to 16-byte aligned rows of dst_stride elements (a multiple of eight, at
+ * least cols), zeros behind them. */
+int gs_rows_pack(const void* src, int64_t rows, int64_t cols, int64_t stride, void* dst, int64_t dst_stride, int dtype,
+                 void* stream);
 size_t gs_linear_fwd_workspace_size(const gs_linear* args);
 int gs_linear_fwd(const gs_linear* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t gs_linear_bwd_workspace_size(const gs_linear* args);

@@ -151,6 +151,18 @@ def test_linear_arguments(kw, code, text):
 
 def test_linear_calls():
     L = _lib.lib()
+    # few rows are read at any address, but for gradients
+    expect(L.gs_linear_fwd(C.byref(linear_args(rows=32, x=260, x_stride=65, weight=258)), None, 0, None), ALIGN, "misaligned")
+    expect(L.gs_linear_bwd(C.byref(linear_args(rows=32, x=260)), 256, 256, 256, 256, 256, 1 << 62, None), ALIGN, "misaligned")
+    pack = lambda src=256, rows=4, cols=60, dst=256, ld=64, dtype=0: L.gs_rows_pack(src, rows, cols, 70, dst, ld, dtype, None)  # noqa: E731
+    expect(pack(dtype=1), ARG, "dtype")
+    expect(pack(rows=-1), ARG, "size")
+    expect(pack(ld=60), ARG, "size")
+    expect(pack(ld=56), ARG, "size")
+    expect(pack(src=None), ARG, "null")
+    expect(pack(dst=264), ALIGN, "misaligned")
+    expect(pack(src=258), ALIGN, "misaligned")
+    expect(pack(rows=1 << 31, ld=1 << 10), ARG, "too many")
     a = linear_args()
     need = L.gs_linear_bwd_workspace_size(C.byref(a))
     assert need > 0 and L.gs_linear_bwd_workspace_size(None) == 0 and L.gs_linear_fwd_workspace_size(None) == 0
