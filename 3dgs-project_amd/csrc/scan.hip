@@ -6,8 +6,8 @@
 //
 // A step is the map h -> E + P h, and maps compose, so the tokens are cut into chunks of 16 that a wavefront walks, a
 // lane holding four channels: scan_sums_kernel forms every chunk's map and, in LDS, the maps from the start of
-// a part (some chunks of one workgroup) to each of its chunks; scan_apply_kernel joins the parts before its own, which gives every
-// chunk its state, and walks the tokens again with it. The inputs are so read twice, the second time from the last-level
+// a part (the chunks of one workgroup) to each of its chunks; scan_parts_kernel joins the parts; scan_apply_kernel has so every
+// chunk's state, and walks the tokens again with it. The inputs are so read twice, the second time from the last-level
 // cache as far as it holds them. (One pass that waits for the workgroups before it would read them once, but
 // needs them to be running; nothing here waits for another workgroup.)
 //
@@ -17,8 +17,9 @@
 // Accuracy: long memories have a near 1, where 1 - a is what counts. The smaller of a and 1 - a is formed
 // directly, s = e / (1 + e) with e = exp(-|f|), and steps are taken as h + s (x - h) or x + s (h - x). A chunk's P is
 // kept as 1 - P while that is the smaller one; a chunk's sum starts at zero, so its rounding is relative to what
-// the chunk adds; chunks are joined in float64. Rounding so does not pile up over the length of the sequence.
+// the chunk adds; chunks and parts are joined in float64. Rounding so does not pile up over the length of the sequence.
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_attention.h"
 #include "gs_rows.h"
@@ -28,9 +29,10 @@ namespace gs {
 constexpr int kScanChunk = 16;                           // tokens of a chunk
 constexpr int kScanWaves = 8;
 constexpr int kScanThreads = kScanWaves * kWave;
+constexpr int kWalkWaves = 4;                            // of a workgroup where every wavefront has a chunk
 constexpr int kScanVec = 4;                              // channels of a lane
 constexpr int kScanGroup = kWave * kScanVec;             // channels of a workgroup
-constexpr int kScanParts = 256;
+constexpr int kScanParts = 512;
 constexpr int kScanBatch = 8;                            // tokens whose loads are in flight together
 
 struct ScanArgs {
@@ -41,10 +43,12 @@ struct ScanArgs {
   const int32_t* offsets;
   int64_t tokens, x_stride, f_stride, o_stride;
   int docs, width, reverse;
+  int groups;                 // of kScanGroup channels
   int chunks, parts, blocks;  // blocks: of a part
   int serial;                 // one wavefront walks all chunks
   float2* prefix;             // [chunks][width]: the map from the part's start to the chunk
-  double2* part;              // [parts][width]: the map of a part
+  float2* part;               // [parts][width]: the map of a part
+  float* before;              // [parts][width]: the state that a part starts with
   // backward
   const void* d_y;
   const float* d_state;
@@ -54,12 +58,6 @@ struct ScanArgs {
 
 template <typename T>
 using Raw4 = RawN<T, 4>;
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, int n, float (&v)[4]) {
-  Raw4<T> r;
-  r.load(p, n);
-  r.to(v);
-}
 template <typename T>
 __device__ __forceinline__ void put4(T* p, int n, const float (&v)[4]) {
   typedef T Vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -98,9 +96,8 @@ struct Sigmoid {
 struct Factor {
   float p = 1.0f, q = 0.0f;
   __device__ __forceinline__ void by(const Sigmoid& a) {
-    const float rest = 1.0f - q;
-    q = a.up ? fmaf(a.small, rest, q) : fmaf(-a.small, rest, 1.0f);
-    p *= a.up ? 1.0f - a.small : a.small;
+    p *= a.value();
+    q = fmaf(a.rest(), 1.0f - q, q);
   }
   __device__ __forceinline__ void drop() {
     p = 0.0f;
@@ -169,36 +166,54 @@ struct Places {
   __device__ __forceinline__ int doc_of(int k) const { return __builtin_amdgcn_readlane(doc, k); }
 };
 
-// A lane's channels.
+// A lane's four channels. Lanes past the width, and the last one where the width is no multiple of four, take the last four
+// channels: what two lanes hold alike they also write alike, and no access needs a branch. Only rows of fewer than
+// four channels (SMALL) are read and written element by element. at_of: the channels' place in a row whose address is the same for
+// all lanes, which takes scalar registers and 32 bits of the lane's.
+template <bool SMALL>
 struct Channels {
   int at, n;
-  __device__ __forceinline__ explicit Channels(const ScanArgs& a)
-      : at((blockIdx.x * kWave + threadIdx.x % kWave) * kScanVec), n(a.width - at) {}
+  __device__ __forceinline__ Channels(const ScanArgs& a, int group)
+      : at(SMALL ? 0 : min((group * kWave + static_cast<int>(threadIdx.x % kWave)) * kScanVec, a.width - kScanVec)),
+        n(SMALL ? a.width : kScanVec) {}
+  template <typename T>
+  __device__ __forceinline__ T* at_of(T* row) const {
+    using Byte = std::conditional_t<std::is_const_v<T>, const char, char>;
+    return reinterpret_cast<T*>(reinterpret_cast<Byte*>(row) + static_cast<uint32_t>(at * static_cast<int>(sizeof(T))));
+  }
+  // Row `row` of a tensor of whole rows; a tensor that is not there is zero.
+  template <typename T>
+  __device__ __forceinline__ void load(const ScanArgs& a, const T* p, int64_t row, float (&v)[4]) const {
+    Raw4<T> r;
+    r.load(at_of(p + row * a.width), p ? (SMALL ? n : kScanVec) : 0);
+    r.to(v);
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* row, const float (&v)[4]) const {
+    put4(at_of(row), SMALL ? n : kScanVec, v);
+  }
 };
 
 // Rows of the tokens at places p0 .. p0 + 7, whatever they belong to (so that no load waits for the documents); past the last
-// token zeros.
-template <typename T>
+// token that one's again.
+template <typename T, bool SMALL>
 struct Batch {
   Raw4<T> row[kScanBatch];
-  __device__ __forceinline__ void load(const ScanArgs& a, const void* p, int64_t stride, int64_t p0, const Channels& c) {
+  __device__ __forceinline__ void load(const ScanArgs& a, const void* p, int64_t stride, int64_t p0, const Channels<SMALL>& c) {
 #pragma unroll
     for (int k = 0; k < kScanBatch; ++k)
-      row[k].load(static_cast<const T*>(p) + token_at(a, p0 + k) * stride + c.at, p0 + k < a.tokens ? c.n : 0);
+      row[k].load(c.at_of(static_cast<const T*>(p) + token_at(a, min<int64_t>(p0 + k, a.tokens - 1)) * stride),
+                  SMALL ? c.n : kScanVec);
   }
 };
-template <typename T>
-__device__ __forceinline__ void put_row(T* p, const Channels& c, const float (&v)[4]) {
-  if (c.n > 0) put4(p + c.at, c.n, v);
-}
 
 // ---- the maps of chunks and parts --------------------------------------------------------------------
 // BACK: of l, whose walk starts at a chunk's last token.
 
-template <typename T, bool BACK>
+template <typename T, bool BACK, bool SMALL>
 __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
   __shared__ float2 maps[kScanWaves][kScanGroup];
-  const Channels c(a);
+  const Channels<SMALL> c(a, blockIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   // the running map of the part, of one channel a thread (the first four wavefronts)
   double e_run = 0.0, p_run = 1.0;
@@ -215,7 +230,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
 #pragma unroll
       for (int b = 0; b < kScanChunk / kScanBatch; ++b) {
         const int k0 = (BACK ? kScanChunk / kScanBatch - 1 - b : b) * kScanBatch;
-        Batch<T> bf, bx, bo;
+        Batch<T, SMALL> bf, bx, bo;
         bf.load(a, a.f, a.f_stride, p0 + k0, c);
         bx.load(a, BACK ? a.d_y : a.x, BACK ? a.width : a.x_stride, p0 + k0, c);
         if (BACK && a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
@@ -225,7 +240,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
           if (!((pl.inside >> k) & 1)) continue;
           if (((BACK ? pl.last : pl.first) >> k) & 1) {
             const float* from = BACK ? a.d_state : a.initial;
-            load4(from + static_cast<int64_t>(pl.doc_of(k)) * a.width + c.at, from ? c.n : 0, e);
+            c.load(a, from, pl.doc_of(k), e);
 #pragma unroll
             for (int j = 0; j < 4; ++j) f[j].drop();
           }
@@ -249,7 +264,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) maps[wave][(threadIdx.x % kWave) * kScanVec + j] = make_float2(e[j], packed(f[j].p, f[j].q));
+    for (int j = 0; j < 4; ++j) {
+      const int ch = c.at + j - static_cast<int>(blockIdx.x) * kScanGroup;  // (the last four may begin in the group before)
+      if (ch >= 0) maps[wave][ch] = make_float2(e[j], packed(f[j].p, f[j].q));
+    }
     __syncthreads();
     if (threadIdx.x < kScanGroup && own < a.width) {
       for (int w = 0; w < kScanWaves && n0 + w < a.chunks; ++w) {
@@ -262,92 +280,97 @@ __global__ __launch_bounds__(kScanThreads) void scan_sums_kernel(ScanArgs a) {
     }
   }
   if (a.parts > 1 && threadIdx.x < kScanGroup && own < a.width)
-    a.part[static_cast<int64_t>(blockIdx.y) * a.width + own] = make_double2(e_run, p_run);
+    a.part[static_cast<int64_t>(blockIdx.y) * a.width + own] = make_float2(static_cast<float>(e_run), packed(p_run));
 }
 
-// The map of all parts before `part`, of zero: the state that a part starts with. A wavefront joins an eighth of them;
-// the result is in LDS for the workgroup's channels.
-struct PartState {
-  double2 maps[kScanWaves][kScanGroup];
-  double state[kScanGroup];
-};
-__device__ __forceinline__ void join_parts(const ScanArgs& a, int part, PartState& s) {
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int per = (part + kScanWaves - 1) / kScanWaves;
-  const int from = min(wave * per, part), to = min(from + per, part);
+// The state that every part starts with: the maps of the parts before it, joined. 32 lanes have a channel each, and 32 runs of
+// parts are joined side by side, first to the runs' own maps and then, from what comes before a run, part by part.
+constexpr int kRuns = 32, kRunParts = kScanParts / kRuns, kJoinThreads = kRuns * 32;
+__global__ __launch_bounds__(kJoinThreads) void scan_parts_kernel(ScanArgs a) {
+  __shared__ double2 maps[kRuns][32];
+  const int lane = threadIdx.x % 32, run = threadIdx.x / 32, ch = blockIdx.x * 32 + lane, first = run * kRunParts;
+  float2 m[kRunParts];
 #pragma unroll
-  for (int j = 0; j < kScanVec; ++j) {
-    const int ch = lane + j * kWave, at = blockIdx.x * kScanGroup + ch;
-    double e = 0.0, p = 1.0;
-    if (at < a.width) {
-#pragma unroll 4
-      for (int i = from; i < to; ++i) {
-        const double2 m = a.part[static_cast<int64_t>(i) * a.width + at];
-        e = mapped(m.x, m.y, e);
-        p = m.y == 0.0 ? 0.0 : p * m.y;
-      }
-    }
-    s.maps[wave][ch] = make_double2(e, p);
+  for (int i = 0; i < kRunParts; ++i)
+    m[i] = ch < a.width && first + i < a.parts ? a.part[static_cast<int64_t>(first + i) * a.width + ch] : make_float2(0.0f, 0.0f);
+  double e = 0.0, p = 1.0;
+#pragma unroll
+  for (int i = 0; i < kRunParts; ++i) {
+    const double f = factor_of(m[i].y);
+    e = mapped(m[i].x, f, e);
+    p = f == 0.0 ? 0.0 : p * f;
   }
+  maps[run][lane] = make_double2(e, p);
   __syncthreads();
-  if (threadIdx.x < kScanGroup) {
-    double h = 0.0;
-    for (int w = 0; w < kScanWaves; ++w) h = mapped(s.maps[w][threadIdx.x].x, s.maps[w][threadIdx.x].y, h);
-    s.state[threadIdx.x] = h;
+  double h = 0.0;
+  for (int r = 0; r < run; ++r) h = mapped(maps[r][lane].x, maps[r][lane].y, h);
+  if (ch >= a.width) return;
+#pragma unroll
+  for (int i = 0; i < kRunParts; ++i) {
+    if (first + i < a.parts) a.before[static_cast<int64_t>(first + i) * a.width + ch] = static_cast<float>(h);
+    h = mapped(m[i].x, factor_of(m[i].y), h);
   }
-  __syncthreads();
 }
 
 // The state that chunk n (in walking order) starts with.
-__device__ __forceinline__ void state_before(const ScanArgs& a, int n, const Channels& c, const PartState& s, float (&h)[4]) {
+template <bool SMALL>
+__device__ __forceinline__ void state_before(const ScanArgs& a, int n, const Channels<SMALL>& c, float (&h)[4]) {
+  float from[4];
+  c.load(a, a.before, n / (a.blocks * kScanWaves), from);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (j >= c.n) continue;
+    if (SMALL && j >= c.n) continue;
     const float2 m = a.prefix[static_cast<int64_t>(n) * a.width + c.at + j];
-    const double from = a.parts > 1 ? s.state[(threadIdx.x % kWave) * kScanVec + j] : 0.0;
-    h[j] = static_cast<float>(mapped(m.x, factor_of(m.y), from));
+    h[j] = static_cast<float>(mapped(m.x, factor_of(m.y), from[j]));
   }
 }
 
 // Documents without tokens: their state goes through as it is, and so does its gradient.
-__device__ __forceinline__ void pass_empty(const ScanArgs& a, const Channels& c, const float* from, float* to) {
+template <bool SMALL>
+__device__ __forceinline__ void pass_empty(const ScanArgs& a, const Channels<SMALL>& c, const float* from, float* to) {
   if (to == nullptr) return;
-  const int waves = blockDim.x / kWave, lane = threadIdx.x % kWave;
-  for (int d0 = (blockIdx.y * waves + threadIdx.x / kWave) * kWave; d0 < a.docs; d0 += gridDim.y * waves * kWave) {
-    const int d = min(d0 + lane, a.docs - 1);
+  const int lane = threadIdx.x % kWave, waves = gridDim.x / a.groups * (blockDim.x / kWave);
+  for (int64_t d0 = (blockIdx.x / a.groups * (blockDim.x / kWave) + threadIdx.x / kWave) * int64_t(kWave); d0 < a.docs;
+       d0 += static_cast<int64_t>(waves) * kWave) {
+    const int d = static_cast<int>(min<int64_t>(d0 + lane, a.docs - 1));
     uint64_t empty = __ballot(d0 + lane < a.docs && scan_edge(a, d) >= scan_edge(a, d + 1));
     for (; empty; empty &= empty - 1) {
-      const int64_t at = static_cast<int64_t>(doc_at(a, d0 + __builtin_ctzll(empty))) * a.width;
+      const int64_t row = doc_at(a, static_cast<int>(d0) + __builtin_ctzll(empty));
       float v[4];
-      load4(from + at + c.at, from ? c.n : 0, v);
-      put_row(to + at, c, v);
+      c.load(a, from, row, v);
+      c.store(to + row * a.width, v);
     }
   }
 }
 
 // ---- the walk ----------------------------------------------------------------------------------------
 
-template <typename T>
-__global__ __launch_bounds__(kScanThreads) void scan_apply_kernel(ScanArgs a) {
-  __shared__ PartState join;
-  const Channels c(a);
-  // the last part first: what the sums' kernel read last is still in the cache
-  const int part = gridDim.y - 1 - blockIdx.y;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+// The chunks that a wavefront walks: one, or in serial mode all of them.
+struct Walk {
+  int first, end;
+  __device__ __forceinline__ explicit Walk(const ScanArgs& a) {
+    // the last ones first: what the sums' kernel read last is still in the cache
+    const int n = (gridDim.x - 1 - blockIdx.x) / a.groups * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    first = a.serial ? 0 : n;
+    end = a.serial ? a.chunks : min(n + 1, a.chunks);
+  }
+};
+
+template <typename T, bool SMALL>
+__global__ __launch_bounds__(kWalkWaves* kWave, 3) void scan_apply_kernel(ScanArgs a) {
+  const Channels<SMALL> c(a, blockIdx.x % a.groups);
   pass_empty(a, c, a.initial, a.state);
-  if (a.parts > 1) join_parts(a, part, join);
   float h[4] = {};
-  const int step = a.serial ? 1 : kScanWaves;
-  const int end = min((part + 1) * a.blocks * step, a.chunks);
-  for (int n = part * a.blocks * step + wave; n < end; n += step) {
+  const Walk w(a);
+  for (int n = w.first; n < w.end; ++n) {
     const int64_t p0 = static_cast<int64_t>(n) * kScanChunk;
-    if (!a.serial) state_before(a, n, c, join, h);
-    if (a.carry) put_row(a.carry + static_cast<int64_t>(n) * a.width, c, h);
+    if (!a.serial) state_before(a, n, c, h);
+    if (a.carry) c.store(a.carry + static_cast<int64_t>(n) * a.width, h);
     const Places pl(a, p0);
 #pragma unroll
     for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
       if (p0 + k0 >= a.tokens) break;
-      Batch<T> bf, bx, bo;
+      Batch<T, SMALL> bf, bx, bo;
       bf.load(a, a.f, a.f_stride, p0 + k0, c);
       bx.load(a, a.x, a.x_stride, p0 + k0, c);
       if (a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
@@ -356,7 +379,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_apply_kernel(ScanArgs a) {
 #pragma unroll
         for (int k = 0; k < kScanBatch; ++k)
           if ((pl.first >> (k0 + k)) & 1)
-            first[k].load(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0);
+            first[k].load(c.at_of(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width), a.initial ? (SMALL ? c.n : kScanVec) : 0);
       }
 #pragma unroll
       for (int k = 0; k < kScanBatch; ++k) {
@@ -375,67 +398,74 @@ __global__ __launch_bounds__(kScanThreads) void scan_apply_kernel(ScanArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] *= vo[j] * Sigmoid(vo[j]).value();
           }
-          if (a.state && ((pl.last >> (k0 + k)) & 1)) put_row(a.state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width, c, h);
+          if (a.state && ((pl.last >> (k0 + k)) & 1)) c.store(a.state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width, h);
         }
-        put_row(static_cast<T*>(a.y) + token_at(a, p) * a.width, c, y);
+        c.store(static_cast<T*>(a.y) + token_at(a, p) * a.width, y);
       }
     }
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
-  __shared__ PartState join;
-  const Channels c(a);
-  const int part = gridDim.y - 1 - blockIdx.y;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+// Eight tokens at a time from the chunk's end: the states before them are walked to from the chunk's start and held in
+// registers. (All sixteen at once took 235 registers and two wavefronts a SIMD: 32771 x 1024 175 us.)
+template <typename T, bool SMALL>
+__global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs a) {
+  const Channels<SMALL> c(a, blockIdx.x % a.groups);
   pass_empty(a, c, a.d_state, a.d_initial);
-  if (a.parts > 1) join_parts(a, part, join);
   float l[4] = {};  // a l of the token after
-  const int step = a.serial ? 1 : kScanWaves;
-  const int end = min((part + 1) * a.blocks * step, a.chunks);
-  for (int n = part * a.blocks * step + wave; n < end; n += step) {
+  const Walk w(a);
+  for (int n = w.first; n < w.end; ++n) {
     const int chunk = a.chunks - 1 - n;
-    const int64_t p0 = static_cast<int64_t>(chunk) * kScanChunk;
-    if (!a.serial) state_before(a, n, c, join, l);
-    const Places pl(a, p0);
-    // the states before each token
-    float before[kScanChunk][4], h[4];
-    load4(a.carry + static_cast<int64_t>(chunk) * a.width + c.at, c.n, h);
+    if (!a.serial) state_before(a, n, c, l);
+    const Places pl(a, static_cast<int64_t>(chunk) * kScanChunk);
+#pragma unroll 1
+    for (int half = kScanChunk / kScanBatch - 1; half >= 0; --half) {
+      const int64_t p0 = static_cast<int64_t>(chunk) * kScanChunk + half * kScanBatch;
+      const uint32_t inside = pl.inside >> (half * kScanBatch), first = pl.first >> (half * kScanBatch),
+                     last = pl.last >> (half * kScanBatch);
+      float before[kScanBatch][4], h[4];
+      c.load(a, a.carry, chunk, h);
+      const auto begin = [&](int k) {  // the state before token k of the chunk where it is a document's first
+        c.load(a, a.initial, pl.doc_of(k), h);
+      };
+      Batch<T, SMALL> bf, bx, bd, bo;
+      if (half) {
+        bf.load(a, a.f, a.f_stride, p0 - kScanBatch, c);
+        bx.load(a, a.x, a.x_stride, p0 - kScanBatch, c);
 #pragma unroll
-    for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
-      Batch<T> bf, bx;
-      bf.load(a, a.f, a.f_stride, p0 + k0, c);
-      bx.load(a, a.x, a.x_stride, p0 + k0, c);
+        for (int k = 0; k < kScanBatch; ++k) {
+          if ((pl.first >> k) & 1) begin(k);
+          float vf[4], vx[4];
+          bf.row[k].to(vf);
+          bx.row[k].to(vx);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) h[j] = Sigmoid(vf[j]).step(h[j], vx[j]);
+        }
+      }
+      bf.load(a, a.f, a.f_stride, p0, c);
+      bx.load(a, a.x, a.x_stride, p0, c);
+      bd.load(a, a.d_y, a.width, p0, c);
+      if (a.o) bo.load(a, a.o, a.o_stride, p0, c);
 #pragma unroll
       for (int k = 0; k < kScanBatch; ++k) {
-        if ((pl.first >> (k0 + k)) & 1)
-          load4(a.initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.initial ? c.n : 0, h);
+        if ((first >> k) & 1) begin(half * kScanBatch + k);
         float vf[4], vx[4];
         bf.row[k].to(vf);
         bx.row[k].to(vx);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          before[k0 + k][j] = h[j];
+          before[k][j] = h[j];
           h[j] = Sigmoid(vf[j]).step(h[j], vx[j]);
         }
       }
-    }
-#pragma unroll
-    for (int k0 = kScanChunk - kScanBatch; k0 >= 0; k0 -= kScanBatch) {
-      Batch<T> bd, bo, bf, bx;
-      bd.load(a, a.d_y, a.width, p0 + k0, c);
-      if (a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
-      bf.load(a, a.f, a.f_stride, p0 + k0, c);
-      bx.load(a, a.x, a.x_stride, p0 + k0, c);
 #pragma unroll
       for (int k = kScanBatch - 1; k >= 0; --k) {
-        const int64_t p = p0 + k0 + k;
+        const int64_t p = p0 + k;
         if (p >= a.tokens) continue;
         float dx[4] = {}, df[4] = {}, dg[4] = {};
-        if ((pl.inside >> (k0 + k)) & 1) {
-          if ((pl.last >> (k0 + k)) & 1)
-            load4(a.d_state + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width + c.at, a.d_state ? c.n : 0, l);
+        if ((inside >> k) & 1) {
+          if ((last >> k) & 1)
+            c.load(a, a.d_state, pl.doc_of(half * kScanBatch + k), l);
           float vf[4], vx[4], vo[4], vd[4];
           bf.row[k].to(vf);
           bx.row[k].to(vx);
@@ -444,7 +474,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const Sigmoid s(vf[j]);
-            const float was = before[k0 + k][j];
+            const float was = before[k][j];
             float d = vd[j];
             if (a.o) {
               const Sigmoid g(vo[j]);
@@ -457,13 +487,13 @@ __global__ __launch_bounds__(kScanThreads) void scan_bwd_kernel(ScanArgs a) {
             df[j] = whole * (was - vx[j]) * (s.large * s.small);
             l[j] = s.times(whole);
           }
-          if (a.d_initial && ((pl.first >> (k0 + k)) & 1))
-            put_row(a.d_initial + static_cast<int64_t>(pl.doc_of(k0 + k)) * a.width, c, l);
+          if (a.d_initial && ((first >> k) & 1))
+            c.store(a.d_initial + static_cast<int64_t>(pl.doc_of(half * kScanBatch + k)) * a.width, l);
         }
         const int64_t at = token_at(a, p) * a.width;
-        if (a.d_x) put_row(static_cast<T*>(a.d_x) + at, c, dx);
-        if (a.d_f) put_row(static_cast<T*>(a.d_f) + at, c, df);
-        if (a.d_o) put_row(static_cast<T*>(a.d_o) + at, c, dg);
+        if (a.d_x) c.store(static_cast<T*>(a.d_x) + at, dx);
+        if (a.d_f) c.store(static_cast<T*>(a.d_f) + at, df);
+        if (a.d_o) c.store(static_cast<T*>(a.d_o) + at, dg);
       }
     }
   }
@@ -489,7 +519,7 @@ static ScanPlan scan_plan(int64_t tokens, int width) {
   s.blocks = (all + kScanParts - 1) / kScanParts;
   s.parts = (all + s.blocks - 1) / s.blocks;
   s.prefix = (static_cast<size_t>(s.chunks) * width * sizeof(float2) + 15) / 16 * 16;
-  s.part = s.parts > 1 ? static_cast<size_t>(s.parts) * width * sizeof(double2) : 0;
+  s.part = s.parts > 1 ? static_cast<size_t>(s.parts) * width * (sizeof(float2) + sizeof(float)) : 0;
   return s;
 }
 
@@ -507,6 +537,8 @@ static int check_scan(const gs_gated_scan* p, void* workspace, size_t workspace_
                  aligned(p->initial, 4) && aligned(p->state, 4) && aligned(p->carry, 4) && aligned(p->offsets, 4) &&
                  aligned(workspace, 16), GS_ERR_ALIGN, "gated scan: misaligned tensor or workspace");
   const ScanPlan s = scan_plan(p->tokens, p->width);
+  GS_REQUIRE((s.chunks + int64_t(kWalkWaves)) * ((p->width + kScanGroup - 1) / kScanGroup) < (int64_t(1) << 26), GS_ERR_ARG,
+             "gated scan: too many elements");
   GS_REQUIRE(workspace_bytes >= s.prefix + s.part && (workspace || s.prefix == 0), GS_ERR_WORKSPACE,
              "gated scan: workspace too small");
   *a = {};
@@ -525,25 +557,39 @@ static int check_scan(const gs_gated_scan* p, void* workspace, size_t workspace_
   a->docs = p->docs;
   a->width = p->width;
   a->reverse = p->reverse != 0;
+  a->groups = (p->width + kScanGroup - 1) / kScanGroup;
   a->chunks = s.chunks;
   a->parts = s.parts;
   a->blocks = s.blocks;
   a->serial = s.serial;
   a->prefix = static_cast<float2*>(workspace);
-  a->part = reinterpret_cast<double2*>(static_cast<char*>(workspace) + s.prefix);
+  a->part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + s.prefix);
+  if (s.parts > 1) a->before = reinterpret_cast<float*>(a->part + static_cast<size_t>(s.parts) * p->width);
   return GS_OK;
 }
 
-template <typename T, bool BACK>
+template <typename T, bool BACK, bool SMALL>
 static int run_scan(const ScanArgs& a, hipStream_t st) {
-  const dim3 grid((a.width + kScanGroup - 1) / kScanGroup, a.parts), block(a.serial ? kWave : kScanThreads);
   if (!a.serial) {
-    hipLaunchKernelGGL((scan_sums_kernel<T, BACK>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((scan_sums_kernel<T, BACK, SMALL>), dim3(a.groups, a.parts), dim3(kScanThreads), 0, st, a);
     if (const int rc = check_launch("gated scan (sums)")) return rc;
   }
-  if constexpr (BACK) hipLaunchKernelGGL(scan_bwd_kernel<T>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(scan_apply_kernel<T>, grid, block, 0, st, a);
+  if (a.parts > 1) {
+    hipLaunchKernelGGL(scan_parts_kernel, dim3((a.width + 31) / 32), dim3(kJoinThreads), 0, st, a);
+    if (const int rc = check_launch("gated scan (parts)")) return rc;
+  }
+  const dim3 grid(static_cast<unsigned>(a.groups) * (a.serial ? 1 : (a.chunks + kWalkWaves - 1) / kWalkWaves));
+  const dim3 block(a.serial ? kWave : kWalkWaves * kWave);
+  if constexpr (BACK) hipLaunchKernelGGL((scan_bwd_kernel<T, SMALL>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((scan_apply_kernel<T, SMALL>), grid, block, 0, st, a);
   return check_launch("gated scan");
+}
+
+template <bool BACK>
+static int run_scan(const ScanArgs& a, int dtype, hipStream_t st) {
+  const bool small = a.width < kScanVec;
+  if (dtype == GS_BFLOAT16) return small ? run_scan<__bf16, BACK, true>(a, st) : run_scan<__bf16, BACK, false>(a, st);
+  return small ? run_scan<float, BACK, true>(a, st) : run_scan<float, BACK, false>(a, st);
 }
 
 }  // namespace gs
@@ -565,7 +611,7 @@ extern "C" int gs_gated_scan_fwd(const gs_gated_scan* p, void* workspace, size_t
   if (const int rc = check_scan(p, workspace, workspace_bytes, &a)) return rc;
   GS_REQUIRE(a.tokens == 0 || a.y, GS_ERR_ARG, "gated scan: null pointer");
   if (a.tokens == 0 && a.state == nullptr) return GS_OK;
-  return p->dtype == GS_BFLOAT16 ? run_scan<__bf16, false>(a, as_stream(stream)) : run_scan<float, false>(a, as_stream(stream));
+  return run_scan<false>(a, p->dtype, as_stream(stream));
 }
 
 extern "C" int gs_gated_scan_bwd(const gs_gated_scan* p, const void* d_y, const float* d_state, void* d_x, void* d_forget,
@@ -585,5 +631,5 @@ extern "C" int gs_gated_scan_bwd(const gs_gated_scan* p, const void* d_y, const 
   a.d_o = d_gate;
   a.d_initial = d_initial;
   if (a.tokens == 0 && d_initial == nullptr) return GS_OK;
-  return p->dtype == GS_BFLOAT16 ? run_scan<__bf16, true>(a, as_stream(stream)) : run_scan<float, true>(a, as_stream(stream));
+  return run_scan<true>(a, p->dtype, as_stream(stream));
 }

@@ -95,7 +95,7 @@ def scan_args(**kw):
 @pytest.mark.parametrize("kw,code,text", [
     (dict(dtype=1), ARG, "dtype"), (dict(tokens=-1), ARG, "token count"), (dict(tokens=1 << 31), ARG, "token count"),
     (dict(width=0), ARG, "width"), (dict(width=(1 << 20) + 1), ARG, "width"), (dict(docs=0), ARG, "document"),
-    (dict(docs=1 << 30), ARG, "document"), (dict(offsets=None), ARG, "offsets"), (dict(x=None), ARG, "null"),
+    (dict(docs=1 << 30), ARG, "document"), (dict(tokens=1 << 30, width=1 << 12), ARG, "too many"), (dict(offsets=None), ARG, "offsets"), (dict(x=None), ARG, "null"),
     (dict(forget=None), ARG, "null"), (dict(x=258), ALIGN, "misaligned"), (dict(state=258), ALIGN, "misaligned"),
     (dict(offsets=258), ALIGN, "misaligned"), (dict(dtype=BF, gate=257), ALIGN, "misaligned"),
 ])
