@@ -49,6 +49,31 @@ __device__ __forceinline__ void load8(const void* p, bool bf16, int64_t at, int 
   else load8(static_cast<const float*>(p) + at, n, v);
 }
 
+// Eight elements of a tensor whose type is known at run time, as they lie in memory.
+struct RawAny8 {
+  Raw8<float> f;  // bfloat16: in the first part
+  bool bf16;
+  __device__ __forceinline__ void load(const void* p, bool bf16_, int64_t at, int n) {
+    bf16 = bf16_;
+    if (bf16) {
+      Raw8<__bf16> h;
+      h.load(static_cast<const __bf16*>(p) + at, n);
+      f.part[0] = __builtin_bit_cast(Raw8<float>::Vec, h.part[0]);
+    } else {
+      f.load(static_cast<const float*>(p) + at, n);
+    }
+  }
+  __device__ __forceinline__ void to(float (&v)[8]) const {
+    if (bf16) {
+      const auto h = __builtin_bit_cast(Raw8<__bf16>::Vec, f.part[0]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(h[j]);
+    } else {
+      f.to(v);
+    }
+  }
+};
+
 // Rounded once, to nearest.
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int n, const float (&v)[8]) {

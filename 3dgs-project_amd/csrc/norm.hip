@@ -70,9 +70,26 @@ struct RowSum {
   }
 };
 
-// Mean and 1 / deviation of a row held in registers (elements past the width are zero).
-template <int NV, typename S>
-__device__ __forceinline__ float2 row_stats(const NormArgs& a, const float (&v)[NV][8], const int (&left)[NV], S& sum) {
+// Where a lane's vector of eight lies in a row, and how many of its elements are the row's. WHOLE: the width is a multiple of
+// eight, so that a vector is the row's or not; lanes past the end then load the last one and are masked, and
+// no load needs a branch.
+template <bool WHOLE>
+struct Piece8 {
+  int col, n;
+  Piece8() = default;
+  __device__ __forceinline__ Piece8(int col_, int width) : col(col_), n(width - col_) {
+    if constexpr (WHOLE) {
+      col = min(col_, width - 8);
+      n = n > 0 ? 8 : 0;
+    }
+  }
+  __device__ __forceinline__ int loaded() const { return WHOLE ? 8 : n; }
+  __device__ __forceinline__ bool has(int j) const { return WHOLE ? n > 0 : j < n; }
+};
+
+// Mean and 1 / deviation of a row held in registers (elements that are not the row's are zero).
+template <int NV, bool WHOLE, typename S>
+__device__ __forceinline__ float2 row_stats(const NormArgs& a, const float (&v)[NV][8], const Piece8<WHOLE> (&at)[NV], S& sum) {
   float mean = 0.0f;
   if (a.layer) {
     float s = 0.0f;
@@ -87,33 +104,53 @@ __device__ __forceinline__ float2 row_stats(const NormArgs& a, const float (&v)[
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float d = j < left[i] ? v[i][j] - mean : 0.0f;
+      const float d = at[i].has(j) ? v[i][j] - mean : 0.0f;
       q = fmaf(d, d, q);
     }
   const float var = sum(q, 0.0f).x * a.inv_width;
   return make_float2(mean, 1.0f / sqrtf(var + a.eps));
 }
 
-// k b of eight elements from y (given standardised as `hat`).
-__device__ __forceinline__ void branch8(const NormArgs& a, uint64_t seed, int64_t row, int col, int n,
-                                        const float (&hat)[8], float (&keep)[8], float (&u)[8]) {
-  float w[8], b[8];
-  if (a.post) {
-    load8(a.post_weight, a.weights_bf16, col, n, w);
-    if (a.post_bias) load8(a.post_bias, a.weights_bf16, col, n, b);
+// What lies between y and h of eight elements, as loaded.
+struct Between8 {
+  RawAny8 w, b, g;
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const NormArgs& a, int64_t row, const Piece8<WHOLE>& at) {
+    if (a.post) w.load(a.post_weight, a.weights_bf16, at.col, at.loaded());
+    if (a.post_bias) b.load(a.post_bias, a.weights_bf16, at.col, at.loaded());
+    if (a.gate) g.load(a.gate, a.gate_bf16, row * a.gate_stride + at.col, at.loaded());
   }
-  if (a.drop.threshold) keep8(a.drop, seed, static_cast<uint32_t>(row), col / 8, keep);
+  // u = k b from y (given standardised as `hat`), and the factors f = scale gate and k.
+  __device__ __forceinline__ void form(const NormArgs& a, uint64_t seed, int64_t row, int col, const float (&hat)[8],
+                                       float (&f)[8], float (&k)[8], float (&u)[8]) const {
+    float v[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    u[j] = hat[j];
-    if (a.post) u[j] = a.post_bias ? fmaf(hat[j], w[j], b[j]) : hat[j] * w[j];
-    if (a.drop.threshold) u[j] = keep[j] != 0.0f ? u[j] * keep[j] : 0.0f;
-    else keep[j] = 1.0f;
+    for (int j = 0; j < 8; ++j) u[j] = hat[j], f[j] = a.scale, k[j] = 1.0f;
+    if (a.post) {
+      w.to(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] *= v[j];
+      if (a.post_bias) {
+        b.to(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] += v[j];
+      }
+    }
+    if (a.gate) {
+      g.to(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= v[j];
+    }
+    if (a.drop.threshold) {
+      keep8(a.drop, seed, static_cast<uint32_t>(row), col / 8, k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = k[j] != 0.0f ? u[j] * k[j] : 0.0f;
+    }
   }
-}
+};
 
 // G lanes a row, each NV vectors of eight: vector i of lane l begins at 8 (l + G i).
-template <typename X, typename Y, int G, int NV>
+template <typename X, typename Y, int G, int NV, bool WHOLE>
 __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a) {
   constexpr int kGroups = G > 256 ? 1 : 256 / G;
   __shared__ float2 lds[2][kGroups][G / kWave];
@@ -123,24 +160,39 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
   // (groups past the last row repeat it without writing: every lane meets every barrier)
   const bool mine = row_at < a.rows;
   const int64_t row = mine ? row_at : a.rows - 1;
-  float h[NV][8], b[NV][8];
-  int left[NV];
+  Piece8<WHOLE> at[NV];
   Raw8<X> rx[NV];
   Raw8<Y> ry[NV];
+  RawAny8 rw[NV], rb[NV];
+  Between8 mid[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int col = 8 * (lane + G * i);
-    left[i] = a.width - col;
-    rx[i].load(static_cast<const X*>(a.x) + row * a.x_stride + col, left[i]);
-    if (a.y) ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, left[i]);
+    at[i] = {8 * (lane + G * i), a.width};
+    rx[i].load(static_cast<const X*>(a.x) + row * a.x_stride + at[i].col, at[i].loaded());
+    if (a.y) {
+      ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + at[i].col, at[i].loaded());
+      mid[i].load(a, row, at[i]);
+    }
+    if (a.weight) rw[i].load(a.weight, a.weights_bf16, at[i].col, at[i].loaded());
+    if (a.bias) rb[i].load(a.bias, a.weights_bf16, at[i].col, at[i].loaded());
   }
+  float h[NV][8];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) rx[i].to(h[i]);
+  for (int i = 0; i < NV; ++i) {
+    rx[i].to(h[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[i][j] = at[i].has(j) ? h[i][j] : 0.0f;
+  }
   if (a.y) {
+    float b[NV][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) ry[i].to(b[i]);
+    for (int i = 0; i < NV; ++i) {
+      ry[i].to(b[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[i][j] = at[i].has(j) ? b[i][j] : 0.0f;
+    }
     float2 st = {0.0f, 1.0f};
-    if (a.post) st = row_stats(a, b, left, sum);
+    if (a.post) st = row_stats(a, b, at, sum);
     if (mine && lane == 0 && a.stats) {
       a.stats[4 * row + 2] = st.x;
       a.stats[4 * row + 3] = st.y;
@@ -148,46 +200,42 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
     const uint64_t seed = a.drop.threshold ? seed_of(a.drop) : 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (left[i] <= 0) continue;
-      const int col = 8 * (lane + G * i);
-      float keep[8], u[8], g[8], hat[8];
-      if (a.gate) load8(a.gate, a.gate_bf16, row * a.gate_stride + col, left[i], g);
+      float f[8], k[8], u[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) hat[j] = a.post ? (b[i][j] - st.x) * st.y : b[i][j];
-      branch8(a, seed, row, col, left[i], hat, keep, u);
+      for (int j = 0; j < 8; ++j) b[i][j] = (b[i][j] - st.x) * st.y;  // (without a post norm y itself)
+      mid[i].form(a, seed, row, at[i].col, b[i], f, k, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float w = a.gate ? a.scale * g[j] : a.scale;
-        h[i][j] = j < left[i] ? fmaf(w, u[j], h[i][j]) : 0.0f;
-      }
-      if (mine) store8(static_cast<X*>(a.h) + row * a.width + col, left[i], h[i]);
+      for (int j = 0; j < 8; ++j) h[i][j] = at[i].has(j) ? fmaf(f[j], u[j], h[i][j]) : 0.0f;
+      if (mine && at[i].n > 0) store8(static_cast<X*>(a.h) + row * a.width + at[i].col, at[i].n, h[i]);
     }
   }
-  const float2 st = row_stats(a, h, left, sum);
+  const float2 st = row_stats(a, h, at, sum);
   if (mine && lane == 0 && a.stats) {
     a.stats[4 * row] = st.x;
     a.stats[4 * row + 1] = st.y;
   }
-  if (!mine) return;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (left[i] <= 0) continue;
-    const int col = 8 * (lane + G * i);
-    float w[8], c[8], n[8];
-    if (a.weight) load8(a.weight, a.weights_bf16, col, left[i], w);
-    if (a.bias) load8(a.bias, a.weights_bf16, col, left[i], c);
+    float w[8], n[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      n[j] = (h[i][j] - st.x) * st.y;
-      if (a.weight) n[j] *= w[j];
-      if (a.bias) n[j] += c[j];
+    for (int j = 0; j < 8; ++j) n[j] = (h[i][j] - st.x) * st.y;
+    if (a.weight) {
+      rw[i].to(w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n[j] *= w[j];
     }
-    store8(static_cast<Y*>(a.n) + row * a.width + col, left[i], n);
+    if (a.bias) {
+      rb[i].to(w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n[j] += w[j];
+    }
+    if (mine && at[i].n > 0) store8(static_cast<Y*>(a.n) + row * a.width + at[i].col, at[i].n, n);
   }
 }
 
-template <typename X, typename Y, int G, int NV>
-__global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a) {
+// BIAS: a bias' gradient is wanted too.
+template <typename X, typename Y, int G, int NV, bool WHOLE, bool BIAS>
+__global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_kernel(NormArgs a) {
   constexpr int kGroups = G > 256 ? 1 : 256 / G;
   constexpr int kWidth = 8 * G * NV;
   __shared__ float2 lds[2][kGroups][G / kWave];
@@ -195,9 +243,9 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
   RowSum<G, kGroups> sum{lds};
   const int lane = threadIdx.x % G;
   float col_sum[5][NV][8] = {};
-  int left[NV];
+  Piece8<WHOLE> at[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) left[i] = a.width - 8 * (lane + G * i);
+  for (int i = 0; i < NV; ++i) at[i] = {8 * (lane + G * i), a.width};
   const uint64_t seed = a.drop.threshold ? seed_of(a.drop) : 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
   // (the groups of a workgroup take as many turns as its first one: barriers are met by all)
@@ -205,90 +253,92 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
     const int64_t row_at = first + threadIdx.x / G;
     const bool mine = row_at < a.rows;
     const int64_t row = mine ? row_at : a.rows - 1;
-    float hat[NV][8], t[NV][8], d[NV][8], b[NV][8], u[NV][8], keep[NV][8];
     Raw8<X> rx[NV], rdh[NV];
     Raw8<Y> ry[NV], rdn[NV];
+    RawAny8 rw[NV];
+    Between8 mid[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
+      const int col = at[i].col, n = at[i].loaded();
       rx[i].load(static_cast<const X*>(a.x) + row * a.x_stride + col, n);
-      ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, a.y ? n : 0);
       rdn[i].load(static_cast<const Y*>(a.d_n) + row * a.width + col, a.d_n ? n : 0);
       rdh[i].load(static_cast<const X*>(a.d_h) + row * a.width + col, a.d_h ? n : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      rx[i].to(hat[i]);
-      ry[i].to(b[i]);
-      rdn[i].to(t[i]);
-      rdh[i].to(d[i]);
+      if (a.weight) rw[i].load(a.weight, a.weights_bf16, col, n);
+      if (a.y) {
+        ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, n);
+        mid[i].load(a, row, at[i]);
+      }
     }
     const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+    float hat[NV][8], t[NV][8], b[NV][8], u[NV][8], fk[NV][8];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
-      float w[8];
-      if (a.weight && n > 0) load8(a.weight, a.weights_bf16, col, n, w);
-      if (a.y && n > 0) {
-        float g[8];
-        if (a.gate) load8(a.gate, a.gate_bf16, row * a.gate_stride + col, n, g);
+      rx[i].to(hat[i]);
+      if (a.y) {
+        float f[8], k[8];
+        ry[i].to(b[i]);
         if (a.post) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) b[i][j] = (b[i][j] - st.z) * st.w;
         }
-        branch8(a, seed, row, col, n, b[i], keep[i], u[i]);
+        mid[i].form(a, seed, row, at[i].col, b[i], f, k, u[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float f = a.gate ? a.scale * g[j] : a.scale;
-          hat[i][j] = fmaf(f, u[i][j], hat[i][j]);
-          keep[i][j] *= f;
+          hat[i][j] = fmaf(f[j], u[i][j], hat[i][j]);
+          fk[i][j] = f[j] * k[j];
         }
       }
+      rdn[i].to(t[i]);
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = 1.0f;
+      if (a.weight) rw[i].to(w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        hat[i][j] = j < n ? (hat[i][j] - st.x) * st.y : 0.0f;
+        const bool has = mine && at[i].has(j);
+        hat[i][j] = has ? (hat[i][j] - st.x) * st.y : 0.0f;
+        t[i][j] = has ? t[i][j] : 0.0f;
         col_sum[kSumWeight][i][j] = fmaf(t[i][j], hat[i][j], col_sum[kSumWeight][i][j]);
-        col_sum[kSumBias][i][j] += t[i][j];
-        if (a.weight) t[i][j] = j < n ? t[i][j] * w[j] : 0.0f;
+        if (BIAS) col_sum[kSumBias][i][j] += t[i][j];
+        t[i][j] = has ? t[i][j] * w[j] : 0.0f;
         s1 = fmaf(t[i][j], hat[i][j], s1);
         s2 += t[i][j];
       }
     }
     const float2 m = sum(s1, s2);
     const float m1 = m.x * a.inv_width, m2 = a.layer ? m.y * a.inv_width : 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[i][j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
-      if (a.d_x && n > 0) store8(static_cast<X*>(a.d_x) + row * a.width + col, n, d[i]);
-    }
-    if (!a.y) continue;
     s1 = s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = 8 * (lane + G * i), n = mine ? left[i] : 0;
+      const bool some = mine && at[i].n > 0;
+      float d[8];
+      rdh[i].to(d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
+      if (a.d_x && some) store8(static_cast<X*>(a.d_x) + row * a.width + at[i].col, at[i].n, d);
+      if (!a.y) continue;
       float e[8], w[8];
-      if (a.post && n > 0) load8(a.post_weight, a.weights_bf16, col, n, w);
+      if (a.post) mid[i].w.to(w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        e[j] = j < n ? a.scale * d[i][j] * u[i][j] : 0.0f;  // of the gate
+        const bool has = mine && at[i].has(j);
+        e[j] = has ? a.scale * d[j] * u[i][j] : 0.0f;  // of the gate
         col_sum[kSumGate][i][j] += e[j];
-        const float v = j < n ? d[i][j] * keep[i][j] : 0.0f;
+        const float v = has ? d[j] * fk[i][j] : 0.0f;
+        t[i][j] = v;
         if (a.post) {
-          if (j >= n) b[i][j] = 0.0f;
+          b[i][j] = has ? b[i][j] : 0.0f;
           col_sum[kSumPostWeight][i][j] = fmaf(v, b[i][j], col_sum[kSumPostWeight][i][j]);
-          col_sum[kSumPostBias][i][j] += v;
-          t[i][j] = j < n ? v * w[j] : 0.0f;
+          if (BIAS) col_sum[kSumPostBias][i][j] += v;
+          t[i][j] = has ? v * w[j] : 0.0f;
           s1 = fmaf(t[i][j], b[i][j], s1);
           s2 += t[i][j];
-        } else {
-          t[i][j] = v;
         }
       }
-      if (a.d_gate_rows && n > 0) store8(a.d_gate_rows, a.gate_bf16, row * a.width + col, n, e);
+      if (a.d_gate_rows && some) store8(a.d_gate_rows, a.gate_bf16, row * a.width + at[i].col, at[i].n, e);
     }
+    if (!a.y) continue;
     if (a.post) {
       const float2 p = sum(s1, s2);
       const float p1 = p.x * a.inv_width, p2 = a.layer ? p.y * a.inv_width : 0.0f;
@@ -300,7 +350,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
     if (a.d_y) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (mine && left[i] > 0) store8(static_cast<Y*>(a.d_y) + row * a.width + 8 * (lane + G * i), left[i], t[i]);
+        if (mine && at[i].n > 0) store8(static_cast<Y*>(a.d_y) + row * a.width + at[i].col, at[i].n, t[i]);
     }
   }
 #pragma unroll
@@ -310,7 +360,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_bwd_kernel(NormArgs a)
     if constexpr (kGroups == 1) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (left[i] > 0) store8(part + 8 * (lane + G * i), left[i], col_sum[k][i]);
+        if (at[i].n > 0) store8(part + at[i].col, at[i].n, col_sum[k][i]);
     } else {
       __syncthreads();
 #pragma unroll
@@ -405,23 +455,29 @@ static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
 
 // Calls f(kernel, lanes a row) with the instance for a width: a wavefront a row where eight or sixteen elements a
 // lane do, more wavefronts above.
-template <typename X, typename Y, typename F>
+template <typename X, typename Y, bool WHOLE, typename F>
 static int with_fwd(int width, F f) {
-  if (width <= 512) return f(norm_fwd_kernel<X, Y, 64, 1>, 64);
-  if (width <= 1024) return f(norm_fwd_kernel<X, Y, 64, 2>, 64);
-  if (width <= 2048) return f(norm_fwd_kernel<X, Y, 64, 4>, 64);
-  if (width <= 4096) return f(norm_fwd_kernel<X, Y, 256, 2>, 256);
-  if (width <= 8192) return f(norm_fwd_kernel<X, Y, 512, 2>, 512);
-  return f(norm_fwd_kernel<X, Y, 1024, 2>, 1024);
+  if (width <= 512) return f(norm_fwd_kernel<X, Y, 64, 1, WHOLE>, 64);
+  if (width <= 1024) return f(norm_fwd_kernel<X, Y, 64, 2, WHOLE>, 64);
+  if (width <= 2048) return f(norm_fwd_kernel<X, Y, 256, 1, WHOLE>, 256);
+  if (width <= 4096) return f(norm_fwd_kernel<X, Y, 256, 2, WHOLE>, 256);
+  if (width <= 8192) return f(norm_fwd_kernel<X, Y, 512, 2, WHOLE>, 512);
+  return f(norm_fwd_kernel<X, Y, 1024, 2, WHOLE>, 1024);
 }
-template <typename X, typename Y, typename F>
+template <typename X, typename Y, bool WHOLE, bool BIAS, typename F>
 static int with_bwd(int width, F f) {
-  if (width <= 512) return f(norm_bwd_kernel<X, Y, 64, 1>, 64);
-  if (width <= 1024) return f(norm_bwd_kernel<X, Y, 64, 2>, 64);
-  if (width <= 2048) return f(norm_bwd_kernel<X, Y, 256, 1>, 256);
-  if (width <= 4096) return f(norm_bwd_kernel<X, Y, 256, 2>, 256);
-  if (width <= 8192) return f(norm_bwd_kernel<X, Y, 512, 2>, 512);
-  return f(norm_bwd_kernel<X, Y, 1024, 2>, 1024);
+  if (width <= 512) return f(norm_bwd_kernel<X, Y, 64, 1, WHOLE, BIAS>, 64);
+  if (width <= 1024) return f(norm_bwd_kernel<X, Y, 128, 1, WHOLE, BIAS>, 128);
+  if (width <= 2048) return f(norm_bwd_kernel<X, Y, 256, 1, WHOLE, BIAS>, 256);
+  if (width <= 4096) return f(norm_bwd_kernel<X, Y, 512, 1, WHOLE, BIAS>, 512);
+  if (width <= 8192) return f(norm_bwd_kernel<X, Y, 1024, 1, WHOLE, BIAS>, 1024);
+  return f(norm_bwd_kernel<X, Y, 1024, 2, WHOLE, BIAS>, 1024);
+}
+template <typename F>
+static int with_types(const gs_residual_norm* p, F f) {
+  if (p->x_dtype == GS_BFLOAT16) return f(__bf16{}, __bf16{});
+  if (p->y_dtype == GS_BFLOAT16) return f(float{}, __bf16{});
+  return f(float{}, float{});
 }
 
 }  // namespace gs
@@ -439,9 +495,11 @@ extern "C" int gs_residual_norm_fwd(const gs_residual_norm* p, void* stream) {
                        as_stream(stream), a);
     return check_launch("residual norm");
   };
-  if (p->x_dtype == GS_BFLOAT16) return with_fwd<__bf16, __bf16>(a.width, run);
-  if (p->y_dtype == GS_BFLOAT16) return with_fwd<float, __bf16>(a.width, run);
-  return with_fwd<float, float>(a.width, run);
+  return with_types(p, [&](auto x, auto y) {
+    using X = decltype(x);
+    using Y = decltype(y);
+    return a.width % 8 == 0 ? with_fwd<X, Y, true>(a.width, run) : with_fwd<X, Y, false>(a.width, run);
+  });
 }
 
 extern "C" size_t gs_residual_norm_bwd_workspace_size(const gs_residual_norm* p) {
@@ -492,9 +550,13 @@ extern "C" int gs_residual_norm_bwd(const gs_residual_norm* p, const void* d_h, 
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(std::max(256, lanes)), 0, st, a);
       return check_launch("residual norm backward");
     };
-    const int rc = p->x_dtype == GS_BFLOAT16 ? with_bwd<__bf16, __bf16>(a.width, run)
-                   : p->y_dtype == GS_BFLOAT16 ? with_bwd<float, __bf16>(a.width, run)
-                                               : with_bwd<float, float>(a.width, run);
+    const bool bias = d_bias || d_post_bias;
+    const int rc = with_types(p, [&](auto x, auto y) {
+      using X = decltype(x);
+      using Y = decltype(y);
+      if (a.width % 8) return with_bwd<X, Y, false, true>(a.width, run);
+      return bias ? with_bwd<X, Y, true, true>(a.width, run) : with_bwd<X, Y, true, false>(a.width, run);
+    });
     if (rc) return rc;
   }
   if (a.sums == 0) return GS_OK;
