@@ -248,36 +248,49 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
   for (int i = 0; i < NV; ++i) at[i] = {8 * (lane + G * i), a.width};
   const uint64_t seed = a.drop.threshold ? seed_of(a.drop) : 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
+  // What differs from row to row is loaded a row ahead.
+  struct Row {
+    Raw8<X> x[NV], d_h[NV];
+    Raw8<Y> y[NV], d_n[NV];
+    float4 stats;
+  };
+  const auto fetch = [&](Row& r, int64_t row) {
+    row = row < a.rows ? row : a.rows - 1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = at[i].col, n = at[i].loaded();
+      r.x[i].load(static_cast<const X*>(a.x) + row * a.x_stride + col, n);
+      r.d_n[i].load(static_cast<const Y*>(a.d_n) + row * a.width + col, a.d_n ? n : 0);
+      r.d_h[i].load(static_cast<const X*>(a.d_h) + row * a.width + col, a.d_h ? n : 0);
+      if (a.y) r.y[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, n);
+    }
+    r.stats = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+  };
+  Row next;
+  fetch(next, static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G);
   // (the groups of a workgroup take as many turns as its first one: barriers are met by all)
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows; first += step) {
     const int64_t row_at = first + threadIdx.x / G;
     const bool mine = row_at < a.rows;
     const int64_t row = mine ? row_at : a.rows - 1;
-    Raw8<X> rx[NV], rdh[NV];
-    Raw8<Y> ry[NV], rdn[NV];
+    const Row now = next;
     RawAny8 rw[NV];
     Between8 mid[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int col = at[i].col, n = at[i].loaded();
-      rx[i].load(static_cast<const X*>(a.x) + row * a.x_stride + col, n);
-      rdn[i].load(static_cast<const Y*>(a.d_n) + row * a.width + col, a.d_n ? n : 0);
-      rdh[i].load(static_cast<const X*>(a.d_h) + row * a.width + col, a.d_h ? n : 0);
-      if (a.weight) rw[i].load(a.weight, a.weights_bf16, col, n);
-      if (a.y) {
-        ry[i].load(static_cast<const Y*>(a.y) + row * a.y_stride + col, n);
-        mid[i].load(a, row, at[i]);
-      }
+      if (a.weight) rw[i].load(a.weight, a.weights_bf16, at[i].col, at[i].loaded());
+      if (a.y) mid[i].load(a, row, at[i]);
     }
-    const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+    fetch(next, row_at + step);
+    const float4 st = now.stats;
     float hat[NV][8], t[NV][8], b[NV][8], u[NV][8], fk[NV][8];
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      rx[i].to(hat[i]);
+      now.x[i].to(hat[i]);
       if (a.y) {
         float f[8], k[8];
-        ry[i].to(b[i]);
+        now.y[i].to(b[i]);
         if (a.post) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) b[i][j] = (b[i][j] - st.z) * st.w;
@@ -289,7 +302,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
           fk[i][j] = f[j] * k[j];
         }
       }
-      rdn[i].to(t[i]);
+      now.d_n[i].to(t[i]);
       float w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = 1.0f;
@@ -313,7 +326,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
     for (int i = 0; i < NV; ++i) {
       const bool some = mine && at[i].n > 0;
       float d[8];
-      rdh[i].to(d);
+      now.d_h[i].to(d);
 #pragma unroll
       for (int j = 0; j < 8; ++j) d[j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
       if (a.d_x && some) store8(static_cast<X*>(a.d_x) + row * a.width + at[i].col, at[i].n, d);
