@@ -178,6 +178,17 @@ class GsGatedScan(C.Structure):
     ]
 
 
+class GsRows(C.Structure):
+    _fields_ = [
+        ("src", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("src_stride", C.c_int64),
+        ("dst_stride", C.c_int64),
+    ]
+
+
 class GsLinear(C.Structure):
     _fields_ = [
         ("x", C.c_void_p),
@@ -264,7 +275,7 @@ _SIGS = {
     "gs_gated_scan_workspace_size": (_sz, [_i64, _i32]),
     "gs_gated_scan_fwd": (_i32, [_vp, _vp, _sz, _vp]),
     "gs_gated_scan_bwd": (_i32, [_vp] * 8 + [_sz, _vp]),
-    "gs_rows_pack": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _i32, _vp]),
+    "gs_rows_pack": (_i32, [_vp, _i32, _i32, _vp]),
     "gs_linear_fwd_workspace_size": (_sz, [_vp]),
     "gs_linear_fwd": (_i32, [_vp, _vp, _sz, _vp]),
     "gs_linear_bwd_workspace_size": (_sz, [_vp]),

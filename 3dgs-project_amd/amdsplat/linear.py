@@ -24,34 +24,47 @@ def _rows(t):
     return t if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= 0) else t.contiguous()
 
 
-def _packed(t: torch.Tensor) -> torch.Tensor:
-    """Rows of t as the tile kernels read them: t itself where its address, its row stride and its row length are multiples of
-    16 bytes, otherwise a copy with zeros behind the rows, of which this is a view."""
-    code, per = _DTYPES[t.dtype]
-    rows, cols = t.shape
+def _ready(t: torch.Tensor, few: bool) -> bool:
+    """The kernels can read t through its row stride: the tile kernels where its address, row stride and row length are
+    multiples of 16 bytes, a forward of few rows at any."""
     s = t.stride(0)
-    if rows == 0 or (cols % per == 0 and t.stride(1) == 1 and 0 <= s < 1 << 20 and s % per == 0 and t.data_ptr() % 16 == 0):
-        return t
-    t = _rows(t)
-    wide = torch.empty((rows, -(-cols // 8) * 8), dtype=t.dtype, device=t.device)
-    call("gs_rows_pack", t.data_ptr(), rows, cols, t.stride(0), wide.data_ptr(), wide.shape[1], code,
-         _lib.stream_handle(t.device))
-    return wide[:, :cols]
+    if t.shape[0] == 0 or not 0 <= s < 1 << 20:
+        return t.shape[0] == 0
+    per = _DTYPES[t.dtype][1]
+    return few or (t.shape[1] % per == 0 and t.stride(1) == 1 and s % per == 0 and t.data_ptr() % 16 == 0)
 
 
-def _operands(x, weight):
-    if x.shape[0] <= FEW_ROWS and weight.stride(0) < 1 << 20 and x.stride(0) < 1 << 20:
-        return _rows(x), _rows(weight)
-    return _packed(x), _packed(weight)
+def _pack(x, weight, few: bool):
+    """None, or a buffer with what of x and weight the kernels cannot read, as rows with zeros behind them."""
+    away = [t for t in (x, weight) if not _ready(t, few)]
+    if not away:
+        return None
+    wide = -(-x.shape[1] // 8) * 8
+    buffer = torch.empty(sum(t.shape[0] for t in away) * wide, dtype=x.dtype, device=x.device)
+    sets = (_lib.GsRows * 2)()
+    to = buffer.data_ptr()
+    for r, t in zip(sets, away):
+        r.src, r.dst, r.rows, r.cols, r.src_stride, r.dst_stride = t.data_ptr(), to, t.shape[0], t.shape[1], t.stride(0), wide
+        to += t.shape[0] * wide * t.element_size()
+    call("gs_rows_pack", sets, len(away), _DTYPES[x.dtype][0], _lib.stream_handle(x.device))
+    return buffer
 
 
-def _args(x, weight, bias, residual, out, z, out_dtype, activation) -> _lib.GsLinear:
-    rows = x.shape[0]
-    return _lib.GsLinear(x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
-                         None if residual is None else residual.data_ptr(), ptr(out), ptr(z), rows,
-                         x.stride(0) if rows else 0, weight.stride(0), 0 if residual is None else residual.stride(0),
-                         weight.shape[1], weight.shape[0], _DTYPES[x.dtype][0], _DTYPES[out_dtype][0],
-                         0 if z is None else _DTYPES[z.dtype][0], 0 if bias is None else _DTYPES[bias.dtype][0], activation)
+def _args(x, weight, buffer, few, bias, residual, out, z, out_dtype, activation) -> _lib.GsLinear:
+    at = []
+    if buffer is not None:
+        to, wide = buffer.data_ptr(), -(-x.shape[1] // 8) * 8
+    for t in (x, weight):
+        if buffer is None or _ready(t, few):
+            at += (t.data_ptr(), t.stride(0) if t.shape[0] else 0)
+        else:
+            at += (to, wide)
+            to += t.shape[0] * wide * t.element_size()
+    return _lib.GsLinear(at[0], at[2], None if bias is None else bias.data_ptr(),
+                         None if residual is None else residual.data_ptr(), ptr(out), ptr(z), x.shape[0], at[1], at[3],
+                         0 if residual is None else residual.stride(0), weight.shape[1], weight.shape[0],
+                         _DTYPES[x.dtype][0], _DTYPES[out_dtype][0], 0 if z is None else _DTYPES[z.dtype][0],
+                         0 if bias is None else _DTYPES[bias.dtype][0], activation)
 
 
 def _workspace(name: str, a, device):
@@ -60,37 +73,40 @@ def _workspace(name: str, a, device):
 
 
 def _forward(x, weight, bias, residual, activation, out_dtype, keep: bool):
+    few = x.shape[0] <= FEW_ROWS
+    buffer = _pack(x, weight, few)
     out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype, device=x.device)
     z = None
     if keep and activation:  # float32 where a bias' gradient sums its slopes; the products round them anyway
         z = torch.empty(out.shape, dtype=x.dtype if bias is None else torch.float32, device=x.device)
-    a = _args(x, weight, bias, residual, out, z, out_dtype, activation)
+    a = _args(x, weight, buffer, few, bias, residual, out, z, out_dtype, activation)
     ws, n = _workspace("gs_linear_fwd_workspace_size", a, x.device)
     call("gs_linear_fwd", C.byref(a), ptr(ws), n, _lib.stream_handle(x.device))
-    return out, z
+    return out, z, buffer
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, out_dtype):
-        x, weight = _operands(x, weight)
-        out, z = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, bias, z)
+        out, z, buffer = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, z, None if x.shape[0] <= FEW_ROWS else buffer)
         ctx.rule = (out_dtype, activation)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        x, weight, bias, z = ctx.saved_tensors
+        x, weight, bias, z, buffer = ctx.saved_tensors
         grads = [None, None, None]
         if any(ctx.needs_input_grad[:3]):
-            x, weight, d = _packed(x), _packed(weight), d_out.contiguous()
+            if x.shape[0] <= FEW_ROWS:
+                buffer = _pack(x, weight, False)
+            d = d_out.contiguous()
             if d.data_ptr() % 16:
                 d = d.clone()
             grads = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if t is not None and need else None
                      for t, need in zip((x, weight, bias), ctx.needs_input_grad)]
-            a = _args(x, weight, bias, None, None, z, *ctx.rule)
+            a = _args(x, weight, buffer, False, bias, None, None, z, *ctx.rule)
             ws, n = _workspace("gs_linear_bwd_workspace_size", a, x.device)
             call("gs_linear_bwd", C.byref(a), ptr(d), *map(ptr, grads), ptr(ws), n, _lib.stream_handle(x.device))
         return (*grads, d_out if ctx.needs_input_grad[3] else None, None, None)
@@ -128,7 +144,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         out_dtype, residual = residual.dtype, _rows(residual)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
+    x, weight = _rows(x), _rows(weight)
     rest = (bias, residual, ACTIVATIONS[activation], out_dtype)
     if tracked(x, weight, bias, residual):
         return _Linear.apply(x, weight, *rest)
-    return _forward(*_operands(x, weight), *rest, False)[0]
+    return _forward(x, weight, *rest, False)[0]

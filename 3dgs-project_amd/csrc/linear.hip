@@ -470,16 +470,26 @@ __global__ __launch_bounds__(kSlopeThreads) void slope_kernel(SlopeArgs a) {
   }
 }
 
-// Rows copied to rows of a multiple of eight elements, the rest zero.
+// Rows copied to rows of a multiple of eight elements, the rest zero: up to two matrices in one launch.
+struct PackArgs {
+  struct {
+    const void* src;
+    void* dst;
+    int64_t vecs, cols, stride;  // vecs: of eight elements, in all
+    int per_row;                 // of them
+  } m[2];
+};
 template <typename T>
-__global__ __launch_bounds__(kFinishThreads) void pack_kernel(const T* src, int64_t rows, int64_t cols, int64_t stride, T* dst,
-                                                              int vecs) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kFinishThreads + threadIdx.x, row = i / vecs;
-  if (row >= rows) return;
-  const int64_t c = (i - row * vecs) * 8, left = cols - c;
+__global__ __launch_bounds__(kFinishThreads) void pack_kernel(PackArgs a) {
+  int64_t i = static_cast<int64_t>(blockIdx.x) * kFinishThreads + threadIdx.x;
+  const bool second = i >= a.m[0].vecs;
+  if (second) i -= a.m[0].vecs;
+  const auto& m = a.m[second];
+  if (i >= m.vecs) return;
+  const int64_t row = i / m.per_row, c = (i - row * m.per_row) * 8, left = m.cols - c;
   float v[8];  // (float32 holds both types exactly)
-  load8(src + row * stride + c, left < 8 ? static_cast<int>(left) : 8, v);
-  store8(dst + i * 8, 8, v);
+  load8(static_cast<const T*>(m.src) + row * m.stride + c, left < 8 ? static_cast<int>(left) : 8, v);
+  store8(static_cast<T*>(m.dst) + i * 8, 8, v);
 }
 
 // ---- plans and launches ------------------------------------------------------------------------------
@@ -653,25 +663,29 @@ static int check_linear(const gs_linear* p, bool backward) {
 
 using namespace gs;
 
-extern "C" int gs_rows_pack(const void* src, int64_t rows, int64_t cols, int64_t stride, void* dst, int64_t dst_stride,
-                            int dtype, void* stream) {
+extern "C" int gs_rows_pack(const gs_rows* sets, int n, int dtype, void* stream) {
   clear_error();
   GS_REQUIRE(row_type(dtype), GS_ERR_ARG, "row pack: dtype must be GS_FLOAT32 or GS_BFLOAT16");
-  GS_REQUIRE(rows >= 0 && cols >= 0 && dst_stride >= cols && dst_stride % 8 == 0, GS_ERR_ARG, "row pack: invalid size");
-  const int64_t vecs = dst_stride / 8;
-  GS_REQUIRE(rows < (int64_t(1) << 32) && vecs < (int64_t(1) << 31) && rows * vecs < (int64_t(1) << 32) - kFinishThreads,
-             GS_ERR_ARG, "row pack: too many elements");
-  GS_REQUIRE(rows * vecs == 0 || (src && dst), GS_ERR_ARG, "row pack: null pointer");
-  GS_REQUIRE(aligned(src, row_type_bytes(dtype)) && aligned(dst, 16), GS_ERR_ALIGN, "row pack: misaligned tensor");
-  if (rows * vecs == 0) return GS_OK;
-  const dim3 grid(static_cast<unsigned>((rows * vecs + kFinishThreads - 1) / kFinishThreads)), block(kFinishThreads);
-  if (dtype == GS_BFLOAT16) {
-    hipLaunchKernelGGL(pack_kernel<__bf16>, grid, block, 0, as_stream(stream), static_cast<const __bf16*>(src), rows, cols,
-                       stride, static_cast<__bf16*>(dst), static_cast<int>(vecs));
-  } else {
-    hipLaunchKernelGGL(pack_kernel<float>, grid, block, 0, as_stream(stream), static_cast<const float*>(src), rows, cols,
-                       stride, static_cast<float*>(dst), static_cast<int>(vecs));
+  GS_REQUIRE(n >= 0 && n <= 2 && (n == 0 || sets), GS_ERR_ARG, "row pack: up to two sets of rows");
+  PackArgs a = {};
+  int64_t all = 0;
+  for (int i = 0; i < n; ++i) {
+    const gs_rows& r = sets[i];
+    GS_REQUIRE(r.rows >= 0 && r.cols >= 0 && r.dst_stride >= r.cols && r.dst_stride % 8 == 0, GS_ERR_ARG,
+               "row pack: invalid size");
+    const int64_t per = r.dst_stride / 8;
+    GS_REQUIRE(r.rows < (int64_t(1) << 32) && per < (int64_t(1) << 31) && r.rows * per < (int64_t(1) << 31), GS_ERR_ARG,
+               "row pack: too many elements");
+    GS_REQUIRE(r.rows * per == 0 || (r.src && r.dst), GS_ERR_ARG, "row pack: null pointer");
+    GS_REQUIRE(aligned(r.src, row_type_bytes(dtype)) && aligned(r.dst, 16), GS_ERR_ALIGN, "row pack: misaligned tensor");
+    a.m[i] = {r.src, r.dst, r.rows * per, r.cols, r.src_stride, static_cast<int>(per)};
+    all += r.rows * per;
   }
+  GS_REQUIRE(all < (int64_t(1) << 32) - kFinishThreads, GS_ERR_ARG, "row pack: too many elements");
+  if (all == 0) return GS_OK;
+  const dim3 grid(static_cast<unsigned>((all + kFinishThreads - 1) / kFinishThreads)), block(kFinishThreads);
+  if (dtype == GS_BFLOAT16) hipLaunchKernelGGL(pack_kernel<__bf16>, grid, block, 0, as_stream(stream), a);
+  else hipLaunchKernelGGL(pack_kernel<float>, grid, block, 0, as_stream(stream), a);
   return check_launch("row pack");
 }
 

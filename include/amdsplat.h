@@ -772,10 +772,14 @@ typedef struct gs_linear {
   int64_t rows, x_stride, weight_stride, residual_stride;
   int32_t inputs, outputs, dtype, out_dtype, z_dtype, bias_dtype, activation;
 } gs_linear;
-/* Copies rows [rows, cols] of a row stride (elements) to 16-byte aligned rows of dst_stride elements (a multiple of eight, at
- * least cols), zeros behind them. */
-int gs_rows_pack(const void* src, int64_t rows, int64_t cols, int64_t stride, void* dst, int64_t dst_stride, int dtype,
-                 void* stream);
+/* Copies n (up to two) sets of rows [rows, cols] of a row stride (elements) to 16-byte aligned rows of dst_stride elements (a multiple
+ * of eight, at least cols), zeros behind them. sets: host memory. */
+typedef struct gs_rows {
+  const void* src;
+  void* dst;
+  int64_t rows, cols, src_stride, dst_stride;
+} gs_rows;
+int gs_rows_pack(const gs_rows* sets, int n, int dtype, void* stream);
 size_t gs_linear_fwd_workspace_size(const gs_linear* args);
 int gs_linear_fwd(const gs_linear* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t gs_linear_bwd_workspace_size(const gs_linear* args);

@@ -154,15 +154,19 @@ def test_linear_calls():
     # few rows are read at any address, but for gradients
     expect(L.gs_linear_fwd(C.byref(linear_args(rows=32, x=260, x_stride=65, weight=258)), None, 0, None), ALIGN, "misaligned")
     expect(L.gs_linear_bwd(C.byref(linear_args(rows=32, x=260)), 256, 256, 256, 256, 256, 1 << 62, None), ALIGN, "misaligned")
-    pack = lambda src=256, rows=4, cols=60, dst=256, ld=64, dtype=0: L.gs_rows_pack(src, rows, cols, 70, dst, ld, dtype, None)  # noqa: E731
+    rows = lambda **kw: _lib.GsRows(**{**dict(src=256, dst=256, rows=4, cols=60, src_stride=70, dst_stride=64), **kw})  # noqa: E731
+    pack = lambda n=2, dtype=0, **kw: L.gs_rows_pack((_lib.GsRows * 2)(rows(), rows(**kw)), n, dtype, None)  # noqa: E731
     expect(pack(dtype=1), ARG, "dtype")
+    expect(pack(n=3), ARG, "two sets")
+    expect(L.gs_rows_pack(None, 1, 0, None), ARG, "two sets")
     expect(pack(rows=-1), ARG, "size")
-    expect(pack(ld=60), ARG, "size")
-    expect(pack(ld=56), ARG, "size")
+    expect(pack(dst_stride=60), ARG, "size")
+    expect(pack(dst_stride=56), ARG, "size")
     expect(pack(src=None), ARG, "null")
     expect(pack(dst=264), ALIGN, "misaligned")
     expect(pack(src=258), ALIGN, "misaligned")
-    expect(pack(rows=1 << 31, ld=1 << 10), ARG, "too many")
+    expect(pack(rows=1 << 31, dst_stride=1 << 10), ARG, "too many")
+    assert L.gs_rows_pack(None, 0, 0, None) == 0
     a = linear_args()
     need = L.gs_linear_bwd_workspace_size(C.byref(a))
     assert need > 0 and L.gs_linear_bwd_workspace_size(None) == 0 and L.gs_linear_fwd_workspace_size(None) == 0
