@@ -12,6 +12,10 @@ scenes' tokens are packed one after the other), and runs
 `SplatPredictor.cache` and `SplatPredictor.extend` are the serving form: a scene's keys and values are
 kept, and the tokens of one more view are run against them.
 
+With `--fused` the blocks are the library's too: projections with their epilogue (linear), and what lies between
+blocks (residual_norm: norms on both sides, a gate, dropout). Layers may then mix by a recurrence over the
+views in order (gated_scan, `--scan 1,3`), whose time and state do not grow with the capture's square.
+
 The scenes are synthetic (random Gaussians rendered by the same rasterizer).
 """
 from __future__ import annotations
@@ -28,7 +32,8 @@ import torch.nn.functional as F
 if __package__ in (None, ""):
     sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
-from amdsplat import FusedAdam, attention, l1_ssim_loss, rasterize, rasterize_inference, rotary_axes
+from amdsplat import (FusedAdam, attention, gated_scan, l1_ssim_loss, linear, norm, rasterize, rasterize_inference,
+                      residual_norm, rotary_axes)
 from amdsplat.scenes import orbit_cameras
 
 GAUSSIAN = 3 + 3 + 4 + 1 + 3  # offset, log-scale, quaternion, opacity logit, colour coefficients
@@ -47,6 +52,10 @@ class Config:
     softcap: float = 30.0
     sections: tuple = (8, 12, 12)  # pairs of a head that turn with view, row and column
     dtype: torch.dtype = torch.bfloat16  # of the matrix products and attention; parameters are float32
+    fused: bool = False      # blocks of linear and residual_norm; the rest needs it
+    sandwich: bool = False   # a norm and a gate behind every block too
+    dropout: float = 0.0     # of every block's output, in training
+    scan: tuple = ()         # layers that mix by gated_scan instead of attention
 
 
 def rays(cam, device):
@@ -77,20 +86,30 @@ class SplatPredictor(torch.nn.Module):
 
         inputs = 9 * c.patch * c.patch  # colour, ray origin, ray direction
         heads = c.heads + 2 * c.kv_heads
+        if not c.fused and (c.sandwich or c.dropout or c.scan):
+            raise ValueError("sandwich, dropout and scan need fused")
         self.embed = weight(c.width, inputs)
         self.layers = torch.nn.ModuleList()
-        for _ in range(c.depth):
+        inner = c.heads * c.head_dim
+        for i in range(c.depth):
             layer = torch.nn.ParameterDict({
                 "norm1": torch.nn.Parameter(torch.ones(c.width, device=device)),
-                "qkv": weight(heads * c.head_dim, c.width),
+                "qkv": weight(3 * inner if i in c.scan else heads * c.head_dim, c.width),
                 "out": weight(c.width, c.heads * c.head_dim, gain=0.5),
                 "norm2": torch.nn.Parameter(torch.ones(c.width, device=device)),
                 "up": weight(4 * c.width, c.width),
                 "down": weight(c.width, 4 * c.width, gain=0.5),
             })
+            if c.sandwich:
+                for name, value in (("post1", 1.0), ("gate1", 0.5), ("post2", 1.0), ("gate2", 0.5)):
+                    layer[name] = torch.nn.Parameter(torch.full((c.width,), value, device=device))
+            if i in c.scan:  # values, forget gates (a memory of some eight tokens to begin with), output gates
+                layer["gates"] = torch.nn.Parameter(torch.tensor([0.0, 2.0, 0.0]).repeat_interleave(inner).to(device))
             self.layers.append(layer)
         self.norm = torch.nn.Parameter(torch.ones(c.width, device=device))
         self.head = weight(c.per_patch * (GAUSSIAN + 1), c.width, gain=0.1)
+        # of dropout; train_step advances it
+        self.register_buffer("seed", torch.full((1,), seed, dtype=torch.int64, device=device), persistent=False)
 
     def linear(self, x, w):
         return F.linear(x.to(self.config.dtype), w.to(self.config.dtype))
@@ -113,6 +132,34 @@ class SplatPredictor(torch.nn.Module):
         y = F.gelu(self.linear(self.rms(x, layer["norm2"]), layer["up"]))
         return x + self.linear(y, layer["down"]).float()
 
+    # ---- fused blocks: n is the stream x, normed for the next block ----
+
+    def project(self, n, w, **epilogue):
+        return linear(n, w.to(self.config.dtype), **epilogue)
+
+    def between(self, i: int, half: int, x, y):
+        """The stream after block `half` (1: mixer, 2: MLP) of layer i, and its norm for the next block."""
+        c, layer = self.config, self.layers[i]
+        after = layer["norm2"] if half == 1 else (self.layers[i + 1]["norm1"] if i + 1 < c.depth else self.norm)
+        post, gate = (layer[f"post{half}"], layer[f"gate{half}"]) if c.sandwich else (None, None)
+        return residual_norm(x, y, after, post_weight=post, gate=gate, dropout=c.dropout if self.training else 0.0,
+                             seed=self.seed, draw=2 * i + half)
+
+    def blocks(self, x, positions, attend, scan):
+        """All layers: attend(i, q, k, v) and scan(i, values, forget, gate) mix the tokens. Returns the normed stream."""
+        c = self.config
+        n = norm(x, self.layers[0]["norm1"], dtype=c.dtype)
+        for i, layer in enumerate(self.layers):
+            if i in c.scan:
+                a = scan(i, *self.project(n, layer["qkv"], bias=layer["gates"]).chunk(3, 1))
+            else:
+                qkv = self.project(n, layer["qkv"]).view(-1, c.heads + 2 * c.kv_heads, c.head_dim)
+                q, k, v = qkv.split((c.heads, c.kv_heads, c.kv_heads), 1)
+                a = attend(i, *rotary_axes(q, k, positions, c.sections), v).flatten(1)
+            x, n = self.between(i, 1, x, self.project(a, layer["out"]))
+            x, n = self.between(i, 2, x, self.project(self.project(n, layer["up"], activation="gelu"), layer["down"]))
+        return n
+
     def tokens(self, images, cams):
         """Tokens of a scene's views: embeddings [T, width] and places (view, row, column) [T, 3]."""
         c = self.config
@@ -132,6 +179,11 @@ class SplatPredictor(torch.nn.Module):
         lens = [x.shape[0] for x, _ in pairs]
         x, positions = torch.cat([x for x, _ in pairs]), torch.cat([p for _, p in pairs])
         offsets = torch.tensor([0] + lens, device=x.device).cumsum(0).int()
+        if c.fused:
+            n = self.blocks(x, positions, lambda i, q, k, v: attention(q, k, v, offsets=offsets, softcap=c.softcap),
+                            lambda i, v, f, o: gated_scan(v, f, o, offsets=offsets))
+            raw = self.project(n, self.head).float()
+            return [self.gaussians(r, cams) for r, (_, cams) in zip(raw.split(lens), scenes)]
         for layer in self.layers:
             q, k, v = self.heads_of(x, layer, positions)
             x = self.rest(x, attention(q, k, v, offsets=offsets, softcap=c.softcap), layer)
@@ -164,6 +216,20 @@ class SplatPredictor(torch.nn.Module):
         x, positions = self.tokens(images, cams)
         n = x.shape[0]
         kept = []
+        if c.fused:
+            kept = [None] * c.depth
+
+            def attend(i, q, k, v):
+                kept[i] = [torch.empty(room, c.kv_heads, c.head_dim, dtype=c.dtype, device=x.device) for _ in "kv"]
+                kept[i][0][:n], kept[i][1][:n] = k, v
+                return attention(q, k, v, softcap=c.softcap)
+
+            def scan(i, v, f, o):
+                y, kept[i] = gated_scan(v, f, o, return_state=True)
+                return y
+
+            self.blocks(x, positions, attend, scan)
+            return dict(kept=kept, length=n, views=len(cams))
         for layer in self.layers:
             q, k, v = self.heads_of(x, layer, positions)
             keys, values = (torch.empty(room, c.kv_heads, c.head_dim, dtype=c.dtype, device=x.device) for _ in "kv")
@@ -181,6 +247,23 @@ class SplatPredictor(torch.nn.Module):
         positions[:, 0] += cache["views"]
         n, m = cache["length"], x.shape[0]
         as_table = lambda *v: torch.tensor(v, dtype=torch.int32, device=x.device)  # noqa: E731
+        if c.fused:
+            kept = cache["kept"]
+
+            def attend(i, q, k, v):
+                keys, values = kept[i]
+                keys[n:n + m], values[n:n + m] = k, v
+                return attention(q, keys, values, offsets=as_table(0, m), k_offsets=as_table(0, keys.shape[0]),
+                                 k_lengths=as_table(n + m), softcap=c.softcap)
+
+            def scan(i, v, f, o):
+                y, kept[i] = gated_scan(v, f, o, initial=kept[i], return_state=True)
+                return y
+
+            normed = self.blocks(x, positions, attend, scan)
+            cache["length"] += m
+            cache["views"] += 1
+            return self.gaussians(self.project(normed, self.head).float(), [cam])
         for layer, (keys, values) in zip(self.layers, cache["kept"]):
             q, k, v = self.heads_of(x, layer, positions)
             keys[n:n + m], values[n:n + m] = k, v
@@ -213,6 +296,7 @@ def train_step(model, optimizer, scenes, max_norm: float = 1.0):
     Returns (loss, gradient norm) as device tensors."""
     for p in model.parameters():
         p.grad = None
+    model.seed += 1
     loss = 0.0
     for splats, (images, cams) in zip(model([(im[:-1], cams[:-1]) for im, cams in scenes]), scenes):
         cam = cams[-1]
@@ -231,8 +315,12 @@ def main():
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     ap.add_argument("--steps", type=int, default=200)
     ap.add_argument("--scenes", type=int, default=3)
+    ap.add_argument("--fused", action="store_true", help="blocks of linear and residual_norm, with norms, gates and dropout")
+    ap.add_argument("--scan", default="", help="with --fused: layers that mix by gated_scan, as 1,3")
     a = ap.parse_args()
     config = Config()
+    if a.fused:
+        config = Config(fused=True, sandwich=True, dropout=0.05, scan=tuple(int(i) for i in a.scan.split(",") if i))
     model = SplatPredictor(config)
     optimizer = optimizer_for(model)
     scenes = [synthetic_scene(i, 3 + i % 3, config.image) for i in range(a.scenes)]
@@ -240,6 +328,7 @@ def main():
         loss, norm = train_step(model, optimizer, scenes)
         if step % 20 == 0 or step == a.steps - 1:
             print(f"step {step}: loss {float(loss):.4f}, gradient norm {float(norm):.3f}", flush=True)
+    model.eval()
     images, cams = scenes[0]
     cache = model.cache(images[:-1], cams[:-1], room=1024)
     splats = model.extend(cache, images[-1], cams[-1])
