@@ -13,6 +13,7 @@
 //
 // Few rows are bound by reading W once: linear_few_kernel streams it past the matrix unit without LDS.
 #include <algorithm>
+#include <type_traits>
 
 #include "gs_attention.h"
 #include "gs_rows.h"
@@ -160,63 +161,98 @@ struct TileAt {
   }
 };
 
-// Bias, activation, residual and store of columns col .. col + 7 of a row (the first n of them).
+// The epilogue of columns col .. col + 7 of a row (the first n of them): bias, activation, residual and store. The residual is
+// loaded apart, long before.
+struct Epilogue8 {
+  RawAny8 residual;
+  __device__ __forceinline__ void load(const GemmArgs& g, int64_t row, int col, int n) {
+    if (g.residual) residual.load(g.residual, g.residual_bf16, row * g.residual_stride + col, n);
+  }
+  template <typename T>
+  __device__ __forceinline__ void finish(const GemmArgs& g, int64_t row, int col, int n, const float (&bias)[8],
+                                         float (&v)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += bias[j];
+    if (g.z) store8(g.z, g.z_bf16, row * g.n + col, n, v);
+    if (g.act != kActNone) activate8<T>(g.act, v);
+    if (g.residual) {
+      float r[8];
+      residual.to(r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += r[j];
+    }
+    store8(g.out, g.out_bf16, row * g.n + col, n, v);
+  }
+};
+__device__ __forceinline__ void bias8(const GemmArgs& g, int col, int n, float (&bias)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = 0.0f;
+  if (g.bias) load8(g.bias, g.bias_bf16, col, n, bias);
+}
 template <typename T>
 __device__ __forceinline__ void finish8(const GemmArgs& g, int64_t row, int col, int n, float (&v)[8]) {
-  if (g.bias) {
-    float b[8];
-    load8(g.bias, g.bias_bf16, col, n, b);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += b[j];
-  }
-  if (g.z) store8(g.z, g.z_bf16, row * g.n + col, n, v);
-  if (g.act != kActNone) activate8<T>(g.act, v);
-  if (g.residual) {
-    float r[8];
-    load8(g.residual, g.residual_bf16, row * g.residual_stride + col, n, r);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += r[j];
-  }
-  store8(g.out, g.out_bf16, row * g.n + col, n, v);
+  Epilogue8 e;
+  float bias[8];
+  e.load(g, row, col, n);
+  bias8(g, col, n, bias);
+  e.template finish<T>(g, row, col, n, bias, v);
 }
 
 template <typename T>
-constexpr int kStage = 128 / static_cast<int>(sizeof(T));  // contraction of a stage
-template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 
-// One side of a tile: ROWS rows (or columns) of an operand, a stage of them in LDS. ALONG: the operand's rows run
-// along the contraction.
-template <typename T, bool ALONG, int ROWS, int THREADS>
+// One side of a tile: ROWS rows (or columns) of an operand, in LDS a stage of KB of the contraction. ALONG: the operand's
+// rows run along the contraction.
+template <typename T, int KB, bool ALONG, int ROWS, int THREADS>
 struct Side {
-  static constexpr int kWidth = ALONG ? kStage<T> : (ROWS * static_cast<int>(sizeof(T)) < 256 ? ROWS : 256 / static_cast<int>(sizeof(T)));
+  static constexpr int kWidth = ALONG ? KB : (ROWS * static_cast<int>(sizeof(T)) < 256 ? ROWS : 256 / static_cast<int>(sizeof(T)));
   static constexpr int kSubs = ALONG ? 1 : ROWS / kWidth;
-  static constexpr int kBytes = ROWS * 128;
+  static constexpr int kBytes = ROWS * KB * static_cast<int>(sizeof(T));
   using L = Tile<T, kWidth>;
-  using Copy = TileCopy<T, kWidth, ALONG ? ROWS : kStage<T>, THREADS>;
+  using Copy = TileCopy<T, kWidth, THREADS / L::kChunks, THREADS>;  // one step
+  static_assert(Copy::kOneOffset, "steps are whole periods of the chunks' permutation");
   const T* base;
   int64_t ld;
   int rows;  // there are from the tile's first on
   __device__ __forceinline__ Side(const void* p, int64_t ld_, int64_t row0, int64_t all)
       : base(static_cast<const T*>(p) + row0 * (ALONG ? ld_ : 1)), ld(ld_),
         rows(static_cast<int>(all - row0 < ROWS ? all - row0 : ROWS)) {}
-  // Contraction k0 .. of `left` more; what is past the operand's end is zero. Rows are there to a whole vector: where
-  // they run along the contraction its rest is zero in one operand at least, where columns are copied it
-  // ends in results that are not stored.
-  __device__ __forceinline__ void stage(char* lds, int64_t k0, int64_t left) const {
-    const int n = left < kStage<T> ? static_cast<int>(left) : kStage<T>;
+  // A stage's copy, contraction k0 .. of `left` more, which kSteps instructions of every lane make. What is past the operand's
+  // end is zero. Rows are there to a whole vector: where they run along the contraction its rest is zero in one operand
+  // at least, where columns are copied it ends in results that are not stored.
+  static constexpr int kSteps = kBytes / (THREADS * 16), kSubSteps = kSteps / kSubs;
+  struct Stage {
+    uint32_t offset[kSubs];
+    __amdgpu_buffer_rsrc_t src[kSubs];
+  };
+  __device__ __forceinline__ Stage stage(int64_t k0, int64_t left) const {
+    const int n = left < 0 ? 0 : (left < KB ? static_cast<int>(left) : KB);
     if constexpr (ALONG) {
       const int whole = (n + kVec<T> - 1) / kVec<T> * kVec<T>;
-      Copy(ld, whole)(lds, row_buffer(base + k0, ld, rows, whole));
+      return {{Copy(ld, whole).offset}, {row_buffer(base + k0, ld, rows, whole)}};
     } else {
-#pragma unroll
-      for (int s = 0; s < kSubs; ++s) {
-        const int cols = (rows + kVec<T> - 1) / kVec<T> * kVec<T> - s * kWidth;
-        const int dim = cols < 0 ? 0 : (cols < kWidth ? cols : kWidth);
-        Copy(ld, dim)(lds + s * kStage<T> * L::kRowBytes, row_buffer(base + k0 * ld + s * kWidth, ld, dim ? n : 0, dim));
-      }
+      const auto cols = [&](int s) {
+        const int c = (rows + kVec<T> - 1) / kVec<T> * kVec<T> - s * kWidth;
+        return c < 0 ? 0 : (c < kWidth ? c : kWidth);
+      };
+      const auto src = [&](int s) {
+        return row_buffer(base + k0 * ld + s * kWidth, ld, cols(s) ? n : 0, cols(s));
+      };
+      static_assert(kSubs <= 2, "at most two side by side");
+      if constexpr (kSubs == 1) return {{Copy(ld, cols(0)).offset}, {src(0)}};
+      else return {{Copy(ld, cols(0)).offset, Copy(ld, cols(1)).offset}, {src(0), src(1)}};
     }
   }
+  __device__ __forceinline__ void step(char* lds, const Stage& st, int i) const {
+    Copy c(ld, kWidth);
+    c.offset = st.offset[i / kSubSteps] + i % kSubSteps * c.step;  // (kNowhere stays outside)
+    c(lds + i * (THREADS * 16), st.src[i / kSubSteps]);
+  }
+  __device__ __forceinline__ void steps(char* lds, const Stage& st) const {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) step(lds, st, i);
+  }
+
   // Rows row0 + l % 32, contraction slots of group c of sixteen: both sides list them in the same order.
   static __device__ __forceinline__ Frag<T> frag(const char* lds, int row0, int c, int lane) {
     if constexpr (ALONG && sizeof(T) == 2) {
@@ -227,7 +263,7 @@ struct Side {
       const f32x4 b = *reinterpret_cast<const f32x4*>(lds + L::at(row, 4 * c + 2 + h));
       return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     } else {
-      lds += row0 / kWidth * (kStage<T> * L::kRowBytes);
+      lds += row0 / kWidth * (KB * L::kRowBytes);
       row0 %= kWidth;
       if constexpr (sizeof(T) == 4) {
         return L::cols(lds, row0, 16 * c, lane);
@@ -249,12 +285,14 @@ template <typename T, int BM, int BN, int WM, int WN, bool A_ALONG, bool B_ALONG
 __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
   constexpr int kThreads = WM * WN * kWave;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 results of a wavefront
-  constexpr int kStageBytes = (BM + BN) * 128;
+  constexpr bool kDeep = TM * TN == 16;
+  constexpr int KB = 128 / static_cast<int>(sizeof(T)), kStages = 2, kGroups = KB / 16;
+  using A = Side<T, KB, A_ALONG, BM, kThreads>;
+  using B = Side<T, KB, B_ALONG, BN, kThreads>;
+  constexpr int kStageBytes = A::kBytes + B::kBytes;
   constexpr int kRowFloats = TN * 32 + 4;  // of the epilogue's rows, padded against bank conflicts
   constexpr int kOutBytes = WM * WN * 32 * kRowFloats * 4;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStageBytes > kOutBytes ? 2 * kStageBytes : kOutBytes];
-  using A = Side<T, A_ALONG, BM, kThreads>;
-  using B = Side<T, B_ALONG, BN, kThreads>;
+  __shared__ __attribute__((aligned(16))) char lds[kStages * kStageBytes > kOutBytes ? kStages * kStageBytes : kOutBytes];
   const bool whole = static_cast<int>(blockIdx.x) < g.whole;
   const int other = whole ? 0 : xcd_tile(blockIdx.x - g.whole, gridDim.x - g.whole), split = other % g.splits;
   const TileAt at(g, whole ? xcd_tile(blockIdx.x, g.whole) : g.whole + other / g.splits, BM, BN);
@@ -268,51 +306,121 @@ __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   f32x16 acc[TM][TN] = {};
-  char *now = lds, *next = lds + kStageBytes;
-  if (k_begin < k_end) {
-    a.stage(now, k_begin, k_end - k_begin);
-    b.stage(now + A::kBytes, k_begin, k_end - k_begin);
-  }
-  for (int64_t k0 = k_begin; k0 < k_end; k0 += kStage<T>) {
-    copies_done();
-    __syncthreads();  // everyone's copies are there, and everyone has left the other stage
-    if (k0 + kStage<T> < k_end) {
-      a.stage(next, k0 + kStage<T>, k_end - k0 - kStage<T>);
-      b.stage(next + A::kBytes, k0 + kStage<T>, k_end - k0 - kStage<T>);
+  const auto stage = [&](char* to, int64_t k0) {
+    a.steps(to, a.stage(k0, k_end - k0));
+    b.steps(to + A::kBytes, b.stage(k0, k_end - k0));
+  };
+  if constexpr (kDeep) {
+    // One wavefront a SIMD, so that what a tile's sides read of LDS is least; nothing else runs while it waits. Fragments are read
+    // one group of sixteen ahead of the products. Past a stage's last reads the wavefronts meet: the next stage has been
+    // copied, and this one may be overwritten. Reads and copies are sent between products, one at a time: together they
+    // would leave the matrix unit idle while they are issued.
+    char *now = lds, *next = lds + kStageBytes;
+    Frag<T> fa[2][TM], fb[2][TN];
+    const auto fetch = [&](const char* from, int c, int to, int i) {
+      if (i < TM) fa[to][i] = A::frag(from, wm + 32 * i, c, lane);
+      else if (i < TM + TN) fb[to][i - TM] = B::frag(from + A::kBytes, wn + 32 * (i - TM), c, lane);
+    };
+    if (k_begin < k_end) {
+      stage(now, k_begin);
+      copies_done();
+      __syncthreads();
+      if (k_begin + KB < k_end) stage(next, k_begin + KB);
+#pragma unroll
+      for (int i = 0; i < TM + TN; ++i) fetch(now, 0, 0, i);
     }
+    // one stage; MORE: another follows, MOST: one more after that, which is copied here
+    const auto turn = [&](auto more, auto most, int64_t k0) {
+      constexpr bool MORE = decltype(more)::value, MOST = decltype(most)::value;
+      typename A::Stage sa;
+      typename B::Stage sb;
 #pragma unroll
-    for (int c = 0; c < kStage<T> / 16; ++c) {
-      Frag<T> fa[TM], fb[TN];
+      for (int c = 0; c < kGroups; ++c) {
+        const bool last = c + 1 == kGroups;
+        if (last && MORE) {
+          copies_done();
+          __syncthreads();
+        }
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = A::frag(now, wm + 32 * i, c, lane);
+        for (int t = 0; t < TM * TN; ++t) {
+          mma(acc[t / TN][t % TN], fb[c % 2][t % TN], fa[c % 2][t / TN]);
+          if (!last) fetch(now, c + 1, (c + 1) % 2, t);
+          else if (MORE) fetch(next, 0, 0, t);
+          if (MOST && c == 1 && t == 8) sa = a.stage(k0 + 2 * KB, k_end - k0 - 2 * KB);
+          if (MOST && c == 2 && t == 8) sb = b.stage(k0 + 2 * KB, k_end - k0 - 2 * KB);
+          if (MOST && last) {
+            if (t < A::kSteps) a.step(now, sa, t);
+            else b.step(now + A::kBytes, sb, t - A::kSteps);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      char* s = now;
+      now = next;
+      next = s;
+    };
+    static_assert(A::kSteps + B::kSteps == TM * TN && kGroups == 4, "a copy for each product of the last group");
+    using Yes = std::true_type;
+    using No = std::false_type;
+    int64_t k0 = k_begin;
+    for (; k0 + 2 * KB < k_end; k0 += KB) turn(Yes{}, Yes{}, k0);
+    if (k0 + KB < k_end) {
+      turn(Yes{}, No{}, k0);
+      k0 += KB;
+    }
+    if (k0 < k_end) turn(No{}, No{}, k0);
+  } else {
+    char *now = lds, *next = lds + kStageBytes;
+    if (k_begin < k_end) stage(now, k_begin);
+    for (int64_t k0 = k_begin; k0 < k_end; k0 += KB) {
+      copies_done();
+      __syncthreads();  // everyone's copies are there, and everyone has left the other stage
+      if (k0 + KB < k_end) stage(next, k0 + KB);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fb[j] = B::frag(now + A::kBytes, wn + 32 * j, c, lane);
-      if constexpr (sizeof(T) == 2) {
+      for (int c = 0; c < kGroups; ++c) {
+        Frag<T> fa[TM], fb[TN];
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i) fa[i] = A::frag(now, wm + 32 * i, c, lane);
 #pragma unroll
-          for (int j = 0; j < TN; ++j) mma(acc[i][j], fb[j], fa[i]);
-      } else {  // one pair of slots over all results, then the next: no product waits for the one before it
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int j = 0; j < TN; ++j) fb[j] = B::frag(now + A::kBytes, wn + 32 * j, c, lane);
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
           for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][s], fa[i][s], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TN; ++j) mma(acc[i][j], fb[j], fa[i]);
+        } else {  // one pair of slots over all results, then the next: no product waits for the one before it
+#pragma unroll
+          for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int j = 0; j < TN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(fb[j][s], fa[i][s], acc[i][j], 0, 0, 0);
+        }
       }
+      char* s = now;
+      now = next;
+      next = s;
     }
-    char* s = now;
-    now = next;
-    next = s;
   }
   __syncthreads();
   // A lane holds row l % 32 and of every 32 columns 8 (r / 4) + 4 (l / 32) + r % 4: 32 rows at a time through the
-  // wavefront's own LDS, then eight neighbouring columns a lane.
-  constexpr int kLanes = TN * 4;  // of a row
+  // wavefront's own LDS, then eight neighbouring columns a lane, residuals loaded before (more than two turns ahead
+  // the code of 16 x 32 x 32 results is longer than the compiler unrolls, which leaves the results in memory).
+  constexpr int kLanes = TN * 4, kRows = kWave / kLanes, kAhead = TN == 4 ? 2 : 32 / kRows;
   float* own = reinterpret_cast<float*>(lds) + wave * 32 * kRowFloats;
+  const int c8 = lane % kLanes * 8, col = n0 + wn + c8;
+  const int64_t m_lane = m0 + wm + lane / kLanes;
+  const auto left = [&](int r) { return m_lane + r < g.m ? g.n - col : 0; };
+  float bias[8];
+  if (whole) bias8(g, col, g.n - col, bias);
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
+    Epilogue8 e[kAhead];
+    if (whole) {
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) e[q].load(g, m_lane + 32 * i + q * kRows, col, left(32 * i + q * kRows));
+    }
     wave_sync();
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -321,18 +429,21 @@ __global__ __launch_bounds__(WM* WN* kWave) void gemm_kernel(GemmArgs g) {
         store4(own + (lane & 31) * kRowFloats + 32 * j + 2 * r + 4 * (lane >> 5), acc[i][j][r], acc[i][j][r + 1],
                acc[i][j][r + 2], acc[i][j][r + 3]);
     wave_sync();
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += kAhead * kRows) {
 #pragma unroll
-    for (int r = 0; r < 32; r += kWave / kLanes) {
-      const int row = r + lane / kLanes, c = lane % kLanes * 8;
-      const int64_t m = m0 + wm + 32 * i + row;
-      const int col = n0 + wn + c, n = m < g.m ? g.n - col : 0;
-      float v[8];
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(own + row * kRowFloats + c);
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(own + row * kRowFloats + c + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
-      if (!whole) store8(g.part + (static_cast<int64_t>(other) * BM + wm + 32 * i + row) * BN + wn + c, 8, v);
-      else if (n > 0) finish8<T>(g, m, col, n, v);
+      for (int q = 0; q < kAhead; ++q) {
+        const int r = r0 + q * kRows, in = 32 * i + r, n = left(in);
+        const float* at = own + (r + lane / kLanes) * kRowFloats + c8;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(at), hi = *reinterpret_cast<const f32x4*>(at + 4);
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if (whole) {
+          if (n > 0) e[q].template finish<T>(g, m_lane + in, col, n, bias, v);
+          if (r + kAhead * kRows < 32) e[q].load(g, m_lane + in + kAhead * kRows, col, left(in + kAhead * kRows));
+        } else {
+          store8(g.part + (static_cast<int64_t>(other) * BM + wm + in + lane / kLanes) * BN + wn + c8, 8, v);
+        }
+      }
     }
   }
 }
@@ -573,7 +684,7 @@ static int run_gemm(GemmArgs g, const GemmPlan& p, void* workspace, const char* 
   g.split_k = p.split_k;
   g.part = static_cast<float*>(workspace);
   if constexpr (sizeof(T) == 2) {
-    if (p.tile == 256) return launch_gemm<T, 256, 2, 4, A_ALONG, B_ALONG>(g, what, st);
+    if (p.tile == 256) return launch_gemm<T, 256, 2, 2, A_ALONG, B_ALONG>(g, what, st);
   }
   if (p.tile == 128) return launch_gemm<T, 128, 2, 2, A_ALONG, B_ALONG>(g, what, st);
   return launch_gemm<T, 64, 2, 2, A_ALONG, B_ALONG>(g, what, st);
