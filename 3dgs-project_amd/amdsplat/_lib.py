@@ -347,6 +347,18 @@ def call(name: str, *args) -> None:
         raise AmdSplatError(f"{name} failed (code {rc}): {msg}")
 
 
+def call_on(device, name: str, *args) -> None:
+    """call(name, *args, stream) on the current stream of `device`, which is made the current device for it: the null
+    stream's handle says nothing of its device."""
+    import torch
+
+    if torch._C._cuda_getDevice() == device.index:
+        call(name, *args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_handle(device))
+
+
 def size_call(name: str, *args) -> int:
     return int(getattr(lib(), name)(*args))
 

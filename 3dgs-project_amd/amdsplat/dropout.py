@@ -7,7 +7,7 @@ import torch
 
 from . import _lib
 from ._grad import tracked
-from ._lib import call
+from ._lib import call_on
 
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
 
@@ -42,8 +42,8 @@ def _drop(x, rule):
     else:
         x, stride = x.contiguous(), width
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    call("gs_dropout", x.data_ptr(), out.data_ptr(), rows, stride, width, _DTYPES[x.dtype], p,
-         None if seed_at is None else seed_at.data_ptr(), seed, draw, _lib.stream_handle(x.device))
+    call_on(x.device, "gs_dropout", x.data_ptr(), out.data_ptr(), rows, stride, width, _DTYPES[x.dtype], p,
+            None if seed_at is None else seed_at.data_ptr(), seed, draw)
     return out
 
 

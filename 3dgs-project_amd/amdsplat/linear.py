@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._grad import tracked
-from ._lib import call, ptr
+from ._lib import call_on, ptr
 
 MAX_WIDTH, FEW_ROWS = 1 << 19, 32  # GS_LINEAR_MAX_WIDTH, GS_LINEAR_FEW_ROWS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # GS_ACT_*
@@ -46,7 +46,7 @@ def _pack(x, weight, few: bool):
     for r, t in zip(sets, away):
         r.src, r.dst, r.rows, r.cols, r.src_stride, r.dst_stride = t.data_ptr(), to, t.shape[0], t.shape[1], t.stride(0), wide
         to += t.shape[0] * wide * t.element_size()
-    call("gs_rows_pack", sets, len(away), _DTYPES[x.dtype][0], _lib.stream_handle(x.device))
+    call_on(x.device, "gs_rows_pack", sets, len(away), _DTYPES[x.dtype][0])
     return buffer
 
 
@@ -81,7 +81,7 @@ def _forward(x, weight, bias, residual, activation, out_dtype, keep: bool):
         z = torch.empty(out.shape, dtype=x.dtype if bias is None else torch.float32, device=x.device)
     a = _args(x, weight, buffer, few, bias, residual, out, z, out_dtype, activation)
     ws, n = _workspace("gs_linear_fwd_workspace_size", a, x.device)
-    call("gs_linear_fwd", C.byref(a), ptr(ws), n, _lib.stream_handle(x.device))
+    call_on(x.device, "gs_linear_fwd", C.byref(a), ptr(ws), n)
     return out, z, buffer
 
 
@@ -108,7 +108,7 @@ class _Linear(torch.autograd.Function):
                      for t, need in zip((x, weight, bias), ctx.needs_input_grad)]
             a = _args(x, weight, buffer, False, bias, None, None, z, *ctx.rule)
             ws, n = _workspace("gs_linear_bwd_workspace_size", a, x.device)
-            call("gs_linear_bwd", C.byref(a), ptr(d), *map(ptr, grads), ptr(ws), n, _lib.stream_handle(x.device))
+            call_on(x.device, "gs_linear_bwd", C.byref(a), ptr(d), *map(ptr, grads), ptr(ws), n)
         return (*grads, d_out if ctx.needs_input_grad[3] else None, None, None)
 
 

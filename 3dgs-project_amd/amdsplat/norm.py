@@ -14,7 +14,7 @@ import torch
 
 from . import _lib
 from ._grad import tracked
-from ._lib import call, ptr
+from ._lib import call_on, ptr
 from .dropout import check_rule
 
 MAX_WIDTH = 16384  # GS_NORM_MAX_WIDTH
@@ -45,7 +45,7 @@ def _forward(x, y, weight, bias, post_weight, post_bias, gate, seed_at, rule, ke
     n = torch.empty(x.shape, dtype=rule[-1], device=x.device)
     stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device) if keep else None
     a = _args(x, y, weight, bias, post_weight, post_bias, gate, seed_at, h, n, stats, rule)
-    call("gs_residual_norm_fwd", C.byref(a), _lib.stream_handle(x.device))
+    call_on(x.device, "gs_residual_norm_fwd", C.byref(a))
     return h, n, stats
 
 
@@ -70,9 +70,7 @@ class _ResidualNorm(torch.autograd.Function):
         a = _args(x, y, *weights, gate, seed_at, None, None, stats, ctx.rule)
         size = _lib.size_call("gs_residual_norm_bwd_workspace_size", C.byref(a))
         ws = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
-        d_x, d_y, d_weight, d_bias, d_post_weight, d_post_bias, d_gate = outs
-        call("gs_residual_norm_bwd", C.byref(a), ptr(d_h), ptr(d_n), ptr(d_x), ptr(d_y), ptr(d_weight), ptr(d_bias),
-             ptr(d_post_weight), ptr(d_post_bias), ptr(d_gate), ws.data_ptr(), size, _lib.stream_handle(x.device))
+        call_on(x.device, "gs_residual_norm_bwd", C.byref(a), ptr(d_h), ptr(d_n), *map(ptr, outs), ws.data_ptr(), size)
         return (*outs, None, None)
 
 

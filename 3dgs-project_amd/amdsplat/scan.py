@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._grad import tracked
-from ._lib import call, ptr
+from ._lib import call_on, ptr
 
 MAX_WIDTH = 1 << 20  # GS_SCAN_MAX_WIDTH
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
@@ -45,7 +45,7 @@ def _forward(x, forget, gate, initial, offsets, reverse, keep: bool, want_state:
         carry = torch.empty((chunks, x.shape[1]), dtype=torch.float32, device=x.device)
     a = _args(x, forget, gate, initial, offsets, reverse, y, state, carry)
     ws, n = _workspace(x)
-    call("gs_gated_scan_fwd", C.byref(a), ptr(ws), n, _lib.stream_handle(x.device))
+    call_on(x.device, "gs_gated_scan_fwd", C.byref(a), ptr(ws), n)
     return y, state, carry
 
 
@@ -70,8 +70,7 @@ class _GatedScan(torch.autograd.Function):
                 for t, need in zip((x, forget, gate, initial), ctx.needs_input_grad)]
         a = _args(x, forget, gate, initial, offsets, ctx.reverse, None, None, carry)
         ws, n = _workspace(x)
-        call("gs_gated_scan_bwd", C.byref(a), ptr(d_y), ptr(d_state), *map(ptr, outs), ptr(ws), n,
-             _lib.stream_handle(x.device))
+        call_on(x.device, "gs_gated_scan_bwd", C.byref(a), ptr(d_y), ptr(d_state), *map(ptr, outs), ptr(ws), n)
         return (*outs, None, None, None)
 
 

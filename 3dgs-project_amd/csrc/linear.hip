@@ -730,9 +730,10 @@ static BackPlan back_plan(const gs_linear* p, bool bias) {
   // the output's gradient is the product's operand as it is where there is no activation, no rounding and no padding
   b.make_dz = p->activation != kActNone || p->out_dtype != p->dtype || p->outputs % per != 0;
   b.ld = (p->outputs + per - 1) / per * per;
-  // some thousand workgroups, of at most 64 rows, of one for each wavefront at least
+  // some thousand workgroups, of at most 64 rows (more only where a grid would pass its limit), of one for each wavefront at least
   const int64_t across = (p->outputs + kWave * 8 - 1) / (kWave * 8);
   b.rows = static_cast<int>(std::max<int64_t>(4, std::min<int64_t>(64, p->rows * across / 1024 / 4 * 4)));
+  b.rows = static_cast<int>(std::max<int64_t>(b.rows, p->rows * across >> 23));
   b.down = static_cast<int>((p->rows + b.rows - 1) / b.rows);
   b.dz = b.make_dz ? round16(static_cast<size_t>(p->rows) * b.ld * es) : 0;
   b.parts = bias ? round16(static_cast<size_t>(b.down) * p->outputs * sizeof(float)) : 0;

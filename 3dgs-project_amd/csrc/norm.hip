@@ -502,8 +502,10 @@ extern "C" int gs_residual_norm_fwd(const gs_residual_norm* p, void* stream) {
   NormArgs a;
   if (const int rc = check_norm(p, false, &a)) return rc;
   if (a.rows == 0) return GS_OK;
-  const auto run = [&](auto kernel, int lanes) {
+  const auto run = [&](auto kernel, int lanes) -> int {
     const int groups = std::max(1, 256 / lanes);
+    GS_REQUIRE((a.rows + groups - 1) / groups * std::max(256, lanes) < (int64_t(1) << 32), GS_ERR_ARG,
+               "residual norm: too many rows of this width");
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)), dim3(std::max(256, lanes)), 0,
                        as_stream(stream), a);
     return check_launch("residual norm");

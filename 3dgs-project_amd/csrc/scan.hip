@@ -303,6 +303,7 @@ __global__ __launch_bounds__(kJoinThreads) void scan_parts_kernel(ScanArgs a) {
   maps[run][lane] = make_double2(e, p);
   __syncthreads();
   double h = 0.0;
+#pragma unroll 4
   for (int r = 0; r < run; ++r) h = mapped(maps[r][lane].x, maps[r][lane].y, h);
   if (ch >= a.width) return;
 #pragma unroll

@@ -53,6 +53,7 @@ def test_norm_calls():
     back = lambda a, dh=256, dx=256, dy=256, dpw=256, dg=256, ws=256, n=need: L.gs_residual_norm_bwd(  # noqa: E731
         C.byref(a), dh, 256, dx, dy, 256, 256, dpw, 256, dg, ws, n, None)
     expect(L.gs_residual_norm_fwd(None, None), ARG, "NULL")
+    expect(L.gs_residual_norm_fwd(C.byref(norm_args(rows=(1 << 31) - 1, width=16384)), None), ARG, "too many")
     expect(L.gs_residual_norm_fwd(C.byref(norm_args(n=None)), None), ARG, "null")
     expect(L.gs_residual_norm_fwd(C.byref(norm_args(h=None)), None), ARG, "null")
     expect(back(norm_args(stats=None)), ARG, "statistics")
