@@ -14,7 +14,7 @@ from . import _lib
 from ._grad import tracked
 from ._lib import call_on, ptr
 
-MAX_WIDTH, FEW_ROWS = 1 << 19, 32  # GS_LINEAR_MAX_WIDTH, GS_LINEAR_FEW_ROWS
+MAX_WIDTH, FEW_ROWS = 1 << 19, 16  # GS_LINEAR_MAX_WIDTH, GS_LINEAR_FEW_ROWS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # GS_ACT_*
 _DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8)}
 
@@ -122,7 +122,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     keeps: in float32, or without a bias in x's dtype. No forward-mode derivative.
 
     x and weight are read through their row strides where these, the addresses and K are multiples of 16 bytes, and in a
-    forward of up to 32 rows wherever the last dimension is contiguous; otherwise they are copied first, at every call."""
+    forward of up to 16 rows wherever the last dimension is contiguous; otherwise they are copied first, at every call."""
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"x must be [tokens, inputs] and weight [outputs, inputs], got {tuple(x.shape)} and {tuple(weight.shape)}")
     if x.dtype not in _DTYPES or weight.dtype != x.dtype:

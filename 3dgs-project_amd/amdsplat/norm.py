@@ -17,7 +17,7 @@ from ._grad import tracked
 from ._lib import call_on, ptr
 from .dropout import check_rule
 
-MAX_WIDTH = 16384  # GS_NORM_MAX_WIDTH
+MAX_WIDTH = 8192  # GS_NORM_MAX_WIDTH
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
 
 
@@ -106,7 +106,7 @@ def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor
          eps: float = 1e-6, dtype: torch.dtype | None = None) -> torch.Tensor:
     """weight x^ + bias over the rows of x [T, C], x^ = x / sqrt(mean x^2 + eps), or with kind "layer"
     (x - mean x) / sqrt(var x + eps); differentiable in x, weight and bias ([C], one dtype, either may be None). dtype
-    of the result: x's by default, or bfloat16 of a float32 x. C up to 16384; the mean of a row's squares
+    of the result: x's by default, or bfloat16 of a float32 x. C up to 8192; the mean of a row's squares
     has to be finite in float32. No forward-mode derivative."""
     dtype = x.dtype if dtype is None else dtype
     layer, eps = _rule(x, kind, eps, dtype)

@@ -44,7 +44,7 @@ __device__ __forceinline__ float sigmoid(float v) {
 }
 // The normal distribution function, and exp(-z^2 / 2). float32: the library's erfc. bfloat16: Phi(-u) = exp(-u^2 / 2)
 // t P(t), t = 1 / (1 + 0.27 u), P of degree six fitted to erfcx(u / sqrt 2) / 2 over t by reweighted least squares:
-// off by 1.6e-6 of itself at most, so the tail is as exact as the middle (8203 x 4096 outputs: 9 us less than erfc).
+// off by 1.6e-6 of itself at most, so the tail is as exact as the middle (8203 x 1024 x 4096: 97 us, with erfc 115).
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& bell) {
   bell = exp_down<T>(-0.5f * z * z);
@@ -147,15 +147,17 @@ struct GemmArgs {
   float* part;       // [other tiles][splits][rows of a tile][columns of a tile]
 };
 
-// The first row and column of tile t. Tiles are taken in groups of eight rows of them, down a group's columns, and an XCD has a
-// contiguous share of that order: what its CUs work on together is a block of some eight by four tiles.
-constexpr int kTileGroup = 8;
+// The first row and column of tile t. Tiles are taken in groups of a few rows of them, down a group's columns, and an XCD has a
+// contiguous share of that order: what its 32 CUs work on together is a block of four by eight tiles of 256, or eight by
+// eight of 128 (two a CU), which reads the least of both operands. With eight by four of 256, a second turn reads the long
+// operand again: 16384 x 8192 x 4096 in groups of 4, 8, 16 rows 895, 960 and 966 us; of 128 8203 x 1024 x 4096 89, 88 and 89.
 struct TileAt {
   int64_t m0;
   int n0;
   __device__ __forceinline__ TileAt(const GemmArgs& g, int t, int bm, int bn) {
-    const int group = t / (kTileGroup * g.tiles_n), first = group * kTileGroup;
-    const int high = min(kTileGroup, g.tiles_m - first), in = t - first * g.tiles_n;
+    const int rows = bm == 256 ? 4 : 8;
+    const int group = t / (rows * g.tiles_n), first = group * rows;
+    const int high = min(rows, g.tiles_m - first), in = t - first * g.tiles_n;
     m0 = static_cast<int64_t>(first + in % high) * bm;
     n0 = in / high * bn;
   }
@@ -470,21 +472,23 @@ __global__ __launch_bounds__(kFinishThreads) void gemm_finish_kernel(GemmArgs g)
 
 // ---- few rows ----------------------------------------------------------------------------------------
 
-// Sixteen columns a workgroup, all rows (16 MT of them): its wavefronts take the contraction in turn, straight from
-// memory into the matrix instruction's operands, four loads of W in flight each, and are joined in LDS. Rows at any address
+// Sixteen columns a workgroup, up to sixteen rows: its wavefronts take the contraction in turn, from memory straight into the
+// matrix instruction's operands, four loads of W in flight each, and are joined in LDS. Rows at any address
 // and stride: loads are of an element's alignment, and the contraction's last vector is read element by element.
+// One row of 1024 x 4096 takes 4.1 us on the GPU, 8192 x 8192 31.5 us (4.3 TB/s). (32 rows in two sets read x twice as often as W:
+// 1024 x 4096 5.1 us, by tiles 8.1; 4096 x 1024 12.8 and 11.9; 8192 x 8192 45 and 26: those go to the tiles.)
 constexpr int kFewWaves = 8, kFewUnroll = 4;
-template <typename T, int MT>
+template <typename T>
 __global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g) {
   constexpr int kGroup = 64 / static_cast<int>(sizeof(T));  // contraction of one load: 4 x 16 bytes a row
   constexpr int kTurn = kFewWaves * kGroup;
-  __shared__ __attribute__((aligned(16))) float join[kFewWaves][MT * 16][16 + 4];
+  __shared__ __attribute__((aligned(16))) float join[kFewWaves][16][16 + 4];
   typedef T Vec __attribute__((ext_vector_type(kVec<T>), aligned(sizeof(T))));
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, row = lane % 16;
   const int n0 = blockIdx.x * 16, k_lane = wave * kGroup + lane / 16 * kVec<T>;
   const T* w = static_cast<const T*>(g.b) + (n0 + row) * g.ldb + k_lane;
   const T* x = static_cast<const T*>(g.a) + row * g.lda + k_lane;
-  const int rows_n = n0 + row < g.n ? static_cast<int>(g.k) : 0;
+  const int k_all = static_cast<int>(g.k), rows_n = n0 + row < g.n ? k_all : 0, rows_m = row < g.m ? k_all : 0;
   const auto fetch = [](const T* p, int left) {
     Vec v;
     if (left >= kVec<T>) {
@@ -495,43 +499,34 @@ __global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g
     }
     return v;
   };
-  f32x4 acc[MT] = {};
+  f32x4 acc = {};
   for (int k = 0; k < g.k; k += kFewUnroll * kTurn) {
-    Vec fw[kFewUnroll], fx[kFewUnroll][MT];
+    Vec fw[kFewUnroll], fx[kFewUnroll];
 #pragma unroll
     for (int u = 0; u < kFewUnroll; ++u) fw[u] = fetch(w + k + u * kTurn, rows_n - k_lane - k - u * kTurn);
 #pragma unroll
-    for (int u = 0; u < kFewUnroll; ++u)
+    for (int u = 0; u < kFewUnroll; ++u) fx[u] = fetch(x + k + u * kTurn, rows_m - k_lane - k - u * kTurn);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        fx[u][i] = fetch(x + 16 * i * g.lda + k + u * kTurn,
-                         16 * i + row < g.m ? static_cast<int>(g.k) - k_lane - k - u * kTurn : 0);
+    for (int u = 0; u < kFewUnroll; ++u) {
+      if constexpr (sizeof(T) == 2) {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u], fx[u], acc, 0, 0, 0);
+      } else {
 #pragma unroll
-    for (int u = 0; u < kFewUnroll; ++u)
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u], fx[u][i], acc[i], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[u][j], fx[u][i][j], acc[i], 0, 0, 0);
-        }
+        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[u][j], fx[u][j], acc, 0, 0, 0);
       }
+    }
   }
   // a lane holds row l % 16 and columns 4 (l / 16) .. + 3
-#pragma unroll
-  for (int i = 0; i < MT; ++i) store4(&join[wave][16 * i + row][lane / 16 * 4], acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+  store4(&join[wave][row][lane / 16 * 4], acc[0], acc[1], acc[2], acc[3]);
   __syncthreads();
-  for (int e = threadIdx.x; e < MT * 16 * 2; e += kFewWaves * kWave) {
-    const int r = e / 2, c = e % 2 * 8, n = g.n - n0 - c;
-    if (r >= g.m || n <= 0) continue;
-    float v[8] = {};
+  const int r = threadIdx.x / 2, c = threadIdx.x % 2 * 8, n = g.n - n0 - c;
+  if (r >= g.m || n <= 0) return;
+  float v[8] = {};
 #pragma unroll
-    for (int s = 0; s < kFewWaves; ++s)
+  for (int s = 0; s < kFewWaves; ++s)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += join[s][r][c + j];
-    finish8<T>(g, r, n0 + c, n, v);
-  }
+    for (int j = 0; j < 8; ++j) v[j] += join[s][r][c + j];
+  finish8<T>(g, r, n0 + c, n, v);
 }
 
 // ---- the activation's gradient -----------------------------------------------------------------------
@@ -708,9 +703,9 @@ static GemmPlan weight_plan(const gs_linear* p) {
 template <typename T>
 static int run_forward(const gs_linear* p, const GemmArgs& g, void* workspace, hipStream_t st) {
   const dim3 grid((g.n + 15) / 16), block(kFewWaves * kWave);
-  if (g.m <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, block, 0, st, g);
-  else if (g.m <= kFewRows) hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, st, g);
-  else return run_gemm<T, true, true>(g, forward_plan(p), workspace, "linear", st);
+  static_assert(kFewRows == 16, "rows of a matrix instruction");
+  if (g.m > kFewRows) return run_gemm<T, true, true>(g, forward_plan(p), workspace, "linear", st);
+  hipLaunchKernelGGL(linear_few_kernel<T>, grid, block, 0, st, g);
   return check_launch("linear");
 }
 

@@ -4,7 +4,7 @@
 //   h = x + scale gate k b                k: the dropout's factors, formed from the counter (gs_philox.h)
 //   n = w h^ + b                          h^: h standardised in the same way
 //
-// and dropout alone. A row is held in the registers of 64 to 1024 lanes from its one reading to its one writing;
+// and dropout alone. A row is held in the registers of 64 to 512 lanes from its one reading to its one writing;
 // deviations are taken from the mean, not from the sum of squares. The backward pass forms h and its
 // standardised rows again from x, y and four saved statistics a row, so that nothing else is kept:
 //
@@ -233,9 +233,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
   }
 }
 
-// BIAS: a bias' gradient is wanted too.
-template <typename X, typename Y, int G, int NV, bool WHOLE, bool BIAS>
-__global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_kernel(NormArgs a) {
+// NV 1: what differs from row to row is loaded a row ahead, which takes the registers that 256 lanes' workgroups of two
+// wavefronts a SIMD have left (32771 x 1024: 168 us without, 139 with; sixteen elements a lane, a row a wavefront: 217).
+template <typename X, typename Y, int G, int NV, bool WHOLE>
+__global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs a) {
   constexpr int kGroups = G > 256 ? 1 : 256 / G;
   constexpr int kWidth = 8 * G * NV;
   __shared__ float2 lds[2][kGroups][G / kWave];
@@ -248,7 +249,6 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
   for (int i = 0; i < NV; ++i) at[i] = {8 * (lane + G * i), a.width};
   const uint64_t seed = a.drop.threshold ? seed_of(a.drop) : 0;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups;
-  // What differs from row to row is loaded a row ahead.
   struct Row {
     Raw8<X> x[NV], d_h[NV];
     Raw8<Y> y[NV], d_n[NV];
@@ -266,13 +266,15 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
     }
     r.stats = *reinterpret_cast<const float4*>(a.stats + 4 * row);
   };
+  constexpr bool kAhead = NV == 1;
   Row next;
-  fetch(next, static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G);
+  if (kAhead) fetch(next, static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G);
   // (the groups of a workgroup take as many turns as its first one: barriers are met by all)
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows; first += step) {
     const int64_t row_at = first + threadIdx.x / G;
     const bool mine = row_at < a.rows;
     const int64_t row = mine ? row_at : a.rows - 1;
+    if (!kAhead) fetch(next, row_at);
     const Row now = next;
     RawAny8 rw[NV];
     Between8 mid[NV];
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
       if (a.weight) rw[i].load(a.weight, a.weights_bf16, at[i].col, at[i].loaded());
       if (a.y) mid[i].load(a, row, at[i]);
     }
-    fetch(next, row_at + step);
+    if (kAhead) fetch(next, row_at + step);
     const float4 st = now.stats;
     float hat[NV][8], t[NV][8], b[NV][8], u[NV][8], fk[NV][8];
     float s1 = 0.0f, s2 = 0.0f;
@@ -313,7 +315,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
         hat[i][j] = has ? (hat[i][j] - st.x) * st.y : 0.0f;
         t[i][j] = has ? t[i][j] : 0.0f;
         col_sum[kSumWeight][i][j] = fmaf(t[i][j], hat[i][j], col_sum[kSumWeight][i][j]);
-        if (BIAS) col_sum[kSumBias][i][j] += t[i][j];
+        col_sum[kSumBias][i][j] += t[i][j];
         t[i][j] = has ? t[i][j] * w[j] : 0.0f;
         s1 = fmaf(t[i][j], hat[i][j], s1);
         s2 += t[i][j];
@@ -343,7 +345,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, G > 512 ? 4 : 2) void norm_bwd_k
         if (a.post) {
           b[i][j] = has ? b[i][j] : 0.0f;
           col_sum[kSumPostWeight][i][j] = fmaf(v, b[i][j], col_sum[kSumPostWeight][i][j]);
-          if (BIAS) col_sum[kSumPostBias][i][j] += v;
+          col_sum[kSumPostBias][i][j] += v;
           t[i][j] = has ? v * w[j] : 0.0f;
           s1 = fmaf(t[i][j], b[i][j], s1);
           s2 += t[i][j];
@@ -466,25 +468,25 @@ static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
   return GS_OK;
 }
 
-// Calls f(kernel, lanes a row) with the instance for a width: a wavefront a row where eight or sixteen elements a
-// lane do, more wavefronts above.
+// Calls f(kernel, lanes a row) with the instance for a width: as many lanes as leave eight elements each (sixteen in the
+// forward, where a wavefront's own row needs no barrier; above 4096 in the backward, which a workgroup of 1024 has
+// too few registers for). Widths that are no multiple of eight take branches for their last vector: 32771 x 1024 by those
+// instances 88 us forward and 220 with its backward, so 77 and 212.
 template <typename X, typename Y, bool WHOLE, typename F>
 static int with_fwd(int width, F f) {
   if (width <= 512) return f(norm_fwd_kernel<X, Y, 64, 1, WHOLE>, 64);
   if (width <= 1024) return f(norm_fwd_kernel<X, Y, 64, 2, WHOLE>, 64);
   if (width <= 2048) return f(norm_fwd_kernel<X, Y, 256, 1, WHOLE>, 256);
   if (width <= 4096) return f(norm_fwd_kernel<X, Y, 256, 2, WHOLE>, 256);
-  if (width <= 8192) return f(norm_fwd_kernel<X, Y, 512, 2, WHOLE>, 512);
-  return f(norm_fwd_kernel<X, Y, 1024, 2, WHOLE>, 1024);
+  return f(norm_fwd_kernel<X, Y, 512, 2, WHOLE>, 512);
 }
-template <typename X, typename Y, bool WHOLE, bool BIAS, typename F>
+template <typename X, typename Y, bool WHOLE, typename F>
 static int with_bwd(int width, F f) {
-  if (width <= 512) return f(norm_bwd_kernel<X, Y, 64, 1, WHOLE, BIAS>, 64);
-  if (width <= 1024) return f(norm_bwd_kernel<X, Y, 128, 1, WHOLE, BIAS>, 128);
-  if (width <= 2048) return f(norm_bwd_kernel<X, Y, 256, 1, WHOLE, BIAS>, 256);
-  if (width <= 4096) return f(norm_bwd_kernel<X, Y, 512, 1, WHOLE, BIAS>, 512);
-  if (width <= 8192) return f(norm_bwd_kernel<X, Y, 1024, 1, WHOLE, BIAS>, 1024);
-  return f(norm_bwd_kernel<X, Y, 1024, 2, WHOLE, BIAS>, 1024);
+  if (width <= 512) return f(norm_bwd_kernel<X, Y, 64, 1, WHOLE>, 64);
+  if (width <= 1024) return f(norm_bwd_kernel<X, Y, 128, 1, WHOLE>, 128);
+  if (width <= 2048) return f(norm_bwd_kernel<X, Y, 256, 1, WHOLE>, 256);
+  if (width <= 4096) return f(norm_bwd_kernel<X, Y, 512, 1, WHOLE>, 512);
+  return f(norm_bwd_kernel<X, Y, 512, 2, WHOLE>, 512);
 }
 template <typename F>
 static int with_types(const gs_residual_norm* p, F f) {
@@ -565,12 +567,10 @@ extern "C" int gs_residual_norm_bwd(const gs_residual_norm* p, const void* d_h, 
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(std::max(256, lanes)), 0, st, a);
       return check_launch("residual norm backward");
     };
-    const bool bias = d_bias || d_post_bias;
     const int rc = with_types(p, [&](auto x, auto y) {
       using X = decltype(x);
       using Y = decltype(y);
-      if (a.width % 8) return with_bwd<X, Y, false, true>(a.width, run);
-      return bias ? with_bwd<X, Y, true, true>(a.width, run) : with_bwd<X, Y, true, false>(a.width, run);
+      return a.width % 8 == 0 ? with_bwd<X, Y, true>(a.width, run) : with_bwd<X, Y, false>(a.width, run);
     });
     if (rc) return rc;
   }

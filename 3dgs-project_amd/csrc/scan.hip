@@ -500,7 +500,8 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs
   }
 }
 
-// Up to so many tokens one wavefront a channel group walks them all, in one launch.
+// Up to so many tokens one wavefront a channel group walks them all, in one launch: 1, 16, 24 (of 24 documents), 32 and 48
+// tokens of 1024 channels 4.1, 9.3, 14.6, 16.2 and 23.1 us, by chunks 8.1, 15.8, 18.3, 16.2 and 16.3.
 constexpr int kScanSerial = 32;
 
 struct ScanPlan {

@@ -680,7 +680,7 @@ int gs_attention_bwd(const gs_attention* args, const void* d_out, void* d_q, voi
  * NULL, each in its tensor's type and shape. Sums over rows are float32 in a fixed order: the same inputs
  * give the same bits.
  * ------------------------------------------------------------------------------------- */
-#define GS_NORM_MAX_WIDTH 16384
+#define GS_NORM_MAX_WIDTH 8192
 typedef struct gs_residual_norm {
   const void *x, *y, *weight, *bias, *post_weight, *post_bias, *gate;
   void *h, *n;
@@ -760,7 +760,7 @@ int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d
  * ------------------------------------------------------------------------------------- */
 #define GS_LINEAR_MAX_WIDTH (1 << 19)
 #define GS_LINEAR_MAX_STRIDE (1 << 20)
-#define GS_LINEAR_FEW_ROWS 32
+#define GS_LINEAR_FEW_ROWS 16
 #define GS_ACT_NONE 0
 #define GS_ACT_RELU 1
 #define GS_ACT_GELU 2

@@ -31,7 +31,7 @@ BF = _lib.GS_BFLOAT16
 @pytest.mark.parametrize("kw,code,text", [
     (dict(x_dtype=1), ARG, "dtypes"), (dict(y_dtype=7), ARG, "dtypes"), (dict(x_dtype=BF), ARG, "bfloat16 stream"),
     (dict(weight_dtype=1), ARG, "weight dtype"), (dict(gate_dtype=1), ARG, "gate dtype"), (dict(rows=-1), ARG, "row count"),
-    (dict(rows=1 << 31), ARG, "row count"), (dict(width=0), ARG, "width"), (dict(width=16385), ARG, "width"),
+    (dict(rows=1 << 31), ARG, "row count"), (dict(width=0), ARG, "width"), (dict(width=8193), ARG, "width"),
     (dict(eps=0.0), ARG, "eps"), (dict(eps=math.inf), ARG, "eps"), (dict(eps=math.nan), ARG, "eps"),
     (dict(scale=math.nan), ARG, "scale"), (dict(scale=math.inf), ARG, "scale"), (dict(dropout=1.0), ARG, "dropout"),
     (dict(dropout=-0.1), ARG, "dropout"), (dict(dropout=math.nan), ARG, "dropout"), (dict(y=None), ARG, "needs y"),
@@ -53,7 +53,7 @@ def test_norm_calls():
     back = lambda a, dh=256, dx=256, dy=256, dpw=256, dg=256, ws=256, n=need: L.gs_residual_norm_bwd(  # noqa: E731
         C.byref(a), dh, 256, dx, dy, 256, 256, dpw, 256, dg, ws, n, None)
     expect(L.gs_residual_norm_fwd(None, None), ARG, "NULL")
-    expect(L.gs_residual_norm_fwd(C.byref(norm_args(rows=(1 << 31) - 1, width=16384)), None), ARG, "too many")
+    expect(L.gs_residual_norm_fwd(C.byref(norm_args(rows=(1 << 31) - 1, width=8192)), None), ARG, "too many")
     expect(L.gs_residual_norm_fwd(C.byref(norm_args(n=None)), None), ARG, "null")
     expect(L.gs_residual_norm_fwd(C.byref(norm_args(h=None)), None), ARG, "null")
     expect(back(norm_args(stats=None)), ARG, "statistics")
@@ -153,8 +153,8 @@ def test_linear_arguments(kw, code, text):
 def test_linear_calls():
     L = _lib.lib()
     # few rows are read at any address, but for gradients
-    expect(L.gs_linear_fwd(C.byref(linear_args(rows=32, x=260, x_stride=65, weight=258)), None, 0, None), ALIGN, "misaligned")
-    expect(L.gs_linear_bwd(C.byref(linear_args(rows=32, x=260)), 256, 256, 256, 256, 256, 1 << 62, None), ALIGN, "misaligned")
+    expect(L.gs_linear_fwd(C.byref(linear_args(rows=16, x=260, x_stride=65, weight=258)), None, 0, None), ALIGN, "misaligned")
+    expect(L.gs_linear_bwd(C.byref(linear_args(rows=16, x=260)), 256, 256, 256, 256, 256, 1 << 62, None), ALIGN, "misaligned")
     rows = lambda **kw: _lib.GsRows(**{**dict(src=256, dst=256, rows=4, cols=60, src_stride=70, dst_stride=64), **kw})  # noqa: E731
     pack = lambda n=2, dtype=0, **kw: L.gs_rows_pack((_lib.GsRows * 2)(rows(), rows(**kw)), n, dtype, None)  # noqa: E731
     expect(pack(dtype=1), ARG, "dtype")

@@ -64,7 +64,7 @@ def test_forms(stream, branch, kind, gate):
               v(6) if post else None, v(7) if post and layer else None, g, kind, 0.7, p)
 
 
-@pytest.mark.parametrize("width", [1, 2, 8, 63, 512, 520, 645, 1024, 1025, 2048, 2050, 4096, 5000, 8192, 8193, 16384])
+@pytest.mark.parametrize("width", [1, 2, 8, 63, 512, 520, 645, 1024, 1025, 2048, 2050, 4096, 5000, 8191, 8192])
 def test_widths(width):
     stream, branch = TYPES[width % 3]
     v = lambda s: rand(s, width, gain=0.3, shift=1.0)  # noqa: E731
@@ -239,7 +239,7 @@ def test_refusals():
         ((x, y, w), dict(dropout=1.0, seed=1), "probability"), ((x, y, w), dict(dropout=0.5), "seed"),
         ((x, y, w), dict(dropout=0.5, seed=torch.zeros(1, dtype=torch.int64)), "seed"),
         ((x, y, w), dict(dropout=0.5, seed=1 << 64), "64 bits"), ((x, y, w), dict(dropout=0.5, seed=1, draw=-1), "draw"),
-        ((z(2, 16385), z(2, 16385)), {}, "width"), ((z(2, 0), z(2, 0)), {}, "width"),
+        ((z(2, 8193), z(2, 8193)), {}, "width"), ((z(2, 0), z(2, 0)), {}, "width"),
     ]:
         with pytest.raises(ValueError, match=text):
             residual_norm(*args, **kw)
