@@ -472,49 +472,69 @@ __global__ __launch_bounds__(kFinishThreads) void gemm_finish_kernel(GemmArgs g)
 
 // ---- few rows ----------------------------------------------------------------------------------------
 
-// Sixteen columns a workgroup, up to sixteen rows: its wavefronts take the contraction in turn, from memory straight into the
-// matrix instruction's operands, four loads of W in flight each, and are joined in LDS. Rows at any address
-// and stride: loads are of an element's alignment, and the contraction's last vector is read element by element.
-// One row of 1024 x 4096 takes 4.1 us on the GPU, 8192 x 8192 31.5 us (4.3 TB/s). (32 rows in two sets read x twice as often as W:
-// 1024 x 4096 5.1 us, by tiles 8.1; 4096 x 1024 12.8 and 11.9; 8192 x 8192 45 and 26: those go to the tiles.)
-constexpr int kFewWaves = 8, kFewUnroll = 4;
+// Sixteen columns a workgroup, up to sixteen rows: its wavefronts take the contraction in turn, from memory straight into
+// the matrix instruction's operands, four loads of W sent while the four before them are multiplied, and are joined in
+// LDS. Rows at any address and stride: loads are of an element's alignment. Reading W bounds it, and at 1024 columns that
+// 64 workgroups leave most CUs without loads: one row of 1024 x 4096 takes 3.5 us on the GPU, 4096 x 1024 6.6,
+// 8192 x 8192 27.8 (4.8 TB/s); with eight wavefronts 3.7, 6.9 and 25.5. (32 rows in two sets read x twice as often as W:
+// 1024 x 4096 5.1 us, by tiles 8.1; 4096 x 1024 12.8 and 11.9; 8192 x 8192 45 and 26: those go to the tiles. With 16 rows
+// these take 4.2 and 8.0, 9.3 and 11.4, 31 and 25.)
+constexpr int kFewWaves = 4, kFewUnroll = 4;
 template <typename T>
 __global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g) {
-  constexpr int kGroup = 64 / static_cast<int>(sizeof(T));  // contraction of one load: 4 x 16 bytes a row
-  constexpr int kTurn = kFewWaves * kGroup;
+  constexpr int kGroup = 128 / static_cast<int>(sizeof(T));  // contraction of two loads: a cache line of every row
+  constexpr int kTurn = kFewWaves * kGroup, kStep = kFewUnroll / 2 * kTurn;
   __shared__ __attribute__((aligned(16))) float join[kFewWaves][16][16 + 4];
   typedef T Vec __attribute__((ext_vector_type(kVec<T>), aligned(sizeof(T))));
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, row = lane % 16;
-  const int n0 = blockIdx.x * 16, k_lane = wave * kGroup + lane / 16 * kVec<T>;
-  const T* w = static_cast<const T*>(g.b) + (n0 + row) * g.ldb + k_lane;
-  const T* x = static_cast<const T*>(g.a) + row * g.lda + k_lane;
-  const int k_all = static_cast<int>(g.k), rows_n = n0 + row < g.n ? k_all : 0, rows_m = row < g.m ? k_all : 0;
-  const auto fetch = [](const T* p, int left) {
-    Vec v;
-    if (left >= kVec<T>) {
-      v = *reinterpret_cast<const Vec*>(p);
+  const int n0 = blockIdx.x * 16, k_lane = wave * kGroup + lane / 16 * 2 * kVec<T>;
+  // (rows past the last repeat it: their results are not stored)
+  const T* w = static_cast<const T*>(g.b) + min(n0 + row, g.n - 1) * g.ldb;
+  const T* x = static_cast<const T*>(g.a) + min(row, static_cast<int>(g.m) - 1) * g.lda;
+  const int k_all = static_cast<int>(g.k), k_whole = k_all / kVec<T> * kVec<T>;
+  f32x4 acc = {};
+  const auto product = [&](const Vec& fw, const Vec& fx) {
+    if constexpr (sizeof(T) == 2) {
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fx, acc, 0, 0, 0);
     } else {
 #pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) v[j] = j < left ? p[j] : static_cast<T>(0.0f);
+      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[j], fx[j], acc, 0, 0, 0);
     }
-    return v;
   };
-  f32x4 acc = {};
-  for (int k = 0; k < g.k; k += kFewUnroll * kTurn) {
-    Vec fw[kFewUnroll], fx[kFewUnroll];
+  // Whole vectors: lanes past the last one load it again, so that no load needs a branch, and take zeros.
+  struct Step {
+    Vec w[kFewUnroll], x[kFewUnroll];
+  };
+  const auto fetch = [&](Step& s, int k) {
 #pragma unroll
-    for (int u = 0; u < kFewUnroll; ++u) fw[u] = fetch(w + k + u * kTurn, rows_n - k_lane - k - u * kTurn);
+    for (int u = 0; u < kFewUnroll; ++u)
+      s.w[u] = *reinterpret_cast<const Vec*>(w + min(k + u / 2 * kTurn + u % 2 * kVec<T>, k_whole - kVec<T>));
 #pragma unroll
-    for (int u = 0; u < kFewUnroll; ++u) fx[u] = fetch(x + k + u * kTurn, rows_m - k_lane - k - u * kTurn);
+    for (int u = 0; u < kFewUnroll; ++u)
+      s.x[u] = *reinterpret_cast<const Vec*>(x + min(k + u / 2 * kTurn + u % 2 * kVec<T>, k_whole - kVec<T>));
+  };
+  if (k_whole > 0) {
+    Step next;
+    fetch(next, k_lane);
+    for (int k = 0; k < k_whole; k += kStep) {
+      const Step now = next;
+      if (k + kStep < k_whole) fetch(next, k + kStep + k_lane);
 #pragma unroll
-    for (int u = 0; u < kFewUnroll; ++u) {
-      if constexpr (sizeof(T) == 2) {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u], fx[u], acc, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[u][j], fx[u][j], acc, 0, 0, 0);
+      for (int u = 0; u < kFewUnroll; ++u) {
+        const bool has = k + k_lane + u / 2 * kTurn + u % 2 * kVec<T> < k_whole;
+        product(has ? now.w[u] : Vec{}, has ? now.x[u] : Vec{});
       }
     }
+  }
+  if (k_whole < k_all && wave == 0) {  // the contraction's last vector, element by element
+    Vec fw = {}, fx = {};
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j)
+      if (lane < 16 && k_whole + j < k_all) {
+        fw[j] = w[k_whole + j];
+        fx[j] = x[k_whole + j];
+      }
+    product(fw, fx);
   }
   // a lane holds row l % 16 and columns 4 (l / 16) .. + 3
   store4(&join[wave][row][lane / 16 * 4], acc[0], acc[1], acc[2], acc[3]);
