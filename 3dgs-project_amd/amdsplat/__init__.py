@@ -3,8 +3,8 @@
 `rasterize(means, scales, quats, opacities, sh, viewmat, K, W, H) -> (image, alpha, aux)` runs
 the 3D path through hand-written HIP kernels behind a C ABI (include/amdsplat.h). The 2D
 drop-in surfaces live in the sibling packages `gs2d` and `splat2d`. For a network that predicts
-Gaussians from images there are `attention`, `rotary_axes`, and `grad_norm` / `clip_grad_norm` beside
-`FusedAdam`.
+Gaussians from images there are `attention`, `rotary_axes`, `linear`, `norm` / `residual_norm`, `dropout`,
+`gated_scan`, and `grad_norm` / `clip_grad_norm` beside `FusedAdam`.
 """
 from .adam import FusedAdam, adam_step, adam_step_sparse
 from .attention import attention

@@ -11,6 +11,11 @@
 // cache as far as it holds them. (One pass that waits for the workgroups before it would read them once, but
 // needs them to be running; nothing here waits for another workgroup.)
 //
+// Memory bounds it beside the chain of a chunk's steps: 32771 x 1024 with a gate in bfloat16, forward sums 41 us, parts 10,
+// walk 56 (268 MB, 4.8 TB/s); backward sums 51, parts 10, walk 128 (470 MB, 3.7 TB/s); one pass over inputs and
+// results alone 737 MB, at a copy's 5.1 TB/s 145 us. With the loads of all sixteen tokens sent together
+// the sums took 43 and 70 us, the walk 71.
+//
 // A document's first token replaces the state, so P = 0 there, and a map with P = 0 drops what came before it whatever
 // that was: documents do not see each other's infinities and NaN.
 //
