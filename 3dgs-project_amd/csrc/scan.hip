@@ -51,6 +51,7 @@ struct ScanArgs {
   int groups;                 // of kScanGroup channels
   int chunks, parts, blocks;  // blocks: of a part
   int serial;                 // one wavefront walks all chunks
+  int single;                 // one wavefront walks a document's
   float2* prefix;             // [chunks][width]: the map from the part's start to the chunk
   float2* part;               // [parts][width]: the map of a part
   float* before;              // [parts][width]: the state that a part starts with
@@ -134,11 +135,23 @@ __device__ __forceinline__ int64_t token_at(const ScanArgs& a, int64_t p) { retu
 // in lane k the document of token k.
 struct Places {
   uint32_t inside, first, last;
+  uint32_t mine = 0;  // of one document's: are walked with it
   int doc;
+  // of one document, places from .. to, walked with all of lo .. hi
+  __device__ __forceinline__ Places(const ScanArgs& a, int64_t p0, int doc_, int from, int to, int lo, int hi) : doc(doc_at(a, doc_)) {
+    const auto bits = [&](int b, int e) {
+      const auto up_to = [&](int p) { return (1u << min(max(static_cast<int>(p - p0), 0), kScanChunk)) - 1; };
+      return up_to(e) & ~up_to(b);
+    };
+    inside = bits(from, to);
+    mine = bits(lo, hi);
+    first = inside & bits(from, from + 1);
+    last = inside & bits(to - 1, to);
+  }
   __device__ __forceinline__ Places(const ScanArgs& a, int64_t p0) {
     const int lane = threadIdx.x % kWave;
     const int64_t p = p0 + lane;
-    const bool mine = lane < kScanChunk && p < a.tokens;
+    const bool there = lane < kScanChunk && p < a.tokens;
     // i: the last edge at or before p, so that empty documents are passed over
     int i = -1;
     int64_t at = -1, next = -1;
@@ -151,7 +164,7 @@ struct Places {
       }
       at = __shfl(e, max(i, 0));
       next = __shfl(e, min(i + 1, a.docs));
-    } else if (mine) {
+    } else if (there) {
       int lo = 0, hi = a.docs + 1;  // edges before lo are at or before p, those from hi on are not
       while (lo < hi) {
         const int mid = (lo + hi) / 2;
@@ -162,7 +175,7 @@ struct Places {
       at = scan_edge(a, max(i, 0));
       next = scan_edge(a, min(i + 1, a.docs));
     }
-    const bool in = mine && i >= 0 && i < a.docs;
+    const bool in = there && i >= 0 && i < a.docs;
     doc = in ? doc_at(a, i) : 0;
     inside = static_cast<uint32_t>(__ballot(in));
     first = static_cast<uint32_t>(__ballot(in && at == p));
@@ -200,15 +213,21 @@ struct Channels {
 };
 
 // Rows of the tokens at places p0 .. p0 + 7, whatever they belong to (so that no load waits for the documents); past the last
-// token that one's again.
+// token that one's again. within: outside lo .. hi - 1 the nearest one's again.
 template <typename T, bool SMALL>
 struct Batch {
   Raw4<T> row[kScanBatch];
   __device__ __forceinline__ void load(const ScanArgs& a, const void* p, int64_t stride, int64_t p0, const Channels<SMALL>& c) {
 #pragma unroll
-    for (int k = 0; k < kScanBatch; ++k)
-      row[k].load(c.at_of(static_cast<const T*>(p) + token_at(a, min<int64_t>(p0 + k, a.tokens - 1)) * stride),
-                  SMALL ? c.n : kScanVec);
+    for (int k = 0; k < kScanBatch; ++k) at(a, k, p, stride, min<int64_t>(p0 + k, a.tokens - 1), c);
+  }
+  __device__ __forceinline__ void within(const ScanArgs& a, const void* p, int64_t stride, int64_t p0, const Channels<SMALL>& c,
+                                         int lo, int hi) {
+#pragma unroll
+    for (int k = 0; k < kScanBatch; ++k) at(a, k, p, stride, min(max<int64_t>(p0 + k, lo), int64_t(hi) - 1), c);
+  }
+  __device__ __forceinline__ void at(const ScanArgs& a, int k, const void* p, int64_t stride, int64_t place, const Channels<SMALL>& c) {
+    row[k].load(c.at_of(static_cast<const T*>(p) + token_at(a, place) * stride), SMALL ? c.n : kScanVec);
   }
 };
 
@@ -351,35 +370,64 @@ __device__ __forceinline__ void pass_empty(const ScanArgs& a, const Channels<SMA
 
 // ---- the walk ----------------------------------------------------------------------------------------
 
-// The chunks that a wavefront walks: one, or in serial mode all of them.
+// The chunks that a wavefront walks: one; in serial mode all of them. ONE: those of its document (and of what belongs to none
+// before the first document or behind the last).
+template <bool ONE>
 struct Walk {
   int first, end;
+  int doc, from, to, lo, hi;  // ONE: in walking order, its places, and the places walked
   __device__ __forceinline__ explicit Walk(const ScanArgs& a) {
-    // the last ones first: what the sums' kernel read last is still in the cache
-    const int n = (gridDim.x - 1 - blockIdx.x) / a.groups * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    first = a.serial ? 0 : n;
-    end = a.serial ? a.chunks : min(n + 1, a.chunks);
+    if constexpr (ONE) {
+      doc = blockIdx.x / a.groups;
+      from = __builtin_amdgcn_readfirstlane(static_cast<int>(scan_edge(a, doc)));
+      to = max(from, __builtin_amdgcn_readfirstlane(static_cast<int>(scan_edge(a, doc + 1))));
+      lo = doc == 0 ? 0 : from;
+      hi = doc == a.docs - 1 ? static_cast<int>(a.tokens) : to;
+      first = lo / kScanChunk;
+      end = hi > lo ? (hi - 1) / kScanChunk + 1 : first;
+    } else {
+      // the last ones first: what the sums' kernel read last is still in the cache
+      const int n = (gridDim.x - 1 - blockIdx.x) / a.groups * (blockDim.x / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+      first = a.serial ? 0 : n;
+      end = a.serial ? a.chunks : min(n + 1, a.chunks);
+    }
+  }
+  __device__ __forceinline__ Places places(const ScanArgs& a, int64_t p0) const {
+    if constexpr (ONE) return Places(a, p0, doc, from, to, lo, hi);
+    else return Places(a, p0);
+  }
+  template <typename B, typename C>
+  __device__ __forceinline__ void load(B& b, const ScanArgs& a, const void* p, int64_t stride, int64_t p0, const C& c) const {
+    if constexpr (ONE) b.within(a, p, stride, p0, c, lo, hi);
+    else b.load(a, p, stride, p0, c);
+  }
+  // Token k of a chunk, at place p, is walked here.
+  __device__ __forceinline__ bool has(const ScanArgs& a, const Places& pl, int k, int64_t p) const {
+    return ONE ? (pl.mine >> k) & 1 : p < a.tokens;
+  }
+  __device__ __forceinline__ bool some(const ScanArgs& a, const Places& pl, int k, int64_t p) const {
+    return ONE ? ((pl.mine >> k) & ((1u << kScanBatch) - 1)) != 0 : p < a.tokens;
   }
 };
 
-template <typename T, bool SMALL>
+template <typename T, bool SMALL, bool ONE>
 __global__ __launch_bounds__(kWalkWaves* kWave, 3) void scan_apply_kernel(ScanArgs a) {
   const Channels<SMALL> c(a, blockIdx.x % a.groups);
   pass_empty(a, c, a.initial, a.state);
   float h[4] = {};
-  const Walk w(a);
+  const Walk<ONE> w(a);
   for (int n = w.first; n < w.end; ++n) {
     const int64_t p0 = static_cast<int64_t>(n) * kScanChunk;
-    if (!a.serial) state_before(a, n, c, h);
-    if (a.carry) c.store(a.carry + static_cast<int64_t>(n) * a.width, h);
-    const Places pl(a, p0);
+    if (!ONE && !a.serial) state_before(a, n, c, h);
+    const Places pl = w.places(a, p0);
+    if (a.carry && w.has(a, pl, 0, p0)) c.store(a.carry + static_cast<int64_t>(n) * a.width, h);
 #pragma unroll
     for (int k0 = 0; k0 < kScanChunk; k0 += kScanBatch) {
-      if (p0 + k0 >= a.tokens) break;
+      if (!w.some(a, pl, k0, p0 + k0)) continue;
       Batch<T, SMALL> bf, bx, bo;
-      bf.load(a, a.f, a.f_stride, p0 + k0, c);
-      bx.load(a, a.x, a.x_stride, p0 + k0, c);
-      if (a.o) bo.load(a, a.o, a.o_stride, p0 + k0, c);
+      w.load(bf, a, a.f, a.f_stride, p0 + k0, c);
+      w.load(bx, a, a.x, a.x_stride, p0 + k0, c);
+      if (a.o) w.load(bo, a, a.o, a.o_stride, p0 + k0, c);
       Raw4<float> first[kScanBatch];
       if ((pl.first >> k0) & ((1u << kScanBatch) - 1)) {
 #pragma unroll
@@ -390,7 +438,7 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 3) void scan_apply_kernel(ScanAr
 #pragma unroll
       for (int k = 0; k < kScanBatch; ++k) {
         const int64_t p = p0 + k0 + k;
-        if (p >= a.tokens) break;
+        if (!w.has(a, pl, k0 + k, p)) continue;
         float y[4] = {};
         if ((pl.inside >> (k0 + k)) & 1) {
           if ((pl.first >> (k0 + k)) & 1) first[k].to(h);
@@ -414,21 +462,22 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 3) void scan_apply_kernel(ScanAr
 
 // Eight tokens at a time from the chunk's end: the states before them are walked to from the chunk's start and held in
 // registers. (All sixteen at once took 235 registers and two wavefronts a SIMD: 32771 x 1024 175 us.)
-template <typename T, bool SMALL>
+template <typename T, bool SMALL, bool ONE>
 __global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs a) {
   const Channels<SMALL> c(a, blockIdx.x % a.groups);
   pass_empty(a, c, a.d_state, a.d_initial);
   float l[4] = {};  // a l of the token after
-  const Walk w(a);
+  const Walk<ONE> w(a);
   for (int n = w.first; n < w.end; ++n) {
-    const int chunk = a.chunks - 1 - n;
-    if (!a.serial) state_before(a, n, c, l);
-    const Places pl(a, static_cast<int64_t>(chunk) * kScanChunk);
+    const int chunk = (ONE ? w.first + w.end : a.chunks) - 1 - n;
+    if (!ONE && !a.serial) state_before(a, n, c, l);
+    const Places pl = w.places(a, static_cast<int64_t>(chunk) * kScanChunk);
 #pragma unroll 1
     for (int half = kScanChunk / kScanBatch - 1; half >= 0; --half) {
       const int64_t p0 = static_cast<int64_t>(chunk) * kScanChunk + half * kScanBatch;
       const uint32_t inside = pl.inside >> (half * kScanBatch), first = pl.first >> (half * kScanBatch),
                      last = pl.last >> (half * kScanBatch);
+      if (!w.some(a, pl, half * kScanBatch, p0)) continue;
       float before[kScanBatch][4], h[4];
       c.load(a, a.carry, chunk, h);
       const auto begin = [&](int k) {  // the state before token k of the chunk where it is a document's first
@@ -436,8 +485,8 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs
       };
       Batch<T, SMALL> bf, bx, bd, bo;
       if (half) {
-        bf.load(a, a.f, a.f_stride, p0 - kScanBatch, c);
-        bx.load(a, a.x, a.x_stride, p0 - kScanBatch, c);
+        w.load(bf, a, a.f, a.f_stride, p0 - kScanBatch, c);
+        w.load(bx, a, a.x, a.x_stride, p0 - kScanBatch, c);
 #pragma unroll
         for (int k = 0; k < kScanBatch; ++k) {
           if ((pl.first >> k) & 1) begin(k);
@@ -448,10 +497,10 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs
           for (int j = 0; j < 4; ++j) h[j] = Sigmoid(vf[j]).step(h[j], vx[j]);
         }
       }
-      bf.load(a, a.f, a.f_stride, p0, c);
-      bx.load(a, a.x, a.x_stride, p0, c);
-      bd.load(a, a.d_y, a.width, p0, c);
-      if (a.o) bo.load(a, a.o, a.o_stride, p0, c);
+      w.load(bf, a, a.f, a.f_stride, p0, c);
+      w.load(bx, a, a.x, a.x_stride, p0, c);
+      w.load(bd, a, a.d_y, a.width, p0, c);
+      if (a.o) w.load(bo, a, a.o, a.o_stride, p0, c);
 #pragma unroll
       for (int k = 0; k < kScanBatch; ++k) {
         if ((first >> k) & 1) begin(half * kScanBatch + k);
@@ -467,7 +516,7 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs
 #pragma unroll
       for (int k = kScanBatch - 1; k >= 0; --k) {
         const int64_t p = p0 + k;
-        if (p >= a.tokens) continue;
+        if (!w.has(a, pl, half * kScanBatch + k, p)) continue;
         float dx[4] = {}, df[4] = {}, dg[4] = {};
         if ((inside >> k) & 1) {
           if ((last >> k) & 1)
@@ -508,6 +557,11 @@ __global__ __launch_bounds__(kWalkWaves* kWave, 2) void scan_bwd_kernel(ScanArgs
 // Up to so many tokens one wavefront a channel group walks them all, in one launch: 1, 16, 24 (of 24 documents), 32 and 48
 // tokens of 1024 channels 4.1, 9.3, 14.6, 16.2 and 23.1 us, by chunks 8.1, 15.8, 18.3, 16.2 and 16.3.
 constexpr int kScanSerial = 32;
+// Documents of few tokens, no more than 32 of them together or than there are documents, are walked by a wavefront each, which
+// is what single tokens of many scenes want: 24, 64, 256 of 1024 channels 3.9, 3.9 and 4.2 us, by the rules above 14.5, 21.3 and
+// 30.4. Lengths are not known here: if one document has all 256 tokens it takes 134 us for 39, and with
+// 1024 documents 519 for 42 (single tokens 7.1 for 34), so that more than 256 go by chunks.
+constexpr int kScanWalkers = 256;
 
 struct ScanPlan {
   int chunks, parts, blocks, serial;
@@ -568,15 +622,25 @@ static int check_scan(const gs_gated_scan* p, void* workspace, size_t workspace_
   a->chunks = s.chunks;
   a->parts = s.parts;
   a->blocks = s.blocks;
-  a->serial = s.serial;
+  a->single = p->docs > 1 && p->docs <= kScanWalkers && (s.serial || p->tokens <= p->docs);
+  a->serial = s.serial && !a->single;
   a->prefix = static_cast<float2*>(workspace);
   a->part = reinterpret_cast<float2*>(static_cast<char*>(workspace) + s.prefix);
   if (s.parts > 1) a->before = reinterpret_cast<float*>(a->part + static_cast<size_t>(s.parts) * p->width);
   return GS_OK;
 }
 
+template <typename T, bool BACK, bool SMALL, bool ONE>
+static int run_walk(const ScanArgs& a, hipStream_t st) {
+  const int walkers = ONE ? a.docs : (a.serial ? 1 : (a.chunks + kWalkWaves - 1) / kWalkWaves);
+  const dim3 grid(static_cast<unsigned>(a.groups) * walkers), block(ONE || a.serial ? kWave : kWalkWaves * kWave);
+  if constexpr (BACK) hipLaunchKernelGGL((scan_bwd_kernel<T, SMALL, ONE>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((scan_apply_kernel<T, SMALL, ONE>), grid, block, 0, st, a);
+  return check_launch("gated scan");
+}
 template <typename T, bool BACK, bool SMALL>
 static int run_scan(const ScanArgs& a, hipStream_t st) {
+  if (a.single) return run_walk<T, BACK, SMALL, true>(a, st);
   if (!a.serial) {
     hipLaunchKernelGGL((scan_sums_kernel<T, BACK, SMALL>), dim3(a.groups, a.parts), dim3(kScanThreads), 0, st, a);
     if (const int rc = check_launch("gated scan (sums)")) return rc;
@@ -585,11 +649,7 @@ static int run_scan(const ScanArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(scan_parts_kernel, dim3((a.width + 31) / 32), dim3(kJoinThreads), 0, st, a);
     if (const int rc = check_launch("gated scan (parts)")) return rc;
   }
-  const dim3 grid(static_cast<unsigned>(a.groups) * (a.serial ? 1 : (a.chunks + kWalkWaves - 1) / kWalkWaves));
-  const dim3 block(a.serial ? kWave : kWalkWaves * kWave);
-  if constexpr (BACK) hipLaunchKernelGGL((scan_bwd_kernel<T, SMALL>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((scan_apply_kernel<T, SMALL>), grid, block, 0, st, a);
-  return check_launch("gated scan");
+  return run_walk<T, BACK, SMALL, false>(a, st);
 }
 
 template <bool BACK>

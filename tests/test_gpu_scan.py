@@ -88,6 +88,19 @@ def test_documents(offsets, reverse, dtype):
     check(x, f, o, offsets=offsets, reverse=reverse, through="state")
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("tokens,offsets", [
+    (30, [0, 5, 20, 30]), (31, [2, 2, 18, 25]), (32, [0, 0, 32, 32]), (17, [16, 17]), (20, [3] * 40 + [19]), (9, [0, 9] + [9] * 1030),
+    (200, [5] * 50 + [9] * 60 + [120] * 40 + [190] * 60), (200, [0] * 100 + [200] * 101), (200, [200] * 201),
+    (250, list(range(0, 251)) + [250] * 6), (250, list(range(0, 251)) + [250] * 7), (70, [i // 2 for i in range(8, 141)])])
+def test_documents_of_few_tokens(tokens, offsets, reverse, dtype):
+    """No more tokens than 32, or than documents: a wavefront walks a document's."""
+    x, f, o = data(len(offsets), tokens, 20, dtype)
+    check(x, f, o, offsets=offsets, initial=rand(5, len(offsets) - 1, 20), reverse=reverse)
+    check(x, f, None, offsets=offsets, reverse=reverse, through="state")
+
+
 @pytest.mark.parametrize("reverse", [False, True])
 def test_many_parts(reverse):
     """More chunks than one part has, and parts of more than one step, in one document and in many."""
