@@ -16,7 +16,7 @@ from ._lib import call_on, ptr
 
 MAX_WIDTH, FEW_ROWS = 1 << 19, 16  # GS_LINEAR_MAX_WIDTH, GS_LINEAR_FEW_ROWS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}  # GS_ACT_*
-_DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8)}
+_DTYPES = {torch.float32: (_lib.GS_FLOAT32, 4, 4), torch.bfloat16: (_lib.GS_BFLOAT16, 8, 2)}  # code, elements of 16 bytes, bytes
 
 
 def _rows(t):
@@ -35,36 +35,43 @@ def _ready(t: torch.Tensor, few: bool) -> bool:
 
 
 def _pack(x, weight, few: bool):
-    """None, or a buffer with what of x and weight the kernels cannot read, as rows with zeros behind them."""
-    away = [t for t in (x, weight) if not _ready(t, few)]
-    if not away:
-        return None
-    wide = -(-x.shape[1] // 8) * 8
-    buffer = torch.empty(sum(t.shape[0] for t in away) * wide, dtype=x.dtype, device=x.device)
-    sets = (_lib.GsRows * 2)()
-    to = buffer.data_ptr()
-    for r, t in zip(sets, away):
-        r.src, r.dst, r.rows, r.cols, r.src_stride, r.dst_stride = t.data_ptr(), to, t.shape[0], t.shape[1], t.stride(0), wide
-        to += t.shape[0] * wide * t.element_size()
-    call_on(x.device, "gs_rows_pack", sets, len(away), _DTYPES[x.dtype][0])
-    return buffer
+    """Which of x and weight the kernels cannot read, and None or a buffer with these as rows with zeros behind them."""
+    away = (not _ready(x, few), not _ready(weight, few))
+    if not (away[0] or away[1]):
+        return away, None
+    dtype, wide = x.dtype, -(-x.shape[1] // 8) * 8
+    buffer = torch.empty(((x.shape[0] if away[0] else 0) + (weight.shape[0] if away[1] else 0)) * wide, dtype=dtype,
+                         device=x.device)
+    to, sets = buffer.data_ptr(), []
+    for t, copied in ((x, away[0]), (weight, away[1])):
+        if copied:
+            rows, cols = t.shape
+            sets.append((t.data_ptr(), to, rows, cols, t.stride(0), wide))
+            to += rows * wide * _DTYPES[dtype][2]
+    call_on(x.device, "gs_rows_pack", (_lib.GsRows * 2)(*sets), len(sets), _DTYPES[dtype][0])
+    return away, buffer
 
 
-def _args(x, weight, buffer, few, bias, residual, out, z, out_dtype, activation) -> _lib.GsLinear:
-    at = []
+def _args(x, weight, buffer, away, bias, residual, out, z, out_dtype, activation) -> _lib.GsLinear:
+    (rows, inputs), outputs = x.shape, weight.shape[0]
+    code, _, size = _DTYPES[x.dtype]
     if buffer is not None:
-        to, wide = buffer.data_ptr(), -(-x.shape[1] // 8) * 8
-    for t in (x, weight):
-        if buffer is None or _ready(t, few):
-            at += (t.data_ptr(), t.stride(0) if t.shape[0] else 0)
-        else:
-            at += (to, wide)
-            to += t.shape[0] * wide * t.element_size()
-    return _lib.GsLinear(at[0], at[2], None if bias is None else bias.data_ptr(),
-                         None if residual is None else residual.data_ptr(), ptr(out), ptr(z), x.shape[0], at[1], at[3],
-                         0 if residual is None else residual.stride(0), weight.shape[1], weight.shape[0],
-                         _DTYPES[x.dtype][0], _DTYPES[out_dtype][0], 0 if z is None else _DTYPES[z.dtype][0],
-                         0 if bias is None else _DTYPES[bias.dtype][0], activation)
+        to, wide = buffer.data_ptr(), -(-inputs // 8) * 8
+    if away[0]:
+        x_at, x_stride = to, wide
+        to += rows * wide * size
+    else:
+        x_at, x_stride = x.data_ptr(), x.stride(0) if rows else 0
+    w_at, w_stride = (to, wide) if away[1] else (weight.data_ptr(), weight.stride(0))
+    return _lib.GsLinear(x_at, w_at, None if bias is None else bias.data_ptr(),
+                         None if residual is None else residual.data_ptr(), None if out is None else out.data_ptr(),
+                         None if z is None else z.data_ptr(), rows, x_stride, w_stride,
+                         0 if residual is None else residual.stride(0), inputs, outputs, code, _DTYPES[out_dtype][0],
+                         0 if z is None else _DTYPES[z.dtype][0], 0 if bias is None else _DTYPES[bias.dtype][0], activation)
+
+
+def _empty(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _workspace(name: str, a, device):
@@ -74,42 +81,43 @@ def _workspace(name: str, a, device):
 
 def _forward(x, weight, bias, residual, activation, out_dtype, keep: bool):
     few = x.shape[0] <= FEW_ROWS
-    buffer = _pack(x, weight, few)
+    away, buffer = _pack(x, weight, few)
     out = torch.empty((x.shape[0], weight.shape[0]), dtype=out_dtype, device=x.device)
     z = None
     if keep and activation:  # float32 where a bias' gradient sums its slopes; the products round them anyway
         z = torch.empty(out.shape, dtype=x.dtype if bias is None else torch.float32, device=x.device)
-    a = _args(x, weight, buffer, few, bias, residual, out, z, out_dtype, activation)
+    a = _args(x, weight, buffer, away, bias, residual, out, z, out_dtype, activation)
     ws, n = _workspace("gs_linear_fwd_workspace_size", a, x.device)
     call_on(x.device, "gs_linear_fwd", C.byref(a), ptr(ws), n)
-    return out, z, buffer
+    return out, z, buffer, away
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, out_dtype):
-        out, z, buffer = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
+        out, z, buffer, away = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, weight, bias, z, None if x.shape[0] <= FEW_ROWS else buffer)
-        ctx.rule = (out_dtype, activation)
+        ctx.rule, ctx.away = (out_dtype, activation), away
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         x, weight, bias, z, buffer = ctx.saved_tensors
-        grads = [None, None, None]
-        if any(ctx.needs_input_grad[:3]):
+        need = ctx.needs_input_grad
+        grads = (None, None, None)
+        if need[0] or need[1] or need[2]:
+            away = ctx.away
             if x.shape[0] <= FEW_ROWS:
-                buffer = _pack(x, weight, False)
+                away, buffer = _pack(x, weight, False)
             d = d_out.contiguous()
             if d.data_ptr() % 16:
                 d = d.clone()
-            grads = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if t is not None and need else None
-                     for t, need in zip((x, weight, bias), ctx.needs_input_grad)]
-            a = _args(x, weight, buffer, False, bias, None, None, z, *ctx.rule)
+            grads = (_empty(x) if need[0] else None, _empty(weight) if need[1] else None, _empty(bias) if need[2] else None)
+            a = _args(x, weight, buffer, away, bias, None, None, z, *ctx.rule)
             ws, n = _workspace("gs_linear_bwd_workspace_size", a, x.device)
-            call_on(x.device, "gs_linear_bwd", C.byref(a), ptr(d), *map(ptr, grads), ptr(ws), n)
-        return (*grads, d_out if ctx.needs_input_grad[3] else None, None, None)
+            call_on(x.device, "gs_linear_bwd", C.byref(a), ptr(d), ptr(grads[0]), ptr(grads[1]), ptr(grads[2]), ptr(ws), n)
+        return (*grads, d_out if need[3] else None, None, None)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str = "none",

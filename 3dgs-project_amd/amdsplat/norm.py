@@ -65,7 +65,7 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 9
         x, y, *weights, gate, seed_at, stats = ctx.saved_tensors
         d_h, d_n = (None if t is None else t.contiguous() for t in (d_h, d_n))
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=x.device) if t is not None and need else None
+        outs = [torch.empty_like(t, memory_format=torch.contiguous_format) if need and t is not None else None
                 for t, need in zip((x, y, *weights, gate), ctx.needs_input_grad)]
         a = _args(x, y, *weights, gate, seed_at, None, None, stats, ctx.rule)
         size = _lib.size_call("gs_residual_norm_bwd_workspace_size", C.byref(a))
