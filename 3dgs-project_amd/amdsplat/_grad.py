@@ -8,8 +8,13 @@ from torch.autograd import forward_ad
 def tracked(*tensors) -> bool:
     """An input takes a gradient, or a forward-mode level is entered, where an input may carry a tangent: the
     functions have no forward-mode derivative and say so, while reading the input's data alone would drop it."""
-    return forward_ad._current_level >= 0 or (
-        torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def refuse_tangents(tensors, what: str) -> None:

@@ -352,8 +352,9 @@ def call_on(device, name: str, *args) -> None:
     stream's handle says nothing of its device."""
     import torch
 
-    if torch._C._cuda_getDevice() == device.index:
-        call(name, *args, stream_handle(device))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index) or None)
     else:
         with torch.cuda.device(device):
             call(name, *args, stream_handle(device))

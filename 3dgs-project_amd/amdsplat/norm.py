@@ -21,31 +21,33 @@ MAX_WIDTH = 8192  # GS_NORM_MAX_WIDTH
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
 
 
-def _at(t):
-    return None if t is None else t.data_ptr()
-
-
 def _rows(t):
     return t if t is None or ((t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= 0) else t.contiguous()
 
 
 def _args(x, y, weight, bias, post_weight, post_bias, gate, seed_at, h, n, stats, rule) -> _lib.GsResidualNorm:
     layer, eps, scale, p, seed, draw, n_dtype = rule
-    w = next((t for t in (weight, bias, post_weight, post_bias) if t is not None), None)
+    w = weight if weight is not None else bias if bias is not None else post_weight  # (there is no post bias without it)
     token = gate is not None and gate.dim() == 2
+    rows, width = x.shape
     return _lib.GsResidualNorm(
-        x.data_ptr(), _at(y), _at(weight), _at(bias), _at(post_weight), _at(post_bias), _at(gate), _at(h), _at(n),
-        _at(stats), _at(seed_at), seed, draw, x.shape[0], x.stride(0), 0 if y is None else y.stride(0),
-        gate.stride(0) if token else 0, p, eps, scale, x.shape[1], _DTYPES[x.dtype], _DTYPES[n_dtype],
-        0 if w is None else _DTYPES[w.dtype], 0 if gate is None else _DTYPES[gate.dtype], token, layer)
+        x.data_ptr(), None if y is None else y.data_ptr(), None if weight is None else weight.data_ptr(),
+        None if bias is None else bias.data_ptr(), None if post_weight is None else post_weight.data_ptr(),
+        None if post_bias is None else post_bias.data_ptr(), None if gate is None else gate.data_ptr(),
+        None if h is None else h.data_ptr(), None if n is None else n.data_ptr(),
+        None if stats is None else stats.data_ptr(), None if seed_at is None else seed_at.data_ptr(), seed, draw, rows,
+        x.stride(0), 0 if y is None else y.stride(0), gate.stride(0) if token else 0, p, eps, scale, width,
+        _DTYPES[x.dtype], _DTYPES[n_dtype], 0 if w is None else _DTYPES[w.dtype],
+        0 if gate is None else _DTYPES[gate.dtype], token, layer)
 
 
 def _forward(x, y, weight, bias, post_weight, post_bias, gate, seed_at, rule, keep: bool):
-    h = None if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    n = torch.empty(x.shape, dtype=rule[-1], device=x.device)
-    stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device) if keep else None
+    shape, device = x.shape, x.device
+    h = None if y is None else torch.empty(shape, dtype=x.dtype, device=device)
+    n = torch.empty(shape, dtype=rule[-1], device=device)
+    stats = torch.empty((shape[0], 4), dtype=torch.float32, device=device) if keep else None
     a = _args(x, y, weight, bias, post_weight, post_bias, gate, seed_at, h, n, stats, rule)
-    call_on(x.device, "gs_residual_norm_fwd", C.byref(a))
+    call_on(device, "gs_residual_norm_fwd", C.byref(a))
     return h, n, stats
 
 
@@ -136,11 +138,13 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor | None 
         raise ValueError("x and y must be on one GPU")
     layer, eps = _rule(x, kind, eps, y.dtype)
     width, device = x.shape[1], x.device
-    given = [t for t in (weight, bias, post_weight, post_bias) if t is not None]
-    dtype = given[0].dtype if given else None
-    weight, bias, post_weight, post_bias = (
-        _vector(t, name, width, device, dtype) for t, name in (
-            (weight, "weight"), (bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias")))
+    w = weight if weight is not None else bias if bias is not None else post_weight if post_weight is not None else post_bias
+    if w is not None:
+        dtype = w.dtype
+        weight = None if weight is None else _vector(weight, "weight", width, device, dtype)
+        bias = None if bias is None else _vector(bias, "bias", width, device, dtype)
+        post_weight = None if post_weight is None else _vector(post_weight, "post_weight", width, device, dtype)
+        post_bias = None if post_bias is None else _vector(post_bias, "post_bias", width, device, dtype)
     if post_bias is not None and post_weight is None:
         raise ValueError("post_bias without post_weight")
     if gate is not None:
@@ -153,6 +157,6 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor | None 
     p, seed_at, seed, draw = check_rule(dropout, seed, draw, device)
     args = (_rows(x), _rows(y), weight, bias, post_weight, post_bias, gate, seed_at,
             (layer, eps, scale, p, seed, draw, y.dtype))
-    if tracked(x, y, *given, gate):
+    if tracked(x, y, weight, bias, post_weight, post_bias, gate):
         return _ResidualNorm.apply(*args)
     return _forward(*args, False)[:2]
