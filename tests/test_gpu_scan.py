@@ -178,6 +178,54 @@ def test_documents_do_not_reach_each_other(bad, reverse):
             assert torch.equal(a[keep], b[keep]), (spoiled, i)
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_documents_of_few_tokens_do_not_reach_each_other(bad, reverse):
+    """As above where a wavefront walks a document, tokens of none among them; then offsets outside the tensor, and a
+    replayed graph whose documents move between replays."""
+    tokens, cuts = 200, [5] * 50 + [9] * 60 + [120] * 40 + [131] * 30 + [190] * 30
+    x, f, o = data(17, tokens, 12, torch.float32)
+    table = torch.tensor(cuts, dtype=torch.int32, device=DEV)
+    docs, d = len(cuts) - 1, rand(18, tokens, 12)
+    initial = rand(19, docs, 12)
+
+    def run(x, f, o, d, table=table):
+        x, f, o, i = (t.detach().requires_grad_(True) for t in (x, f, o, initial))
+        y, s = gated_scan(x, f, o, offsets=table, initial=i, reverse=reverse, return_state=True)
+        return (y.detach(), s.detach(), *torch.autograd.grad((y, s), (x, f, o, i), (d, torch.ones_like(s))))
+
+    want = run(x, f, o, d)
+    assert all(bool((want[i][:5] == 0).all()) and bool((want[i][190:] == 0).all()) for i in (0, 2, 3, 4))
+    others = [i for i in range(docs) if i != cuts.index(120) - 1]
+    for spoiled in range(4):
+        v = [x.clone(), f.clone(), o.clone(), d.clone()]
+        v[spoiled][9:120:7] = bad
+        v[spoiled][:5] = bad
+        v[spoiled][190:] = bad
+        for i, (a, b) in enumerate(zip(run(*v), want)):
+            keep = others if i in (1, 5) else [*range(0, 9), *range(120, tokens)]
+            assert torch.equal(a[keep], b[keep]), (spoiled, i)
+    outside = table.clone()
+    outside[outside == 5], outside[outside == 190] = -7, 1 << 30
+    inside = outside.clamp(0, tokens)
+    assert all(torch.equal(a, b) for a, b in zip(run(x, f, o, d, outside), run(x, f, o, d, inside)))
+    moving = table.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(x, f, o, d, moving)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(x, f, o, d, moving)
+    for to in (table, inside, torch.arange(docs + 1, dtype=torch.int32, device=DEV).clamp(max=tokens), table):
+        moving.copy_(to)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, run(x, f, o, d, moving)))
+
+
 def test_offsets_outside_the_tensor_are_cut():
     x, f, o = data(9, 100, 8, torch.float32)
     t = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
