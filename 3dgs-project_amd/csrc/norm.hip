@@ -17,7 +17,7 @@
 //
 // Memory bounds all of it: 32771 x 1024 of a float32 stream and a bfloat16 branch, rms norms, gate and dropout, forward
 // 403 MB in 76 us (5.3 TB/s), backward 604 MB in 139 us (4.3 TB/s; its two sums over a row stand between loads and stores),
-// the column sums' join 5 us; one row 4.0 us. Widths above 4096 go backward at a quarter of that: see with_bwd.
+// the column sums' join 5 us; one row 4.0 us. Widths above 4096 go backward at less than half of that: see with_bwd.
 #include <algorithm>
 
 #include "gs_philox.h"
@@ -247,7 +247,35 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
   __shared__ float join[kGroups > 1 ? kGroups * kWidth : 1];
   RowSum<G, kGroups> sum{lds};
   const int lane = threadIdx.x % G;
+  // Column sums: in registers, or with sixteen elements a lane, but for the bias', in the lane's own place in LDS
+  constexpr bool kInLds = NV > 1;
+  __shared__ float4 held[kInLds ? 4 : 1][kInLds ? NV : 1][2][kInLds ? G : 1];
   float col_sum[5][NV][8] = {};
+  const auto place = [&](int k, int i, int half) -> float4& { return held[k - (k > kSumBias)][i][half][lane]; };
+  const auto add = [&](int k, int i, const float (&p)[8], const float (&q)[8]) {
+    if (kInLds && k != kSumBias) {
+      if (a.slot[k] < 0) return;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float4& to = place(k, i, half);
+        float4 c = to;
+        c.x = fmaf(p[4 * half], q[4 * half], c.x);
+        c.y = fmaf(p[4 * half + 1], q[4 * half + 1], c.y);
+        c.z = fmaf(p[4 * half + 2], q[4 * half + 2], c.z);
+        c.w = fmaf(p[4 * half + 3], q[4 * half + 3], c.w);
+        to = c;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) col_sum[k][i][j] = fmaf(p[j], q[j], col_sum[k][i][j]);
+    }
+  };
+  constexpr float kOnes[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+  if constexpr (kInLds) {
+    for (int k = 0; k < 5; ++k)
+      for (int i = 0; i < NV; ++i)
+        if (k != kSumBias) place(k, i, 0) = place(k, i, 1) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   Piece8<WHOLE> at[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) at[i] = {8 * (lane + G * i), a.width};
@@ -282,10 +310,13 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
     const Row now = next;
     RawAny8 rw[NV];
     Between8 mid[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    const auto weights = [&](int i) {
       if (a.weight) rw[i].load(a.weight, a.weights_bf16, at[i].col, at[i].loaded());
       if (a.y) mid[i].load(a, row, at[i]);
+    };
+    if (!kInLds) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) weights(i);
     }
     if (kAhead) fetch(next, row_at + step);
     const float4 st = now.stats;
@@ -293,6 +324,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (kInLds) weights(i);
       now.x[i].to(hat[i]);
       if (a.y) {
         float f[8], k[8];
@@ -318,12 +350,16 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
         const bool has = mine && at[i].has(j);
         hat[i][j] = has ? (hat[i][j] - st.x) * st.y : 0.0f;
         t[i][j] = has ? t[i][j] : 0.0f;
-        col_sum[kSumWeight][i][j] = fmaf(t[i][j], hat[i][j], col_sum[kSumWeight][i][j]);
-        col_sum[kSumBias][i][j] += t[i][j];
-        t[i][j] = has ? t[i][j] * w[j] : 0.0f;
+      }
+      add(kSumWeight, i, t[i], hat[i]);
+      add(kSumBias, i, t[i], kOnes);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        t[i][j] = mine && at[i].has(j) ? t[i][j] * w[j] : 0.0f;
         s1 = fmaf(t[i][j], hat[i][j], s1);
         s2 += t[i][j];
       }
+      if (kInLds) __builtin_amdgcn_sched_barrier(0);
     }
     const float2 m = sum(s1, s2);
     const float m1 = m.x * a.inv_width, m2 = a.layer ? m.y * a.inv_width : 0.0f;
@@ -338,24 +374,28 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
       if (a.d_x && some) store8(static_cast<X*>(a.d_x) + row * a.width + at[i].col, at[i].n, d);
       if (!a.y) continue;
       float e[8], w[8];
+      if (a.post && kInLds) mid[i].w.load(a.post_weight, a.weights_bf16, at[i].col, at[i].loaded());
       if (a.post) mid[i].w.to(w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const bool has = mine && at[i].has(j);
         e[j] = has ? a.scale * d[j] * u[i][j] : 0.0f;  // of the gate
-        col_sum[kSumGate][i][j] += e[j];
-        const float v = has ? d[j] * fk[i][j] : 0.0f;
-        t[i][j] = v;
-        if (a.post) {
-          b[i][j] = has ? b[i][j] : 0.0f;
-          col_sum[kSumPostWeight][i][j] = fmaf(v, b[i][j], col_sum[kSumPostWeight][i][j]);
-          col_sum[kSumPostBias][i][j] += v;
-          t[i][j] = has ? v * w[j] : 0.0f;
+        t[i][j] = has ? d[j] * fk[i][j] : 0.0f;
+        if (a.post) b[i][j] = has ? b[i][j] : 0.0f;
+      }
+      add(kSumGate, i, e, kOnes);
+      if (a.post) {
+        add(kSumPostWeight, i, t[i], b[i]);
+        add(kSumPostBias, i, t[i], kOnes);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          t[i][j] = mine && at[i].has(j) ? t[i][j] * w[j] : 0.0f;
           s1 = fmaf(t[i][j], b[i][j], s1);
           s2 += t[i][j];
         }
       }
       if (a.d_gate_rows && some) store8(a.d_gate_rows, a.gate_bf16, row * a.width + at[i].col, at[i].n, e);
+      if (kInLds) __builtin_amdgcn_sched_barrier(0);
     }
     if (!a.y) continue;
     if (a.post) {
@@ -378,8 +418,15 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
     float* part = a.parts + (static_cast<int64_t>(blockIdx.x) * a.sums + a.slot[k]) * a.width;
     if constexpr (kGroups == 1) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (at[i].n > 0) store8(part + at[i].col, at[i].n, col_sum[k][i]);
+      for (int i = 0; i < NV; ++i) {
+        if (kInLds && k != kSumBias) {
+          const float4 lo = place(k, i, 0), hi = place(k, i, 1);
+          const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          if (at[i].n > 0) store8(part + at[i].col, at[i].n, v);
+        } else if (at[i].n > 0) {
+          store8(part + at[i].col, at[i].n, col_sum[k][i]);
+        }
+      }
     } else {
       __syncthreads();
 #pragma unroll
@@ -475,9 +522,9 @@ static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
 }
 
 // Calls f(kernel, lanes a row) with the instance for a width: as many lanes as leave eight elements each (sixteen in the
-// forward, where a wavefront's own row needs no barrier). Above 4096 the backward has too few registers for its column sums and
-// keeps some in memory: 4096 x 8192 trained by 512 lanes of sixteen 831 us, by 1024 of eight 880; wider rows
-// are refused. Widths that are no multiple of eight take branches for their last vector: 32771 x 1024 by those
+// forward, where a wavefront's own row needs no barrier). Above 4096 the backward has too few registers: it keeps its column sums in
+// LDS and loads the weights twice, and still some of a row goes through memory: 4096 x 8192 trained by 512 lanes of
+// sixteen 408 us (829 with the sums in registers), by 1024 of eight 511; wider rows are refused. Widths that are no multiple of eight take branches for their last vector: 32771 x 1024 by those
 // instances 88 us forward and 220 with its backward, so 77 and 212.
 template <typename X, typename Y, bool WHOLE, typename F>
 static int with_fwd(int width, F f) {
