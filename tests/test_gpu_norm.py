@@ -96,6 +96,21 @@ def test_no_rows_and_plain_norm():
             near(norm(x, kind=kind, dtype=to), *(r["n"] for r in R.residual_norm(x, None, kind=kind)), "no weight")
 
 
+@pytest.mark.parametrize("stream,branch", TYPES)
+@pytest.mark.parametrize("width", [4104, 6001])
+@pytest.mark.parametrize("rows", [3, 1100])
+def test_wide_rows(rows, width, stream, branch):
+    """Above 4096 columns the backward keeps its column sums elsewhere: all five, some and none of them, rows than which there
+    are fewer workgroups."""
+    v = lambda s: rand(s, width, gain=0.3, shift=1.0)  # noqa: E731
+    x, y = rand(1, rows, width, dtype=stream), rand(2, rows, width, dtype=branch)
+    check(x, y, v(3), v(4), v(5), v(6), v(7), "layer", 0.5, 0.1)
+    if rows == 3:
+        check(x, y, None, v(4), v(5), None, rand(8, rows, width), "rms", 1.0, 0.0)
+        check(x, y, None, None, None, None, v(7), "rms", 1.0, 0.3)
+        check(x, y, None, None, None, None, None, "layer", 1.0, 0.0)
+
+
 def test_one_of_the_gradients():
     """Only h or only n goes on, only some inputs take a gradient, weights in bfloat16."""
     x, y = rand(1, 20, 96).requires_grad_(True), rand(2, 20, 96, dtype=BF16)
