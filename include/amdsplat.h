@@ -746,15 +746,17 @@ int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d
 /* ---------------------------------------------------------------------------------------
  * out [rows, outputs] = act(x weight^T + bias) + residual, x [rows, inputs] and weight [outputs, inputs] of dtype, read
  * through row strides (multiples of 16 bytes below GS_LINEAR_MAX_STRIDE elements, pointers 16-byte aligned; a stride of 0
- * repeats one row). Where inputs is no multiple of 16 bytes, rows go on to the next one with zeros (gs_rows_pack makes such rows). A
- * forward of up to GS_LINEAR_FEW_ROWS rows reads x and weight at any element's address and row stride, and no further than inputs. bias [outputs] of bias_dtype and residual [rows, outputs] of out_dtype (row
- * stride residual_stride) may be NULL. out is of out_dtype: dtype, or GS_FLOAT32 for bfloat16 products. Products and the
+ * repeats one row). Where inputs is no multiple of 16 bytes, rows go on to the next one with zeros (gs_rows_pack makes
+ * such rows). A forward of up to GS_LINEAR_FEW_ROWS rows reads x and weight at any element's address and row stride, and
+ * no further than inputs. bias [outputs] of bias_dtype and residual [rows, outputs] of out_dtype (row stride
+ * residual_stride) may be NULL. out is of out_dtype: dtype, or GS_FLOAT32 for bfloat16 products. Products and the
  * epilogue are float32, rounded once. z (of z_dtype: GS_FLOAT32, or dtype; may be NULL): x weight^T + bias, for the backward
  * of an activation, whose slopes are taken there (a float32 d_bias needs a float32 z).
  * Activations: relu, gelu z Phi(z), its tanh form, silu z sigmoid(z).
  *
  * gs_linear_bwd takes the same arguments (out and residual are not used, z is needed but for GS_ACT_NONE) and d_out [rows,
- * outputs] of out_dtype (16-byte aligned), and writes those of d_x [rows, inputs], d_weight (dtype) and d_bias (bias_dtype) that are not NULL;
+ * outputs] of out_dtype (16-byte aligned), and writes those of d_x [rows, inputs], d_weight (dtype) and d_bias
+ * (bias_dtype) that are not NULL;
  * the residual's gradient is d_out. d_out act'(z) is rounded to dtype as an operand.
  * No atomics: the same inputs give the same bits.
  * ------------------------------------------------------------------------------------- */
