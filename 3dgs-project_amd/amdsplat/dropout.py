@@ -64,7 +64,8 @@ class _Dropout(torch.autograd.Function):
 
 def dropout(x: torch.Tensor, p: float, seed, *, draw: int = 0) -> torch.Tensor:
     """x with elements dropped with probability p (0 <= p < 1, taken as a multiple of 2^-16) and the others
-    divided by 1 - p; bfloat16 or float32 on the GPU, differentiable in x. Every dimension but the last counts as rows.
+    divided by 1 - p; bfloat16 or float32 on the GPU, differentiable in x. Every dimension but the last, which is
+    below 2^31, counts as rows.
 
     seed: an integer, or an int64 CUDA tensor of one element, read when the kernels run (so a captured graph
     may be replayed with another seed; the backward pass reads it again, and autograd refuses one that was written
@@ -76,6 +77,8 @@ def dropout(x: torch.Tensor, p: float, seed, *, draw: int = 0) -> torch.Tensor:
     if not x.is_cuda:
         raise ValueError("x must be on the GPU")
     rule = check_rule(p, seed, draw, x.device)
+    if x.dim() and x.shape[-1] >= 1 << 31:
+        raise ValueError("the last dimension must be below 2^31")
     if x.dim() and x.numel() // max(x.shape[-1], 1) >= 1 << 32:
         raise ValueError("at most 2^32 - 1 rows")
     return _Dropout.apply(x, *rule) if tracked(x) else _drop(x, rule)
