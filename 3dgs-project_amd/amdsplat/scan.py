@@ -14,7 +14,7 @@ from . import _lib
 from ._grad import tracked
 from ._lib import call_on, ptr
 
-MAX_WIDTH = 1 << 20  # GS_SCAN_MAX_WIDTH
+MAX_WIDTH, MAX_DOCS = 1 << 20, (1 << 30) - 1  # GS_SCAN_MAX_WIDTH, and what gs_gated_scan_fwd takes
 _DTYPES = {torch.float32: _lib.GS_FLOAT32, torch.bfloat16: _lib.GS_BFLOAT16}
 
 
@@ -107,6 +107,8 @@ def gated_scan(x: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | None 
                 and offsets.is_contiguous() and offsets.device == x.device and offsets.shape[0] >= 2):
             raise ValueError("offsets must be a contiguous int32 tensor of at least 2 entries on x's device")
         docs = offsets.shape[0] - 1
+        if docs > MAX_DOCS:
+            raise ValueError(f"{docs} documents: up to {MAX_DOCS} are provided")
     if initial is not None:
         if initial.shape != (docs, x.shape[1]) or initial.dtype != torch.float32 or initial.device != x.device:
             raise ValueError(f"initial must be float32 [{docs}, {x.shape[1]}] on x's device")

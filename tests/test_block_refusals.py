@@ -3,7 +3,7 @@ calls would cut to another, valid one. The tensors are of the meta device and cl
 import pytest
 import torch
 
-from amdsplat import dropout
+from amdsplat import dropout, gated_scan
 
 
 class Claimed(torch.Tensor):
@@ -21,3 +21,12 @@ def test_dropout_over_a_long_dimension(width, grad):
     for shape in ((width,), (1, width), (3, 2, width)):
         with pytest.raises(ValueError, match="last dimension"):
             dropout(claimed(*shape, dtype=torch.bfloat16).requires_grad_(grad), 0.5, 1)
+
+
+@pytest.mark.parametrize("docs", [1 << 30, 1 << 32, (1 << 32) + 2])
+def test_a_recurrence_over_many_documents(docs):
+    """2^32 + 2 documents would be taken as 2, and the other documents' states never be written."""
+    x, offsets = claimed(10, 8), claimed(docs + 1, dtype=torch.int32)
+    for initial in (None, claimed(docs, 8)):
+        with pytest.raises(ValueError, match="documents"):
+            gated_scan(x, x, offsets=offsets, initial=initial, return_state=True)
