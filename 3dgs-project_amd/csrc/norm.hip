@@ -321,6 +321,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
     if (kAhead) fetch(next, row_at + step);
     const float4 st = now.stats;
     float hat[NV][8], t[NV][8], b[NV][8], u[NV][8], fk[NV][8];
+    uint32_t kept[NV] = {};  // a bit an element: a dropped one's gradient is zero whatever arrives
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -338,6 +339,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
         for (int j = 0; j < 8; ++j) {
           hat[i][j] = fmaf(f[j], u[i][j], hat[i][j]);
           fk[i][j] = f[j] * k[j];
+          kept[i] |= static_cast<uint32_t>(k[j] != 0.0f) << j;
         }
       }
       now.d_n[i].to(t[i]);
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
       for (int j = 0; j < 8; ++j) {
         const bool has = mine && at[i].has(j);
         e[j] = has ? a.scale * d[j] * u[i][j] : 0.0f;  // of the gate
-        t[i][j] = has ? d[j] * fk[i][j] : 0.0f;
+        t[i][j] = has && (kept[i] >> j & 1) ? d[j] * fk[i][j] : 0.0f;
         if (a.post) b[i][j] = has ? b[i][j] : 0.0f;
       }
       add(kSumGate, i, e, kOnes);

@@ -1,0 +1,39 @@
+"""What is not finite beside the block operators' dropped, masked and padded elements, and calls at their limits."""
+import math
+
+import pytest
+import torch
+
+import block_ref as R
+from amdsplat import residual_norm
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def rand(seed, *shape, dtype=F32, gain=1.0):
+    return (gain * torch.randn(shape, generator=torch.Generator().manual_seed(seed))).to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("width", [77, 96, 1100, 4104])
+def test_a_dropped_elements_gradient_is_zero(width, post, bad):
+    """Whatever arrives at it (h's gradient alone is spoiled, so no sum over a row is), as from `dropout` by itself."""
+    rows, seed, p = 11, 7, 0.4
+    x, y = rand(1, rows, width).requires_grad_(True), rand(2, rows, width, dtype=BF16).requires_grad_(True)
+    w, gate, pw = rand(3, width), rand(4, width), rand(5, width).requires_grad_(True) if post else None
+    d_h, d_n = rand(6, rows, width), rand(7, rows, width, dtype=BF16)
+    dropped = R.keep(rows, width, seed, 0, p).to(DEV) == 0
+    leaves = [y] + ([pw] if post else [])
+
+    def grads(d_h, gate):
+        h, n = residual_norm(x, y, w, post_weight=pw, gate=gate, dropout=p, seed=seed)
+        return torch.autograd.grad((h, n), leaves, (d_h, d_n))
+
+    want = grads(d_h, gate)
+    got = grads(torch.where(dropped, torch.full_like(d_h, bad), d_h), gate)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert bool((want[0][dropped] == 0).all()) or post
