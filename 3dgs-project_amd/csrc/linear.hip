@@ -105,33 +105,42 @@ __device__ __forceinline__ void activate8(int act, float (&v)[8]) {
     default: return;
   }
 }
-// act'(z) in place of z.
+// d act'(z) in place of d. relu passes d or does not: where z is not positive the gradient is 0 whatever arrives, and where z is
+// NaN it goes on.
 template <typename T>
-__device__ __forceinline__ void slope8(int act, float (&v)[8]) {
+__device__ __forceinline__ void slope8(int act, float (&v)[8], float (&d)[8]) {
   const auto near = [](float z) { return z < -kFar ? -kFar : (z > kFar ? kFar : z); };
   switch (act) {
-    case kActRelu: return each8(v, [](float z) { return z > 0.0f ? 1.0f : 0.0f; });
+    case kActRelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = v[j] <= 0.0f ? 0.0f : d[j];
+      return;
     case kActGelu:
-      return each8(v, [&](float z) {
+      each8(v, [&](float z) {
         float bell;
         z = near(z);
         const float p = normal_cdf<T>(z, bell);
         return fmaf(z * 0.3989422804014327f, bell, p);
       });
+      break;
     case kActGeluTanh:
-      return each8(v, [&](float z) {
+      each8(v, [&](float z) {
         z = near(z);
         const float p = sigmoid<T>(kTanhOuter * fmaf(kTanhInner * z * z, z, z));
         return fmaf(z * p * (1.0f - p), kTanhOuter * fmaf(3.0f * kTanhInner * z, z, 1.0f), p);
       });
+      break;
     case kActSilu:
-      return each8(v, [&](float z) {
+      each8(v, [&](float z) {
         z = near(z);
         const float p = sigmoid<T>(z);
         return fmaf(z * p, 1.0f - p, p);
       });
-    default: return each8(v, [](float) { return 1.0f; });
+      break;
+    default: return;
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d[j] *= v[j];
 }
 
 // ---- the tile kernel ---------------------------------------------------------------------------------
@@ -580,9 +589,7 @@ __global__ __launch_bounds__(kSlopeThreads) void slope_kernel(SlopeArgs a) {
     load8(static_cast<const O*>(a.d_out) + row * a.n + col, n, d);
     if (a.act != kActNone) {
       load8(a.z, a.z_bf16, row * a.n + col, n, z);
-      slope8<T>(a.act, z);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] *= z[j];
+      slope8<T>(a.act, z, d);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] += d[j];

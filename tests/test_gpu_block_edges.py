@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import block_ref as R
-from amdsplat import residual_norm
+from amdsplat import linear, residual_norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -37,3 +37,26 @@ def test_a_dropped_elements_gradient_is_zero(width, post, bad):
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert bool((want[0][dropped] == 0).all()) or post
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [7, 70])
+def test_relus_gradient_beside_what_is_not_finite(rows, dtype):
+    """With the identity for a weight the products are exact: z is x, and x's gradient the output's where z is positive, 0 where it is
+    not, whatever arrives there. A row of NaN lets its gradient through, as torch's relu does."""
+    n = 64
+    x = rand(1, rows, n, dtype=dtype)
+    bias = torch.zeros(n, device=DEV, requires_grad=True)
+    eye, d = torch.eye(n, dtype=dtype, device=DEV), rand(2, rows, n, dtype=dtype)
+    d = torch.where((x <= 0) & (rand(3, rows, n) > 0), torch.full_like(d, math.inf), d)
+    x[5, 3] = math.nan  # (all of z's row 5: 0 times NaN)
+    d[5] = rand(4, n, dtype=dtype)
+    want = torch.where(x <= 0, torch.zeros_like(d), d)
+    want[5] = d[5]
+    for b in (None, bias):
+        leaves = [x.clone().requires_grad_(True)] + ([] if b is None else [b])
+        got = torch.autograd.grad(linear(leaves[0], eye, b, activation="relu"), leaves, d)
+        assert torch.equal(got[0], want)
+        if b is not None:
+            size = want.double().abs().sum(0)
+            assert bool(((got[1].double() - want.double().sum(0)).abs() <= (rows + 2) * 2.0 ** -24 * size).all())
