@@ -34,9 +34,14 @@ def _ready(t: torch.Tensor, few: bool) -> bool:
     return few or (t.shape[1] % per == 0 and t.stride(1) == 1 and s % per == 0 and t.data_ptr() % 16 == 0)
 
 
-def _pack(x, weight, few: bool):
-    """Which of x and weight the kernels cannot read, and None or a buffer with these as rows with zeros behind them."""
-    away = (not _ready(x, few), not _ready(weight, few))
+def _overlaps(t: torch.Tensor) -> bool:
+    return t.shape[0] > 1 and t.stride(0) < t.shape[1]
+
+
+def _pack(x, weight, few: bool, apart: bool = False):
+    """Which of x and weight the kernels cannot read, and None or a buffer with these as rows with zeros behind them. apart:
+    rows that overlap are among these."""
+    away = (not _ready(x, few) or (apart and _overlaps(x)), not _ready(weight, few) or (apart and _overlaps(weight)))
     if not (away[0] or away[1]):
         return away, None
     dtype, wide = x.dtype, -(-x.shape[1] // 8) * 8
@@ -96,8 +101,9 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, out_dtype):
         out, z, buffer, away = _forward(x, weight, bias, residual, activation, out_dtype, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, bias, z, None if x.shape[0] <= FEW_ROWS else buffer)
-        ctx.rule, ctx.away = (out_dtype, activation), away
+        again = x.shape[0] <= FEW_ROWS or _overlaps(x) or _overlaps(weight)  # the backward reads them in other ways
+        ctx.save_for_backward(x, weight, bias, z, None if again else buffer)
+        ctx.rule, ctx.away = (out_dtype, activation), None if again else away
         return out
 
     @staticmethod
@@ -108,8 +114,8 @@ class _Linear(torch.autograd.Function):
         grads = (None, None, None)
         if need[0] or need[1] or need[2]:
             away = ctx.away
-            if x.shape[0] <= FEW_ROWS:
-                away, buffer = _pack(x, weight, False)
+            if away is None:
+                away, buffer = _pack(x, weight, False, apart=True)
             d = d_out.contiguous()
             if d.data_ptr() % 16:
                 d = d.clone()
@@ -130,7 +136,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     keeps: in float32, or without a bias in x's dtype. No forward-mode derivative.
 
     x and weight are read through their row strides where these, the addresses and K are multiples of 16 bytes, and in a
-    forward of up to 16 rows wherever the last dimension is contiguous; otherwise they are copied first, at every call."""
+    forward of up to 16 rows wherever the last dimension is contiguous; otherwise they are copied first, at every call, and so are
+    rows that overlap (an expanded tensor's) for the backward."""
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"x must be [tokens, inputs] and weight [outputs, inputs], got {tuple(x.shape)} and {tuple(weight.shape)}")
     if x.dtype not in _DTYPES or weight.dtype != x.dtype:

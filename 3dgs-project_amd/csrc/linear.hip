@@ -792,6 +792,9 @@ static int check_linear(const gs_linear* p, bool backward) {
   GS_REQUIRE(aligned(p->x, few ? es : 16) && aligned(p->weight, few ? es : 16) && aligned(p->z, row_type_bytes(p->z_dtype)) &&
                  aligned(p->bias, row_type_bytes(p->bias_dtype)) && aligned(p->residual, os) && aligned(p->out, os),
              GS_ERR_ALIGN, "linear: misaligned tensor (x and weight: 16 bytes)");
+  // The gradients' products run over rows, and what is past the last one is outside the operand (Side::stage) only where rows do not overlap.
+  GS_REQUIRE(!backward || ((p->rows <= 1 || p->x_stride >= p->inputs) && (p->outputs == 1 || p->weight_stride >= p->inputs)),
+             GS_ERR_ARG, "linear: rows that overlap have no backward pass: copy them first");
   // grids of a dimension below 2^32 threads; results indexed below 2^62
   const int64_t m = p->rows, n = p->outputs, k = p->inputs;
   GS_REQUIRE((m + 63) / 64 * ((std::max(n, k) + 63) / 64) < (int64_t(1) << 23) && m * ((std::max(n, k) + 7) / 8) < (int64_t(1) << 32),
@@ -900,11 +903,13 @@ static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* 
   g.out_bf16 = sizeof(T) == 2;
   const void* dz = make_dz ? static_cast<const void*>(ws) : d_out;
   const int64_t ld = make_dz ? b.ld : p->outputs;
+  // a single row's stride says nothing, and may be 0
+  const int64_t per = 16 / static_cast<int64_t>(sizeof(T)), apart = (p->inputs + per - 1) / per * per;
   if (d_x && p->rows > 0) {
     g.a = dz;
     g.lda = ld;
     g.b = p->weight;
-    g.ldb = p->weight_stride;
+    g.ldb = std::max(p->weight_stride, apart);
     g.m = p->rows;
     g.n = p->inputs;
     g.k = p->outputs;
@@ -915,7 +920,7 @@ static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* 
     g.a = dz;
     g.lda = ld;
     g.b = p->x;
-    g.ldb = p->x_stride;
+    g.ldb = std::max(p->x_stride, apart);
     g.m = p->outputs;
     g.n = p->inputs;
     g.k = p->rows;

@@ -756,8 +756,8 @@ int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d
  *
  * gs_linear_bwd takes the same arguments (out and residual are not used, z is needed but for GS_ACT_NONE) and d_out [rows,
  * outputs] of out_dtype (16-byte aligned), and writes those of d_x [rows, inputs], d_weight (dtype) and d_bias
- * (bias_dtype) that are not NULL;
- * the residual's gradient is d_out. d_out act'(z) is rounded to dtype as an operand.
+ * (bias_dtype) that are not NULL; the residual's gradient is d_out. Rows of x or of weight that overlap (a stride below inputs, of
+ * more than one row) are refused there: copies have a backward pass (gs_rows_pack). d_out act'(z) is rounded to dtype as an operand.
  * No atomics: the same inputs give the same bits.
  * ------------------------------------------------------------------------------------- */
 #define GS_LINEAR_MAX_WIDTH (1 << 19)

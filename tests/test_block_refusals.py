@@ -1,9 +1,12 @@
 """Sizes that the block operators refuse before anything is allocated or launched: counts that a 32-bit argument of the C
 calls would cut to another, valid one. The tensors are of the meta device and claim to be on the GPU."""
+import ctypes as C
+
 import pytest
 import torch
 
-from amdsplat import dropout, gated_scan
+from amdsplat import _lib, dropout, gated_scan
+from test_block_errors import ARG, WORKSPACE, expect, linear_args
 
 
 class Claimed(torch.Tensor):
@@ -30,3 +33,13 @@ def test_a_recurrence_over_many_documents(docs):
     for initial in (None, claimed(docs, 8)):
         with pytest.raises(ValueError, match="documents"):
             gated_scan(x, x, offsets=offsets, initial=initial, return_state=True)
+
+
+@pytest.mark.parametrize("kw", [dict(x_stride=32), dict(weight_stride=0), dict(x_stride=0), dict(rows=16, x_stride=60)])
+def test_a_projections_gradient_of_rows_that_overlap(kw):
+    """(In Python they are copied first.) A single row has any stride."""
+    L = _lib.lib()
+    a = linear_args(**kw)
+    expect(L.gs_linear_bwd(C.byref(a), 256, 256, 256, 256, 256, 1 << 62, None), ARG, "overlap")
+    one = linear_args(rows=1, outputs=1, x_stride=0, weight_stride=0)
+    expect(L.gs_linear_bwd(C.byref(one), 256, 256, 256, 256, None, 0, None), WORKSPACE, "workspace")

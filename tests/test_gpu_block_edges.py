@@ -60,3 +60,27 @@ def test_relus_gradient_beside_what_is_not_finite(rows, dtype):
         if b is not None:
             size = want.double().abs().sum(0)
             assert bool(((got[1].double() - want.double().sum(0)).abs() <= (rows + 2) * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 9, 40, 300])
+def test_gradients_of_rows_that_overlap(rows, dtype):
+    """Windows that move by a quarter of their width (or a single row of stride 0), with an infinity in the last one: in the
+    gradients it reaches its own columns, as in those of copies."""
+    k, step = 128, 32 if rows > 1 else 0
+    flat = rand(1, (rows - 1) * step + k, dtype=dtype)
+    flat[(rows - 1) * step + 40] = math.inf
+    windows, plain, d = flat.as_strided((rows, k), (step, 1)), rand(2, 40, k, dtype=dtype), rand(3, rows, 40, dtype=dtype)
+
+    def grads(x, w, d, bias=None):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        return torch.autograd.grad(linear(x, w, bias), (x, w), d)
+
+    for a, b in ((windows, plain), (plain, windows)):
+        g = d if a is windows else d.t().contiguous()
+        got, want = grads(a, b, g), grads(a.clone(memory_format=torch.contiguous_format), b.clone(memory_format=torch.contiguous_format), g)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        finite = torch.ones(k, dtype=torch.bool, device=DEV)
+        finite[[i for i in range(k) if not math.isfinite(float(windows[:, i].float().abs().max()))]] = False
+        assert 0 < int((~finite).sum()) <= 3
+        assert bool(torch.isfinite(got[1] if a is windows else got[0])[:, finite].all())
