@@ -349,7 +349,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
       if (a.weight) rw[i].to(w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool has = mine && at[i].has(j);
+        const bool has = mine && a.d_n && at[i].has(j);
         hat[i][j] = has ? (hat[i][j] - st.x) * st.y : 0.0f;
         t[i][j] = has ? t[i][j] : 0.0f;
       }
@@ -371,8 +371,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
       const bool some = mine && at[i].n > 0;
       float d[8];
       now.d_h[i].to(d);
+      if (a.d_n) {  // (a norm whose result goes nowhere adds nothing, whatever the row holds)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
+        for (int j = 0; j < 8; ++j) d[j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
+      }
       if (a.d_x && some) store8(static_cast<X*>(a.d_x) + row * a.width + at[i].col, at[i].n, d);
       if (!a.y) continue;
       float e[8], w[8];

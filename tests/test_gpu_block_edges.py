@@ -84,3 +84,18 @@ def test_gradients_of_rows_that_overlap(rows, dtype):
         finite[[i for i in range(k) if not math.isfinite(float(windows[:, i].float().abs().max()))]] = False
         assert 0 < int((~finite).sum()) <= 3
         assert bool(torch.isfinite(got[1] if a is windows else got[0])[:, finite].all())
+
+
+@pytest.mark.parametrize("width", [50, 64, 2000, 5000])
+def test_a_norm_that_goes_nowhere_adds_nothing(width):
+    """h alone is used, and rows of it are not finite: x's gradient is h's, the next norm's weight has none."""
+    x, y, w = rand(1, 9, width), rand(2, 9, width).requires_grad_(True), rand(3, width).requires_grad_(True)
+    x[2, 5], x[4, 49], x[6, 0] = math.inf, math.nan, -math.inf
+    x.requires_grad_(True)
+    gate, d = rand(4, width), rand(5, 9, width)
+    for kind in ("rms", "layer"):
+        h, _ = residual_norm(x, y, w, w, kind=kind, gate=gate, scale=0.5)
+        dx, dy, dw = torch.autograd.grad(h, (x, y, w), d)
+        assert torch.equal(dx, d) and bool((dw == 0).all())
+        want = (0.5 * gate.double() * d.double())
+        assert bool(((dy.double() - want).abs() <= 2 * 2.0 ** -24 * want.abs()).all())
