@@ -108,8 +108,8 @@ def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor
          eps: float = 1e-6, dtype: torch.dtype | None = None) -> torch.Tensor:
     """weight x^ + bias over the rows of x [T, C], x^ = x / sqrt(mean x^2 + eps), or with kind "layer"
     (x - mean x) / sqrt(var x + eps); differentiable in x, weight and bias ([C], one dtype, either may be None). dtype
-    of the result: x's by default, or bfloat16 of a float32 x. C up to 8192; the mean of a row's squares
-    has to be finite in float32. No forward-mode derivative."""
+    of the result: x's by default, or bfloat16 of a float32 x. C up to 8192, T below 2^31, T C below 2^38; the mean of a
+    row's squares has to be finite in float32. No forward-mode derivative."""
     dtype = x.dtype if dtype is None else dtype
     layer, eps = _rule(x, kind, eps, dtype)
     weight = _vector(weight, "weight", x.shape[1], x.device)

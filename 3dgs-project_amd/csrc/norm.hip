@@ -30,6 +30,7 @@ struct NormArgs {
   void *h, *n;
   float* stats;  // [rows][4]: mean and 1 / deviation of h, of y
   int64_t rows, x_stride, y_stride, gate_stride;
+  int64_t first;  // row of a forward launch
   int width;
   bool layer, post, weights_bf16, gate_bf16;
   float eps, scale, inv_width;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(NormArgs a)
   __shared__ float2 lds[2][kGroups][G / kWave];
   RowSum<G, kGroups> sum{lds};
   const int lane = threadIdx.x % G;
-  const int64_t row_at = static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
+  const int64_t row_at = a.first + static_cast<int64_t>(blockIdx.x) * kGroups + threadIdx.x / G;
   // (groups past the last row repeat it without writing: every lane meets every barrier)
   const bool mine = row_at < a.rows;
   const int64_t row = mine ? row_at : a.rows - 1;
@@ -474,6 +475,9 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(const T* x, T* ou
 constexpr int64_t kNormParts = 512;
 static int64_t norm_parts(int64_t rows) { return std::min<int64_t>(kNormParts, rows); }
 
+// Workgroups of one launch of the forward, below the 2^32 threads that a grid may have: more rows take several.
+constexpr int64_t kNormLaunch = 1 << 22;
+
 static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
   GS_REQUIRE(p, GS_ERR_ARG, "residual norm: args is NULL");
   GS_REQUIRE(row_type(p->x_dtype) && row_type(p->y_dtype), GS_ERR_ARG,
@@ -486,6 +490,7 @@ static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
   GS_REQUIRE(p->rows >= 0 && p->rows < (int64_t(1) << 31), GS_ERR_ARG, "residual norm: invalid row count");
   GS_REQUIRE(p->width >= 1 && p->width <= GS_NORM_MAX_WIDTH, GS_ERR_ARG, "residual norm: width %d: 1 to %d are provided",
              p->width, GS_NORM_MAX_WIDTH);
+  GS_REQUIRE(p->rows * p->width < (int64_t(1) << 38), GS_ERR_ARG, "residual norm: too many elements");
   GS_REQUIRE(p->eps > 0.0f && p->eps <= 1e30f, GS_ERR_ARG, "residual norm: eps must be positive and finite");
   GS_REQUIRE(p->scale - p->scale == 0.0f, GS_ERR_ARG, "residual norm: scale must be finite");
   GS_REQUIRE(p->dropout >= 0.0 && p->dropout < 1.0, GS_ERR_ARG, "residual norm: dropout must be at least 0 and below 1");
@@ -564,11 +569,12 @@ extern "C" int gs_residual_norm_fwd(const gs_residual_norm* p, void* stream) {
   if (a.rows == 0) return GS_OK;
   const auto run = [&](auto kernel, int lanes) -> int {
     const int groups = std::max(1, 256 / lanes);
-    GS_REQUIRE((a.rows + groups - 1) / groups * std::max(256, lanes) < (int64_t(1) << 32), GS_ERR_ARG,
-               "residual norm: too many rows of this width");
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((a.rows + groups - 1) / groups)), dim3(std::max(256, lanes)), 0,
-                       as_stream(stream), a);
-    return check_launch("residual norm");
+    for (a.first = 0; a.first < a.rows; a.first += kNormLaunch * groups) {
+      const int64_t blocks = std::min(kNormLaunch, (a.rows - a.first + groups - 1) / groups);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(std::max(256, lanes)), 0, as_stream(stream), a);
+      if (const int rc = check_launch("residual norm")) return rc;
+    }
+    return GS_OK;
   };
   return with_types(p, [&](auto x, auto y) {
     using X = decltype(x);

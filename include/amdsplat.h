@@ -671,8 +671,9 @@ int gs_attention_bwd(const gs_attention* args, const void* d_out, void* d_q, voi
  * post_bias and gate may be NULL; gate is [width], or with gate_rows [rows, width]. k is the dropout's factors (see
  * gs_dropout; dropout 0: one). x and h are of x_dtype, y and n of y_dtype (float32 streams take either,
  * bfloat16 streams bfloat16), the weights and biases of weight_dtype. x, y and gate are read through row
- * strides (elements); the rest is contiguous, at an element's alignment. Sums are float32: the mean of a row's squares
- * has to be finite there. stats (float32 [rows, 4], 16-byte aligned; NULL if no backward pass follows): the
+ * strides (elements); the rest is contiguous, at an element's alignment. Fewer than 2^31 rows and 2^38 elements. Sums are
+ * float32: the mean of a row's squares has to be finite there. stats (float32 [rows, 4], 16-byte aligned; NULL if no
+ * backward pass follows): the
  * rows' mean and 1 / deviation of h and of y.
  *
  * gs_residual_norm_bwd takes the same arguments (h and n are not used), d_h of x_dtype and d_n of y_dtype (either may be

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import block_ref as R
-from amdsplat import linear, residual_norm
+from amdsplat import dropout, linear, norm, residual_norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -99,3 +99,40 @@ def test_a_norm_that_goes_nowhere_adds_nothing(width):
         assert torch.equal(dx, d) and bool((dw == 0).all())
         want = (0.5 * gate.double() * d.double())
         assert bool(((dy.double() - want).abs() <= 2 * 2.0 ** -24 * want.abs()).all())
+
+
+def test_rows_of_several_launches():
+    """2^26 rows and more: norms of heads over a long batch. Pieces of the rows give the same bits; the dropout's rows go on being
+    counted, so the parts of a branch by themselves give h and n."""
+    t, c, piece = (1 << 26) + 5, 8, 1 << 23
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(t, c, generator=g, device=DEV, dtype=BF16).requires_grad_(True)
+    w = rand(2, c).requires_grad_(True)
+    n = norm(x, w)
+    with torch.no_grad():
+        for at in range(0, t, piece):
+            assert torch.equal(n[at:at + piece], norm(x[at:at + piece], w)), at
+    d = torch.randn(t, c, generator=g, device=DEV, dtype=BF16)
+    dx, dw = torch.autograd.grad(n, (x, w), d)
+    want, size = torch.zeros(2, c, dtype=torch.float64, device=DEV)
+    for at in range(0, t, piece):
+        r = slice(at, at + piece)
+        near = x[r].detach().requires_grad_(True)
+        assert torch.equal(dx[r], torch.autograd.grad(norm(near, w), near, d[r])[0])
+        hat = x[r].detach().double()
+        hat *= (hat.square().mean(1, keepdim=True) + 1e-6).rsqrt()
+        want += (d[r].double() * hat).sum(0)
+        size += (d[r].double() * hat).abs().sum(0)
+    # 512 workgroups of four rows at a time, their sums and their join
+    assert bool(((dw.double() - want).abs() <= (t / 2048 + 600 + 32) * 2.0 ** -24 * size).all())
+    del n, d, dx
+    x = x.detach()
+    y = torch.randn(t, c, generator=g, device=DEV, dtype=BF16)
+    h, n = residual_norm(x.float(), y, w.detach(), dropout=0.25, seed=9)
+    for at in range(0, t, piece):
+        r = slice(at, at + piece)
+        assert torch.equal(n[r], norm(h[r], w.detach(), dtype=BF16)), at
+    kept = h != x.float()
+    assert torch.equal(kept, (dropout(torch.ones_like(y), 0.25, 9) != 0) & (y != 0) & kept)
+    missed = (dropout(torch.ones_like(y), 0.25, 9) != 0) & ~kept  # only where the branch vanishes beside the stream
+    assert bool((y[missed].float().abs() <= 2.0 ** -23 * x[missed].float().abs()).all())
