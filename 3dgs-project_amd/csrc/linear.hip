@@ -658,7 +658,7 @@ constexpr TileCost kTileCost[2][3] = {{{128, 2, 1.96f, 2.4f}, {64, 4, 0.51f, 0.7
 // stages, which costs a second launch, and the parts written and read. 8203 rows are 65 tiles of 128, so that 512 of 65 x 8
 // tiles fill the chip and the other eight would take half as long again: 8203 x 1024 results over 4096 take 103 us
 // whole, 77 us with those eight in sixteen parts each; 4096 x 1024 over 8203 88 us in 256 tiles, 73 us in 2 x 256 parts.
-static GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, size_t es, size_t result) {
+static GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, size_t es, size_t result, bool cut = true) {
   GemmPlan best = {};
   float least = FLT_MAX;
   const int64_t stage = 128 / static_cast<int64_t>(es);
@@ -683,7 +683,7 @@ static GemmPlan gemm_plan(int64_t m, int64_t n, int64_t k, size_t es, size_t res
     };
     take(0, stages);
     const int others = tiles <= kCus ? tiles : tiles % kCus;
-    if (others == 0 || (tiles > kCus && others > kCus / 2)) continue;
+    if (!cut || others == 0 || (tiles > kCus && others > kCus / 2)) continue;
     for (const int p : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
       if (stages < 4 * p) break;
       take(others, (stages + p - 1) / p);
@@ -717,11 +717,13 @@ static int run_gemm(GemmArgs g, const GemmPlan& p, void* workspace, const char* 
   if (p.tile == 128) return launch_gemm<T, 128, 2, 2, A_ALONG, B_ALONG>(g, what, st);
   return launch_gemm<T, 64, 2, 2, A_ALONG, B_ALONG>(g, what, st);
 }
-static size_t result_bytes(const gs_linear* p) {
-  return row_type_bytes(p->out_dtype) + (p->z ? row_type_bytes(p->z_dtype) : 0) + (p->residual ? row_type_bytes(p->out_dtype) : 0);
-}
+// A call that keeps z gives the same bits as one that does not: where the contraction is cut goes without z. Tiles that are made whole sum in one
+// order whatever their side is, so that z's stores may choose it.
 static GemmPlan forward_plan(const gs_linear* p) {
-  return gemm_plan(p->rows, p->outputs, p->inputs, row_type_bytes(p->dtype), result_bytes(p));
+  const size_t es = row_type_bytes(p->dtype), result = row_type_bytes(p->out_dtype) * (p->residual ? 2 : 1);
+  const GemmPlan g = gemm_plan(p->rows, p->outputs, p->inputs, es, result);
+  if (!p->z || g.part) return g;
+  return gemm_plan(p->rows, p->outputs, p->inputs, es, result + row_type_bytes(p->z_dtype), false);
 }
 // of d_x and of d_weight
 static GemmPlan input_plan(const gs_linear* p) {

@@ -136,3 +136,17 @@ def test_rows_of_several_launches():
     assert torch.equal(kept, (dropout(torch.ones_like(y), 0.25, 9) != 0) & (y != 0) & kept)
     missed = (dropout(torch.ones_like(y), 0.25, 9) != 0) & ~kept  # only where the branch vanishes beside the stream
     assert bool((y[missed].float().abs() <= 2.0 ** -23 * x[missed].float().abs()).all())
+
+
+@pytest.mark.parametrize("dtype,shape", [
+    (BF16, (2763, 3821, 4951)), (BF16, (3099, 4101, 201)), (BF16, (981, 1113, 3081)), (BF16, (10009, 1167, 307)), (BF16, (2305, 1565, 1801)),
+    (F32, (943, 1099, 2491)), (F32, (1299, 3493, 1027)), (F32, (8251, 835, 59))])
+def test_a_projection_is_the_same_with_and_without_gradients(dtype, shape):
+    """What is kept for the backward pass changes neither where the contraction is cut nor a bit of the result."""
+    m, n, k = shape
+    x, w, b = rand(1, m, k, dtype=dtype), rand(2, n, k, dtype=dtype, gain=1 / math.sqrt(k)).requires_grad_(True), rand(3, n)
+    for bias in (None, b):
+        out = linear(x, w, bias, activation="gelu")
+        assert out.requires_grad
+        with torch.no_grad():
+            assert torch.equal(out.detach(), linear(x, w, bias, activation="gelu"))
