@@ -276,6 +276,7 @@ _SIGS = {
     "gs_gated_scan_fwd": (_i32, [_vp, _vp, _sz, _vp]),
     "gs_gated_scan_bwd": (_i32, [_vp] * 8 + [_sz, _vp]),
     "gs_rows_pack": (_i32, [_vp, _i32, _i32, _vp]),
+    "gs_linear_plan": (_i32, [_vp, _i32, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "gs_linear_fwd_workspace_size": (_sz, [_vp]),
     "gs_linear_fwd": (_i32, [_vp, _vp, _sz, _vp]),
     "gs_linear_bwd_workspace_size": (_sz, [_vp]),

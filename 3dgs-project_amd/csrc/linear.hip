@@ -834,6 +834,21 @@ extern "C" int gs_rows_pack(const gs_rows* sets, int n, int dtype, void* stream)
   return check_launch("row pack");
 }
 
+extern "C" int gs_linear_plan(const gs_linear* p, int product, int32_t* tile, int32_t* whole, int32_t* parts) {
+  clear_error();
+  GS_REQUIRE(tile && whole && parts, GS_ERR_ARG, "linear plan: null pointer");
+  GS_REQUIRE(product >= GS_LINEAR_FORWARD && product <= GS_LINEAR_D_WEIGHT, GS_ERR_ARG, "linear plan: unknown product");
+  if (const int rc = check_linear(p, product != GS_LINEAR_FORWARD)) return rc;
+  GemmPlan g = {};
+  if (product == GS_LINEAR_D_WEIGHT) g = weight_plan(p);
+  else if (product == GS_LINEAR_D_X && p->rows > 0) g = input_plan(p);
+  else if (product == GS_LINEAR_FORWARD && p->rows > kFewRows) g = forward_plan(p);
+  *tile = g.tile;
+  *whole = g.whole;
+  *parts = g.whole < g.tiles_m * g.tiles_n ? g.splits : 0;
+  return GS_OK;
+}
+
 extern "C" size_t gs_linear_fwd_workspace_size(const gs_linear* p) {
   clear_error();
   if (!p || p->rows <= kFewRows || p->inputs <= 0 || p->outputs <= 0 || !row_type(p->dtype)) return 0;

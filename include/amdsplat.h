@@ -783,6 +783,12 @@ typedef struct gs_rows {
   int64_t rows, cols, src_stride, dst_stride;
 } gs_rows;
 int gs_rows_pack(const gs_rows* sets, int n, int dtype, void* stream);
+/* How a product is cut, for those who measure: the side of its tiles of results (256, 128 or 64; 0: none, the forward of few rows), how
+ * many of them one workgroup makes alone, and into how many parts along the contraction each of the others is cut (0: there are none). */
+#define GS_LINEAR_FORWARD 0
+#define GS_LINEAR_D_X 1
+#define GS_LINEAR_D_WEIGHT 2
+int gs_linear_plan(const gs_linear* args, int product, int32_t* tile, int32_t* whole, int32_t* parts);
 size_t gs_linear_fwd_workspace_size(const gs_linear* args);
 int gs_linear_fwd(const gs_linear* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t gs_linear_bwd_workspace_size(const gs_linear* args);
