@@ -88,6 +88,8 @@ class SplatPredictor(torch.nn.Module):
         heads = c.heads + 2 * c.kv_heads
         if not c.fused and (c.sandwich or c.dropout or c.scan):
             raise ValueError("sandwich, dropout and scan need fused")
+        if any(i not in range(c.depth) for i in c.scan):
+            raise ValueError(f"scan: layers 0 to {c.depth - 1} are there, got {tuple(c.scan)}")
         self.embed = weight(c.width, inputs)
         self.layers = torch.nn.ModuleList()
         inner = c.heads * c.head_dim
@@ -318,6 +320,8 @@ def main():
     ap.add_argument("--fused", action="store_true", help="blocks of linear and residual_norm, with norms, gates and dropout")
     ap.add_argument("--scan", default="", help="with --fused: layers that mix by gated_scan, as 1,3")
     a = ap.parse_args()
+    if a.scan and not a.fused:
+        ap.error("--scan needs --fused")
     config = Config()
     if a.fused:
         config = Config(fused=True, sandwich=True, dropout=0.05, scan=tuple(int(i) for i in a.scan.split(",") if i))
