@@ -322,7 +322,6 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
     if (kAhead) fetch(next, row_at + step);
     const float4 st = now.stats;
     float hat[NV][8], t[NV][8], b[NV][8], u[NV][8], fk[NV][8];
-    uint32_t kept[NV] = {};  // a bit an element: a dropped one's gradient is zero whatever arrives
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -339,8 +338,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           hat[i][j] = fmaf(f[j], u[i][j], hat[i][j]);
-          fk[i][j] = f[j] * k[j];
-          kept[i] |= static_cast<uint32_t>(k[j] != 0.0f) << j;
+          // (+0 + -0 is +0: only what is dropped has -0, so that its gradient can be zero whatever arrives)
+          fk[i][j] = k[j] != 0.0f ? fmaf(f[j], k[j], 0.0f) : -0.0f;
         }
       }
       now.d_n[i].to(t[i]);
@@ -366,16 +365,15 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
     }
     const float2 m = sum(s1, s2);
     const float m1 = m.x * a.inv_width, m2 = a.layer ? m.y * a.inv_width : 0.0f;
+    const float inv = a.d_n ? st.y : 0.0f;  // (a norm whose result goes nowhere adds nothing, whatever the row holds)
     s1 = s2 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const bool some = mine && at[i].n > 0;
       float d[8];
       now.d_h[i].to(d);
-      if (a.d_n) {  // (a norm whose result goes nowhere adds nothing, whatever the row holds)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] += st.y * (t[i][j] - fmaf(hat[i][j], m1, m2));
-      }
+      for (int j = 0; j < 8; ++j) d[j] += inv * (t[i][j] - fmaf(hat[i][j], m1, m2));
       if (a.d_x && some) store8(static_cast<X*>(a.d_x) + row * a.width + at[i].col, at[i].n, d);
       if (!a.y) continue;
       float e[8], w[8];
@@ -385,7 +383,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 2) void norm_bwd_kernel(NormArgs
       for (int j = 0; j < 8; ++j) {
         const bool has = mine && at[i].has(j);
         e[j] = has ? a.scale * d[j] * u[i][j] : 0.0f;  // of the gate
-        t[i][j] = has && (kept[i] >> j & 1) ? d[j] * fk[i][j] : 0.0f;
+        t[i][j] = has && __float_as_uint(fk[i][j]) != 0x80000000u ? d[j] * fk[i][j] : 0.0f;
         if (a.post) b[i][j] = has ? b[i][j] : 0.0f;
       }
       add(kSumGate, i, e, kOnes);
