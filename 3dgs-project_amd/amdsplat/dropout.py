@@ -65,7 +65,7 @@ class _Dropout(torch.autograd.Function):
 def dropout(x: torch.Tensor, p: float, seed, *, draw: int = 0) -> torch.Tensor:
     """x with elements dropped with probability p (0 <= p < 1, taken as a multiple of 2^-16) and the others
     divided by 1 - p; bfloat16 or float32 on the GPU, differentiable in x. Every dimension but the last, which is
-    below 2^31, counts as rows.
+    below 2^31, counts as rows; rows times an eighth of it (rounded up) stay below 2^32 - 256.
 
     seed: an integer, or an int64 CUDA tensor of one element, read when the kernels run (so a captured graph
     may be replayed with another seed; the backward pass reads it again, and autograd refuses one that was written

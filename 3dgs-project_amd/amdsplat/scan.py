@@ -86,8 +86,10 @@ def gated_scan(x: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | None 
     non-decreasing: document d's tokens are offsets[d] .. offsets[d + 1] (None: one document of all tokens); tokens
     outside all documents give 0. A state is h after the document's last step, an empty document's its initial
     one: given back as `initial`, the next tokens continue where these ended. Differentiable in x, forget, gate
-    and initial, through y and the states. h is float32. Documents do not reach each other, whatever they
-    hold; differences x - h have to be finite in float32. No forward-mode derivative."""
+    and initial, through y and the states. h is float32; the smaller of a and 1 - a is off by 2^-23 |forget| of itself (the
+    hardware's exponential, in float32 too). Documents do not reach each other, whatever they hold; differences
+    x - h have to be finite in float32. C up to 2^20, T times C / 256 (rounded up) up to 2^29, docs below
+    2^30. No forward-mode derivative."""
     if x.dim() != 2:
         raise ValueError("x must be [tokens, width]")
     if x.dtype not in _DTYPES:

@@ -11,11 +11,12 @@
 // rounded once. The last tiles, which would leave CUs idle, are cut along the contraction into float32 parts, which a
 // second launch sums in order and finishes (gemm_plan).
 //
-// The matrix units bound large products: bfloat16 8192 x 8192 x 8192 846 us (1300 TF/s), 8192 x 4096 x 4096 226 us (1217),
-// 16384 x 8192 x 2048 467 us (1176; with bias and residual 498), float32 4096 x 4096 x 4096 1002 us (137 of the 157 TF/s there
-// are). 8203 x 1024 x 4096 takes 87 us bare, and 105 with a bias, gelu and both results stored, 201 MB of them.
-// Products of a few tiles are bound by the chain of a tile's stages, 0.3 us each: 181 x 1024 x 1024 8.1 us (four
-// stages ahead of the products instead of one: 8.6).
+// Large products: bfloat16 8192 x 8192 x 8192 846 us (1300 TF/s), 8192 x 4096 x 4096 226 us (1217), 16384 x 8192 x 2048 467 us
+// (1176; with bias and residual 498). The matrix units are busy for half of that (51%), the one wavefront a SIMD waits for a
+// quarter (27%), and a plain library product takes 674, 196 and 355 us. float32 4096 x 4096 x 4096 is bound by the matrix units: 1002 us,
+// 137 of the 157 TF/s there are. 8203 x 1024 x 4096 takes 87 us bare, and 105 with a bias, gelu and both results stored, 201 MB
+// of them, for which the matrix units stand still. Products of a few tiles are bound by the chain of a tile's stages, 0.3 us each:
+// 181 x 1024 x 1024 8.1 us (four stages ahead of the products instead of one: 8.6).
 //
 // Few rows are bound by reading W once: linear_few_kernel streams it past the matrix unit without LDS.
 #include <algorithm>
@@ -30,6 +31,9 @@ enum { kActNone = GS_ACT_NONE, kActRelu = GS_ACT_RELU, kActGelu = GS_ACT_GELU, k
        kActSilu = GS_ACT_SILU, kActs };
 
 // ---- activations -------------------------------------------------------------------------------------
+
+// T is the operands' type here: beside operands known to 2^-8 of themselves the forms below that are off by some 2^-17 lose
+// nothing, in float32 results too (a float32 residual's), and save a sixth of a product of 1024 inputs.
 
 // exp(v), v <= 0: in bfloat16 by the hardware's exponential, off by 2^-23 |v| of itself.
 template <typename T>
@@ -49,8 +53,9 @@ __device__ __forceinline__ float sigmoid(float v) {
   return v >= 0.0f ? r : e * r;
 }
 // The normal distribution function, and exp(-z^2 / 2). float32: the library's erfc. bfloat16: Phi(-u) = exp(-u^2 / 2)
-// t P(t), t = 1 / (1 + 0.27 u), P of degree six fitted to erfcx(u / sqrt 2) / 2 over t by reweighted least squares:
-// off by 1.6e-6 of itself at most, so the tail is as exact as the middle (8203 x 1024 x 4096: 97 us, with erfc 115).
+// t P(t), t = 1 / (1 + 0.27 u), P of degree six fitted to erfcx(u / sqrt 2) / 2 over t by reweighted least squares: off by
+// 1.3e-6 of itself up to u = 14, below which Phi leaves float32. The exponential's argument adds 2^-23 u^2 / 2, so that
+// in all it is 1.6e-6 of itself up to u = 3, 3.1e-6 at 6, 6.9e-6 at 12 (8203 x 1024 x 4096: 97 us, with erfc 115).
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& bell) {
   bell = exp_down<T>(-0.5f * z * z);
@@ -567,7 +572,10 @@ __global__ __launch_bounds__(kFewWaves* kWave) void linear_few_kernel(GemmArgs g
 // ---- the activation's gradient -----------------------------------------------------------------------
 
 // dz = dout act'(z) in the operands' type, rows padded with zeros to a multiple of 16 bytes, and the column sums of
-// the unrounded dz over a workgroup's rows. Memory bounds it: 8203 x 4096 of bfloat16 with z in float32 54 us (268 MB, 5.0 TB/s).
+// the unrounded dz over a workgroup's rows. Rounded to bfloat16, since that is what the matrix instruction takes: half a step of every
+// term, so that the gradients of x and weight are off by 2.3e-3 of themselves where rounding them alone is 1.7e-3 (2-norm, 8203 x
+// 1024 -> 4096); a second term for the rest would double the products. A bias' gradient has no such rounding.
+// Memory bounds it: 8203 x 4096 of bfloat16 with z in float32 54 us (268 MB, 5.0 TB/s).
 constexpr int kSlopeThreads = 256;
 struct SlopeArgs {
   const void *d_out, *z;
@@ -753,7 +761,7 @@ struct BackPlan {
   int rows, down;  // of a workgroup of the slope kernel, and workgroups down a column
   size_t dz, parts, product;
 };
-static BackPlan back_plan(const gs_linear* p, bool bias) {
+static BackPlan back_plan(const gs_linear* p) {
   BackPlan b = {};
   const size_t es = row_type_bytes(p->dtype);
   const int64_t per = 16 / static_cast<int64_t>(es);
@@ -766,7 +774,7 @@ static BackPlan back_plan(const gs_linear* p, bool bias) {
   b.rows = static_cast<int>(std::max<int64_t>(b.rows, p->rows * across >> 23));
   b.down = static_cast<int>((p->rows + b.rows - 1) / b.rows);
   b.dz = b.make_dz ? round16(static_cast<size_t>(p->rows) * b.ld * es) : 0;
-  b.parts = bias ? round16(static_cast<size_t>(b.down) * p->outputs * sizeof(float)) : 0;
+  b.parts = round16(static_cast<size_t>(b.down) * p->outputs * sizeof(float));
   b.product = std::max(input_plan(p).part, weight_plan(p).part);
   return b;
 }
@@ -886,14 +894,14 @@ extern "C" int gs_linear_fwd(const gs_linear* p, void* workspace, size_t workspa
 extern "C" size_t gs_linear_bwd_workspace_size(const gs_linear* p) {
   clear_error();
   if (!p || p->rows <= 0 || p->inputs <= 0 || p->outputs <= 0 || !row_type(p->dtype)) return 0;
-  const BackPlan b = back_plan(p, true);
+  const BackPlan b = back_plan(p);
   return b.dz + b.parts + b.product;
 }
 
 template <typename T>
 static int run_backward(const gs_linear* p, const void* d_out, void* d_x, void* d_weight, void* d_bias, void* workspace,
                         hipStream_t st) {
-  const BackPlan b = back_plan(p, true);
+  const BackPlan b = back_plan(p);
   char* ws = static_cast<char*>(workspace);
   float* parts = reinterpret_cast<float*>(ws + b.dz);
   void* product = ws + b.dz + b.parts;

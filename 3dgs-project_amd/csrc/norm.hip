@@ -531,8 +531,9 @@ static int check_norm(const gs_residual_norm* p, bool backward, NormArgs* a) {
 // Calls f(kernel, lanes a row) with the instance for a width: as many lanes as leave eight elements each (sixteen in the
 // forward, where a wavefront's own row needs no barrier). Above 4096 the backward has too few registers: it keeps its column sums in
 // LDS and loads the weights twice, and still some of a row goes through memory: 4096 x 8192 trained by 512 lanes of
-// sixteen 408 us (829 with the sums in registers), by 1024 of eight 511; wider rows are refused. Widths that are no multiple of eight take branches for their last vector: 32771 x 1024 by those
-// instances 88 us forward and 220 with its backward, so 77 and 212.
+// sixteen 412 us (829 with the sums in registers), by 1024 of eight 511; rows wider than 8192 are refused. Widths that
+// are no multiple of eight take branches for their last vector: 32771 x 1024 by those instances 88 us forward and 220 with
+// its backward, so 77 and 211.
 template <typename X, typename Y, bool WHOLE, typename F>
 static int with_fwd(int width, F f) {
   if (width <= 512) return f(norm_fwd_kernel<X, Y, 64, 1, WHOLE>, 64);

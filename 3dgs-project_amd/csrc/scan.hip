@@ -20,9 +20,10 @@
 // that was: documents do not see each other's infinities and NaN.
 //
 // Accuracy: long memories have a near 1, where 1 - a is what counts. The smaller of a and 1 - a is formed
-// directly, s = e / (1 + e) with e = exp(-|f|), and steps are taken as h + s (x - h) or x + s (h - x). A chunk's P is
-// kept as 1 - P while that is the smaller one; a chunk's sum starts at zero, so its rounding is relative to what
-// the chunk adds; chunks and parts are joined in float64. Rounding so does not pile up over the length of the sequence.
+// directly, s = e / (1 + e) with e = exp(-|f|), by the hardware's exponential and reciprocal in both types: s is off by 2^-23 |f|
+// and a few 2^-24 of itself, beside float32 roundings of the steps. These are taken as h + s (x - h) or x + s (h - x). A chunk's P
+// is kept as 1 - P while that is the smaller one; a chunk's sum starts at zero, so its rounding is relative to what the
+// chunk adds; chunks and parts are joined in float64. Rounding so does not pile up over the length of the sequence.
 #include <algorithm>
 #include <type_traits>
 

@@ -720,7 +720,8 @@ int gs_dropout(const void* x, void* out, int64_t rows, int64_t stride, int width
  * Document d owns the tokens offsets[d] .. offsets[d + 1] (device int32, non-decreasing, docs + 1 of them; NULL for one
  * document of all tokens; values outside the tensors are cut to them). An empty document's state is its initial
  * one. Tokens outside the documents give y = 0. h is float32, and the states of long sequences are joined in
- * float64; differences x - h have to be finite in float32. Documents do not reach each other, whatever they hold.
+ * float64; differences x - h have to be finite in float32. Documents do not reach each other, whatever they hold. Fewer than 2^30
+ * documents; tokens times width / 256 (rounded up) up to 2^29.
  * carry (float32 [gs_gated_scan_chunks(tokens), width]; NULL if no backward pass follows) is written by the
  * forward and read by the backward.
  *
@@ -752,7 +753,8 @@ int gs_gated_scan_bwd(const gs_gated_scan* args, const void* d_y, const float* d
  * no further than inputs. bias [outputs] of bias_dtype and residual [rows, outputs] of out_dtype (row stride
  * residual_stride) may be NULL. out is of out_dtype: dtype, or GS_FLOAT32 for bfloat16 products. Products and the
  * epilogue are float32, rounded once. z (of z_dtype: GS_FLOAT32, or dtype; may be NULL): x weight^T + bias, for the backward
- * of an activation, whose slopes are taken there (a float32 d_bias needs a float32 z).
+ * of an activation, whose slopes are taken there (a float32 d_bias needs a float32 z). Up to 2^28 rows; rows
+ * times inputs or outputs, and inputs times outputs, up to 2^33.
  * Activations: relu, gelu z Phi(z), its tanh form, silu z sigmoid(z).
  *
  * gs_linear_bwd takes the same arguments (out and residual are not used, z is needed but for GS_ACT_NONE) and d_out [rows,
