@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import block_ref as R
-from amdsplat import dropout, linear, norm, residual_norm
+from amdsplat import dropout, gated_scan, linear, norm, residual_norm
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -150,3 +150,128 @@ def test_a_projection_is_the_same_with_and_without_gradients(dtype, shape):
         assert out.requires_grad
         with torch.no_grad():
             assert torch.equal(out.detach(), linear(x, w, bias, activation="gelu"))
+
+
+def test_a_recurrence_without_tokens():
+    """Every document is empty: states go through, and so do their gradients."""
+    for docs in (1, 5, 70, 300):
+        x = torch.zeros(0, 20, device=DEV, requires_grad=True)
+        initial = rand(1, docs, 20).requires_grad_(True)
+        offsets = None if docs == 1 else torch.zeros(docs + 1, dtype=torch.int32, device=DEV)
+        for reverse in (False, True):
+            y, state = gated_scan(x, x, x, offsets=offsets, initial=initial, reverse=reverse, return_state=True)
+            assert y.shape == (0, 20) and torch.equal(state, initial)
+            d = rand(2, docs, 20)
+            dx, di = torch.autograd.grad((y, state), (x, initial), (torch.zeros_like(y), d))
+            assert dx.shape == (0, 20) and torch.equal(di, d)
+            assert gated_scan(x, x, offsets=offsets, return_state=True)[1].eq(0).all()
+
+
+@pytest.mark.parametrize("tokens", [3, 70])
+def test_the_widest_recurrence(tokens):
+    """2^20 channels; channels do not reach each other, so some of them alone give the same bits."""
+    c = 1 << 20
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, f, o, d = (torch.randn(tokens, c, generator=g, device=DEV, dtype=BF16) for _ in range(4))
+    offsets = torch.tensor([0, 1, tokens], dtype=torch.int32, device=DEV)
+    parts = (slice(0, 8), slice(c // 2 - 4, c // 2 + 4), slice(c - 8, c))
+
+    def run(x, f, o, d):
+        v = [t.detach().clone().requires_grad_(True) for t in (x, f, o)]
+        y, state = gated_scan(*v, offsets=offsets, return_state=True)
+        return y.detach(), state.detach(), *torch.autograd.grad((y, state), v, (d, torch.ones_like(state)))
+
+    whole = run(x, f, o, d)
+    for p in parts:
+        for a, b in zip(whole, run(x[:, p], f[:, p], o[:, p], d[:, p].contiguous())):
+            assert torch.equal(a[:, p], b)
+    with pytest.raises(ValueError, match="width"):
+        gated_scan(*[torch.empty(1, c + 1, device=DEV, dtype=BF16)] * 2)
+
+
+def test_dropout_over_the_longest_dimension():
+    """2^31 - 1 elements in one row: the first ones are those of a shorter row, the last ones the generator's."""
+    n = (1 << 31) - 1
+    x = torch.ones(n, dtype=BF16, device=DEV)
+    out = dropout(x, 0.25, 9)
+    assert torch.equal(out[:1 << 20], dropout(x[:1 << 20], 0.25, 9))
+    for group in (n // 8, n // 8 - 1, n // 16):
+        words = R.philox([group, 0, 0, 0], [9, 0])
+        bits = torch.tensor([h for word in words for h in (word & 0xffff, word >> 16)])
+        mine = out[8 * group:8 * group + 8]
+        assert torch.equal(mine == 0, (bits < 16384).to(DEV)[:len(mine)])
+    kept = float((out != 0).sum()) / n
+    assert abs(kept - 0.75) < 6 * math.sqrt(0.75 * 0.25 / n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_widest_projections(dtype):
+    """2^19 inputs, 2^19 outputs, rows nearly 2^20 elements apart; few rows and tiles; all gradients, against float64."""
+    from test_gpu_linear import check
+
+    wide = 1 << 19
+    g = torch.Generator(device=DEV).manual_seed(3)
+    randn = lambda *s: torch.randn(s, generator=g, device=DEV).to(dtype)  # noqa: E731
+    far = torch.zeros(40, (1 << 20) - 8, dtype=dtype, device=DEV)
+    for rows in (9, 40):
+        far[:rows, 8:wide + 8] = randn(rows, wide)
+        check(far[:rows, 8:wide + 8], randn(24, wide) / 700, randn(24).float(), "silu")
+        check(randn(rows, 64), randn(wide, 64) / 8, None, "none", randn(rows, wide).float())
+    for shape in ((4, wide + 8), (wide + 8, 4)):
+        with pytest.raises(ValueError, match="provided"):
+            linear(torch.zeros(2, shape[1], dtype=dtype, device=DEV), torch.zeros(shape, dtype=dtype, device=DEV))
+
+
+@pytest.mark.parametrize("rows,k", [(200, 101), (9, 101), (40, 128)])
+def test_copied_rows_in_a_captured_step(rows, k):
+    """What is copied first (rows of an odd length, windows that overlap) is copied again in every replay."""
+    flat = rand(1, rows * 160, dtype=BF16)
+    x = flat.as_strided((rows, k), (32, 1) if k == 128 else (k, 1)).detach().requires_grad_(True)
+    w, b = rand(2, 72, k, dtype=BF16).requires_grad_(True), rand(3, 72).requires_grad_(True)
+    d = rand(4, rows, 72, dtype=BF16)
+
+    def step():
+        out = linear(x, w, b, activation="gelu")
+        first = torch.autograd.grad(out, (x, w, b), d, retain_graph=True)
+        second = torch.autograd.grad(out, (x, w, b), d)
+        return out.detach(), *first, *second
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (11, 12, 13):
+        flat.copy_(rand(seed, rows * 160, dtype=BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(p, q) for p, q in zip(got[1:4], got[4:]))
+        assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+def test_two_threads():
+    """Calls from two threads on streams of their own, refused ones among them: results and messages are each call's own."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    x, w = rand(1, 300, 200, dtype=BF16), rand(2, 136, 200, dtype=BF16)
+    y, s = rand(3, 500, 640), rand(4, 640)
+    want = linear(x, w, activation="gelu"), norm(y, s), gated_scan(y, y)
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for k in range(30):
+                got = linear(x, w, activation="gelu"), norm(y, s), gated_scan(y, y)
+                with pytest.raises(Exception, match="eps" if i else "activation"):
+                    norm(y, s, eps=-1.0) if i else linear(x, w, activation="x")
+                stream.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+        return True
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(work, range(2)))
