@@ -54,8 +54,8 @@ __device__ __forceinline__ float sigmoid(float v) {
 }
 // The normal distribution function, and exp(-z^2 / 2). float32: the library's erfc. bfloat16: Phi(-u) = exp(-u^2 / 2)
 // t P(t), t = 1 / (1 + 0.27 u), P of degree six fitted to erfcx(u / sqrt 2) / 2 over t by reweighted least squares: off by
-// 1.3e-6 of itself up to u = 14, below which Phi leaves float32. The exponential's argument adds 2^-23 u^2 / 2, so that
-// in all it is 1.6e-6 of itself up to u = 3, 3.1e-6 at 6, 6.9e-6 at 12 (8203 x 1024 x 4096: 97 us, with erfc 115).
+// 1.3e-6 of itself up to u = 14, where Phi(-u) is below float32's smallest number. The exponential's argument adds 2^-23 u^2 / 2, so
+// that in all it is 1.6e-6 of itself up to u = 3, 3.1e-6 at 6, 6.9e-6 at 12 (8203 x 1024 x 4096: 97 us, with erfc 115).
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& bell) {
   bell = exp_down<T>(-0.5f * z * z);
